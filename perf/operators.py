@@ -129,7 +129,7 @@ def _summary(fmt, rows, live):
     """Codes and scales of the mean rows of pages [..., page, row], over the live positions [..., page]."""
     s = (_values(fmt, rows).double() * live[..., None]).sum(-2)
     top = s.abs().amax(-1)
-    codes = torch.round(s * torch.where(top > 0, 127.0 / top, 0.0)[..., None])
+    codes = torch.round(s * 127.0 / torch.where(top > 0, top, 1.0)[..., None])
     return codes.to(torch.int8), (top / (127.0 * live.sum(-1).clamp(min=1))).float()
 
 
@@ -239,7 +239,7 @@ def _select(st):
     B, M, H, _ = st["qabs"].shape
     q = torch.cat([st["qabs"], st["q_rope"]], -1).double()
     top = q.abs().amax(-1)
-    codes = torch.round(q * torch.where(top > 0, 127.0 / top, 0.0)[..., None]).float().reshape(B, M * H, -1)
+    codes = torch.round(q * 127.0 / torch.where(top > 0, top, 1.0)[..., None]).float().reshape(B, M * H, -1)
     at = st["table"].clamp(min=0).long()
     # sums of 576 products of 7 bits are whole numbers under 2^24: exact in f32
     dots = torch.bmm(codes, st["mean"][at].float().transpose(1, 2).contiguous()).reshape(B, M, H, -1)
@@ -314,7 +314,7 @@ def _exact_mean(case, pages, phys, live):
     x = pages[phys, :live]
     s = (x.double() if case["fmt"] == "bf16" else x[:, 0].double() + x[:, 1].double() * 2.0 ** -11).sum(0)
     top = s.abs().max()
-    return torch.round(s * (127.0 / top)) * (top / (127.0 * live)).float().double() if top > 0 else s * 0
+    return torch.round(s * 127.0 / top) * (top / (127.0 * live)).float().double() if top > 0 else s * 0
 
 
 def exact(case, seed):
@@ -346,7 +346,7 @@ def exact(case, seed):
                 k = -(-(n - M + j + 1) // page)
                 at = table[b, :k].long()
                 top = q[b, j].abs().amax(-1)
-                dots = torch.round(q[b, j] * (127.0 / top)[:, None]) @ st["mean"][at].double().T
+                dots = torch.round(q[b, j] * 127.0 / top[:, None]) @ st["mean"][at].double().T
                 score = (dots.relu() * (top / 127.0)[:, None]).sum(0) * st["mean_scale"][at].double()
                 score = score.tolist()
                 forced = set(range(min(KEEP_FIRST, k))) | set(range(max(0, k - KEEP_LAST), k))
