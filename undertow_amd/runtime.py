@@ -465,7 +465,7 @@ def mla_attend(ctx: Context, qabs, q_rope, latent, krot, pos_base: int, scale: f
     if out is None:
         out = torch.empty((R, H, L), dtype=torch.float32, device=qabs.device)
     elif tuple(out.shape) != (R, H, L) or out.dtype != torch.float32 or not out.is_contiguous():
-        raise ShapeError(f"mla_attend: out must be a contiguous float32 [{R}, {H}, {L}] tensor")
+        raise ShapeError(UT_ERR_SHAPE, f"mla_attend: out must be a contiguous float32 [{R}, {H}, {L}] tensor")
     ctx.check(lib().ut_mla_attend(ctx.handle, _ptr(qabs), _ptr(q_rope), _ptr(latent), _ptr(krot),
                                   R, H, L, P, pos_base, scale, _ptr(out)))
     return out
@@ -487,7 +487,7 @@ def mla_attend_split(ctx: Context, qabs, q_rope, kc, pos_base: int, scale: float
     R, H, L = qabs.shape
     P = q_rope.shape[2]
     if kc.shape[-1] != L + P:
-        raise ShapeError(f"mla_attend_split: cache width {kc.shape[-1]} != {L} + {P}")
+        raise ShapeError(UT_ERR_SHAPE, f"mla_attend_split: cache width {kc.shape[-1]} != {L} + {P}")
     if out is None:
         out = torch.empty((R, H, L), dtype=torch.float32, device=qabs.device)
     ctx.check(lib().ut_mla_attend_split(ctx.handle, _ptr(qabs), _ptr(q_rope), _ptr(kc), R, H, L, P,
