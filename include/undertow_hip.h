@@ -45,7 +45,8 @@ enum {
     UT_ERR_BAD_TOKEN = -8,        /* token id >= vocab_size */
     UT_ERR_NOT_FOUND = -9,        /* a required tensor was never set */
     UT_ERR_STATE = -10,           /* call out of order (e.g. no MTP head) */
-    UT_ERR_IO = -11               /* EngineError::Io: a checkpoint file could not be read */
+    UT_ERR_IO = -11,              /* EngineError::Io: a checkpoint file could not be read */
+    UT_ERR_BAD_PAGE = -12         /* a length beyond its table, or a page outside its pool */
 };
 
 /* QuantFormat (undertow-quant/src/qtensor.rs:17-21).  UT_FMT_INFER asks
@@ -77,7 +78,7 @@ const char *ut_last_error(const ut_ctx *ctx);
 int32_t     ut_ctx_set_stream(ut_ctx *ctx, void *stream);
 void       *ut_ctx_stream(ut_ctx *ctx);
 /* Waits for the context's stream; also reports errors detected on device
- * since the last call (UT_ERR_BAD_EXPERT). */
+ * since the last call (UT_ERR_BAD_EXPERT, UT_ERR_BAD_PAGE). */
 int32_t     ut_ctx_synchronize(ut_ctx *ctx);
 /* Per-kernel timing with HIP events on the context stream (bench tooling):
  * while enabled, every kernel the library launches is bracketed by events;
@@ -287,6 +288,87 @@ int32_t ut_mla_cache_split(ut_ctx *ctx, const float *latent_dev, const float *kr
 int32_t ut_mla_attend_split(ut_ctx *ctx, const float *qabs_dev, const float *q_rope_dev,
                             const void *kc_dev, int64_t R, int64_t H, int64_t L, int64_t P,
                             int64_t pos_base, float scale, float *clat_dev);
+
+/* ---------------------------------------------------------- paged cache */
+/* No reference counterpart (the reference keeps one LayerKvCache per
+ * session): one layer's latent cache of many sequences in a pool of pages.
+ * Every page holds `page` positions (a power of two of at most 1024), each
+ * the row [latent | krot] of D = latent + rope values (multiples of 8, D at
+ * most 1024) as
+ *   UT_KV_BF16   [n_pages][page][D] bf16; queries and contexts are bf16 too;
+ *   UT_KV_F16X2  [n_pages][page][2][D] f16, x = hi + lo / 2048 to 2^-23 |x|
+ *                (|x| up to 65504; finite values beyond take that), the bytes
+ *                of f32 rows; queries and contexts are f32.
+ * mean / mean_scale (both or neither NULL) summarise each page for
+ * ut_mla_page_select: the mean row is mean_scale[p] * mean[p][d] to 1/254 of
+ * its largest value.  pages and mean are 16-byte aligned.  The struct is
+ * read during the call only; the memory is the caller's.
+ *
+ * A batch: table_dev holds `batch` rows, table_stride entries apart, each of
+ * max_pages physical page ids in the sequence's order; lens_dev [batch]
+ * counts a sequence's positions, the `rows` rows of the present step
+ * included.  Row j of a sequence stands at position lens - rows + j and sees
+ * the positions up to its own: lens - rows + j + 1 of them.  Where that is not
+ * positive (a batch padded with lens 0, fewer new rows than `rows`, aligned
+ * to the end) the row has no position and sees nothing.  Sequences may share pages; entries behind a
+ * sequence's last page are not read.  Lengths and tables stay on the device
+ * and may change between replays of a captured call.  A length that is
+ * negative or beyond its table is cut, a page id outside the pool reads page
+ * 0 (an append writes nothing there), and the next ut_ctx_synchronize returns
+ * UT_ERR_BAD_PAGE; the values of that sequence are then unspecified.  At most
+ * 65535 sequences, and rows in all for the calls with queries.
+ * All calls run on the context's device and stream; those that need working
+ * memory take the context's arena. */
+enum { UT_KV_BF16 = 0, UT_KV_F16X2 = 1 };
+typedef struct {
+    void *pages;
+    int8_t *mean;      /* [n_pages][D] or NULL */
+    float *mean_scale; /* [n_pages] or NULL */
+    int64_t n_pages, page, latent, rope;
+    int32_t fmt;
+} ut_mla_pages;
+
+/* Writes the rows latent [batch, rows, latent] and krot [batch, rows, rope]
+ * (f32) to their positions, and the summary of every page they fall into
+ * anew from its stored positions below lens.  A position before the cache's
+ * start is not written.  Two rows must not fall on one place of the pool. */
+int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
+                            int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
+                            int64_t batch, int64_t rows, const float *latent_dev,
+                            const float *krot_dev);
+/* ut_mla_attend for each row over its sequence's pages: qabs [batch, rows,
+ * heads, latent], q_rope [batch, rows, heads, rope], clat like qabs, in the
+ * cache format's type.  A row that sees nothing gets zeros.  What a row does
+ * not see does not reach it, NaN and infinities included.  Equal calls give
+ * equal bits; a row's rounding may depend on the lengths of the batch (the
+ * work is cut evenly over the device). */
+int32_t ut_mla_paged_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
+                            int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
+                            int64_t batch, int64_t rows, int64_t heads, const void *qabs_dev,
+                            const void *q_rope_dev, float scale, void *clat_dev);
+/* The pages each row shall attend to: of the pages it sees, the first
+ * keep_first, the last keep_last, and then those of the largest score, ties
+ * to the lower page; top_k in all, written to sel [batch, rows, top_k] in
+ * ascending order (the sequence's page numbers, not physical ids), -1 behind
+ * them.  The score of a page is
+ *   mean_scale * sum_h weight_h * max|q_h| / 127 * max(0, code(q_h) . mean)
+ * with q_h = [qabs | q_rope] of head h and code(q) = rint(q * 127 / max|q|):
+ * the products are exact in integers and the sum runs in 64 bits.  weights
+ * [batch, rows, heads] f32 or NULL (all 1).  A head whose query is not finite
+ * is left out; a NaN score ranks last. */
+int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
+                           int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
+                           int64_t batch, int64_t rows, int64_t heads, const void *qabs_dev,
+                           const void *q_rope_dev, const float *weights_dev, int64_t keep_first,
+                           int64_t keep_last, int64_t top_k, int32_t *sel_dev);
+/* ut_mla_paged_attend over the listed pages only: sel [batch, rows, top_k]
+ * sequence page numbers in any order.  Negative entries and pages behind the
+ * row's end are skipped; a page listed twice counts twice. */
+int32_t ut_mla_sparse_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
+                             int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
+                             int64_t batch, int64_t rows, int64_t heads, const void *qabs_dev,
+                             const void *q_rope_dev, float scale, const int32_t *sel_dev,
+                             int64_t top_k, void *clat_dev);
 
 /* ---------------------------------------------------------------- model */
 /* DeepseekConfig fields the forward pass reads (adapters/undertow-deepseek-

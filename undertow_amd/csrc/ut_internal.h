@@ -63,8 +63,8 @@ struct ut_ctx {
     std::vector<ut::KernelStat> stats;
     std::vector<ut::PendingTiming> pending;
     int multiprocessors = 256;
-    // Sticky device-side error flag (invalid expert ids), reported by the
-    // next ut_ctx_synchronize().
+    // Sticky device-side error words (invalid expert ids; lengths and pages of
+    // paged calls), reported by the next ut_ctx_synchronize().
     int32_t *dev_err = nullptr;
     // Split-K GEMV partial totals (allocated on first use).
     void *splitk = nullptr;
@@ -148,8 +148,8 @@ void timing_end(ut_ctx *ctx, int token);
 int32_t launch_check(ut_ctx *ctx, const char *name);
 void ctx_retain(ut_ctx *ctx);
 void ctx_release(ut_ctx *ctx);
-// The context's device error flag (allocated when the context is created)
-// and its check.
+// The context's device error words (allocated when the context is created),
+// the expert word first and the page word behind it, and their check.
 int32_t device_error_flag(ut_ctx *ctx, int32_t **flag);
 // Looks up this device's copy of the expert block's fixed working array
 // (hipGetSymbolAddress, the device current) into ctx->noalloc_scratch.

@@ -1,0 +1,527 @@
+// ut_paged.hip -- the paged MLA latent cache: appending a step's rows, the
+// score that selects pages, and attention for any latent width.
+#include "ut_paged.h"
+
+namespace ut {
+
+struct Bf16 {
+    static constexpr int kPlanes = 1;
+    typedef __bf16 q_t;
+    __device__ static float value(const uint16_t *row, int D, int d) {
+        return __uint_as_float((uint32_t)row[d] << 16);
+    }
+};
+struct F16x2 {
+    static constexpr int kPlanes = 2;
+    typedef float q_t;
+    __device__ static float value(const uint16_t *row, int D, int d) {
+        const _Float16 *h = (const _Float16 *)row;
+        return __fadd_rn((float)h[d], __fmul_rn((float)h[D + d], 1.0f / kF16x2Step));
+    }
+};
+
+// -------------------------------------------------------------- append ---
+// A workgroup takes one page that a sequence's new rows fall into: it writes
+// the new rows and, where summaries are kept, adds the page's rows up dim by
+// dim in 64 bits (sums of values of 8 or 22 bits: exact but for extreme
+// ranges), the older ones read back and the new ones as stored:
+//   S_d = sum x_d, A = max_d |S_d|, code = rint(S_d 127 / A),
+//   scale = A / (127 n)   (code * scale is the mean row to 1/254 of its max).
+// A thread holds four dims of every fourth position.
+template <class F>
+__global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__restrict__ pages,
+                                                      const float *__restrict__ latent,
+                                                      const float *__restrict__ krot,
+                                                      int8_t *__restrict__ mean,
+                                                      float *__restrict__ mean_scale) {
+    extern __shared__ double sum[];  // [4][D]
+    __shared__ double red[16];
+    const int b = blockIdx.y, tid = threadIdx.x, D = a.L + a.P, nq = D / 4;
+    const int32_t len = paged_len(a, b);
+    const int32_t from = len > a.M ? len - a.M : 0;  // the first new position
+    const int k = (from >> a.shift) + (int)blockIdx.x;
+    const int32_t page = 1 << a.shift;
+    const int64_t p0 = (int64_t)k << a.shift;
+    if (p0 >= len) return;
+    bool bad = false;
+    const int32_t phys = paged_phys(a, b, k, bad);
+    if (bad) return;
+    const int live = len - p0 < page ? (int)(len - p0) : page;
+    const int first = from > p0 ? (int)(from - p0) : 0;  // the page's first new row
+    const int64_t row16 = (int64_t)D * F::kPlanes;
+    uint16_t *base = pages + ((int64_t)phys << a.shift) * row16;
+    for (int u = tid; u < 4 * nq; u += blockDim.x) {
+        const int s = u / nq, d = (u - s * nq) * 4;
+        double t[4] = {0.0, 0.0, 0.0, 0.0};
+        if (mean)
+            for (int o = s; o < first; o += 4)
+#pragma unroll
+                for (int i = 0; i < 4; i++) t[i] += (double)F::value(base + o * row16, D, d + i);
+        for (int o = first + ((s - first) & 3); o < live; o += 4) {
+            const int64_t r = (int64_t)b * a.M + (p0 + o - (len - a.M));
+            const float4 v = d < a.L ? *(const float4 *)(latent + r * a.L + d)
+                                     : *(const float4 *)(krot + r * a.P + (d - a.L));
+            const float x[4] = {v.x, v.y, v.z, v.w};
+            uint16_t *row = base + o * row16 + d;
+            if (F::kPlanes == 1) {
+                __bf16 h[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    h[i] = (__bf16)x[i];
+                    t[i] += (double)(float)h[i];
+                }
+                *(uint2 *)row = *(const uint2 *)h;
+            } else {
+                _Float16 h[4], l[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    f16x2_split(x[i], h[i], l[i]);
+                    t[i] += (double)__fadd_rn((float)h[i], __fmul_rn((float)l[i], 1.0f / kF16x2Step));
+                }
+                *(uint2 *)row = *(const uint2 *)h;
+                *(uint2 *)(row + D) = *(const uint2 *)l;
+            }
+        }
+        if (mean)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sum[s * D + d + i] = t[i];
+    }
+    if (!mean) return;
+    __syncthreads();
+    double top = 0.0;
+    for (int d = tid; d < D; d += blockDim.x) {
+        const double t = (sum[d] + sum[D + d]) + (sum[2 * D + d] + sum[3 * D + d]);
+        sum[d] = t;
+        top = fmax(top, fabs(t));
+    }
+    for (int off = 32; off >= 1; off >>= 1) top = fmax(top, __shfl_xor(top, off, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+    __syncthreads();
+    for (int w = 0; w < (int)(blockDim.x >> 6); w++) top = fmax(top, red[w]);
+    for (int d = tid; d < D; d += blockDim.x) {
+        const double c = top > 0.0 ? rint(sum[d] * 127.0 / top) : 0.0;
+        mean[(int64_t)phys * D + d] = (int8_t)(c >= -127.0 && c <= 127.0 ? (int)c : 0);
+    }
+    if (tid == 0) mean_scale[phys] = (float)(top / (127.0 * live));
+}
+
+// ----------------------------------------------------------- attention ---
+// Any latent width: a workgroup takes one head of one row and goes over its
+// positions 64 at a time, four lanes to a position, with the running maximum
+// and sum of the softmax.  Only visible positions are read.
+constexpr int kGenChunk = 64;
+template <class F>
+__global__ __launch_bounds__(256) void k_paged_attend(PagedArgs a) {
+    extern __shared__ float sm[];
+    const int h = blockIdx.x, j = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    const int D = a.L + a.P;
+    float *q = sm, *o = q + D, *p = o + a.L;  // [D], [L], [kGenChunk]
+    __shared__ int64_t at[kGenChunk];
+    const int64_t r = ((int64_t)b * a.M + j) * a.H + h;
+    const int32_t n = paged_len(a, b) - a.M + j + 1;
+    for (int d = tid; d < D; d += 256)
+        q[d] = d < a.L ? (float)((const typename F::q_t *)a.qabs)[r * a.L + d]
+                       : (float)((const typename F::q_t *)a.qrope)[r * a.P + (d - a.L)];
+    for (int d = tid; d < a.L; d += 256) o[d] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const int64_t total = a.sel ? (int64_t)a.top_k << a.shift : (int64_t)(n > 0 ? n : 0);
+    const int64_t row16 = (int64_t)D * F::kPlanes;
+    for (int64_t t0 = 0; t0 < total; t0 += kGenChunk) {
+        __syncthreads();
+        if (tid < kGenChunk) {
+            const int64_t t = t0 + tid;
+            int64_t row = -1;
+            if (t < total) {
+                int64_t k = t >> a.shift;
+                if (a.sel) k = a.sel[((int64_t)b * a.M + j) * a.top_k + k];
+                const int64_t pos = (k << a.shift) + (t & ((1 << a.shift) - 1));
+                if (k >= 0 && pos < n)
+                    row = ((int64_t)paged_phys(a, b, (int)k) << a.shift) + (t & ((1 << a.shift) - 1));
+            }
+            at[tid] = row;
+        }
+        __syncthreads();
+        const int t = tid >> 2, s = tid & 3;
+        float acc = 0.0f;
+        const int64_t row = at[t];
+        if (row >= 0) {
+            const uint16_t *src = (const uint16_t *)a.pages + row * row16;
+            for (int d = s; d < D; d += 4) acc = __builtin_fmaf(q[d], F::value(src, D, d), acc);
+        }
+        acc += __shfl_xor(acc, 1, 64);
+        acc += __shfl_xor(acc, 2, 64);
+        if (s == 0) p[t] = row >= 0 ? __fmul_rn(acc, a.scale) : -INFINITY;
+        __syncthreads();
+        // NaN scores reach the output: a maximum that skips them, then e^NaN
+        float mn = m;
+        for (int i = 0; i < kGenChunk; i++) mn = fmaxf(mn, p[i]);
+        const float base = mn > -INFINITY ? mn : 0.0f, f = m > -INFINITY ? expf(m - base) : 0.0f;
+        float ls = 0.0f;
+        for (int i = 0; i < kGenChunk; i++)
+            if (at[i] >= 0) ls += expf(p[i] - base);
+        l = l * f + ls;
+        m = mn;
+        for (int d = tid; d < a.L; d += 256) {
+            float v = o[d] * f;
+            for (int i = 0; i < kGenChunk; i++)
+                if (at[i] >= 0)
+                    v = __builtin_fmaf(expf(p[i] - base),
+                                       F::value((const uint16_t *)a.pages + at[i] * row16, D, d), v);
+            o[d] = v;
+        }
+    }
+    __syncthreads();
+    for (int d = tid; d < a.L; d += 256)
+        ((typename F::q_t *)a.out)[r * a.L + d] = (typename F::q_t)(l != 0.0f ? o[d] / l : 0.0f);
+}
+
+// -------------------------------------------------------------- select ---
+// A head's query in 8 bits: code = rint(q 127 / max|q|); its share of a score
+// is weight max|q| / 127.  A head with a value that is not finite has none.
+template <class F>
+__global__ __launch_bounds__(64) void k_select_codes(PagedArgs a, const float *__restrict__ weights,
+                                                     int8_t *__restrict__ codes,
+                                                     double *__restrict__ share) {
+    const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x, D = a.L + a.P;
+    auto q = [&](int d) {
+        return d < a.L ? (float)((const typename F::q_t *)a.qabs)[r * a.L + d]
+                       : (float)((const typename F::q_t *)a.qrope)[r * a.P + (d - a.L)];
+    };
+    uint32_t top = 0;  // |q|'s bits: NaN lies above infinity
+    for (int d = lane; d < D; d += 64) {
+        const uint32_t v = __float_as_uint(q(d)) & 0x7fffffffu;
+        top = v > top ? v : top;
+    }
+    for (int off = 32; off >= 1; off >>= 1) {
+        const uint32_t v = __shfl_xor(top, off, 64);
+        top = v > top ? v : top;
+    }
+    const bool live = top > 0 && top < 0x7f800000u;
+    const double m = (double)__uint_as_float(top);
+    for (int d = lane; d < D; d += 64)
+        codes[r * D + d] = live ? (int8_t)(int)rint((double)q(d) * 127.0 / m) : 0;
+    if (lane == 0) share[r] = live ? (weights ? (double)weights[r] : 1.0) * (m / 127.0) : 0.0;
+}
+
+// A score's order as an unsigned number; NaN below everything.
+__device__ __forceinline__ uint64_t score_key(double s) {
+    if (!(s == s)) return 0;
+    const uint64_t u = (uint64_t)__double_as_longlong(s + 0.0);  // -0 counts as 0
+    return u >> 63 ? ~u : u | (1ull << 63);
+}
+
+// score = (sum_h share_h max(0, code_h . mean)) mean_scale, a wave to a page.
+__global__ __launch_bounds__(256) void k_select_score(PagedArgs a, const int8_t *__restrict__ codes,
+                                                      const double *__restrict__ share,
+                                                      const int8_t *__restrict__ mean,
+                                                      const float *__restrict__ mean_scale,
+                                                      uint64_t *__restrict__ keys) {
+    const int row = blockIdx.y, b = row / a.M, j = row - b * a.M, lane = threadIdx.x & 63;
+    const int k = blockIdx.x * 4 + (threadIdx.x >> 6), D = a.L + a.P;
+    const int32_t n = paged_len(a, b) - a.M + j + 1;
+    if (n <= 0 || k > (n - 1) >> a.shift) return;
+    const int32_t phys = paged_phys(a, b, k);
+    const uint32_t *mw = (const uint32_t *)(mean + (int64_t)phys * D);
+    double t = 0.0;
+    for (int h = 0; h < a.H; h++) {
+        const int64_t r = (int64_t)row * a.H + h;
+        const uint32_t *cw = (const uint32_t *)(codes + r * D);
+        int dot = 0;
+        for (int w = lane; w < D / 4; w += 64) dot = __builtin_amdgcn_sdot4(mw[w], cw[w], dot, false);
+        for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off, 64);
+        t += share[r] * (double)(dot > 0 ? dot : 0);
+    }
+    if (lane == 0) keys[(int64_t)row * a.max_pages + k] = score_key(t * (double)mean_scale[phys]);
+}
+
+// The top_k pages of a row: the first keep_first, the last keep_last, then by
+// score, ties to the lower page; ascending, -1 behind them.  The top_k-th
+// largest key is found digit by digit (eight of 8 bits, counted in LDS), then
+// one pass writes the pages above it and the first of those equal to it.
+constexpr int kPickThreads = 1024;
+__global__ __launch_bounds__(kPickThreads) void k_select_pick(PagedArgs a,
+                                                              const uint64_t *__restrict__ keys,
+                                                              int keep_first, int keep_last,
+                                                              int32_t *__restrict__ out) {
+    __shared__ int hist[256];
+    __shared__ int s_digit, s_above, scan[kPickThreads / 64 * 2];
+    const int row = blockIdx.x, b = row / a.M, j = row - b * a.M, tid = threadIdx.x;
+    const int32_t n = paged_len(a, b) - a.M + j + 1;
+    const int np = n > 0 ? ((n - 1) >> a.shift) + 1 : 0;
+    out += (int64_t)row * a.top_k;
+    if (np <= a.top_k) {
+        for (int i = tid; i < a.top_k; i += kPickThreads) out[i] = i < np ? i : -1;
+        return;
+    }
+    keys += (int64_t)row * a.max_pages;
+    auto key = [&](int k) {
+        return k < keep_first || k >= np - keep_last ? ~0ull : keys[k];
+    };
+    uint64_t prefix = 0;
+    int need = a.top_k;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (int k = tid; k < np; k += kPickThreads) {
+            const uint64_t v = key(k);
+            if (shift == 56 || (v >> (shift + 8)) == (prefix >> (shift + 8)))
+                atomicAdd(&hist[(v >> shift) & 255], 1);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int above = 0, d = 255;
+            while (above + hist[d] < need) above += hist[d--];
+            s_digit = d;
+            s_above = above;
+        }
+        __syncthreads();
+        prefix |= (uint64_t)s_digit << shift;
+        need -= s_above;
+    }
+    // `need` of the pages equal to the key are taken, the lowest first
+    int done = 0, equal = 0;
+    const int lane = tid & 63, w = tid >> 6;
+    for (int k0 = 0; k0 < np; k0 += kPickThreads) {
+        const int k = k0 + tid;
+        const uint64_t v = k < np ? key(k) : 0;
+        const bool gt = k < np && v > prefix, eq = k < np && v == prefix;
+        const uint64_t be = __ballot(eq), bg = __ballot(gt);
+        __syncthreads();
+        if (lane == 0) scan[w] = __popcll(be);
+        __syncthreads();
+        int e = equal + __popcll(be & ((1ull << lane) - 1)), te = equal;
+        for (int i = 0; i < kPickThreads / 64; i++) {
+            if (i < w) e += scan[i];
+            te += scan[i];
+        }
+        equal = te;
+        const bool take = gt || (eq && e < need);
+        const uint64_t bt = __ballot(take);
+        if (lane == 0) scan[kPickThreads / 64 + w] = __popcll(bt);
+        __syncthreads();
+        int at = done + __popcll(bt & ((1ull << lane) - 1)), td = done;
+        for (int i = 0; i < kPickThreads / 64; i++) {
+            if (i < w) at += scan[kPickThreads / 64 + i];
+            td += scan[kPickThreads / 64 + i];
+        }
+        if (take) out[at] = k;
+        done = td;
+    }
+}
+
+// ------------------------------------------------------------ the calls ---
+// The context's device while a call runs: its allocations and launches go
+// there whichever device the caller has current.
+struct DeviceScope {
+    int before = -1;
+    bool ok = true;
+    explicit DeviceScope(int device) {
+        int d = -1;
+        ok = hipGetDevice(&d) == hipSuccess;
+        if (ok && d != device) {
+            before = d;
+            ok = hipSetDevice(device) == hipSuccess;
+        }
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+static int32_t paged_args(ut_ctx *ctx, const char *what, const ut_mla_pages *kv,
+                          const int32_t *table, int64_t stride, int64_t max_pages,
+                          const int32_t *lens, int64_t B, int64_t M, int64_t H, PagedArgs &a) {
+    auto bad = [&](const char *why) {
+        set_error(ctx, "%s: %s", what, why);
+        return UT_ERR_ARG;
+    };
+    if (!kv || !kv->pages || !table || !lens) return bad("null pointer");
+    if (kv->fmt != UT_KV_BF16 && kv->fmt != UT_KV_F16X2) return bad("unknown cache format");
+    if (kv->n_pages <= 0 || max_pages <= 0 || B <= 0 || M <= 0 || H <= 0 || stride < max_pages)
+        return bad("sizes must be positive and the table's stride cover its pages");
+    if (((uintptr_t)kv->pages & 15) != 0) return bad("pages must be 16-byte aligned");
+    const int64_t page = kv->page, L = kv->latent, P = kv->rope;
+    auto shape = [&](const char *why) {
+        set_error(ctx, "%s: %s (page %lld, latent %lld, rope %lld, sequences %lld, rows %lld, heads %lld)",
+                  what, why, (long long)page, (long long)L, (long long)P, (long long)B, (long long)M,
+                  (long long)H);
+        return UT_ERR_SHAPE;
+    };
+    if (page < 1 || page > 1024 || (page & (page - 1)) != 0)
+        return shape("a page is a power of two of at most 1024 positions");
+    if (L <= 0 || P <= 0 || L % 8 != 0 || P % 8 != 0 || L + P > 1024)
+        return shape("latent and rope must be multiples of 8 that add up to at most 1024");
+    if (kv->n_pages > INT32_MAX / page || max_pages > INT32_MAX / page)
+        return shape("a pool and a sequence hold fewer than 2^31 positions");
+    if (B > 65535 || H > 65535 || M > INT32_MAX / B / H || (H > 1 && B * M > 65535))
+        return shape("too many sequences, rows or heads");
+    a = PagedArgs{};
+    a.pages = kv->pages;
+    a.table = table;
+    a.stride = stride;
+    a.lens = lens;
+    UT_TRY(device_error_flag(ctx, &a.err));
+    a.err += 1;  // the page word
+    a.n_pages = (int32_t)kv->n_pages;
+    a.max_pages = (int32_t)max_pages;
+    a.shift = __builtin_ctzll((uint64_t)page);
+    a.B = (int32_t)B;
+    a.M = (int32_t)M;
+    a.H = (int32_t)H;
+    a.L = (int32_t)L;
+    a.P = (int32_t)P;
+    return UT_OK;
+}
+
+static int32_t launch_paged_generic(ut_ctx *ctx, const PagedArgs &a, int32_t fmt) {
+    const size_t lds = (size_t)(2 * a.L + a.P + kGenChunk) * 4;
+    const dim3 grid((unsigned)a.H, (unsigned)a.M, (unsigned)a.B);
+    int tok = timing_begin(ctx, "paged_attend");
+    if (fmt == UT_KV_BF16) hipLaunchKernelGGL(k_paged_attend<Bf16>, grid, dim3(256), lds, ctx->stream, a);
+    else hipLaunchKernelGGL(k_paged_attend<F16x2>, grid, dim3(256), lds, ctx->stream, a);
+    timing_end(ctx, tok);
+    return launch_check(ctx, "k_paged_attend");
+}
+
+static int32_t paged_attend(ut_ctx *ctx, const char *what, const ut_mla_pages *kv,
+                            const int32_t *table, int64_t stride, int64_t max_pages,
+                            const int32_t *lens, int64_t B, int64_t M, int64_t H, const void *qabs,
+                            const void *qrope, float scale, const int32_t *sel, int64_t top_k,
+                            void *out) {
+    DeviceScope dev(ctx->device);
+    PagedArgs a;
+    UT_TRY(paged_args(ctx, what, kv, table, stride, max_pages, lens, B, M, H, a));
+    if (!qabs || !qrope || !out || ((uintptr_t)qabs & 15) != 0 || ((uintptr_t)qrope & 15) != 0 ||
+        ((uintptr_t)out & 15) != 0) {
+        set_error(ctx, "%s: queries and output must be 16-byte aligned device memory", what);
+        return UT_ERR_ARG;
+    }
+    a.qabs = qabs;
+    a.qrope = qrope;
+    a.scale = scale;
+    a.sel = sel;
+    a.top_k = (int32_t)top_k;
+    a.out = out;
+    return launch_paged_generic(ctx, a, kv->fmt);
+}
+
+}  // namespace ut
+
+using namespace ut;
+
+extern "C" int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv,
+                                       const int32_t *table_dev, int64_t table_stride,
+                                       int64_t max_pages, const int32_t *lens_dev, int64_t batch,
+                                       int64_t rows, const float *latent_dev,
+                                       const float *krot_dev) {
+    if (!ctx) return UT_ERR_ARG;
+    DeviceScope dev(ctx->device);
+    PagedArgs a;
+    UT_TRY(paged_args(ctx, "ut_mla_paged_append", kv, table_dev, table_stride, max_pages, lens_dev,
+                      batch, rows, 1, a));
+    if (!latent_dev || !krot_dev || ((uintptr_t)latent_dev & 15) != 0 ||
+        ((uintptr_t)krot_dev & 15) != 0 || !kv->mean != !kv->mean_scale) {
+        set_error(ctx, "ut_mla_paged_append: rows must be 16-byte aligned device memory, and mean "
+                       "and mean_scale be given together");
+        return UT_ERR_ARG;
+    }
+    // pages that `rows` positions can fall into
+    const int64_t page = kv->page, touched = (rows + page - 2) / page + 1;
+    const size_t lds = kv->mean ? (size_t)(a.L + a.P) * 4 * sizeof(double) : 0;
+    const dim3 grid((unsigned)(touched < max_pages ? touched : max_pages), (unsigned)batch);
+    int tok = timing_begin(ctx, "paged_append");
+    if (kv->fmt == UT_KV_BF16)
+        hipLaunchKernelGGL(k_paged_append<Bf16>, grid, dim3(576), lds, ctx->stream, a,
+                           (uint16_t *)kv->pages, latent_dev, krot_dev, kv->mean, kv->mean_scale);
+    else
+        hipLaunchKernelGGL(k_paged_append<F16x2>, grid, dim3(576), lds, ctx->stream, a,
+                           (uint16_t *)kv->pages, latent_dev, krot_dev, kv->mean, kv->mean_scale);
+    timing_end(ctx, tok);
+    return launch_check(ctx, "k_paged_append");
+}
+
+extern "C" int32_t ut_mla_paged_attend(ut_ctx *ctx, const ut_mla_pages *kv,
+                                       const int32_t *table_dev, int64_t table_stride,
+                                       int64_t max_pages, const int32_t *lens_dev, int64_t batch,
+                                       int64_t rows, int64_t heads, const void *qabs_dev,
+                                       const void *q_rope_dev, float scale, void *clat_dev) {
+    if (!ctx) return UT_ERR_ARG;
+    return paged_attend(ctx, "ut_mla_paged_attend", kv, table_dev, table_stride, max_pages,
+                        lens_dev, batch, rows, heads, qabs_dev, q_rope_dev, scale, nullptr, 0,
+                        clat_dev);
+}
+
+extern "C" int32_t ut_mla_sparse_attend(ut_ctx *ctx, const ut_mla_pages *kv,
+                                        const int32_t *table_dev, int64_t table_stride,
+                                        int64_t max_pages, const int32_t *lens_dev, int64_t batch,
+                                        int64_t rows, int64_t heads, const void *qabs_dev,
+                                        const void *q_rope_dev, float scale, const int32_t *sel_dev,
+                                        int64_t top_k, void *clat_dev) {
+    if (!ctx) return UT_ERR_ARG;
+    if (!sel_dev || top_k <= 0 || (kv && kv->page > 0 && top_k > INT32_MAX / kv->page)) {
+        set_error(ctx, "ut_mla_sparse_attend: a selection of at least one page is needed");
+        return UT_ERR_ARG;
+    }
+    return paged_attend(ctx, "ut_mla_sparse_attend", kv, table_dev, table_stride, max_pages,
+                        lens_dev, batch, rows, heads, qabs_dev, q_rope_dev, scale, sel_dev, top_k,
+                        clat_dev);
+}
+
+extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
+                                      int64_t table_stride, int64_t max_pages,
+                                      const int32_t *lens_dev, int64_t batch, int64_t rows,
+                                      int64_t heads, const void *qabs_dev, const void *q_rope_dev,
+                                      const float *weights_dev, int64_t keep_first,
+                                      int64_t keep_last, int64_t top_k, int32_t *sel_dev) {
+    if (!ctx) return UT_ERR_ARG;
+    DeviceScope dev(ctx->device);
+    PagedArgs a;
+    UT_TRY(paged_args(ctx, "ut_mla_page_select", kv, table_dev, table_stride, max_pages, lens_dev,
+                      batch, rows, heads, a));
+    if (!qabs_dev || !q_rope_dev || !sel_dev || !kv->mean || !kv->mean_scale ||
+        ((uintptr_t)qabs_dev & 15) != 0 || ((uintptr_t)q_rope_dev & 15) != 0 ||
+        ((uintptr_t)kv->mean & 15) != 0) {
+        set_error(ctx, "ut_mla_page_select: queries and page means must be 16-byte aligned device "
+                       "memory");
+        return UT_ERR_ARG;
+    }
+    if (keep_first < 0 || keep_last < 0 || top_k <= 0 || top_k > INT32_MAX / 2 ||
+        keep_first > top_k || keep_last > top_k - keep_first) {
+        set_error(ctx, "ut_mla_page_select: top_k %lld must hold the %lld first and %lld last pages",
+                  (long long)top_k, (long long)keep_first, (long long)keep_last);
+        return UT_ERR_ARG;
+    }
+    a.qabs = qabs_dev;
+    a.qrope = q_rope_dev;
+    a.top_k = (int32_t)top_k;
+    const int64_t R = batch * rows, D = a.L + a.P;
+    ScratchPlan plan;
+    plan.add((size_t)(R * heads * D));
+    plan.add((size_t)(R * heads) * 8);
+    plan.add((size_t)(R * max_pages) * 8);
+    std::vector<void *> ptrs;
+    UT_TRY(scratch_acquire(ctx, plan, ptrs));
+    int8_t *codes = (int8_t *)ptrs[0];
+    double *share = (double *)ptrs[1];
+    uint64_t *keys = (uint64_t *)ptrs[2];
+    int tok = timing_begin(ctx, "select_codes");
+    if (kv->fmt == UT_KV_BF16)
+        hipLaunchKernelGGL(k_select_codes<Bf16>, dim3((unsigned)(R * heads)), dim3(64), 0,
+                           ctx->stream, a, weights_dev, codes, share);
+    else
+        hipLaunchKernelGGL(k_select_codes<F16x2>, dim3((unsigned)(R * heads)), dim3(64), 0,
+                           ctx->stream, a, weights_dev, codes, share);
+    timing_end(ctx, tok);
+    UT_TRY(launch_check(ctx, "k_select_codes"));
+    tok = timing_begin(ctx, "select_score");
+    hipLaunchKernelGGL(k_select_score, dim3((unsigned)((max_pages + 3) / 4), (unsigned)R), dim3(256), 0,
+                       ctx->stream, a, codes, share, kv->mean, kv->mean_scale, keys);
+    timing_end(ctx, tok);
+    UT_TRY(launch_check(ctx, "k_select_score"));
+    tok = timing_begin(ctx, "select_pick");
+    hipLaunchKernelGGL(k_select_pick, dim3((unsigned)R), dim3(kPickThreads), 0, ctx->stream, a, keys,
+                       (int)keep_first, (int)keep_last, sel_dev);
+    timing_end(ctx, tok);
+    return launch_check(ctx, "k_select_pick");
+}

@@ -1,0 +1,48 @@
+// ut_paged_plan.h -- how a batch over the paged cache is cut into equal
+// ranges of work, and the bounds of what its lengths and tables may say.
+// Plain arithmetic for the kernels and for the host.
+//
+// The sequences' tiles stand in one row, one sequence after another: W in
+// all, sequence u's from pre_u on.  Range r of N takes the tiles
+// [W r / N, W (r + 1) / N), so a ragged batch is cut as evenly as a square
+// one, and a long sequence spreads over many ranges.  A range meets at most
+// one sequence that began before it and one that goes on behind it; those two
+// leave a partial result each (plan_slot), every other sequence in it is whole.
+#pragma once
+
+#include <cstdint>
+
+#if defined(__HIPCC__)
+#define UT_PLAN_FN __host__ __device__ inline
+#else
+#define UT_PLAN_FN inline
+#endif
+
+namespace ut {
+
+// How many ranges: as many as may be, with `least` tiles in each.
+UT_PLAN_FN int64_t plan_ranges(int64_t W, int64_t most, int64_t least) {
+    const int64_t n = (W + least - 1) / least;
+    return n < 1 ? 1 : n < most ? n : most;
+}
+UT_PLAN_FN int64_t plan_begin(int64_t W, int64_t N, int64_t r) { return W * r / N; }
+// The range that holds tile t.
+UT_PLAN_FN int64_t plan_range_of(int64_t W, int64_t N, int64_t t) { return ((t + 1) * N - 1) / W; }
+// Where range r leaves its part of the sequence whose tiles begin at pre.
+UT_PLAN_FN int64_t plan_slot(int64_t W, int64_t N, int64_t r, int64_t pre) {
+    return 2 * r + (plan_begin(W, N, r) <= pre ? 1 : 0);
+}
+
+// A length cut to what the table can hold; a page id cut to the pool.
+UT_PLAN_FN int32_t plan_len(int32_t n, int64_t cap, bool &bad) {
+    if (n >= 0 && n <= cap) return n;
+    bad = true;
+    return n < 0 ? 0 : (int32_t)cap;
+}
+UT_PLAN_FN int32_t plan_page(int32_t p, int32_t n_pages, bool &bad) {
+    if (p >= 0 && p < n_pages) return p;
+    bad = true;
+    return 0;
+}
+
+}  // namespace ut

@@ -144,12 +144,12 @@ void timing_end(ut_ctx *ctx, int token) {
 
 int32_t device_error_flag(ut_ctx *ctx, int32_t **flag) {
     if (!ctx->dev_err) {
-        if (hipMalloc((void **)&ctx->dev_err, 4) != hipSuccess) {
+        if (hipMalloc((void **)&ctx->dev_err, 8) != hipSuccess) {
             (void)hipGetLastError();
             set_error(ctx, "error flag allocation failed");
             return UT_ERR_OOM;
         }
-        UT_CHECK_HIP(ctx, hipMemset(ctx->dev_err, 0, 4));
+        UT_CHECK_HIP(ctx, hipMemset(ctx->dev_err, 0, 8));
     }
     *flag = ctx->dev_err;
     return UT_OK;
@@ -175,10 +175,15 @@ void splitk_reserve(ut_ctx *ctx) {
 
 int32_t check_device_error(ut_ctx *ctx) {
     if (!ctx->dev_err) return UT_OK;
-    int32_t f = 0;
-    UT_CHECK_HIP(ctx, hipMemcpy(&f, ctx->dev_err, 4, hipMemcpyDeviceToHost));
-    if (!f) return UT_OK;
-    UT_CHECK_HIP(ctx, hipMemset(ctx->dev_err, 0, 4));
+    int32_t f[2] = {0, 0};
+    UT_CHECK_HIP(ctx, hipMemcpy(f, ctx->dev_err, 8, hipMemcpyDeviceToHost));
+    if (!f[0] && !f[1]) return UT_OK;
+    UT_CHECK_HIP(ctx, hipMemset(ctx->dev_err, 0, 8));
+    if (!f[0]) {
+        set_error(ctx, "a paged call met a length beyond its table or a page outside its pool "
+                       "(reported by a kernel)");
+        return UT_ERR_BAD_PAGE;
+    }
     set_error(ctx, "an expert id was out of range or not loaded (reported by a kernel)");
     return UT_ERR_BAD_EXPERT;
 }

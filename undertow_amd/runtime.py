@@ -38,6 +38,9 @@ UT_ERR_BAD_TOKEN = -8
 UT_ERR_NOT_FOUND = -9
 UT_ERR_STATE = -10
 UT_ERR_IO = -11
+UT_ERR_BAD_PAGE = -12
+
+KV_BF16, KV_F16X2 = 0, 1
 
 
 class UtError(RuntimeError):
@@ -100,6 +103,13 @@ _SIGS = [
     ("ut_mla_attend", _i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp]),
     ("ut_mla_cache_split", _i32, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     ("ut_mla_attend_split", _i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp]),
+    ("ut_mla_paged_append", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp]),
+    ("ut_mla_paged_attend", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _f32,
+                                   _vp]),
+    ("ut_mla_page_select", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp,
+                                  _i64, _i64, _i64, _vp]),
+    ("ut_mla_sparse_attend", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _f32,
+                                    _vp, _i64, _vp]),
     ("ut_model_create", _i32, [_vp, _vp, C.POINTER(_vp)]),
     ("ut_model_set_tensor", _i32, [_vp, C.c_char_p, _i32, _vp, _i64, _vp, _i64, _i64]),
     ("ut_model_finalize", _i32, [_vp]),
@@ -181,6 +191,12 @@ class ModelConfig(C.Structure):
             if k in d:
                 setattr(c, k, d[k])
         return c
+
+
+class MlaPages(C.Structure):
+    """ut_mla_pages: a pool of pages and their summaries."""
+    _fields_ = [("pages", _vp), ("mean", _vp), ("mean_scale", _vp), ("n_pages", _i64),
+                ("page", _i64), ("latent", _i64), ("rope", _i64), ("fmt", _i32)]
 
 
 class StoreConfig(C.Structure):
@@ -493,6 +509,145 @@ def mla_attend_split(ctx: Context, qabs, q_rope, kc, pos_base: int, scale: float
     ctx.check(lib().ut_mla_attend_split(ctx.handle, _ptr(qabs), _ptr(q_rope), _ptr(kc), R, H, L, P,
                                         pos_base, scale, _ptr(out)))
     return out
+
+
+class PagedCache:
+    """One layer's latent cache of many sequences in a pool of pages.
+
+    pages: bfloat16 [n_pages, page, latent + rope], or float16 [n_pages, page,
+    2, latent + rope] whose two planes stand for f32 values hi + lo / 2048;
+    mean (int8 [n_pages, latent + rope]) and mean_scale (float32 [n_pages])
+    hold a summary per page for ``select``.  The tensors are the caller's and
+    stay theirs.
+
+    Every call takes a batch: table [B, max_pages] int32 (physical pages in a
+    sequence's order; the rows may be slices of a wider table) and lens [B]
+    int32, the positions of each sequence with the present step's rows
+    included, so that row j of M sees lens - M + j + 1 of them.  A length or
+    page out of range is reported by the context's next ``synchronize``."""
+
+    def __init__(self, ctx: Context, pages, latent: int = 512, rope: int = 64, mean=None,
+                 mean_scale=None):
+        torch = _torch()
+        D = latent + rope
+        if pages.dtype == torch.bfloat16:
+            self.fmt, self.dtype, shape = KV_BF16, torch.bfloat16, tuple(pages.shape[:2]) + (D,)
+        elif pages.dtype == torch.float16:
+            self.fmt, self.dtype, shape = KV_F16X2, torch.float32, tuple(pages.shape[:2]) + (2, D)
+        else:
+            raise UtError(UT_ERR_ARG, f"PagedCache: pages are bfloat16 or float16, got {pages.dtype}")
+        if len(pages.shape) < 2:
+            raise ShapeError(UT_ERR_SHAPE, "PagedCache: pages must have a page and a position axis")
+        if (mean is None) != (mean_scale is None):
+            raise UtError(UT_ERR_ARG, "PagedCache: mean and mean_scale are given together")
+        self.ctx, self.latent, self.rope = ctx, latent, rope
+        self.pages, self.mean, self.mean_scale = pages, mean, mean_scale
+        n, self.page = int(pages.shape[0]), int(pages.shape[1])
+        self._tensor("pages", pages, pages.dtype, shape)
+        if mean is not None:
+            self._tensor("mean", mean, torch.int8, (n, D))
+            self._tensor("mean_scale", mean_scale, torch.float32, (n,))
+        self._kv = MlaPages(_ptr(pages), _ptr(mean), _ptr(mean_scale), n, self.page, latent, rope,
+                            self.fmt)
+
+    @classmethod
+    def empty(cls, ctx: Context, n_pages: int, page: int = 64, latent: int = 512, rope: int = 64,
+              fmt: int = KV_BF16, summaries: bool = True) -> "PagedCache":
+        """A cache over a pool of its own."""
+        torch = _torch()
+        d, D = f"cuda:{ctx.device}", latent + rope
+        pages = (torch.zeros((n_pages, page, D), dtype=torch.bfloat16, device=d) if fmt == KV_BF16
+                 else torch.zeros((n_pages, page, 2, D), dtype=torch.float16, device=d))
+        if not summaries:
+            return cls(ctx, pages, latent, rope)
+        return cls(ctx, pages, latent, rope, torch.zeros((n_pages, D), dtype=torch.int8, device=d),
+                   torch.zeros(n_pages, device=d))
+
+    def _tensor(self, name: str, t, dtype, shape) -> Optional[int]:
+        if tuple(t.shape) != tuple(shape):
+            raise ShapeError(UT_ERR_SHAPE, f"PagedCache: {name} must be {list(shape)}, got {list(t.shape)}")
+        if t.dtype != dtype or not t.is_contiguous() or not t.is_cuda or t.device.index != self.ctx.device:
+            raise UtError(UT_ERR_ARG, f"PagedCache: {name} must be a contiguous {dtype} tensor on "
+                                      f"cuda:{self.ctx.device}")
+        return t.data_ptr()
+
+    def _batch(self, table, lens, rows: int):
+        torch = _torch()
+        if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
+            raise ShapeError(UT_ERR_SHAPE, f"PagedCache: table must be [B, max_pages], got {list(table.shape)}")
+        B, n = table.shape
+        stride = table.stride(0) if B > 1 else max(n, table.stride(0))
+        if (table.dtype != torch.int32 or not table.is_cuda or table.device.index != self.ctx.device
+                or (n > 1 and table.stride(1) != 1) or stride < n):
+            raise UtError(UT_ERR_ARG, f"PagedCache: table must be int32 rows of adjacent entries on "
+                                      f"cuda:{self.ctx.device}")
+        return (self.ctx.handle, C.byref(self._kv), table.data_ptr(), stride, n,
+                self._tensor("lens", lens, torch.int32, (B,)), B, rows)
+
+    def _queries(self, table, lens, qabs, q_rope):
+        if qabs.dim() != 4:
+            raise ShapeError(UT_ERR_SHAPE, f"PagedCache: qabs must be [B, rows, heads, latent], got {list(qabs.shape)}")
+        _, M, H, _ = qabs.shape
+        batch = self._batch(table, lens, M)
+        B = batch[6]
+        return batch + (H, self._tensor("qabs", qabs, self.dtype, (B, M, H, self.latent)),
+                        self._tensor("q_rope", q_rope, self.dtype, (B, M, H, self.rope)))
+
+    def _context(self, qabs, out):
+        torch = _torch()
+        if out is None:
+            return torch.empty_like(qabs)
+        self._tensor("out", out, self.dtype, qabs.shape)
+        return out
+
+    def append(self, table, lens, latent, krot) -> None:
+        """Writes latent [B, M, latent] and krot [B, M, rope] (f32) to each
+        sequence's last M positions, and their pages' summaries anew."""
+        torch = _torch()
+        if latent.dim() != 3:
+            raise ShapeError(UT_ERR_SHAPE, f"PagedCache: latent must be [B, rows, latent], got {list(latent.shape)}")
+        batch = self._batch(table, lens, latent.shape[1])
+        B, M = batch[6:]
+        self.ctx.check(lib().ut_mla_paged_append(
+            *batch, self._tensor("latent", latent, torch.float32, (B, M, self.latent)),
+            self._tensor("krot", krot, torch.float32, (B, M, self.rope))))
+
+    def attend(self, table, lens, qabs, q_rope, scale: float, out=None):
+        """Absorbed attention of qabs [B, M, H, latent] and q_rope [B, M, H,
+        rope] over each row's positions -> [B, M, H, latent]."""
+        q = self._queries(table, lens, qabs, q_rope)
+        out = self._context(qabs, out)
+        self.ctx.check(lib().ut_mla_paged_attend(*q, scale, _ptr(out)))
+        return out
+
+    def select(self, table, lens, qabs, q_rope, top_k: int, keep_first: int = 1, keep_last: int = 1,
+               weights=None, out=None):
+        """The pages each row shall attend to -> [B, M, top_k] int32 (page
+        numbers of the sequence, ascending, -1 behind them): the first
+        keep_first, the last keep_last, then the best scores.  weights [B, M,
+        H] f32 weigh the heads."""
+        torch = _torch()
+        q = self._queries(table, lens, qabs, q_rope)
+        B, M, H = q[6:9]
+        w = None if weights is None else self._tensor("weights", weights, torch.float32, (B, M, H))
+        if out is None:
+            out = torch.empty((B, M, max(top_k, 0)), dtype=torch.int32, device=qabs.device)
+        else:
+            self._tensor("out", out, torch.int32, (B, M, top_k))
+        self.ctx.check(lib().ut_mla_page_select(*q, w, keep_first, keep_last, top_k, _ptr(out)))
+        return out
+
+    def attend_pages(self, table, lens, qabs, q_rope, scale: float, sel, out=None):
+        """``attend`` over the pages that sel [B, M, top_k] int32 lists."""
+        torch = _torch()
+        q = self._queries(table, lens, qabs, q_rope)
+        if sel.dim() != 3:
+            raise ShapeError(UT_ERR_SHAPE, f"PagedCache: sel must be [B, rows, top_k], got {list(sel.shape)}")
+        k = sel.shape[2]
+        self._tensor("sel", sel, torch.int32, tuple(q[6:8]) + (k,))
+        out = self._context(qabs, out)
+        self.ctx.check(lib().ut_mla_sparse_attend(*q, scale, _ptr(sel), k, _ptr(out)))
+        return out
 
 
 class ExpertTable:
