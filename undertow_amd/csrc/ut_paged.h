@@ -52,4 +52,8 @@ __device__ __forceinline__ void f16x2_split(float x, _Float16 &hi, _Float16 &lo)
                              : (_Float16)0.0f;
 }
 
+// The matrix-core attention (latent 512 + rope 64, pages of 8 and more).
+bool paged_mfma_ok(const PagedArgs &a);
+int32_t launch_paged_mfma(ut_ctx *ctx, const PagedArgs &a, int32_t fmt);
+
 }  // namespace ut

@@ -403,6 +403,7 @@ static int32_t paged_attend(ut_ctx *ctx, const char *what, const ut_mla_pages *k
     a.sel = sel;
     a.top_k = (int32_t)top_k;
     a.out = out;
+    if (paged_mfma_ok(a)) return launch_paged_mfma(ctx, a, kv->fmt);
     return launch_paged_generic(ctx, a, kv->fmt);
 }
 

@@ -1,0 +1,707 @@
+// ut_paged_mfma.hip -- attention over the paged latent cache on the matrix
+// cores, for latent 512 + rope 64 and pages of 8 positions and more.
+#include "ut_paged.h"
+
+namespace ut {
+
+typedef __bf16 pbf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pbf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 pbf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 pf16x8 __attribute__((ext_vector_type(8)));
+typedef float pf32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t pu32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef const __attribute__((address_space(4))) int32_t const_i32;
+
+constexpr int kPT = 32;             // positions per tile
+constexpr int kPL = 512, kPD = 576;
+constexpr int kCols = 16;           // heads per column group (a wave's)
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLow = -3.402823466e38f;  // the offset before any score
+
+struct PagedMfmaArgs {
+    PagedArgs a;
+    int32_t units;    // sequences, or rows where each has pages of its own
+    int32_t groups;   // column groups (16 heads of one row) of a unit
+    int32_t chunks;   // workgroups that share a unit's positions
+    int32_t per;      // column groups of a workgroup
+    int32_t most;     // ranges at most
+    int32_t least;    // tiles a range at least
+    float *part_o;    // [slot][group][128 quads][16 columns][4]
+    float *part_ml;   // [slot][group][16 columns][2]
+    int64_t *plan;    // [units] first tile of each, then W
+};
+
+// Tiles of a unit.
+template <bool SPARSE> __device__ __forceinline__ int32_t unit_tiles(const PagedArgs &a, int u) {
+    if (!SPARSE) return (int32_t)(((int64_t)paged_len(a, u) + kPT - 1) / kPT);
+    const int b = u / a.M, n = paged_len(a, b) - a.M + (u - b * a.M) + 1;
+    return n > 0 ? (int32_t)((((int64_t)a.top_k << a.shift) + kPT - 1) / kPT) : 0;
+}
+
+// The sum of v over the workgroup's threads before this one, and in all.
+template <int NW> __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *s, int64_t &all) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int64_t x = v;
+    for (int off = 1; off < 64; off <<= 1) {
+        const int64_t y = __shfl_up(x, off, 64);
+        if (lane >= off) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) s[w] = x;
+    __syncthreads();
+    int64_t before = x - v;
+    all = 0;
+    for (int i = 0; i < NW; i++) {
+        if (i < w) before += s[i];
+        all += s[i];
+    }
+    return before;
+}
+
+// A value that every lane has, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+    return (int64_t)((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32)) << 32 | lo);
+}
+
+struct Range {
+    int64_t W, N, s, e;  // the range takes tiles [s, e) of W
+    int u;               // the unit that holds tile s, and its first tile
+    int64_t pre;
+};
+
+// Every workgroup works its range out from the lengths: one pass over the
+// units for their sum, one up to the unit where the range begins.  `leave`:
+// the units' first tiles are written down for the join.
+template <bool SPARSE, int NW>
+__device__ bool find_range(const PagedMfmaArgs &p, int64_t r, bool leave, Range &g) {
+    __shared__ int64_t s[NW];
+    __shared__ int64_t found[2];
+    const int tid = threadIdx.x;
+    int64_t W = 0;
+    for (int c = 0; c < p.units; c += NW * 64) {
+        const int u = c + tid;
+        int64_t all;
+        const int64_t t = u < p.units ? unit_tiles<SPARSE>(p.a, u) : 0;
+        const int64_t pre = W + block_scan<NW>(t, s, all);
+        if (leave && u < p.units) p.plan[u] = pre;
+        W += all;
+    }
+    if (leave && tid == 0) p.plan[p.units] = W;
+    g.W = W = uniform(W);
+    if (W == 0) return false;
+    g.N = plan_ranges(W, p.most, p.least);
+    if (r >= g.N) return false;
+    g.s = plan_begin(W, g.N, r);
+    g.e = plan_begin(W, g.N, r + 1);
+    int64_t at = 0;
+    for (int c = 0; c < p.units && at <= g.s; c += NW * 64) {
+        const int u = c + tid;
+        int64_t all;
+        const int64_t t = u < p.units ? unit_tiles<SPARSE>(p.a, u) : 0;
+        const int64_t pre = at + block_scan<NW>(t, s, all);
+        if (pre <= g.s && g.s < pre + t) {
+            found[0] = u;
+            found[1] = pre;
+        }
+        at += all;
+    }
+    __syncthreads();
+    g.u = __builtin_amdgcn_readfirstlane((int)found[0]);
+    g.pre = uniform(found[1]);
+    return true;
+}
+
+// ------------------------------------------------------------- the tile ---
+// A tile holds 32 positions in LDS as blocks of 1 KiB: block (rg, cg) has rows
+// 8 rg .. 8 rg + 7 and 128 bytes (64 values) of each, the bytes that one load
+// instruction of a wave brings, straight to LDS: nine column blocks a plane.
+// In a row's 128 bytes the eight 16-byte chunks are XORed with tile_swz(row),
+// so that the score reads (16 rows, one chunk) and the transposing reads (8
+// rows, two chunks) both meet each of the LDS's 16 slots of 16 bytes once.
+__device__ __forceinline__ int tile_swz(int row) { return (((row >> 1) & 3) << 1) | ((row >> 3) & 1); }
+
+// A column's lanes l, l ^ 16, l ^ 32, l ^ 48 combined.
+__device__ __forceinline__ float col_max(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float col_sum(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __fadd_rn(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __fadd_rn(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// LDS by its 32-bit address.
+template <class V> __device__ __forceinline__ V lds_read(uint32_t at) {
+    return *(const __attribute__((address_space(3))) V *)at;
+}
+__device__ __forceinline__ pu32x4 tr_read(uint32_t x, uint32_t y) {
+    typedef __attribute__((address_space(3))) pbf16x4 lds4;
+    const pbf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)x);
+    const pbf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)y);
+    return __builtin_bit_cast(pu32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// A lane's first score read and first transposing read in a tile.  The others
+// lie 1 KiB steps away, with chunk bits flipped: chunk 4 (ks & 1) + g in the
+// score reads (^ 64 bytes), 2 (mt & 3) + .. in the transposing ones (^ 32, ^ 64).
+struct LaneAddr {
+    uint32_t k, v;
+};
+template <int PLANES> __device__ __forceinline__ LaneAddr lane_addr(int l) {
+    const int row = l & 15, g = l >> 4, j = l & 15, r = 4 * g + (j >> 2);
+    return {(uint32_t)((row >> 3) * 9 * PLANES * 1024 + (row & 7) * 128 + ((g ^ tile_swz(row)) << 4)),
+            (uint32_t)((r >> 3) * 9 * PLANES * 1024 + (r & 7) * 128 + ((((j & 3) >> 1) ^ tile_swz(r)) << 4) +
+                       8 * (j & 1))};
+}
+
+// bf16 pages: queries and weights in bf16.
+struct MfmaBf16 {
+    static constexpr int kPlanes = 1, kWaves = 8;
+    static constexpr int kDepth = 5;
+    static constexpr float kRise = 11.5f;  // log2 units a score may exceed the offset (8 nats)
+    typedef __bf16 out_t;
+    struct Query {
+        pbf16x8 q[18];
+    };
+    // column l & 15, dims 32 ks + 8 (l >> 4) + [0, 8); the scale that the scores then need
+    __device__ __forceinline__ static float load(Query &x, const void *qabs, const void *qrope, int64_t row, int g) {
+        const __bf16 *qa = (const __bf16 *)qabs + row * kPL, *qr = (const __bf16 *)qrope + row * (kPD - kPL);
+#pragma unroll
+        for (int ks = 0; ks < 18; ks++) x.q[ks] = *(const pbf16x8 *)(ks < 16 ? qa + 32 * ks + 8 * g : qr + 32 * (ks - 16) + 8 * g);
+        return 1.0f;
+    }
+    // waits for the loads here: left to their first use, the wait would stand
+    // in the loop and hold up the copies too
+    __device__ __forceinline__ static void arrive(Query &x) {
+#pragma unroll
+        for (int ks = 0; ks < 18; ks++) asm volatile("" : "+v"(x.q[ks]));
+    }
+    // both halves of the tile in turn, kDepth reads ahead of the products
+    __device__ __forceinline__ static void scores(const Query &x, uint32_t T, pf32x4 (&s)[2]) {
+        pbf16x8 k[36];
+        auto read = [&](int i) {
+            k[i] = lds_read<pbf16x8>((T ^ (((i >> 1) & 1) << 6)) + (i >> 2) * 1024 + (i & 1) * 18 * 1024);
+        };
+#pragma unroll
+        for (int i = 0; i < kDepth; i++) read(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 36; i++) {
+            s[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i], x.q[i >> 1], s[i & 1], 0, 0, 0);
+            if (i + kDepth < 36) read(i + kDepth);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    struct Weights {
+        pbf16x8 p;
+    };
+    // the sum is of the rounded weights that V meets
+    __device__ __forceinline__ static float weigh(Weights &x, const float (&e)[8]) {
+        float sum = 0.0f;
+        const pbf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const pbf16x2 v = {(__bf16)e[i], (__bf16)e[i + 1]};
+            sum = __builtin_amdgcn_fdot2_f32_bf16(v, one, sum, false);
+            x.p[i] = v[0];
+            x.p[i + 1] = v[1];
+        }
+        return sum;
+    }
+    __device__ __forceinline__ static void context(const Weights &x, uint32_t T, pf32x4 (&o)[32]) {
+        pu32x4 v[32];
+        auto read = [&](int i) {
+            const uint32_t b = (T ^ ((i & 3) << 5)) + (i >> 2) * 1024;
+            v[i] = tr_read(b, b + 18 * 1024);
+        };
+#pragma unroll
+        for (int i = 0; i < kDepth; i++) read(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pbf16x8, v[i]), x.p, o[i], 0, 0, 0);
+            if (i + kDepth < 32) read(i + kDepth);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+
+// f16x2 pages.  Every operand is a pair of f16, and a product is taken as
+// hi*hi + lo*hi + hi*lo (lo*lo lies 2^-22 below).  Stored low parts are
+// scaled by 2^11; the partner of such a part is the high part of the other
+// operand times 2^-11, so all three products add up in one accumulator.
+// Queries are scaled by a power of two to a maximum in [2^14, 2^15) and
+// weights by 2^14 (at most 2^15), so that neither their low parts nor the
+// scaled high parts fall out of f16's range where they matter.
+struct MfmaF16x2 {
+    static constexpr int kPlanes = 2, kWaves = 4;
+    static constexpr int kDepth = 4;
+    static constexpr float kRise = 1.0f;
+    typedef float out_t;
+    struct Query {
+        pf16x8 h[18], l[18];
+    };
+    __device__ __forceinline__ static float load(Query &x, const void *qabs, const void *qrope, int64_t row, int g) {
+        const float *qa = (const float *)qabs + row * kPL, *qr = (const float *)qrope + row * (kPD - kPL);
+        float top = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < 18; ks++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf((ks < 16 ? qa + 32 * ks : qr + 32 * (ks - 16))[8 * g + i]));
+        top = col_max(top);
+        // 2^e <= top < 2^(e + 1)
+        const int e = (int)(__float_as_uint(top) >> 23) - 127;
+        const int up = top > 0.0f && top < INFINITY ? (14 - e < 120 ? 14 - e : 120) : 0;
+#pragma unroll
+        for (int ks = 0; ks < 18; ks++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float v = ldexpf((ks < 16 ? qa + 32 * ks : qr + 32 * (ks - 16))[8 * g + i], up);
+                const _Float16 h = (_Float16)v;
+                x.h[ks][i] = h;
+                x.l[ks][i] = (_Float16)__fsub_rn(v, (float)h);
+            }
+        return ldexpf(1.0f, -up);
+    }
+    __device__ __forceinline__ static void arrive(Query &) {}  // converted: they are there
+    __device__ __forceinline__ static void scores(const Query &x, uint32_t T, pf32x4 (&s)[2]) {
+        pf32x4 t[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+        pf16x8 k[36], d[36];  // high and low parts
+        auto read = [&](int i) {
+            const uint32_t b = (T ^ (((i >> 1) & 1) << 6)) + (i >> 2) * 1024 + (i & 1) * 36 * 1024;
+            k[i] = lds_read<pf16x8>(b);
+            d[i] = lds_read<pf16x8>(b + 9 * 1024);
+        };
+#pragma unroll
+        for (int i = 0; i < kDepth; i++) read(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 36; i++) {
+            s[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], x.h[i >> 1], s[i & 1], 0, 0, 0);
+            t[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], x.l[i >> 1], t[i & 1], 0, 0, 0);
+            pf16x8 h = x.h[i >> 1];
+            asm volatile("" : "+v"(h));  // scaled here: all of them scaled ahead would not fit
+            t[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[i], h * (_Float16)(1.0f / kF16x2Step), t[i & 1], 0, 0, 0);
+            if (i + kDepth < 36) read(i + kDepth);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            s[0][i] = __fadd_rn(s[0][i], t[0][i]);
+            s[1][i] = __fadd_rn(s[1][i], t[1][i]);
+        }
+    }
+    struct Weights {
+        pf16x8 h, l, d;
+    };
+    __device__ __forceinline__ static float weigh(Weights &x, const float (&e)[8]) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float v = __fmul_rn(e[i], 16384.0f);
+            sum = __fadd_rn(sum, v);
+            x.h[i] = (_Float16)v;
+            x.l[i] = (_Float16)__fsub_rn(v, (float)x.h[i]);
+        }
+        x.d = x.h * (_Float16)(1.0f / kF16x2Step);
+        return sum;
+    }
+    __device__ __forceinline__ static void context(const Weights &x, uint32_t T, pf32x4 (&o)[32]) {
+        pu32x4 h[32], d[32];
+        auto read = [&](int i) {
+            const uint32_t b = (T ^ ((i & 3) << 5)) + (i >> 2) * 1024;
+            h[i] = tr_read(b, b + 36 * 1024);
+            d[i] = tr_read(b + 9 * 1024, b + 45 * 1024);
+        };
+#pragma unroll
+        for (int i = 0; i < kDepth; i++) read(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            const pf16x8 vh = __builtin_bit_cast(pf16x8, h[i]), vl = __builtin_bit_cast(pf16x8, d[i]);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, x.l, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, x.d, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, x.h, o[i], 0, 0, 0);
+            if (i + kDepth < 32) read(i + kDepth);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+
+// One wave's columns: 16 heads of one query row, the whole latent width.
+template <class F> struct Wave {
+    typename F::Query q;
+    pf32x4 o[32];  // context^T: dim 16 mt + 4 (l >> 4) + i, column l & 15
+    float m, l;    // softmax offset (log2 units) and sum
+};
+
+// One tile: S^T = K Q^T (positions x columns), the online softmax per column,
+// O^T += V^T P.  A lane of S holds positions 4 g + i and 16 + 4 g + i of one
+// column (g = lane >> 4); the second product takes its positions in that very
+// order (V's rows are read to match), so P goes from one product into the
+// other without leaving the lane.  The offset m moves only where a score
+// exceeds it by more than kRise.
+// seen: the tile's visible positions.  A hidden position's score is replaced,
+// whatever it is; what V holds there must be finite (tile_clear).
+template <class F>
+__device__ __forceinline__ void tile_step(Wave<F> &w, const LaneAddr &ad, uint32_t T, uint32_t seen, float c, int g) {
+    pf32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    F::scores(w.q, T + ad.k, s);
+    const uint32_t mine = seen >> (4 * g);
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) t[i] = __fmul_rn(s[i >> 2][i & 3], c);
+    if (seen != ~0u)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (!((mine >> ((i >> 2) * 16 + (i & 3))) & 1)) t[i] = -INFINITY;
+    float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+    top = col_max(top);
+    const bool jump = top > __fadd_rn(w.m, F::kRise);
+    if (__any(jump)) {
+        const float mn = jump ? top : w.m, f = __builtin_amdgcn_exp2f(w.m - mn);
+        w.m = mn;
+        w.l *= f;
+#pragma unroll
+        for (int mt = 0; mt < 32; mt++) w.o[mt] *= f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) t[i] = __builtin_amdgcn_exp2f(t[i] - w.m);
+    typename F::Weights p;
+    w.l = __fadd_rn(w.l, F::weigh(p, t));
+    F::context(p, T + ad.v, w.o);
+}
+
+// The latent values of a tile's rows: hidden rows are cleared before V meets
+// them (0 * NaN is NaN), 64 chunks of 16 bytes a plane.
+template <class F> __device__ __forceinline__ uint8_t *tile_chunk(uint8_t *T, int row, int c) {
+    return T + ((row >> 3) * 9 * F::kPlanes + (c >> 6) * 9 + ((c & 63) >> 3)) * 1024 + (row & 7) * 128 +
+           (((c & 7) ^ tile_swz(row)) << 4);
+}
+template <class F> __device__ __forceinline__ void tile_clear(uint8_t *T, uint32_t rows) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < 32 * 64 * F::kPlanes; i += F::kWaves * 64)
+        if ((rows >> (i & 31)) & 1) *(pu32x4 *)tile_chunk<F>(T, i & 31, i >> 5) = pu32x4{0, 0, 0, 0};
+}
+// Whether one of the rows holds a value that is not finite (this thread's share).
+template <class F> __device__ __forceinline__ bool tile_odd(uint8_t *T, uint32_t rows) {
+    const uint32_t ones = F::kPlanes == 1 ? 0x7f80u : 0x7c00u;  // the exponent's bits
+    bool odd = false;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < 32 * 64 * F::kPlanes; i += F::kWaves * 64)
+        if ((rows >> (i & 31)) & 1) {
+            const pu32x4 v = *(const pu32x4 *)tile_chunk<F>(T, i & 31, i >> 5);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                odd |= (v[k] & ones) == ones || ((v[k] >> 16) & ones) == ones;
+        }
+    return odd;
+}
+
+// What a wave needs to look positions up: unit u's sequence and row.
+struct Lookup {
+    const_i32 *table, *sel;  // the sequence's row of the table, the row's pages
+    int32_t n, top_k, shift, n_pages;
+};
+// The pool row of the unit's position v0 (8 aligned positions lie in a page);
+// any row of the pool where it has none.
+template <bool SPARSE>
+__device__ __forceinline__ int32_t look_up(const Lookup &k, int32_t v0) {
+    int32_t page;
+    if (SPARSE) {
+        const int32_t i = v0 >> k.shift;
+        page = i < k.top_k ? k.sel[i] : 0;
+        if (page < 0 || ((int64_t)page << k.shift) >= k.n) page = 0;
+    } else {
+        const int32_t last = (k.n - 1) & ~7;
+        if (v0 > last) v0 = last;
+        page = v0 >> k.shift;
+    }
+    bool bad = false;  // reported before the loop
+    const int32_t phys = plan_page(k.table[page], k.n_pages, bad);
+    return (phys << k.shift) + (v0 & ((1 << k.shift) - 1));
+}
+// The visible positions of the tile at v0 for a row that sees n.
+template <bool SPARSE>
+__device__ __forceinline__ uint32_t visible(const Lookup &k, int32_t v0, int32_t n) {
+    if (!SPARSE) {
+        const int32_t c = n - v0;
+        return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u;
+    }
+    const int per = k.shift >= 5 ? 32 : 1 << k.shift;
+    uint32_t m = 0;
+    for (int i = 0; i < 32; i += per) {
+        const int32_t v = v0 + i, at = v >> k.shift;
+        const int32_t page = at < k.top_k ? k.sel[at] : -1;
+        const int64_t c = page < 0 ? 0 : n - (((int64_t)page << k.shift) + (v & ((1 << k.shift) - 1)));
+        const uint32_t ones = c >= per ? (per == 32 ? ~0u : (1u << per) - 1u) : c <= 0 ? 0u : (1u << c) - 1u;
+        m |= ones << i;
+    }
+    return m;
+}
+
+// Column blocks I .. N - 1 of a lane's row, 128 bytes apart there and 1 KiB
+// apart in LDS, straight to LDS.  An instruction's offset counts on both
+// sides, so lds steps by the rest.  Written out, since the compiler would
+// have every later LDS read wait for every copy under way: the kernel waits
+// itself.  Nothing is loaded into a register, and the address is read when
+// the instruction issues.
+template <int I, int N> __device__ __forceinline__ void copy_blocks(uint32_t off, const uint8_t *src, uint32_t lds) {
+    if constexpr (I < N) {
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3"
+                     :
+                     : "v"(off), "s"(src), "s"(lds + I * (1024 - 128)), "n"(I * 128)
+                     : "memory", "m0");
+        copy_blocks<I + 1, N>(off, src, lds);
+    }
+}
+
+// s_waitcnt of at most n vector memory operations under way (a tile's copies
+// are 5 of one half of the waves and 4 of the other; waiting for the fewer
+// suits both)
+constexpr int kWaitVm0 = 0x0f70, kWaitVm4 = 0x0f74, kWaitVm8 = 0x0f78;
+
+// A workgroup is F::kWaves waves, each with a column group of its own, over
+// the same tiles.  Four (two) tiles fit the LDS: the products of one run while
+// the next three (one) are on their way.
+template <class F, bool SPARSE>
+__global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(PagedMfmaArgs p) {
+    constexpr int NW = F::kWaves, PL = F::kPlanes, STAGES = 4 / PL, BLOCKS = 36 * PL, ROW = kPD * 2 * PL;
+    __shared__ __attribute__((aligned(1024))) uint8_t stage[STAGES][BLOCKS * 1024];
+    __shared__ int s_odd;
+    const PagedArgs &a = p.a;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, col = l & 15;
+    const int share = gridDim.x >> 3;
+    const int id = (blockIdx.x & 7) * share + (blockIdx.x >> 3);  // neighbours on one XCD
+    const int r = id / p.chunks, chunk = id - r * p.chunks;
+    // units without positions: zeros
+    const int64_t vec = (int64_t)(SPARSE ? 1 : a.M) * a.H * kPL * (int)sizeof(typename F::out_t) / 16;
+    for (int u = id; u < p.units; u += gridDim.x)
+        if (unit_tiles<SPARSE>(a, u) == 0)
+            for (int64_t i = tid; i < vec; i += NW * 64) ((pu32x4 *)a.out)[u * vec + i] = pu32x4{0, 0, 0, 0};
+    Range rg;
+    if (r >= p.most || !find_range<SPARSE, NW>(p, r, r == 0 && chunk == 0, rg)) return;
+    const int grp = chunk * p.per + w;
+    const bool active = w < p.per && grp < p.groups;
+    const int per_row = (a.H + kCols - 1) / kCols;
+    const LaneAddr ad = lane_addr<PL>(l);
+    // copies: wave w brings row block w & 3 and, where two waves share it, half of its column blocks
+    const int rb = w & 3, c0 = w < 4 ? 0 : 5;
+    Wave<F> wv;
+    int u = rg.u;
+    int64_t pre = rg.pre, at = rg.s;
+    while (at < rg.e) {
+        const int32_t tiles = __builtin_amdgcn_readfirstlane(unit_tiles<SPARSE>(a, u));
+        if (tiles == 0) {
+            u++;
+            continue;
+        }
+        const int32_t b0 = (int32_t)(at - pre), b1 = rg.e - pre < tiles ? (int32_t)(rg.e - pre) : tiles;
+        const int b = SPARSE ? u / a.M : u;
+        const int gr = active ? grp : 0;
+        const int j = SPARSE ? u - b * a.M : gr / per_row, h0 = (SPARSE ? gr : gr % per_row) * kCols;
+        const int32_t len = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+        const int32_t n = len - a.M + j + 1;
+        const int64_t row = ((int64_t)b * a.M + j) * a.H + (h0 + col < a.H ? h0 + col : a.H - 1);
+        Lookup lk;
+        lk.table = (const_i32 *)(a.table + (int64_t)b * a.stride);
+        lk.sel = SPARSE ? (const_i32 *)(a.sel + (int64_t)u * a.top_k) : nullptr;
+        lk.n = SPARSE ? n : len;
+        lk.top_k = a.top_k;
+        lk.shift = a.shift;
+        lk.n_pages = a.n_pages;
+        auto copy = [&](int32_t x) {
+            // the lane's place in a block, worked out anew: it would be kept in
+            // registers that the products need
+            int t = threadIdx.x;
+            asm volatile("" : "+v"(t));
+            const uint32_t off = ((t >> 3) & 7) * ROW + (((t & 7) ^ tile_swz(8 * rb + ((t >> 3) & 7))) << 4);
+            const uint8_t *src = (const uint8_t *)a.pages + (int64_t)look_up<SPARSE>(lk, x * kPT + 8 * rb) * ROW + c0 * 128;
+            const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)stage[(x - b0) % STAGES] + (rb * 9 * PL + c0) * 1024;
+            copy_blocks<0, NW == 4 ? 9 * PL : 4>(off, src, lds);
+            if (NW == 8 && w < 4) copy_blocks<4, 5>(off, src, lds);
+        };
+        float c = a.scale * kLog2e;
+        auto turn = [&](int32_t x) {
+            uint8_t *T = stage[(x - b0) % STAGES];
+            // tile x's copies have landed: those of the tiles behind it may be on their way
+            const int32_t ahead = b1 - 1 - x < STAGES - 2 ? b1 - 1 - x : STAGES - 2;
+            if (ahead >= 2) __builtin_amdgcn_s_waitcnt(kWaitVm8);
+            else if (ahead == 1) __builtin_amdgcn_s_waitcnt(kWaitVm4);
+            else __builtin_amdgcn_s_waitcnt(kWaitVm0);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            if (x + STAGES - 1 < b1) copy(x + STAGES - 1);
+            const uint32_t seen = visible<SPARSE>(lk, x * kPT, n);
+            // what the unit's last row sees, and its first one
+            const uint32_t most = SPARSE ? seen : visible<false>(lk, x * kPT, len);
+            const uint32_t least = SPARSE ? seen : visible<false>(lk, x * kPT, len - a.M + 1);
+            bool odd = false;
+            if (least != ~0u) {
+                // a value that is not finite where only later rows look: those
+                // rows first, then it is cleared for the rows before
+                if (most != ~0u) tile_clear<F>(T, ~most);
+                if (least != most) {
+                    if (tid == 0) s_odd = 0;
+                    __syncthreads();
+                    if (tile_odd<F>(T, most & ~least)) s_odd = 1;
+                }
+                __syncthreads();
+                odd = least != most && __builtin_amdgcn_readfirstlane(s_odd);
+            }
+            uint32_t now = most;
+            do {
+                if (active && seen && (!odd || seen == now)) tile_step<F>(wv, ad, (uint32_t)(uintptr_t)(lds_u8 *)T, seen, c, g);
+                if (!odd || now == least) break;
+                __syncthreads();
+                tile_clear<F>(T, now & ~(now >> 1));
+                __syncthreads();
+                now >>= 1;
+            } while (true);
+
+        };
+        wv.m = kLow;
+        wv.l = 0.0f;
+#pragma unroll
+        for (int mt = 0; mt < 32; mt++) wv.o[mt] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        // page ids outside the pool among those that the tiles name
+        for (int32_t k = ((b0 * kPT) >> a.shift) + tid; k <= (b1 * kPT - 1) >> a.shift; k += NW * 64) {
+            int32_t page = k;
+            if (SPARSE) page = k < a.top_k ? lk.sel[k] : -1;
+            if (page >= 0 && ((int64_t)page << a.shift) < lk.n) paged_phys(a, b, page);
+        }
+        for (int32_t x = b0; x < b1 && x < b0 + STAGES - 1; x++) copy(x);
+        c *= F::load(wv.q, a.qabs, a.qrope, row, g);
+        F::arrive(wv.q);
+        for (int32_t x = b0; x < b1; x++) turn(x);
+        __syncthreads();  // the stages may be filled again
+        // ---- the unit's context, or this range's part of it
+        const float sum = col_sum(wv.l);
+        if (active && b0 == 0 && b1 == tiles) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            typename F::out_t *out = (typename F::out_t *)a.out + row * kPL + 4 * g;
+            if (h0 + col < a.H)
+#pragma unroll
+                for (int mt = 0; mt < 32; mt++) {
+                    typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
+                    o4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = (typename F::out_t)__fmul_rn(wv.o[mt][i], inv);
+                    *(o4 *)(out + 16 * mt) = v;
+                }
+        } else if (active) {
+            const int64_t slot = plan_slot(rg.W, rg.N, r, pre) * p.groups + grp;
+            pf32x4 *po = (pf32x4 *)p.part_o + slot * 128 * kCols + g * kCols + col;
+#pragma unroll
+            for (int mt = 0; mt < 32; mt++) po[mt * 4 * kCols] = wv.o[mt];
+            if (g == 0) *(float2 *)(p.part_ml + (slot * kCols + col) * 2) = make_float2(wv.m, sum);
+        }
+        at = pre + b1;
+        pre += tiles;
+        u++;
+    }
+}
+
+// Joins the parts of a unit that lies in more than one range:
+// out = sum_r o_r 2^(m_r - M) / sum_r l_r 2^(m_r - M).  A workgroup takes one
+// column group and 128 dims, a thread four dims of two columns.
+template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_join(PagedMfmaArgs p) {
+    constexpr int DIMS = 128;
+    typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
+    __shared__ __attribute__((aligned(16))) typename F::out_t so[kCols][DIMS + 16 / sizeof(typename F::out_t)];
+    const PagedArgs &a = p.a;
+    const int u = blockIdx.x / p.groups, grp = blockIdx.x - u * p.groups, tid = threadIdx.x;
+    const int64_t W = p.plan[p.units], pre = p.plan[u];
+    const int64_t tiles = unit_tiles<SPARSE>(a, u);
+    if (tiles == 0) return;
+    const int64_t N = plan_ranges(W, p.most, p.least);
+    const int64_t r0 = plan_range_of(W, N, pre), r1 = plan_range_of(W, N, pre + tiles - 1);
+    if (r0 == r1) return;
+    auto slot = [&](int64_t r) { return plan_slot(W, N, r, pre) * p.groups + grp; };
+    const int col = tid & 15, qd = tid >> 4;  // quads 32 blockIdx.y + qd, + 16
+    float M = kLow;
+    for (int64_t r = r0; r <= r1; r++) M = fmaxf(M, p.part_ml[(slot(r) * kCols + col) * 2]);
+    float L = 0.0f;
+    pf32x4 t[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll 4
+    for (int64_t r = r0; r <= r1; r++) {
+        const float2 ml = *(const float2 *)(p.part_ml + (slot(r) * kCols + col) * 2);
+        const float f = __builtin_amdgcn_exp2f(ml.x - M);
+        L = __fadd_rn(L, __fmul_rn(ml.y, f));
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const pf32x4 v = ((const pf32x4 *)p.part_o)[(slot(r) * 128 + blockIdx.y * 32 + qd + 16 * k) * kCols + col];
+#pragma unroll
+            for (int i = 0; i < 4; i++) t[k][i] = __builtin_fmaf(v[i], f, t[k][i]);
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        o4 v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (typename F::out_t)__fmul_rn(t[k][i], inv);
+        *(o4 *)&so[col][4 * (qd + 16 * k)] = v;
+    }
+    __syncthreads();
+    const int per_row = (a.H + kCols - 1) / kCols;
+    const int64_t row = SPARSE ? u : (int64_t)u * a.M + grp / per_row;
+    const int c = tid >> 4, h = (SPARSE ? grp : grp % per_row) * kCols + c;
+    if (h < a.H)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            *(o4 *)((typename F::out_t *)a.out + (row * a.H + h) * kPL + blockIdx.y * DIMS + 4 * ((tid & 15) + 16 * k)) =
+                *(const o4 *)&so[c][4 * ((tid & 15) + 16 * k)];
+}
+
+bool paged_mfma_ok(const PagedArgs &a) { return a.L == kPL && a.P == kPD - kPL && a.shift >= 3; }
+
+constexpr int kLeastTiles = 2;
+
+template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const PagedArgs &a) {
+    PagedMfmaArgs p{};
+    p.a = a;
+    p.units = SPARSE ? a.B * a.M : a.B;
+    p.groups = (SPARSE ? 1 : a.M) * ((a.H + kCols - 1) / kCols);
+    p.chunks = (p.groups + F::kWaves - 1) / F::kWaves;
+    p.per = (p.groups + p.chunks - 1) / p.chunks;
+    const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
+    const int64_t W = (int64_t)p.units * ((cap + kPT - 1) / kPT);  // at most
+    const int64_t most = ctx->multiprocessors / p.chunks;
+    p.least = kLeastTiles;
+    p.most = (int32_t)plan_ranges(W, most < 1 ? 1 : most, p.least);
+    const int64_t slots = 2ll * p.most * p.groups;
+    ScratchPlan plan;
+    plan.add((size_t)slots * kPL * kCols * 4);
+    plan.add((size_t)slots * kCols * 8);
+    plan.add((size_t)(p.units + 1) * 8);
+    std::vector<void *> ptrs;
+    UT_TRY(scratch_acquire(ctx, plan, ptrs));
+    p.part_o = (float *)ptrs[0];
+    p.part_ml = (float *)ptrs[1];
+    p.plan = (int64_t *)ptrs[2];
+    const int64_t wgs = ((int64_t)p.most * p.chunks + 7) / 8 * 8;
+    int tok = timing_begin(ctx, "paged_mfma");
+    hipLaunchKernelGGL((k_paged_mfma<F, SPARSE>), dim3((unsigned)wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
+    timing_end(ctx, tok);
+    UT_TRY(launch_check(ctx, "k_paged_mfma"));
+    if (p.most == 1) return UT_OK;
+    tok = timing_begin(ctx, "paged_join");
+    hipLaunchKernelGGL((k_paged_join<F, SPARSE>), dim3((unsigned)((int64_t)p.units * p.groups), kPL / 128), dim3(256), 0,
+                       ctx->stream, p);
+    timing_end(ctx, tok);
+    return launch_check(ctx, "k_paged_join");
+}
+
+int32_t launch_paged_mfma(ut_ctx *ctx, const PagedArgs &a, int32_t fmt) {
+    if (fmt == UT_KV_BF16) return a.sel ? launch_fmt<MfmaBf16, true>(ctx, a) : launch_fmt<MfmaBf16, false>(ctx, a);
+    return a.sel ? launch_fmt<MfmaF16x2, true>(ctx, a) : launch_fmt<MfmaF16x2, false>(ctx, a);
+}
+
+}  // namespace ut
