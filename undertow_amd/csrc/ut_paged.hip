@@ -176,31 +176,60 @@ __global__ __launch_bounds__(256) void k_paged_attend(PagedArgs a) {
 }
 
 // -------------------------------------------------------------- select ---
-// A head's query in 8 bits: code = rint(q 127 / max|q|); its share of a score
-// is weight max|q| / 127.  A head with a value that is not finite has none.
+// A head's query in 8 bits, a wave to a head: code = rint(q 127 / max|q|) of
+// the real quotient, its rows padded with zeros to whole steps of 64; its
+// share of a score is weight max|q| / 127.  A head with a value that is not
+// finite has none.  c = rint(q (127 / max)) may miss by one next to a half;
+// q 127 - c max is exact in 64 bits and tells.
+constexpr int kCodeStep = 64;
+__host__ __device__ inline int64_t code_row(int64_t D) { return (D + kCodeStep - 1) / kCodeStep * kCodeStep; }
+__device__ __forceinline__ int code8(double q, double top, double f) {
+    double c = rint(q * f);
+    const double e = 2.0 * __builtin_fma(-c, top, q * 127.0);
+    if (e > top || (e == top && ((int)c & 1))) c += 1.0;
+    if (e < -top || (e == -top && ((int)c & 1))) c -= 1.0;
+    return (int)c;
+}
 template <class F>
-__global__ __launch_bounds__(64) void k_select_codes(PagedArgs a, const float *__restrict__ weights,
-                                                     int8_t *__restrict__ codes,
-                                                     double *__restrict__ share) {
-    const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x, D = a.L + a.P;
-    auto q = [&](int d) {
-        return d < a.L ? (float)((const typename F::q_t *)a.qabs)[r * a.L + d]
-                       : (float)((const typename F::q_t *)a.qrope)[r * a.P + (d - a.L)];
-    };
+__global__ __launch_bounds__(256) void k_select_codes(PagedArgs a, const float *__restrict__ weights,
+                                                      int64_t heads, int8_t *__restrict__ codes,
+                                                      double *__restrict__ share) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= heads) return;
+    const int lane = threadIdx.x & 63, D = a.L + a.P;
+    typedef typename F::q_t q_t;
+    typedef q_t q8 __attribute__((ext_vector_type(8)));
+    const q_t *qa = (const q_t *)a.qabs + r * a.L, *qr = (const q_t *)a.qrope + r * a.P;
+    // eight dims a lane and turn: D is at most 1024
+    q8 q[2];
     uint32_t top = 0;  // |q|'s bits: NaN lies above infinity
-    for (int d = lane; d < D; d += 64) {
-        const uint32_t v = __float_as_uint(q(d)) & 0x7fffffffu;
-        top = v > top ? v : top;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int d = 8 * (lane + 64 * t);
+        q[t] = q8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (d < D) q[t] = *(const q8 *)(d < a.L ? qa + d : qr + (d - a.L));
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t v = __float_as_uint((float)q[t][i]) & 0x7fffffffu;
+            top = v > top ? v : top;
+        }
     }
     for (int off = 32; off >= 1; off >>= 1) {
         const uint32_t v = __shfl_xor(top, off, 64);
         top = v > top ? v : top;
     }
     const bool live = top > 0 && top < 0x7f800000u;
-    const double m = (double)__uint_as_float(top);
-    for (int d = lane; d < D; d += 64)
-        codes[r * D + d] = live ? (int8_t)(int)rint((double)q(d) * 127.0 / m) : 0;
+    const double m = (double)__uint_as_float(top), f = live ? 127.0 / m : 0.0;
+    const int64_t Dp = code_row(D);
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int d = 8 * (lane + 64 * t);
+        uint32_t c[2] = {0, 0};
+        if (live)
+#pragma unroll
+            for (int i = 0; i < 8; i++) c[i >> 2] |= (uint32_t)(code8((double)(float)q[t][i], m, f) & 255) << (8 * (i & 3));
+        if (d < Dp) *(uint2 *)(codes + r * Dp + d) = make_uint2(c[0], c[1]);
+    }
     if (lane == 0) share[r] = live ? (weights ? (double)weights[r] : 1.0) * (m / 127.0) : 0.0;
 }
 
@@ -211,42 +240,97 @@ __device__ __forceinline__ uint64_t score_key(double s) {
     return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// score = (sum_h share_h max(0, code_h . mean)) mean_scale, a wave to a page.
+// score = (sum_h share_h max(0, code_h . mean)) mean_scale.  A workgroup takes
+// 32 pages of a row; its waves take every fourth tile of 16 heads, the
+// products v_mfma_i32_16x16x64_i8 (pages x heads, exact), the sums over heads
+// in 64 bits in an order that is the same for every page.  FULL: rows of
+// whole steps of 64.
+constexpr int kScorePages = 32;
+typedef int si32x4 __attribute__((ext_vector_type(4)));
+template <bool FULL>
 __global__ __launch_bounds__(256) void k_select_score(PagedArgs a, const int8_t *__restrict__ codes,
                                                       const double *__restrict__ share,
                                                       const int8_t *__restrict__ mean,
                                                       const float *__restrict__ mean_scale,
                                                       uint64_t *__restrict__ keys) {
-    const int row = blockIdx.y, b = row / a.M, j = row - b * a.M, lane = threadIdx.x & 63;
-    const int k = blockIdx.x * 4 + (threadIdx.x >> 6), D = a.L + a.P;
+    constexpr int STEPS = FULL ? 9 : 16;  // at most 1024 dims
+    __shared__ double part[4][kScorePages];
+    const int row = blockIdx.y, b = row / a.M, j = row - b * a.M;
+    const int w = threadIdx.x >> 6, l = threadIdx.x & 63, g = l >> 4;
+    const int D = a.L + a.P, Dp = (int)code_row(D), steps = Dp / kCodeStep;
     const int32_t n = paged_len(a, b) - a.M + j + 1;
-    if (n <= 0 || k > (n - 1) >> a.shift) return;
-    const int32_t phys = paged_phys(a, b, k);
-    const uint32_t *mw = (const uint32_t *)(mean + (int64_t)phys * D);
-    double t = 0.0;
-    for (int h = 0; h < a.H; h++) {
-        const int64_t r = (int64_t)row * a.H + h;
-        const uint32_t *cw = (const uint32_t *)(codes + r * D);
-        int dot = 0;
-        for (int w = lane; w < D / 4; w += 64) dot = __builtin_amdgcn_sdot4(mw[w], cw[w], dot, false);
-        for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off, 64);
-        t += share[r] * (double)(dot > 0 ? dot : 0);
+    const int np = n > 0 ? ((n - 1) >> a.shift) + 1 : 0, k0 = blockIdx.x * kScorePages;
+    if (k0 >= np) return;
+    si32x4 A[2][STEPS];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int k = k0 + 16 * t + (l & 15);
+        const int8_t *src = mean + (int64_t)paged_phys(a, b, k < np ? k : np - 1) * D;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const int d = kCodeStep * s + 16 * g;
+            if (FULL) {
+                A[t][s] = *(const si32x4 *)(src + d);
+            } else {  // rows of a multiple of 8 bytes, zeros behind them
+                const int2 z = make_int2(0, 0), x = d + 8 <= D ? *(const int2 *)(src + d) : z;
+                const int2 y = d + 16 <= D ? *(const int2 *)(src + d + 8) : z;
+                A[t][s] = si32x4{x.x, x.y, y.x, y.y};
+            }
+        }
     }
-    if (lane == 0) keys[(int64_t)row * a.max_pages + k] = score_key(t * (double)mean_scale[phys]);
+    double sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int h0 = 16 * w; h0 < a.H; h0 += 64) {
+        const int h = h0 + (l & 15);
+        const int64_t r = (int64_t)row * a.H + (h < a.H ? h : a.H - 1);
+        const double sh = h < a.H ? share[r] : 0.0;
+        si32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+            if (FULL || s < steps) {
+                const si32x4 B = *(const si32x4 *)(codes + r * Dp + kCodeStep * s + 16 * g);
+                c[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[0][s], B, c[0], 0, 0, 0);
+                c[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[1][s], B, c[1], 0, 0, 0);
+            }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int v = c[i >> 2][i & 3];
+            sum[i] += sh * (double)(v > 0 ? v : 0);
+        }
+    }
+    // lane l holds pages 16 (i >> 2) + 4 g + (i & 3) for its head column
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        for (int off = 1; off < 16; off <<= 1) sum[i] += __shfl_xor(sum[i], off, 64);
+    if ((l & 15) == 0)
+#pragma unroll
+        for (int i = 0; i < 8; i++) part[w][16 * (i >> 2) + 4 * g + (i & 3)] = sum[i];
+    __syncthreads();
+    const int k = k0 + threadIdx.x;
+    if (threadIdx.x < kScorePages && k < np) {
+        const double t = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+        keys[(int64_t)row * a.max_pages + k] = score_key(t * (double)mean_scale[paged_phys(a, b, k)]);
+    }
 }
 
 // The top_k pages of a row: the first keep_first, the last keep_last, then by
-// score, ties to the lower page; ascending, -1 behind them.  The top_k-th
-// largest key is found digit by digit (eight of 8 bits, counted in LDS), then
-// one pass writes the pages above it and the first of those equal to it.
-constexpr int kPickThreads = 1024;
+// score, ties to the lower page; ascending, -1 behind them.  A workgroup per
+// row looks for the key of the last page to be taken: keys between the least
+// and the largest that are left fall into 256 bins by the first eight bits
+// in which those two differ; the bin that holds the one sought is looked
+// into further, until its keys are equal or at most 64, which one wave then
+// ranks.  One more pass writes the pages above that key and the first of
+// those equal to it.
+constexpr int kPickThreads = 512;
 __global__ __launch_bounds__(kPickThreads) void k_select_pick(PagedArgs a,
                                                               const uint64_t *__restrict__ keys,
                                                               int keep_first, int keep_last,
                                                               int32_t *__restrict__ out) {
-    __shared__ int hist[256];
-    __shared__ int s_digit, s_above, scan[kPickThreads / 64 * 2];
+    constexpr int NW = kPickThreads / 64;
+    __shared__ int hist[256], few_n, s_bin, s_above;
+    __shared__ uint64_t ends[2][NW], few[64], s_key;
+    __shared__ int scan[2][NW];
     const int row = blockIdx.x, b = row / a.M, j = row - b * a.M, tid = threadIdx.x;
+    const int lane = tid & 63, w = tid >> 6;
     const int32_t n = paged_len(a, b) - a.M + j + 1;
     const int np = n > 0 ? ((n - 1) >> a.shift) + 1 : 0;
     out += (int64_t)row * a.top_k;
@@ -255,55 +339,128 @@ __global__ __launch_bounds__(kPickThreads) void k_select_pick(PagedArgs a,
         return;
     }
     keys += (int64_t)row * a.max_pages;
-    auto key = [&](int k) {
-        return k < keep_first || k >= np - keep_last ? ~0ull : keys[k];
-    };
-    uint64_t prefix = 0;
-    int need = a.top_k;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int k = tid; k < np; k += kPickThreads) {
-            const uint64_t v = key(k);
-            if (shift == 56 || (v >> (shift + 8)) == (prefix >> (shift + 8)))
-                atomicAdd(&hist[(v >> shift) & 255], 1);
+    const int kept = keep_first + keep_last;  // of np > top_k >= kept pages
+    auto scored = [&](int k) { return k >= keep_first && k < np - keep_last; };
+    int need = a.top_k - kept;  // of the scored pages
+    uint64_t cut = ~0ull;       // pages of larger keys are taken, of equal ones `need`
+    if (need > 0) {
+        // the keys in question: lo <= key <= hi, `need` of them from above
+        uint64_t lo = 0, hi = ~0ull;
+        for (;;) {
+            uint64_t mn = ~0ull, mx = 0;
+            for (int k = tid; k < np; k += kPickThreads)
+                if (scored(k)) {
+                    const uint64_t v = keys[k];
+                    if (v >= lo && v <= hi) {
+                        mn = v < mn ? v : mn;
+                        mx = v > mx ? v : mx;
+                    }
+                }
+            for (int off = 32; off >= 1; off >>= 1) {
+                const uint64_t x = __shfl_xor(mn, off, 64), y = __shfl_xor(mx, off, 64);
+                mn = x < mn ? x : mn;
+                mx = y > mx ? y : mx;
+            }
+            if (lane == 0) {
+                ends[0][w] = mn;
+                ends[1][w] = mx;
+            }
+            if (tid < 256) hist[tid] = 0;
+            if (tid == 0) few_n = 0;
+            __syncthreads();
+            for (int i = 0; i < NW; i++) {
+                mn = ends[0][i] < mn ? ends[0][i] : mn;
+                mx = ends[1][i] > mx ? ends[1][i] : mx;
+            }
+            if (mn == mx) {
+                cut = mn;
+                break;
+            }
+            // the highest bit that differs is the bins' highest
+            const int top = 63 - __builtin_clzll(mn ^ mx), sh = top > 7 ? top - 7 : 0;
+            const uint64_t base = mn >> sh & ~255ull;
+            for (int k = tid; k < np; k += kPickThreads)
+                if (scored(k)) {
+                    const uint64_t v = keys[k];
+                    if (v >= mn && v <= mx) atomicAdd(&hist[(int)((v >> sh) - base)], 1);
+                }
+            __syncthreads();
+            if (w == 0) {
+                // lane l: bins 255 - 4 l - [0, 4), summed from the top
+                int c[4], s = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) s += c[i] = hist[255 - 4 * lane - i];
+                int x = s;
+                for (int off = 1; off < 64; off <<= 1) {
+                    const int y = __shfl_up(x, off, 64);
+                    if (lane >= off) x += y;
+                }
+                int above = x - s;
+                if (above < need && need <= x) {
+                    int i = 0;
+                    while (above + c[i] < need) above += c[i++];
+                    s_bin = 255 - 4 * lane - i;
+                    s_above = above;
+                }
+            }
+            __syncthreads();
+            need -= s_above;
+            lo = (base + (uint64_t)s_bin) << sh;
+            hi = lo | ((1ull << sh) - 1);
+            const int left = hist[s_bin];
+            if (left <= 64) {
+                for (int k = tid; k < np; k += kPickThreads)
+                    if (scored(k)) {
+                        const uint64_t v = keys[k];
+                        if (v >= lo && v <= hi) few[atomicAdd(&few_n, 1)] = v;
+                    }
+                __syncthreads();
+                if (w == 0) {
+                    const uint64_t v = lane < left ? few[lane] : 0;
+                    int more = 0, same = 0;
+                    for (int i = 0; i < left; i++) {
+                        more += few[i] > v;
+                        same += few[i] == v;
+                    }
+                    // the key that holds the place sought
+                    if (lane < left && more < need && need <= more + same) {
+                        s_key = v;
+                        s_above = more;
+                    }
+                }
+                __syncthreads();
+                cut = s_key;
+                need -= s_above;
+                break;
+            }
+            __syncthreads();  // hist and few_n are set anew
         }
-        __syncthreads();
-        if (tid == 0) {
-            int above = 0, d = 255;
-            while (above + hist[d] < need) above += hist[d--];
-            s_digit = d;
-            s_above = above;
-        }
-        __syncthreads();
-        prefix |= (uint64_t)s_digit << shift;
-        need -= s_above;
     }
-    // `need` of the pages equal to the key are taken, the lowest first
+    // of the pages equal to the cut `need` are taken, the lowest first
     int done = 0, equal = 0;
-    const int lane = tid & 63, w = tid >> 6;
     for (int k0 = 0; k0 < np; k0 += kPickThreads) {
         const int k = k0 + tid;
-        const uint64_t v = k < np ? key(k) : 0;
-        const bool gt = k < np && v > prefix, eq = k < np && v == prefix;
-        const uint64_t be = __ballot(eq), bg = __ballot(gt);
+        const bool in = k < np && scored(k);
+        const uint64_t v = in ? keys[k] : 0;
+        const bool eq = in && need > 0 && v == cut;
+        const uint64_t be = __ballot(eq), before = (1ull << lane) - 1;
         __syncthreads();
-        if (lane == 0) scan[w] = __popcll(be);
+        if (lane == 0) scan[0][w] = __popcll(be);
         __syncthreads();
-        int e = equal + __popcll(be & ((1ull << lane) - 1)), te = equal;
-        for (int i = 0; i < kPickThreads / 64; i++) {
-            if (i < w) e += scan[i];
-            te += scan[i];
+        int e = equal + __popcll(be & before), te = equal;
+        for (int i = 0; i < NW; i++) {
+            if (i < w) e += scan[0][i];
+            te += scan[0][i];
         }
         equal = te;
-        const bool take = gt || (eq && e < need);
+        const bool take = (k < np && !in) || (in && v > cut) || (eq && e < need);
         const uint64_t bt = __ballot(take);
-        if (lane == 0) scan[kPickThreads / 64 + w] = __popcll(bt);
+        if (lane == 0) scan[1][w] = __popcll(bt);
         __syncthreads();
-        int at = done + __popcll(bt & ((1ull << lane) - 1)), td = done;
-        for (int i = 0; i < kPickThreads / 64; i++) {
-            if (i < w) at += scan[kPickThreads / 64 + i];
-            td += scan[kPickThreads / 64 + i];
+        int at = done + __popcll(bt & before), td = done;
+        for (int i = 0; i < NW; i++) {
+            if (i < w) at += scan[1][i];
+            td += scan[1][i];
         }
         if (take) out[at] = k;
         done = td;
@@ -498,7 +655,7 @@ extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const
     a.top_k = (int32_t)top_k;
     const int64_t R = batch * rows, D = a.L + a.P;
     ScratchPlan plan;
-    plan.add((size_t)(R * heads * D));
+    plan.add((size_t)(R * heads * code_row(D)));
     plan.add((size_t)(R * heads) * 8);
     plan.add((size_t)(R * max_pages) * 8);
     std::vector<void *> ptrs;
@@ -507,17 +664,19 @@ extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const
     double *share = (double *)ptrs[1];
     uint64_t *keys = (uint64_t *)ptrs[2];
     int tok = timing_begin(ctx, "select_codes");
+    const dim3 four((unsigned)((R * heads + 3) / 4));
     if (kv->fmt == UT_KV_BF16)
-        hipLaunchKernelGGL(k_select_codes<Bf16>, dim3((unsigned)(R * heads)), dim3(64), 0,
-                           ctx->stream, a, weights_dev, codes, share);
+        hipLaunchKernelGGL(k_select_codes<Bf16>, four, dim3(256), 0, ctx->stream, a, weights_dev, R * heads, codes, share);
     else
-        hipLaunchKernelGGL(k_select_codes<F16x2>, dim3((unsigned)(R * heads)), dim3(64), 0,
-                           ctx->stream, a, weights_dev, codes, share);
+        hipLaunchKernelGGL(k_select_codes<F16x2>, four, dim3(256), 0, ctx->stream, a, weights_dev, R * heads, codes, share);
     timing_end(ctx, tok);
     UT_TRY(launch_check(ctx, "k_select_codes"));
     tok = timing_begin(ctx, "select_score");
-    hipLaunchKernelGGL(k_select_score, dim3((unsigned)((max_pages + 3) / 4), (unsigned)R), dim3(256), 0,
-                       ctx->stream, a, codes, share, kv->mean, kv->mean_scale, keys);
+    const dim3 grid((unsigned)((max_pages + kScorePages - 1) / kScorePages), (unsigned)R);
+    if (D == 9 * kCodeStep)
+        hipLaunchKernelGGL(k_select_score<true>, grid, dim3(256), 0, ctx->stream, a, codes, share, kv->mean, kv->mean_scale, keys);
+    else
+        hipLaunchKernelGGL(k_select_score<false>, grid, dim3(256), 0, ctx->stream, a, codes, share, kv->mean, kv->mean_scale, keys);
     timing_end(ctx, tok);
     UT_TRY(launch_check(ctx, "k_select_score"));
     tok = timing_begin(ctx, "select_pick");
