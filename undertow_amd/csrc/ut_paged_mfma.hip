@@ -30,6 +30,7 @@ struct PagedMfmaArgs {
     float *part_o;    // [slot][group][128 quads][16 columns][4]
     float *part_ml;   // [slot][group][16 columns][2]
     int64_t *plan;    // [units] first tile of each, then W
+    int32_t lead;     // empty tiles before every unit with tiles but the first
 };
 
 // Tiles of a unit.
@@ -67,27 +68,30 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 
 struct Range {
     int64_t W, N, s, e;  // the range takes tiles [s, e) of W
-    int u;               // the unit that holds tile s, and its first tile
-    int64_t pre;
+    int u;               // the unit that holds tile s, and its first tile (behind its empty ones)
+    int64_t first;
 };
 
-// Every workgroup works its range out from the lengths: one pass over the
-// units for their sum, one up to the unit where the range begins.  `leave`:
-// the units' first tiles are written down for the join.
+// Every workgroup works its range out from the lengths.  `leave`: the units'
+// first tiles are written down for the join.
 template <bool SPARSE, int NW>
 __device__ bool find_range(const PagedMfmaArgs &p, int64_t r, bool leave, Range &g) {
     __shared__ int64_t s[NW];
     __shared__ int64_t found[2];
     const int tid = threadIdx.x;
     int64_t W = 0;
+    int64_t t, pre;  // the last turn's
     for (int c = 0; c < p.units; c += NW * 64) {
         const int u = c + tid;
         int64_t all;
-        const int64_t t = u < p.units ? unit_tiles<SPARSE>(p.a, u) : 0;
-        const int64_t pre = W + block_scan<NW>(t, s, all);
+        t = u < p.units ? unit_tiles<SPARSE>(p.a, u) : 0;
+        // lead tiles before each unit that has tiles, but for the row's first
+        t += t > 0 ? p.lead : 0;
+        pre = W + block_scan<NW>(t, s, all);
         if (leave && u < p.units) p.plan[u] = pre;
         W += all;
     }
+    W -= W > 0 ? p.lead : 0;
     if (leave && tid == 0) p.plan[p.units] = W;
     g.W = W = uniform(W);
     if (W == 0) return false;
@@ -95,21 +99,31 @@ __device__ bool find_range(const PagedMfmaArgs &p, int64_t r, bool leave, Range 
     if (r >= g.N) return false;
     g.s = plan_begin(W, g.N, r);
     g.e = plan_begin(W, g.N, r + 1);
-    int64_t at = 0;
-    for (int c = 0; c < p.units && at <= g.s; c += NW * 64) {
-        const int u = c + tid;
-        int64_t all;
-        const int64_t t = u < p.units ? unit_tiles<SPARSE>(p.a, u) : 0;
-        const int64_t pre = at + block_scan<NW>(t, s, all);
-        if (pre <= g.s && g.s < pre + t) {
-            found[0] = u;
+    // unit u: [pre - lead, pre - lead + t), the first unit's lead before 0
+    const int64_t at = g.s + p.lead;
+    if (p.units <= NW * 64) {
+        if (pre <= at && at < pre + t) {
+            found[0] = tid;
             found[1] = pre;
         }
-        at += all;
+    } else {
+        int64_t sum = 0;
+        for (int c = 0; c < p.units && sum <= at; c += NW * 64) {
+            const int u = c + tid;
+            int64_t all;
+            t = u < p.units ? unit_tiles<SPARSE>(p.a, u) : 0;
+            t += t > 0 ? p.lead : 0;
+            pre = sum + block_scan<NW>(t, s, all);
+            if (pre <= at && at < pre + t) {
+                found[0] = u;
+                found[1] = pre;
+            }
+            sum += all;
+        }
     }
     __syncthreads();
     g.u = __builtin_amdgcn_readfirstlane((int)found[0]);
-    g.pre = uniform(found[1]);
+    g.first = uniform(found[1]);
     return true;
 }
 
@@ -120,7 +134,7 @@ __device__ bool find_range(const PagedMfmaArgs &p, int64_t r, bool leave, Range 
 // In a row's 128 bytes the eight 16-byte chunks are XORed with tile_swz(row),
 // so that the score reads (16 rows, one chunk) and the transposing reads (8
 // rows, two chunks) both meet each of the LDS's 16 slots of 16 bytes once.
-__device__ __forceinline__ int tile_swz(int row) { return (((row >> 1) & 3) << 1) | ((row >> 3) & 1); }
+__device__ __forceinline__ int tile_swz(int row) { return row & 7; }
 
 // A column's lanes l, l ^ 16, l ^ 32, l ^ 48 combined.
 __device__ __forceinline__ float col_max(float v) {
@@ -409,9 +423,10 @@ struct Lookup {
     int32_t n, top_k, shift, n_pages;
 };
 // The pool row of the unit's position v0 (8 aligned positions lie in a page);
-// any row of the pool where it has none.
+// any row of the pool where it has none, or where the table names a page
+// outside the pool (bad).
 template <bool SPARSE>
-__device__ __forceinline__ int32_t look_up(const Lookup &k, int32_t v0) {
+__device__ __forceinline__ int32_t look_up(const Lookup &k, int32_t v0, bool &bad) {
     int32_t page;
     if (SPARSE) {
         const int32_t i = v0 >> k.shift;
@@ -422,7 +437,6 @@ __device__ __forceinline__ int32_t look_up(const Lookup &k, int32_t v0) {
         if (v0 > last) v0 = last;
         page = v0 >> k.shift;
     }
-    bool bad = false;  // reported before the loop
     const int32_t phys = plan_page(k.table[page], k.n_pages, bad);
     return (phys << k.shift) + (v0 & ((1 << k.shift) - 1));
 }
@@ -493,55 +507,81 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
     // copies: wave w brings row block w & 3 and, where two waves share it, half of its column blocks
     const int rb = w & 3, c0 = w < 4 ? 0 : 5;
     Wave<F> wv;
-    int u = rg.u;
-    int64_t pre = rg.pre, at = rg.s;
-    while (at < rg.e) {
-        const int32_t tiles = __builtin_amdgcn_readfirstlane(unit_tiles<SPARSE>(a, u));
-        if (tiles == 0) {
-            u++;
-            continue;
-        }
-        const int32_t b0 = (int32_t)(at - pre), b1 = rg.e - pre < tiles ? (int32_t)(rg.e - pre) : tiles;
-        const int b = SPARSE ? u / a.M : u;
-        const int gr = active ? grp : 0;
-        const int j = SPARSE ? u - b * a.M : gr / per_row, h0 = (SPARSE ? gr : gr % per_row) * kCols;
-        const int32_t len = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-        const int32_t n = len - a.M + j + 1;
-        const int64_t row = ((int64_t)b * a.M + j) * a.H + (h0 + col < a.H ? h0 + col : a.H - 1);
+    bool bad = false;
+    // the range's part of one unit
+    struct Seg {
+        int32_t u, j, h0, b0, b1, tiles, len, n;
+        int64_t first, row;
         Lookup lk;
-        lk.table = (const_i32 *)(a.table + (int64_t)b * a.stride);
-        lk.sel = SPARSE ? (const_i32 *)(a.sel + (int64_t)u * a.top_k) : nullptr;
-        lk.n = SPARSE ? n : len;
-        lk.top_k = a.top_k;
-        lk.shift = a.shift;
-        lk.n_pages = a.n_pages;
-        auto copy = [&](int32_t x) {
-            // the lane's place in a block, worked out anew: it would be kept in
-            // registers that the products need
-            int t = threadIdx.x;
-            asm volatile("" : "+v"(t));
-            const uint32_t off = ((t >> 3) & 7) * ROW + (((t & 7) ^ tile_swz(8 * rb + ((t >> 3) & 7))) << 4);
-            const uint8_t *src = (const uint8_t *)a.pages + (int64_t)look_up<SPARSE>(lk, x * kPT + 8 * rb) * ROW + c0 * 128;
-            const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)stage[(x - b0) % STAGES] + (rb * 9 * PL + c0) * 1024;
-            copy_blocks<0, NW == 4 ? 9 * PL : 4>(off, src, lds);
-            if (NW == 8 && w < 4) copy_blocks<4, 5>(off, src, lds);
-        };
-        float c = a.scale * kLog2e;
-        auto turn = [&](int32_t x) {
-            uint8_t *T = stage[(x - b0) % STAGES];
+    };
+    int32_t u = rg.u;
+    int64_t first = rg.first, at = rg.s;
+    auto next = [&](Seg &q) {
+        int32_t tiles = 0;
+        while (at < rg.e && !(tiles = __builtin_amdgcn_readfirstlane(unit_tiles<SPARSE>(a, u)))) u++;
+        q.b0 = at > first ? (int32_t)(at - first) : 0;
+        q.b1 = rg.e - first < tiles ? (int32_t)(rg.e - first) : tiles;
+        if (q.b0 >= q.b1) return false;
+        const int b = SPARSE ? u / a.M : u, gr = active ? grp : 0;
+        q.u = u;
+        q.j = SPARSE ? u - b * a.M : gr / per_row;
+        q.h0 = (SPARSE ? gr : gr % per_row) * kCols;
+        q.tiles = tiles;
+        q.len = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+        q.n = q.len - a.M + q.j + 1;
+        q.first = first;
+        q.row = ((int64_t)b * a.M + q.j) * a.H;
+        q.lk.table = (const_i32 *)(a.table + (int64_t)b * a.stride);
+        q.lk.sel = SPARSE ? (const_i32 *)(a.sel + (int64_t)u * a.top_k) : nullptr;
+        q.lk.n = SPARSE ? q.n : q.len;
+        q.lk.top_k = a.top_k;
+        q.lk.shift = a.shift;
+        q.lk.n_pages = a.n_pages;
+        first += tiles + p.lead;
+        at = first;
+        u++;
+        return true;
+    };
+    auto copy = [&](const Seg &q, int32_t x) {
+        // the lane's place in a block, worked out anew: it would be kept in
+        // registers that the products need
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));
+        const uint32_t off = ((t >> 3) & 7) * ROW + (((t & 7) ^ tile_swz(8 * rb + ((t >> 3) & 7))) << 4);
+        const uint8_t *src = (const uint8_t *)a.pages + (int64_t)look_up<SPARSE>(q.lk, x * kPT + 8 * rb, bad) * ROW + c0 * 128;
+        const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)stage[(x - q.b0) % STAGES] + (rb * 9 * PL + c0) * 1024;
+        copy_blocks<0, NW == 4 ? 9 * PL : 4>(off, src, lds);
+        if (NW == 8 && w < 4) copy_blocks<4, 5>(off, src, lds);
+    };
+    auto start = [&](const Seg &q) {
+        for (int32_t x = q.b0; x < q.b1 && x < q.b0 + STAGES - 1; x++) copy(q, x);
+    };
+    Seg q;
+    if (!next(q)) return;
+    start(q);
+    while (true) {
+        const int64_t row = q.row + (q.h0 + col < a.H ? q.h0 + col : a.H - 1);
+        const float c = a.scale * kLog2e * F::load(wv.q, a.qabs, a.qrope, row, g);
+        F::arrive(wv.q);
+        wv.m = kLow;
+        wv.l = 0.0f;
+#pragma unroll
+        for (int mt = 0; mt < 32; mt++) wv.o[mt] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int32_t x = q.b0; x < q.b1; x++) {
+            uint8_t *T = stage[(x - q.b0) % STAGES];
             // tile x's copies have landed: those of the tiles behind it may be on their way
-            const int32_t ahead = b1 - 1 - x < STAGES - 2 ? b1 - 1 - x : STAGES - 2;
+            const int32_t ahead = q.b1 - 1 - x < STAGES - 2 ? q.b1 - 1 - x : STAGES - 2;
             if (ahead >= 2) __builtin_amdgcn_s_waitcnt(kWaitVm8);
             else if (ahead == 1) __builtin_amdgcn_s_waitcnt(kWaitVm4);
             else __builtin_amdgcn_s_waitcnt(kWaitVm0);
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            if (x + STAGES - 1 < b1) copy(x + STAGES - 1);
-            const uint32_t seen = visible<SPARSE>(lk, x * kPT, n);
+            if (x + STAGES - 1 < q.b1) copy(q, x + STAGES - 1);
+            const uint32_t seen = visible<SPARSE>(q.lk, x * kPT, q.n);
             // what the unit's last row sees, and its first one
-            const uint32_t most = SPARSE ? seen : visible<false>(lk, x * kPT, len);
-            const uint32_t least = SPARSE ? seen : visible<false>(lk, x * kPT, len - a.M + 1);
+            const uint32_t most = SPARSE ? seen : visible<false>(q.lk, x * kPT, q.len);
+            const uint32_t least = SPARSE ? seen : visible<false>(q.lk, x * kPT, q.len - a.M + 1);
             bool odd = false;
             if (least != ~0u) {
                 // a value that is not finite where only later rows look: those
@@ -564,29 +604,17 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
                 __syncthreads();
                 now >>= 1;
             } while (true);
-
-        };
-        wv.m = kLow;
-        wv.l = 0.0f;
-#pragma unroll
-        for (int mt = 0; mt < 32; mt++) wv.o[mt] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        // page ids outside the pool among those that the tiles name
-        for (int32_t k = ((b0 * kPT) >> a.shift) + tid; k <= (b1 * kPT - 1) >> a.shift; k += NW * 64) {
-            int32_t page = k;
-            if (SPARSE) page = k < a.top_k ? lk.sel[k] : -1;
-            if (page >= 0 && ((int64_t)page << a.shift) < lk.n) paged_phys(a, b, page);
         }
-        for (int32_t x = b0; x < b1 && x < b0 + STAGES - 1; x++) copy(x);
-        c *= F::load(wv.q, a.qabs, a.qrope, row, g);
-        F::arrive(wv.q);
-        for (int32_t x = b0; x < b1; x++) turn(x);
-        __syncthreads();  // the stages may be filled again
+        __syncthreads();  // the stages may be filled again: with the next part's first tiles
+        Seg nx;
+        const bool more = next(nx);
+        if (more) start(nx);
         // ---- the unit's context, or this range's part of it
         const float sum = col_sum(wv.l);
-        if (active && b0 == 0 && b1 == tiles) {
+        if (active && q.b0 == 0 && q.b1 == q.tiles) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             typename F::out_t *out = (typename F::out_t *)a.out + row * kPL + 4 * g;
-            if (h0 + col < a.H)
+            if (q.h0 + col < a.H)
 #pragma unroll
                 for (int mt = 0; mt < 32; mt++) {
                     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
@@ -596,73 +624,103 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
                     *(o4 *)(out + 16 * mt) = v;
                 }
         } else if (active) {
-            const int64_t slot = plan_slot(rg.W, rg.N, r, pre) * p.groups + grp;
+            const int64_t slot = (2 * r + (rg.s <= q.first ? 1 : 0)) * p.groups + grp;  // plan_slot
             pf32x4 *po = (pf32x4 *)p.part_o + slot * 128 * kCols + g * kCols + col;
 #pragma unroll
             for (int mt = 0; mt < 32; mt++) po[mt * 4 * kCols] = wv.o[mt];
             if (g == 0) *(float2 *)(p.part_ml + (slot * kCols + col) * 2) = make_float2(wv.m, sum);
         }
-        at = pre + b1;
-        pre += tiles;
-        u++;
+        if (!more) break;
+        q = nx;
     }
+    if (bad && l == 0) *a.err = 1;
 }
 
 // Joins the parts of a unit that lies in more than one range:
 // out = sum_r o_r 2^(m_r - M) / sum_r l_r 2^(m_r - M).  A workgroup takes one
-// column group and 128 dims, a thread four dims of two columns.
+// column group and 64 dims, each of its waves every fourth part, four at a
+// time with all their loads under way; the waves' results meet in LDS.
 template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_join(PagedMfmaArgs p) {
-    constexpr int DIMS = 128;
     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
-    __shared__ __attribute__((aligned(16))) typename F::out_t so[kCols][DIMS + 16 / sizeof(typename F::out_t)];
+    __shared__ __attribute__((aligned(16))) pf32x4 so[4][16][kCols];
+    __shared__ float2 sml[4][kCols];
     const PagedArgs &a = p.a;
     const int u = blockIdx.x / p.groups, grp = blockIdx.x - u * p.groups, tid = threadIdx.x;
-    const int64_t W = p.plan[p.units], pre = p.plan[u];
+    const int w = tid >> 6, col = tid & 15, qd = (tid >> 4) & 3;
+    const int64_t W = p.plan[p.units], first = p.plan[u];
     const int64_t tiles = unit_tiles<SPARSE>(a, u);
     if (tiles == 0) return;
     const int64_t N = plan_ranges(W, p.most, p.least);
-    const int64_t r0 = plan_range_of(W, N, pre), r1 = plan_range_of(W, N, pre + tiles - 1);
+    const int r0 = (int)plan_range_of(W, N, first), r1 = (int)plan_range_of(W, N, first + tiles - 1);
     if (r0 == r1) return;
-    auto slot = [&](int64_t r) { return plan_slot(W, N, r, pre) * p.groups + grp; };
-    const int col = tid & 15, qd = tid >> 4;  // quads 32 blockIdx.y + qd, + 16
-    float M = kLow;
-    for (int64_t r = r0; r <= r1; r++) M = fmaxf(M, p.part_ml[(slot(r) * kCols + col) * 2]);
-    float L = 0.0f;
-    pf32x4 t[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll 4
-    for (int64_t r = r0; r <= r1; r++) {
-        const float2 ml = *(const float2 *)(p.part_ml + (slot(r) * kCols + col) * 2);
-        const float f = __builtin_amdgcn_exp2f(ml.x - M);
-        L = __fadd_rn(L, __fmul_rn(ml.y, f));
+    float m = kLow, L = 0.0f;
+    pf32x4 t[4] = {};
+    for (int r = r0 + w; r <= r1; r += 16) {
+        float2 ml[4];
+        pf32x4 v[4][4];
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const pf32x4 v = ((const pf32x4 *)p.part_o)[(slot(r) * 128 + blockIdx.y * 32 + qd + 16 * k) * kCols + col];
+        for (int i = 0; i < 4; i++) {
+            const int x = r + 4 * i <= r1 ? r + 4 * i : r;
+            const int64_t slot = (2ll * x + (x == r0 ? 1 : 0)) * p.groups + grp;  // plan_slot
+            ml[i] = *(const float2 *)(p.part_ml + (slot * kCols + col) * 2);
 #pragma unroll
-            for (int i = 0; i < 4; i++) t[k][i] = __builtin_fmaf(v[i], f, t[k][i]);
+            for (int k = 0; k < 4; k++)
+                v[i][k] = ((const pf32x4 *)p.part_o)[(slot * 128 + blockIdx.y * 16 + qd + 4 * k) * kCols + col];
         }
-    }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        float mn = m;
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        o4 v;
+        for (int i = 0; i < 4; i++) {
+            if (r + 4 * i > r1) ml[i] = make_float2(kLow, 0.0f);
+            mn = fmaxf(mn, ml[i].x);
+        }
+        const float f0 = __builtin_amdgcn_exp2f(m - mn);
+        L *= f0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = (typename F::out_t)__fmul_rn(t[k][i], inv);
-        *(o4 *)&so[col][4 * (qd + 16 * k)] = v;
+        for (int k = 0; k < 4; k++) t[k] *= f0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - mn);
+            if (r + 4 * i <= r1) {
+                L = __builtin_fmaf(ml[i].y, f, L);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) t[k][e] = __builtin_fmaf(v[i][k][e], f, t[k][e]);
+            }
+        }
+        m = mn;
     }
+    if (qd == 0) sml[w][col] = make_float2(m, L);
+#pragma unroll
+    for (int k = 0; k < 4; k++) so[w][qd + 4 * k][col] = t[k];
     __syncthreads();
+    // thread: four dims (tid & 15) of column tid >> 4
+    const int c = tid >> 4, d = tid & 15;
+    float M = kLow, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) M = fmaxf(M, sml[i][c].x);
+    pf32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float f = __builtin_amdgcn_exp2f(sml[i][c].x - M);
+        const pf32x4 v = so[i][d][c];
+        sum = __builtin_fmaf(sml[i][c].y, f, sum);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(v[e], f, o[e]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    o4 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = (typename F::out_t)__fmul_rn(o[e], inv);
     const int per_row = (a.H + kCols - 1) / kCols;
     const int64_t row = SPARSE ? u : (int64_t)u * a.M + grp / per_row;
-    const int c = tid >> 4, h = (SPARSE ? grp : grp % per_row) * kCols + c;
-    if (h < a.H)
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-            *(o4 *)((typename F::out_t *)a.out + (row * a.H + h) * kPL + blockIdx.y * DIMS + 4 * ((tid & 15) + 16 * k)) =
-                *(const o4 *)&so[c][4 * ((tid & 15) + 16 * k)];
+    const int h = (SPARSE ? grp : grp % per_row) * kCols + c;
+    if (h < a.H) *(o4 *)((typename F::out_t *)a.out + (row * a.H + h) * kPL + blockIdx.y * 64 + 4 * d) = v;
 }
 
 bool paged_mfma_ok(const PagedArgs &a) { return a.L == kPL && a.P == kPD - kPL && a.shift >= 3; }
 
-constexpr int kLeastTiles = 2;
+constexpr int kLeastTiles = 2, kLeadTiles = 4;
 
 template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const PagedArgs &a) {
     PagedMfmaArgs p{};
@@ -672,7 +730,8 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     p.chunks = (p.groups + F::kWaves - 1) / F::kWaves;
     p.per = (p.groups + p.chunks - 1) / p.chunks;
     const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
-    const int64_t W = (int64_t)p.units * ((cap + kPT - 1) / kPT);  // at most
+    p.lead = kLeadTiles;
+    const int64_t W = (int64_t)p.units * ((cap + kPT - 1) / kPT + p.lead);  // at most
     const int64_t most = ctx->multiprocessors / p.chunks;
     p.least = kLeastTiles;
     p.most = (int32_t)plan_ranges(W, most < 1 ? 1 : most, p.least);
@@ -693,7 +752,7 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     UT_TRY(launch_check(ctx, "k_paged_mfma"));
     if (p.most == 1) return UT_OK;
     tok = timing_begin(ctx, "paged_join");
-    hipLaunchKernelGGL((k_paged_join<F, SPARSE>), dim3((unsigned)((int64_t)p.units * p.groups), kPL / 128), dim3(256), 0,
+    hipLaunchKernelGGL((k_paged_join<F, SPARSE>), dim3((unsigned)((int64_t)p.units * p.groups), kPL / 64), dim3(256), 0,
                        ctx->stream, p);
     timing_end(ctx, tok);
     return launch_check(ctx, "k_paged_join");

@@ -2,12 +2,14 @@
 // ranges of work, and the bounds of what its lengths and tables may say.
 // Plain arithmetic for the kernels and for the host.
 //
-// The sequences' tiles stand in one row, one sequence after another: W in
-// all, sequence u's from pre_u on.  Range r of N takes the tiles
-// [W r / N, W (r + 1) / N), so a ragged batch is cut as evenly as a square
-// one, and a long sequence spreads over many ranges.  A range meets at most
-// one sequence that began before it and one that goes on behind it; those two
-// leave a partial result each (plan_slot), every other sequence in it is whole.
+// The sequences' tiles stand in one row, one sequence after another, W in
+// all.  Range r of N takes the tiles [W r / N, W (r + 1) / N), so a ragged
+// batch is cut as evenly as a square one, and a long sequence spreads over
+// many ranges.  A sequence that begins inside a range costs that range its
+// queries and its result: some empty tiles stand before each but the first
+// for that.  A range meets at most one sequence whose first tile lies
+// before it and one that goes on behind it; those two leave a partial result
+// each (plan_slot), every other sequence in it is whole.
 #pragma once
 
 #include <cstdint>
@@ -28,11 +30,10 @@ UT_PLAN_FN int64_t plan_ranges(int64_t W, int64_t most, int64_t least) {
 UT_PLAN_FN int64_t plan_begin(int64_t W, int64_t N, int64_t r) { return W * r / N; }
 // The range that holds tile t.
 UT_PLAN_FN int64_t plan_range_of(int64_t W, int64_t N, int64_t t) { return ((t + 1) * N - 1) / W; }
-// Where range r leaves its part of the sequence whose tiles begin at pre.
-UT_PLAN_FN int64_t plan_slot(int64_t W, int64_t N, int64_t r, int64_t pre) {
-    return 2 * r + (plan_begin(W, N, r) <= pre ? 1 : 0);
+// Where range r leaves its part of the sequence whose first tile is `first`.
+UT_PLAN_FN int64_t plan_slot(int64_t W, int64_t N, int64_t r, int64_t first) {
+    return 2 * r + (plan_begin(W, N, r) <= first ? 1 : 0);
 }
-
 // A length cut to what the table can hold; a page id cut to the pool.
 UT_PLAN_FN int32_t plan_len(int32_t n, int64_t cap, bool &bad) {
     if (n >= 0 && n <= cap) return n;
