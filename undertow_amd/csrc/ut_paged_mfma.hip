@@ -79,6 +79,31 @@ __device__ bool find_range(const PagedMfmaArgs &p, int64_t r, bool leave, Range 
     __shared__ int64_t s[NW];
     __shared__ int64_t found[2];
     const int tid = threadIdx.x;
+    if (p.units <= 64) {
+        // every wave by itself
+        const int lane = tid & 63;
+        int32_t t = lane < p.units ? unit_tiles<SPARSE>(p.a, lane) : 0;
+        t += t > 0 ? p.lead : 0;
+        int64_t x = t;
+        for (int off = 1; off < 64; off <<= 1) {
+            const int64_t y = __shfl_up(x, off, 64);
+            if (lane >= off) x += y;
+        }
+        const int64_t all = uniform(__shfl(x, 63, 64)), pre = x - t;
+        g.W = all > 0 ? all - p.lead : 0;
+        if (leave && tid < p.units) p.plan[tid] = pre;
+        if (leave && tid == 0) p.plan[p.units] = g.W;
+        if (g.W == 0) return false;
+        g.N = plan_ranges(g.W, p.most, p.least);
+        if (r >= g.N) return false;
+        g.s = plan_begin(g.W, g.N, r);
+        g.e = plan_begin(g.W, g.N, r + 1);
+        const int64_t at = g.s + p.lead;
+        const int lead = __builtin_ctzll(__ballot(pre <= at && at < pre + t));
+        g.u = __builtin_amdgcn_readfirstlane(lead);
+        g.first = uniform(__shfl(pre, lead, 64));
+        return true;
+    }
     int64_t W = 0;
     int64_t t, pre;  // the last turn's
     for (int c = 0; c < p.units; c += NW * 64) {
@@ -176,7 +201,7 @@ template <int PLANES> __device__ __forceinline__ LaneAddr lane_addr(int l) {
 // bf16 pages: queries and weights in bf16.
 struct MfmaBf16 {
     static constexpr int kPlanes = 1, kWaves = 8;
-    static constexpr int kDepth = 5;
+    static constexpr int kDepth = 4;
     static constexpr float kRise = 11.5f;  // log2 units a score may exceed the offset (8 nats)
     typedef __bf16 out_t;
     struct Query {
@@ -379,10 +404,12 @@ __device__ __forceinline__ void tile_step(Wave<F> &w, const LaneAddr &ad, uint32
     const bool jump = top > __fadd_rn(w.m, F::kRise);
     if (__any(jump)) {
         const float mn = jump ? top : w.m, f = __builtin_amdgcn_exp2f(w.m - mn);
+        // (a column's first scores meet zeros)
+        if (__any(jump && w.m > kLow))
+#pragma unroll
+            for (int mt = 0; mt < 32; mt++) w.o[mt] *= f;
         w.m = mn;
         w.l *= f;
-#pragma unroll
-        for (int mt = 0; mt < 32; mt++) w.o[mt] *= f;
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) t[i] = __builtin_amdgcn_exp2f(t[i] - w.m);
@@ -558,10 +585,12 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
     };
     Seg q;
     if (!next(q)) return;
-    start(q);
+    bool begun = false;
     while (true) {
         const int64_t row = q.row + (q.h0 + col < a.H ? q.h0 + col : a.H - 1);
         const float c = a.scale * kLog2e * F::load(wv.q, a.qabs, a.qrope, row, g);
+        if (!begun) start(q);
+        begun = true;
         F::arrive(wv.q);
         wv.m = kLow;
         wv.l = 0.0f;
