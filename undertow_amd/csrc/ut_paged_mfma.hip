@@ -1,5 +1,7 @@
 // ut_paged_mfma.hip -- attention over the paged latent cache on the matrix
 // cores, for latent 512 + rope 64 and pages of 8 positions and more.
+#include <type_traits>
+
 #include "ut_paged.h"
 
 namespace ut {
@@ -201,6 +203,7 @@ template <int PLANES> __device__ __forceinline__ LaneAddr lane_addr(int l) {
 // bf16 pages: queries and weights in bf16.
 struct MfmaBf16 {
     static constexpr int kPlanes = 1, kWaves = 8;
+    static constexpr bool kBetween = false;  // copies between the products (the branches cost registers)
     static constexpr int kDepth = 4;
     static constexpr float kRise = 11.5f;  // log2 units a score may exceed the offset (8 nats)
     typedef __bf16 out_t;
@@ -220,8 +223,10 @@ struct MfmaBf16 {
 #pragma unroll
         for (int ks = 0; ks < 18; ks++) asm volatile("" : "+v"(x.q[ks]));
     }
-    // both halves of the tile in turn, kDepth reads ahead of the products
-    __device__ __forceinline__ static void scores(const Query &x, uint32_t T, pf32x4 (&s)[2]) {
+    // both halves of the tile in turn, kDepth reads ahead of the products;
+    // between(i) behind product i
+    template <class B> __device__ __forceinline__ static void scores(const Query &x, uint32_t T, pf32x4 (&s)[2], B &&between) {
+        s[0] = s[1] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
         pbf16x8 k[36];
         auto read = [&](int i) {
             k[i] = lds_read<pbf16x8>((T ^ (((i >> 1) & 1) << 6)) + (i >> 2) * 1024 + (i & 1) * 18 * 1024);
@@ -233,6 +238,7 @@ struct MfmaBf16 {
         for (int i = 0; i < 36; i++) {
             s[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i], x.q[i >> 1], s[i & 1], 0, 0, 0);
             if (i + kDepth < 36) read(i + kDepth);
+            between(i);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -272,13 +278,14 @@ struct MfmaBf16 {
 
 // f16x2 pages.  Every operand is a pair of f16, and a product is taken as
 // hi*hi + lo*hi + hi*lo (lo*lo lies 2^-22 below).  Stored low parts are
-// scaled by 2^11; the partner of such a part is the high part of the other
-// operand times 2^-11, so all three products add up in one accumulator.
-// Queries are scaled by a power of two to a maximum in [2^14, 2^15) and
+// scaled by 2^11: the scores' sum with them is scaled back at its end, and in
+// the context such a part meets the weight's high part times 2^-11, so that
+// all three products add up in one accumulator.  Queries are scaled by a power of two to a maximum in [2^14, 2^15) and
 // weights by 2^14 (at most 2^15), so that neither their low parts nor the
 // scaled high parts fall out of f16's range where they matter.
 struct MfmaF16x2 {
     static constexpr int kPlanes = 2, kWaves = 4;
+    static constexpr bool kBetween = true;
     static constexpr int kDepth = 4;
     static constexpr float kRise = 1.0f;
     typedef float out_t;
@@ -308,8 +315,10 @@ struct MfmaF16x2 {
         return ldexpf(1.0f, -up);
     }
     __device__ __forceinline__ static void arrive(Query &) {}  // converted: they are there
-    __device__ __forceinline__ static void scores(const Query &x, uint32_t T, pf32x4 (&s)[2]) {
-        pf32x4 t[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    // three sums a half tile, so that no product waits for the one before it
+    template <class B> __device__ __forceinline__ static void scores(const Query &x, uint32_t T, pf32x4 (&s)[2], B &&between) {
+        s[0] = s[1] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        pf32x4 t[2] = {s[0], s[0]}, v[2] = {s[0], s[0]};
         pf16x8 k[36], d[36];  // high and low parts
         auto read = [&](int i) {
             const uint32_t b = (T ^ (((i >> 1) & 1) << 6)) + (i >> 2) * 1024 + (i & 1) * 36 * 1024;
@@ -320,20 +329,25 @@ struct MfmaF16x2 {
         for (int i = 0; i < kDepth; i++) read(i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 36; i++) {
-            s[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], x.h[i >> 1], s[i & 1], 0, 0, 0);
-            t[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], x.l[i >> 1], t[i & 1], 0, 0, 0);
-            pf16x8 h = x.h[i >> 1];
-            asm volatile("" : "+v"(h));  // scaled here: all of them scaled ahead would not fit
-            t[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[i], h * (_Float16)(1.0f / kF16x2Step), t[i & 1], 0, 0, 0);
-            if (i + kDepth < 36) read(i + kDepth);
+        for (int i = 0; i < 36; i += 2) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) s[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i + e], x.h[i >> 1], s[e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; e++) t[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i + e], x.l[i >> 1], t[e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; e++) v[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[i + e], x.h[i >> 1], v[e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                if (i + e + kDepth < 36) read(i + e + kDepth);
+            between(i);
+            between(i + 1);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            s[0][i] = __fadd_rn(s[0][i], t[0][i]);
-            s[1][i] = __fadd_rn(s[1][i], t[1][i]);
-        }
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                s[e][i] = __fadd_rn(s[e][i], __builtin_fmaf(v[e][i], 1.0f / kF16x2Step, t[e][i]));
     }
     struct Weights {
         pf16x8 h, l, d;
@@ -361,12 +375,16 @@ struct MfmaF16x2 {
         for (int i = 0; i < kDepth; i++) read(i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-            const pf16x8 vh = __builtin_bit_cast(pf16x8, h[i]), vl = __builtin_bit_cast(pf16x8, d[i]);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, x.l, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, x.d, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, x.h, o[i], 0, 0, 0);
-            if (i + kDepth < 32) read(i + kDepth);
+        for (int i = 0; i < 32; i += 2) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) o[i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pf16x8, h[i + e]), x.l, o[i + e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; e++) o[i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pf16x8, d[i + e]), x.d, o[i + e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; e++) o[i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pf16x8, h[i + e]), x.h, o[i + e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                if (i + e + kDepth < 32) read(i + e + kDepth);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -387,10 +405,10 @@ template <class F> struct Wave {
 // exceeds it by more than kRise.
 // seen: the tile's visible positions.  A hidden position's score is replaced,
 // whatever it is; what V holds there must be finite (tile_clear).
-template <class F>
-__device__ __forceinline__ void tile_step(Wave<F> &w, const LaneAddr &ad, uint32_t T, uint32_t seen, float c, int g) {
-    pf32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-    F::scores(w.q, T + ad.k, s);
+template <class F, class B>
+__device__ __forceinline__ void tile_step(Wave<F> &w, const LaneAddr &ad, uint32_t T, uint32_t seen, float c, int g, B &&between) {
+    pf32x4 s[2];
+    F::scores(w.q, T + ad.k, s, between);
     const uint32_t mine = seen >> (4 * g);
     float t[8];
 #pragma unroll
@@ -447,25 +465,20 @@ template <class F> __device__ __forceinline__ bool tile_odd(uint8_t *T, uint32_t
 // What a wave needs to look positions up: unit u's sequence and row.
 struct Lookup {
     const_i32 *table, *sel;  // the sequence's row of the table, the row's pages
-    int32_t n, top_k, shift, n_pages;
+    int32_t n, top_k, shift;
 };
-// The pool row of the unit's position v0 (8 aligned positions lie in a page);
-// any row of the pool where it has none, or where the table names a page
-// outside the pool (bad).
-template <bool SPARSE>
-__device__ __forceinline__ int32_t look_up(const Lookup &k, int32_t v0, bool &bad) {
-    int32_t page;
+// The page of the sequence that holds the unit's position v0; one that it
+// does have, where there is none or it lies behind the end.
+template <bool SPARSE> __device__ __forceinline__ int32_t page_of(const Lookup &k, int32_t v0) {
     if (SPARSE) {
         const int32_t i = v0 >> k.shift;
-        page = i < k.top_k ? k.sel[i] : 0;
-        if (page < 0 || ((int64_t)page << k.shift) >= k.n) page = 0;
-    } else {
-        const int32_t last = (k.n - 1) & ~7;
-        if (v0 > last) v0 = last;
-        page = v0 >> k.shift;
+        return i < k.top_k ? k.sel[i] : 0;
     }
-    const int32_t phys = plan_page(k.table[page], k.n_pages, bad);
-    return (phys << k.shift) + (v0 & ((1 << k.shift) - 1));
+    return (v0 < k.n ? v0 : k.n - 1) >> k.shift;
+}
+template <bool SPARSE> __device__ __forceinline__ int32_t page_entry(const Lookup &k, int32_t page) {
+    if (SPARSE && (page < 0 || ((int64_t)page << k.shift) >= k.n)) page = 0;
+    return k.table[page];
 }
 // The visible positions of the tile at v0 for a row that sees n.
 template <bool SPARSE>
@@ -486,19 +499,29 @@ __device__ __forceinline__ uint32_t visible(const Lookup &k, int32_t v0, int32_t
     return m;
 }
 
-// Column blocks I .. N - 1 of a lane's row, 128 bytes apart there and 1 KiB
-// apart in LDS, straight to LDS.  An instruction's offset counts on both
-// sides, so lds steps by the rest.  Written out, since the compiler would
-// have every later LDS read wait for every copy under way: the kernel waits
-// itself.  Nothing is loaded into a register, and the address is read when
-// the instruction issues.
+// Column block I of a lane's row, 128 bytes apart there and 1 KiB apart in
+// LDS, straight to LDS.  An instruction's offset counts on both sides, so lds
+// steps by the rest.  Written out, since the compiler would have every later
+// LDS read wait for every copy under way: the kernel waits itself.  Nothing
+// is loaded into a register, and the address is read when the instruction
+// issues.
+template <int I> __device__ __forceinline__ void copy_block(uint32_t off, const uint8_t *src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3"
+                 :
+                 : "v"(off), "s"(src), "s"(lds + I * (1024 - 128)), "n"(I * 128)
+                 : "memory");
+}
 template <int I, int N> __device__ __forceinline__ void copy_blocks(uint32_t off, const uint8_t *src, uint32_t lds) {
     if constexpr (I < N) {
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3"
-                     :
-                     : "v"(off), "s"(src), "s"(lds + I * (1024 - 128)), "n"(I * 128)
-                     : "memory", "m0");
+        copy_block<I>(off, src, lds);
         copy_blocks<I + 1, N>(off, src, lds);
+    }
+}
+// Block i of N, i known where this is expanded.
+template <int I, int N> __device__ __forceinline__ void copy_nth(int i, uint32_t off, const uint8_t *src, uint32_t lds) {
+    if constexpr (I < N) {
+        if (i == I) copy_block<I>(off, src, lds);
+        else copy_nth<I + 1, N>(i, off, src, lds);
     }
 }
 
@@ -507,13 +530,52 @@ template <int I, int N> __device__ __forceinline__ void copy_blocks(uint32_t off
 // suits both)
 constexpr int kWaitVm0 = 0x0f70, kWaitVm4 = 0x0f74, kWaitVm8 = 0x0f78;
 
+// The part of a range that lies in one unit.
+struct Seg {
+    int32_t u, j, h0, b0, b1, tiles, len, n;
+    int64_t first, row;
+    Lookup lk;
+};
+// Goes over a range's parts.
+template <bool SPARSE> struct Walk {
+    int32_t u;
+    int64_t first, at;
+    __device__ __forceinline__ bool next(const PagedMfmaArgs &p, const Range &rg, int gr, Seg &q) {
+        const PagedArgs &a = p.a;
+        int32_t tiles = 0;
+        while (at < rg.e && !(tiles = __builtin_amdgcn_readfirstlane(unit_tiles<SPARSE>(a, u)))) u++;
+        q.b0 = at > first ? (int32_t)(at - first) : 0;
+        q.b1 = rg.e - first < tiles ? (int32_t)(rg.e - first) : tiles;
+        if (q.b0 >= q.b1) return false;
+        const int per_row = (a.H + kCols - 1) / kCols, b = SPARSE ? u / a.M : u;
+        q.u = u;
+        q.j = SPARSE ? u - b * a.M : gr / per_row;
+        q.h0 = (SPARSE ? gr : gr % per_row) * kCols;
+        q.tiles = tiles;
+        q.len = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+        q.n = q.len - a.M + q.j + 1;
+        q.first = first;
+        q.row = ((int64_t)b * a.M + q.j) * a.H;
+        q.lk.table = (const_i32 *)(a.table + (int64_t)b * a.stride);
+        q.lk.sel = SPARSE ? (const_i32 *)(a.sel + (int64_t)u * a.top_k) : nullptr;
+        q.lk.n = SPARSE ? q.n : q.len;
+        q.lk.top_k = a.top_k;
+        q.lk.shift = a.shift;
+        first += tiles + p.lead;
+        at = first;
+        u++;
+        return true;
+    }
+};
+
 // A workgroup is F::kWaves waves, each with a column group of its own, over
-// the same tiles.  Four (two) tiles fit the LDS: the products of one run while
-// the next three (one) are on their way.
+// the same tiles.  Four (f16x2: two) tiles fit the LDS: the products of one
+// run while the next three (one) are on their way.  A table entry is read a
+// tile before its copy, and the copies issue between the products.
 template <class F, bool SPARSE>
 __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(PagedMfmaArgs p) {
-    constexpr int NW = F::kWaves, PL = F::kPlanes, STAGES = 4 / PL, BLOCKS = 36 * PL, ROW = kPD * 2 * PL;
-    __shared__ __attribute__((aligned(1024))) uint8_t stage[STAGES][BLOCKS * 1024];
+    constexpr int NW = F::kWaves, PL = F::kPlanes, STAGES = 4 / PL, ROW = kPD * 2 * PL, TILE = 36 * PL * 1024;
+    __shared__ __attribute__((aligned(1024))) uint8_t stage[STAGES * TILE];
     __shared__ int s_odd;
     const PagedArgs &a = p.a;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, col = l & 15;
@@ -529,62 +591,45 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
     if (r >= p.most || !find_range<SPARSE, NW>(p, r, r == 0 && chunk == 0, rg)) return;
     const int grp = chunk * p.per + w;
     const bool active = w < p.per && grp < p.groups;
-    const int per_row = (a.H + kCols - 1) / kCols;
+    const int gr = active ? grp : 0;
     const LaneAddr ad = lane_addr<PL>(l);
+    const uint32_t stage0 = (uint32_t)(uintptr_t)(lds_u8 *)stage;
     // copies: wave w brings row block w & 3 and, where two waves share it, half of its column blocks
-    const int rb = w & 3, c0 = w < 4 ? 0 : 5;
+    const int rb = w & 3, c0 = NW == 8 && w >= 4 ? 5 : 0;
+    constexpr int COPIES = NW == 4 ? 9 * PL : 4;  // and a fifth of waves 0 to 3
     Wave<F> wv;
     bool bad = false;
-    // the range's part of one unit
-    struct Seg {
-        int32_t u, j, h0, b0, b1, tiles, len, n;
-        int64_t first, row;
-        Lookup lk;
-    };
-    int32_t u = rg.u;
-    int64_t first = rg.first, at = rg.s;
-    auto next = [&](Seg &q) {
-        int32_t tiles = 0;
-        while (at < rg.e && !(tiles = __builtin_amdgcn_readfirstlane(unit_tiles<SPARSE>(a, u)))) u++;
-        q.b0 = at > first ? (int32_t)(at - first) : 0;
-        q.b1 = rg.e - first < tiles ? (int32_t)(rg.e - first) : tiles;
-        if (q.b0 >= q.b1) return false;
-        const int b = SPARSE ? u / a.M : u, gr = active ? grp : 0;
-        q.u = u;
-        q.j = SPARSE ? u - b * a.M : gr / per_row;
-        q.h0 = (SPARSE ? gr : gr % per_row) * kCols;
-        q.tiles = tiles;
-        q.len = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-        q.n = q.len - a.M + q.j + 1;
-        q.first = first;
-        q.row = ((int64_t)b * a.M + q.j) * a.H;
-        q.lk.table = (const_i32 *)(a.table + (int64_t)b * a.stride);
-        q.lk.sel = SPARSE ? (const_i32 *)(a.sel + (int64_t)u * a.top_k) : nullptr;
-        q.lk.n = SPARSE ? q.n : q.len;
-        q.lk.top_k = a.top_k;
-        q.lk.shift = a.shift;
-        q.lk.n_pages = a.n_pages;
-        first += tiles + p.lead;
-        at = first;
-        u++;
-        return true;
-    };
-    auto copy = [&](const Seg &q, int32_t x) {
+    // the next copy: its table entry, and where it goes
+    int32_t entry = 0;
+    uint32_t off, dst;
+    const uint8_t *src;
+    auto aim = [&](const Seg &q, int32_t x) {
         // the lane's place in a block, worked out anew: it would be kept in
         // registers that the products need
         int t = threadIdx.x;
         asm volatile("" : "+v"(t));
-        const uint32_t off = ((t >> 3) & 7) * ROW + (((t & 7) ^ tile_swz(8 * rb + ((t >> 3) & 7))) << 4);
-        const uint8_t *src = (const uint8_t *)a.pages + (int64_t)look_up<SPARSE>(q.lk, x * kPT + 8 * rb, bad) * ROW + c0 * 128;
-        const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)stage[(x - q.b0) % STAGES] + (rb * 9 * PL + c0) * 1024;
-        copy_blocks<0, NW == 4 ? 9 * PL : 4>(off, src, lds);
-        if (NW == 8 && w < 4) copy_blocks<4, 5>(off, src, lds);
+        off = ((t >> 3) & 7) * ROW + (((t & 7) ^ tile_swz(8 * rb + ((t >> 3) & 7))) << 4);
+        const int32_t phys = plan_page(entry, a.n_pages, bad);
+        const int32_t at = (phys << a.shift) + ((x * kPT + 8 * rb) & ((1 << a.shift) - 1));
+        src = (const uint8_t *)uniform((int64_t)a.pages + (int64_t)at * ROW + c0 * 128);
+        dst = __builtin_amdgcn_readfirstlane(stage0 + (x - q.b0) % STAGES * TILE + (rb * 9 * PL + c0) * 1024);
     };
+    auto fifth = [&]() {
+        if (NW == 8 && w < 4) copy_block<4>(off, src, dst);
+    };
+    auto entry_of = [&](const Seg &q, int32_t x) { return page_entry<SPARSE>(q.lk, page_of<SPARSE>(q.lk, x * kPT + 8 * rb)); };
     auto start = [&](const Seg &q) {
-        for (int32_t x = q.b0; x < q.b1 && x < q.b0 + STAGES - 1; x++) copy(q, x);
+        for (int32_t x = q.b0; x < q.b1 && x < q.b0 + STAGES - 1; x++) {
+            entry = entry_of(q, x);
+            aim(q, x);
+            copy_blocks<0, COPIES>(off, src, dst);
+            fifth();
+        }
+        entry = entry_of(q, q.b0 + STAGES - 1);
     };
+    Walk<SPARSE> walk = {rg.u, rg.first, rg.s};
     Seg q;
-    if (!next(q)) return;
+    if (!walk.next(p, rg, gr, q)) return;
     bool begun = false;
     while (true) {
         const int64_t row = q.row + (q.h0 + col < a.H ? q.h0 + col : a.H - 1);
@@ -596,8 +641,10 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
         wv.l = 0.0f;
 #pragma unroll
         for (int mt = 0; mt < 32; mt++) wv.o[mt] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t seen = visible<SPARSE>(q.lk, q.b0 * kPT, q.n);
         for (int32_t x = q.b0; x < q.b1; x++) {
-            uint8_t *T = stage[(x - q.b0) % STAGES];
+            const uint32_t ps = (uint32_t)(x - q.b0) % STAGES * TILE;
+            uint8_t *T = stage + ps;
             // tile x's copies have landed: those of the tiles behind it may be on their way
             const int32_t ahead = q.b1 - 1 - x < STAGES - 2 ? q.b1 - 1 - x : STAGES - 2;
             if (ahead >= 2) __builtin_amdgcn_s_waitcnt(kWaitVm8);
@@ -606,8 +653,14 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            if (x + STAGES - 1 < q.b1) copy(q, x + STAGES - 1);
-            const uint32_t seen = visible<SPARSE>(q.lk, x * kPT, q.n);
+            bool due = x + STAGES - 1 < q.b1;
+            if (due) {
+                aim(q, x + STAGES - 1);
+                if (!F::kBetween) {
+                    copy_blocks<0, COPIES>(off, src, dst);
+                    fifth();
+                }
+            }
             // what the unit's last row sees, and its first one
             const uint32_t most = SPARSE ? seen : visible<false>(q.lk, x * kPT, q.len);
             const uint32_t least = SPARSE ? seen : visible<false>(q.lk, x * kPT, q.len - a.M + 1);
@@ -624,19 +677,30 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
                 __syncthreads();
                 odd = least != most && __builtin_amdgcn_readfirstlane(s_odd);
             }
+            const int32_t page = page_of<SPARSE>(q.lk, (x + STAGES) * kPT + 8 * rb);
             uint32_t now = most;
             do {
-                if (active && seen && (!odd || seen == now)) tile_step<F>(wv, ad, (uint32_t)(uintptr_t)(lds_u8 *)T, seen, c, g);
+                if (active && seen && (!odd || seen == now))
+                    tile_step<F>(wv, ad, stage0 + ps, seen, c, g, [&](int i) {
+                        // a copy every few products
+                        constexpr int EVERY = 36 / COPIES;
+                        if (F::kBetween && i % EVERY == 0 && due) copy_nth<0, COPIES>(i / EVERY, off, src, dst);
+                    });
+                else if (F::kBetween && due)
+                    copy_blocks<0, COPIES>(off, src, dst);
+                due = false;
                 if (!odd || now == least) break;
                 __syncthreads();
                 tile_clear<F>(T, now & ~(now >> 1));
                 __syncthreads();
                 now >>= 1;
             } while (true);
+            entry = page_entry<SPARSE>(q.lk, page);
+            seen = visible<SPARSE>(q.lk, (x + 1) * kPT, q.n);
         }
         __syncthreads();  // the stages may be filled again: with the next part's first tiles
         Seg nx;
-        const bool more = next(nx);
+        const bool more = walk.next(p, rg, gr, nx);
         if (more) start(nx);
         // ---- the unit's context, or this range's part of it
         const float sum = col_sum(wv.l);
@@ -667,8 +731,8 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
 
 // Joins the parts of a unit that lies in more than one range:
 // out = sum_r o_r 2^(m_r - M) / sum_r l_r 2^(m_r - M).  A workgroup takes one
-// column group and 64 dims, each of its waves every fourth part, four at a
-// time with all their loads under way; the waves' results meet in LDS.
+// column group and 64 dims, each of its waves every fourth part, as many
+// at a time as there are, with all their loads under way; the waves' results meet in LDS.
 template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_join(PagedMfmaArgs p) {
     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
     __shared__ __attribute__((aligned(16))) pf32x4 so[4][16][kCols];
@@ -684,12 +748,14 @@ template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_j
     if (r0 == r1) return;
     float m = kLow, L = 0.0f;
     pf32x4 t[4] = {};
-    for (int r = r0 + w; r <= r1; r += 16) {
-        float2 ml[4];
-        pf32x4 v[4][4];
+    // N parts, r and every fourth behind it
+    auto add = [&](int r, auto many) {
+        constexpr int COUNT = decltype(many)::value;
+        float2 ml[COUNT];
+        pf32x4 v[COUNT][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int x = r + 4 * i <= r1 ? r + 4 * i : r;
+        for (int i = 0; i < COUNT; i++) {
+            const int x = r + 4 * i;
             const int64_t slot = (2ll * x + (x == r0 ? 1 : 0)) * p.groups + grp;  // plan_slot
             ml[i] = *(const float2 *)(p.part_ml + (slot * kCols + col) * 2);
 #pragma unroll
@@ -698,27 +764,33 @@ template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_j
         }
         float mn = m;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (r + 4 * i > r1) ml[i] = make_float2(kLow, 0.0f);
-            mn = fmaxf(mn, ml[i].x);
-        }
+        for (int i = 0; i < COUNT; i++) mn = fmaxf(mn, ml[i].x);
         const float f0 = __builtin_amdgcn_exp2f(m - mn);
         L *= f0;
 #pragma unroll
         for (int k = 0; k < 4; k++) t[k] *= f0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < COUNT; i++) {
             const float f = __builtin_amdgcn_exp2f(ml[i].x - mn);
-            if (r + 4 * i <= r1) {
-                L = __builtin_fmaf(ml[i].y, f, L);
+            L = __builtin_fmaf(ml[i].y, f, L);
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+            for (int k = 0; k < 4; k++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) t[k][e] = __builtin_fmaf(v[i][k][e], f, t[k][e]);
-            }
+                for (int e = 0; e < 4; e++) t[k][e] = __builtin_fmaf(v[i][k][e], f, t[k][e]);
         }
         m = mn;
+    };
+    int r = r0 + w;
+    for (; r + 28 <= r1; r += 32) add(r, std::integral_constant<int, 8>());
+    if (r + 12 <= r1) {
+        add(r, std::integral_constant<int, 4>());
+        r += 16;
     }
+    if (r + 4 <= r1) {
+        add(r, std::integral_constant<int, 2>());
+        r += 8;
+    }
+    if (r <= r1) add(r, std::integral_constant<int, 1>());
     if (qd == 0) sml[w][col] = make_float2(m, L);
 #pragma unroll
     for (int k = 0; k < 4; k++) so[w][qd + 4 * k][col] = t[k];
