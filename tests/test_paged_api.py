@@ -9,8 +9,9 @@ from undertow_amd.runtime import UT_ERR_ARG, UT_ERR_SHAPE, PagedCache
 
 class OnDevice(torch.Tensor):
     """A CPU tensor that says it lies on cuda:0."""
-    is_cuda = True
-    device = torch.device("cuda", 0)
+
+    def get_device(self):
+        return 0
 
 
 def dev(*shape, dtype=torch.float32):

@@ -22,17 +22,21 @@ struct PagedArgs {
     void *out;
 };
 
+// Lengths and tables do not change while a kernel runs: read as constants,
+// through the scalar cache where the index is the same for a wave.
+typedef const __attribute__((address_space(4))) int32_t const_i32;
+
 // Positions of sequence b, bounded by what its row of the table can hold.
 __device__ __forceinline__ int32_t paged_len(const PagedArgs &a, int b) {
     bool bad = false;
-    const int32_t n = plan_len(a.lens[b], (int64_t)a.max_pages << a.shift, bad);
+    const int32_t n = plan_len(((const_i32 *)a.lens)[b], (int64_t)a.max_pages << a.shift, bad);
     if (bad) *a.err = 1;
     return n;
 }
 // The physical page of a sequence's k-th page (k < max_pages); an id outside
 // the pool is reported and page 0 stands in for it.
 __device__ __forceinline__ int32_t paged_phys(const PagedArgs &a, int b, int k, bool &bad) {
-    const int32_t p = plan_page(a.table[(int64_t)b * a.stride + k], a.n_pages, bad);
+    const int32_t p = plan_page(((const_i32 *)a.table)[(int64_t)b * a.stride + k], a.n_pages, bad);
     if (bad) *a.err = 1;
     return p;
 }

@@ -7,16 +7,40 @@ namespace ut {
 struct Bf16 {
     static constexpr int kPlanes = 1;
     typedef __bf16 q_t;
+    typedef float code_t;
     __device__ static float value(const uint16_t *row, int D, int d) {
         return __uint_as_float((uint32_t)row[d] << 16);
+    }
+    // four values as a row holds them, and back
+    __device__ static void store(const float (&x)[4], uint2 (&h)[1]) {
+        __bf16 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (__bf16)x[i];
+        h[0] = *(const uint2 *)v;
+    }
+    __device__ static float stored(const uint2 (&h)[1], int i) {
+        const uint32_t w = i < 2 ? h[0].x : h[0].y;
+        return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
     }
 };
 struct F16x2 {
     static constexpr int kPlanes = 2;
     typedef float q_t;
+    typedef double code_t;
     __device__ static float value(const uint16_t *row, int D, int d) {
         const _Float16 *h = (const _Float16 *)row;
         return __fadd_rn((float)h[d], __fmul_rn((float)h[D + d], 1.0f / kF16x2Step));
+    }
+    __device__ static void store(const float (&x)[4], uint2 (&h)[2]) {
+        _Float16 v[2][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) f16x2_split(x[i], v[0][i], v[1][i]);
+        h[0] = *(const uint2 *)v[0];
+        h[1] = *(const uint2 *)v[1];
+    }
+    __device__ static float stored(const uint2 (&h)[2], int i) {
+        const _Float16 *hi = (const _Float16 *)&h[0], *lo = (const _Float16 *)&h[1];
+        return __fadd_rn((float)hi[i], __fmul_rn((float)lo[i], 1.0f / kF16x2Step));
     }
 };
 
@@ -53,34 +77,41 @@ __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__r
     for (int u = tid; u < 4 * nq; u += blockDim.x) {
         const int s = u / nq, d = (u - s * nq) * 4;
         double t[4] = {0.0, 0.0, 0.0, 0.0};
+        // kOld (kNew) rows at a time, so that as many loads are under way
+        constexpr int kOld = 16, kNew = 8;
         if (mean)
-            for (int o = s; o < first; o += 4)
+            for (int o0 = s; o0 < first; o0 += 4 * kOld) {
+                uint2 v[kOld][F::kPlanes];
 #pragma unroll
-                for (int i = 0; i < 4; i++) t[i] += (double)F::value(base + o * row16, D, d + i);
-        for (int o = first + ((s - first) & 3); o < live; o += 4) {
-            const int64_t r = (int64_t)b * a.M + (p0 + o - (len - a.M));
-            const float4 v = d < a.L ? *(const float4 *)(latent + r * a.L + d)
-                                     : *(const float4 *)(krot + r * a.P + (d - a.L));
-            const float x[4] = {v.x, v.y, v.z, v.w};
-            uint16_t *row = base + o * row16 + d;
-            if (F::kPlanes == 1) {
-                __bf16 h[4];
+                for (int k = 0; k < kOld; k++) {
+                    const int o = o0 + 4 * k < first ? o0 + 4 * k : o0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    h[i] = (__bf16)x[i];
-                    t[i] += (double)(float)h[i];
+                    for (int i = 0; i < F::kPlanes; i++) v[k][i] = *(const uint2 *)(base + o * row16 + i * D + d);
                 }
-                *(uint2 *)row = *(const uint2 *)h;
-            } else {
-                _Float16 h[4], l[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    f16x2_split(x[i], h[i], l[i]);
-                    t[i] += (double)__fadd_rn((float)h[i], __fmul_rn((float)l[i], 1.0f / kF16x2Step));
-                }
-                *(uint2 *)row = *(const uint2 *)h;
-                *(uint2 *)(row + D) = *(const uint2 *)l;
+                for (int k = 0; k < kOld; k++)
+                    if (o0 + 4 * k < first) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) t[i] += (double)F::stored(v[k], i);
+                    }
             }
+        const float *src = d < a.L ? latent + d : krot + (d - a.L);
+        const int64_t width = d < a.L ? a.L : a.P, r0 = (int64_t)b * a.M + (p0 - (len - a.M));
+        for (int o0 = first + ((s - first) & 3); o0 < live; o0 += 4 * kNew) {
+            float4 v[kNew];
+#pragma unroll
+            for (int k = 0; k < kNew; k++) v[k] = *(const float4 *)(src + (r0 + (o0 + 4 * k < live ? o0 + 4 * k : o0)) * width);
+#pragma unroll
+            for (int k = 0; k < kNew; k++)
+                if (o0 + 4 * k < live) {
+                    const float x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                    uint2 h[F::kPlanes];
+                    F::store(x, h);
+#pragma unroll
+                    for (int i = 0; i < F::kPlanes; i++) *(uint2 *)(base + (o0 + 4 * k) * row16 + i * D + d) = h[i];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) t[i] += (double)F::stored(h, i);
+                }
         }
         if (mean)
 #pragma unroll
@@ -176,61 +207,67 @@ __global__ __launch_bounds__(256) void k_paged_attend(PagedArgs a) {
 }
 
 // -------------------------------------------------------------- select ---
-// A head's query in 8 bits, a wave to a head: code = rint(q 127 / max|q|) of
-// the real quotient, its rows padded with zeros to whole steps of 64; its
-// share of a score is weight max|q| / 127.  A head with a value that is not
-// finite has none.  c = rint(q (127 / max)) may miss by one next to a half;
-// q 127 - c max is exact in 64 bits and tells.
+// A head's query in 8 bits: code = rint(q 127 / max|q|) of the real quotient;
+// its share of a score is weight max|q| / 127.  A head with a value that is
+// not finite has none.  c = rint(q (127 / max)) may miss by one next to a
+// half; q 127 - c max is exact and tells: a bf16 query's numbers fit f32 (15
+// bits), a f32 one's take 64 bits.
 constexpr int kCodeStep = 64;
 __host__ __device__ inline int64_t code_row(int64_t D) { return (D + kCodeStep - 1) / kCodeStep * kCodeStep; }
-__device__ __forceinline__ int code8(double q, double top, double f) {
-    double c = rint(q * f);
-    const double e = 2.0 * __builtin_fma(-c, top, q * 127.0);
-    if (e > top || (e == top && ((int)c & 1))) c += 1.0;
-    if (e < -top || (e == -top && ((int)c & 1))) c -= 1.0;
-    return (int)c;
+__device__ __forceinline__ float exact_fma(float x, float y, float z) { return __builtin_fmaf(x, y, z); }
+__device__ __forceinline__ double exact_fma(double x, double y, double z) { return __builtin_fma(x, y, z); }
+template <class T> __device__ __forceinline__ int code8(T q, T top, T f) {
+    const T c = rint(q * f), e = exact_fma(c, -2 * top, q * 254);  // twice the rest
+    const int k = (int)c;
+    const bool next = e > top || -e > top || ((e == top || -e == top) && (k & 1));
+    return next ? (e > 0 ? k + 1 : k - 1) : k;
 }
+// The codes of head r (none from `end` on), by a wave: code_row(D) bytes,
+// zeros behind the D; its share.
 template <class F>
-__global__ __launch_bounds__(256) void k_select_codes(PagedArgs a, const float *__restrict__ weights,
-                                                      int64_t heads, int8_t *__restrict__ codes,
-                                                      double *__restrict__ share) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= heads) return;
-    const int lane = threadIdx.x & 63, D = a.L + a.P;
+__device__ __forceinline__ void head_codes(const PagedArgs &a, int64_t r, int64_t end, const float *weights,
+                                           int8_t *codes, double *share) {
+    const int lane = threadIdx.x & 63, D = a.L + a.P, Dp = (int)code_row(D);
     typedef typename F::q_t q_t;
+    typedef typename F::code_t T;
     typedef q_t q8 __attribute__((ext_vector_type(8)));
+    const bool any = r < end;
+    if (!any) r = end - 1;
     const q_t *qa = (const q_t *)a.qabs + r * a.L, *qr = (const q_t *)a.qrope + r * a.P;
-    // eight dims a lane and turn: D is at most 1024
-    q8 q[2];
-    uint32_t top = 0;  // |q|'s bits: NaN lies above infinity
+    auto at = [&](int d) { return (float)(d < a.L ? qa[d] : qr[d - a.L]); };
+    auto bits = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };  // NaN lies above infinity
+    // eight dims a lane, then (D is at most 1024) up to eight single ones
+    q8 q = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (8 * lane < D) q = *(const q8 *)(8 * lane < a.L ? qa + 8 * lane : qr + (8 * lane - a.L));
+    const float one = 512 + lane < D ? at(512 + lane) : 0.0f, weight = weights ? weights[r] : 1.0f;
+    uint32_t top = bits(one);
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const int d = 8 * (lane + 64 * t);
-        q[t] = q8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (d < D) q[t] = *(const q8 *)(d < a.L ? qa + d : qr + (d - a.L));
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t v = __float_as_uint((float)q[t][i]) & 0x7fffffffu;
-            top = v > top ? v : top;
-        }
+    for (int k = 0; k < 8; k++) {
+        const uint32_t v = bits((float)q[k]);
+        top = v > top ? v : top;
+    }
+#pragma unroll 1
+    for (int d = 576 + lane; d < D; d += 64) {
+        const uint32_t v = bits(at(d));
+        top = v > top ? v : top;
     }
     for (int off = 32; off >= 1; off >>= 1) {
         const uint32_t v = __shfl_xor(top, off, 64);
         top = v > top ? v : top;
     }
-    const bool live = top > 0 && top < 0x7f800000u;
-    const double m = (double)__uint_as_float(top), f = live ? 127.0 / m : 0.0;
-    const int64_t Dp = code_row(D);
+    const bool live = any && top > 0 && top < 0x7f800000u;
+    const float m = __uint_as_float(top);
+    // a power of two keeps the numbers within f32's normal range
+    const T up = m < 1e-30f ? (T)0x1p90f : m > 1e30f ? (T)0x1p-30f : (T)1, mt = (T)m * up, f = live ? (T)127 / mt : (T)0;
+    auto code = [&](float x) { return live ? code8<T>((T)x * up, mt, f) : 0; };
+    uint32_t c[2] = {0, 0};
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const int d = 8 * (lane + 64 * t);
-        uint32_t c[2] = {0, 0};
-        if (live)
-#pragma unroll
-            for (int i = 0; i < 8; i++) c[i >> 2] |= (uint32_t)(code8((double)(float)q[t][i], m, f) & 255) << (8 * (i & 3));
-        if (d < Dp) *(uint2 *)(codes + r * Dp + d) = make_uint2(c[0], c[1]);
-    }
-    if (lane == 0) share[r] = live ? (weights ? (double)weights[r] : 1.0) * (m / 127.0) : 0.0;
+    for (int k = 0; k < 8; k++) c[k >> 2] |= (uint32_t)(code((float)q[k]) & 255) << (8 * (k & 3));
+    if (8 * lane < Dp) *(uint2 *)(codes + 8 * lane) = make_uint2(c[0], c[1]);
+    if (512 + lane < Dp) codes[512 + lane] = (int8_t)code(one);
+#pragma unroll 1
+    for (int d = 576 + lane; d < Dp; d += 64) codes[d] = d < D ? (int8_t)code(at(d)) : 0;
+    if (lane == 0) *share = live ? (double)weight * ((double)m / 127.0) : 0.0;
 }
 
 // A score's order as an unsigned number; NaN below everything.
@@ -239,23 +276,55 @@ __device__ __forceinline__ uint64_t score_key(double s) {
     const uint64_t u = (uint64_t)__double_as_longlong(s + 0.0);  // -0 counts as 0
     return u >> 63 ? ~u : u | (1ull << 63);
 }
+template <int CTRL> __device__ __forceinline__ double dpp_double(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)u, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
 
-// score = (sum_h share_h max(0, code_h . mean)) mean_scale.  A workgroup takes
-// 32 pages of a row; its waves take every fourth tile of 16 heads, the
-// products v_mfma_i32_16x16x64_i8 (pages x heads, exact), the sums over heads
-// in 64 bits in an order that is the same for every page.  FULL: rows of
-// whole steps of 64.
-constexpr int kScorePages = 32;
+// score = (sum_h share_h max(0, code_h . mean)) mean_scale; the products are
+// v_mfma_i32_16x16x64_i8 (pages x heads, exact), the sums over heads run in 64
+// bits in an order that is the same for every page.  Two ways to the sums:
+//
+// many rows: a launch makes all codes; then a workgroup takes 32 pages of a
+// row, its waves every fourth tile of 16 heads, so that a page's mean is read
+// once for all heads;
+// few rows (and rows of nine whole steps of 64): one launch, a workgroup takes
+// 16 heads, whose codes its waves make first, and 256 pages or more, and
+// leaves its heads' part of each sum.
+// The one launch reads the means again for every 16 heads.  Whole calls over
+// 512 pages, 128 heads: one row 14.4 us (two launches 16.4), 8 rows 15.0
+// (16.5), 16 rows 15.3 (17.3), 48 rows 28.3 (26.2); 32 rows of 64 heads 16.5
+// (19.2).  So one launch up to as many tiles of 16 heads as CUs.
 typedef int si32x4 __attribute__((ext_vector_type(4)));
+// The sum over a row of 16 lanes, in all of them: lanes ^ 1, ^ 2, then each
+// eight and sixteen mirrored (a quad agrees by then).
+__device__ __forceinline__ double sum16(double v) {
+    v += dpp_double<0xB1>(v);   // quad_perm [1, 0, 3, 2]
+    v += dpp_double<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+    v += dpp_double<0x141>(v);  // row_half_mirror
+    v += dpp_double<0x140>(v);  // row_mirror
+    return v;
+}
+
+template <class F>
+__global__ __launch_bounds__(256) void k_select_codes(PagedArgs a, const float *__restrict__ weights, int64_t r0,
+                                                      int64_t heads, int8_t *__restrict__ codes,
+                                                      double *__restrict__ share) {
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i < heads) head_codes<F>(a, r0 + i, r0 + heads, weights, codes + i * code_row(a.L + a.P), share + i);
+}
+
+constexpr int kScorePages = 32;
 template <bool FULL>
 __global__ __launch_bounds__(256) void k_select_score(PagedArgs a, const int8_t *__restrict__ codes,
                                                       const double *__restrict__ share,
-                                                      const int8_t *__restrict__ mean,
-                                                      const float *__restrict__ mean_scale,
-                                                      uint64_t *__restrict__ keys) {
+                                                      const int8_t *__restrict__ mean, int row0,
+                                                      double *__restrict__ part) {
     constexpr int STEPS = FULL ? 9 : 16;  // at most 1024 dims
-    __shared__ double part[4][kScorePages];
-    const int row = blockIdx.y, b = row / a.M, j = row - b * a.M;
+    __shared__ double wave_part[4][kScorePages];
+    const int row = row0 + blockIdx.y, b = row / a.M, j = row - b * a.M;
     const int w = threadIdx.x >> 6, l = threadIdx.x & 63, g = l >> 4;
     const int D = a.L + a.P, Dp = (int)code_row(D), steps = Dp / kCodeStep;
     const int32_t n = paged_len(a, b) - a.M + j + 1;
@@ -279,57 +348,99 @@ __global__ __launch_bounds__(256) void k_select_score(PagedArgs a, const int8_t 
         }
     }
     double sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int h0 = 16 * w; h0 < a.H; h0 += 64) {
+    // the next tile of heads is loaded under this one's products
+    si32x4 B[STEPS];
+    double sh = 0.0;
+    auto load = [&](int h0) {
         const int h = h0 + (l & 15);
-        const int64_t r = (int64_t)row * a.H + (h < a.H ? h : a.H - 1);
-        const double sh = h < a.H ? share[r] : 0.0;
+        const int64_t r = (int64_t)blockIdx.y * a.H + (h < a.H ? h : a.H - 1);
+        sh = h < a.H ? share[r] : 0.0;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+            if (FULL || s < steps) B[s] = *(const si32x4 *)(codes + r * Dp + kCodeStep * s + 16 * g);
+    };
+    if (16 * w < a.H) load(16 * w);
+    for (int h0 = 16 * w; h0 < a.H; h0 += 64) {
         si32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        const double share_h = sh;
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
             if (FULL || s < steps) {
-                const si32x4 B = *(const si32x4 *)(codes + r * Dp + kCodeStep * s + 16 * g);
-                c[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[0][s], B, c[0], 0, 0, 0);
-                c[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[1][s], B, c[1], 0, 0, 0);
+                c[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[0][s], B[s], c[0], 0, 0, 0);
+                c[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[1][s], B[s], c[1], 0, 0, 0);
             }
+        if (h0 + 64 < a.H) load(h0 + 64);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int v = c[i >> 2][i & 3];
-            sum[i] += sh * (double)(v > 0 ? v : 0);
+            sum[i] += share_h * (double)(v > 0 ? v : 0);
         }
     }
-    // lane l holds pages 16 (i >> 2) + 4 g + (i & 3) for its head column
+    // lane l: pages 16 (i >> 2) + 4 g + (i & 3) for its head column
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        for (int off = 1; off < 16; off <<= 1) sum[i] += __shfl_xor(sum[i], off, 64);
+    for (int i = 0; i < 8; i++) sum[i] = sum16(sum[i]);
     if ((l & 15) == 0)
 #pragma unroll
-        for (int i = 0; i < 8; i++) part[w][16 * (i >> 2) + 4 * g + (i & 3)] = sum[i];
+        for (int i = 0; i < 8; i++) wave_part[w][16 * (i >> 2) + 4 * g + (i & 3)] = sum[i];
     __syncthreads();
-    const int k = k0 + threadIdx.x;
-    if (threadIdx.x < kScorePages && k < np) {
-        const double t = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
-        keys[(int64_t)row * a.max_pages + k] = score_key(t * (double)mean_scale[paged_phys(a, b, k)]);
-    }
+    const int t = threadIdx.x;
+    if (t < kScorePages && k0 + t < np)
+        part[(int64_t)blockIdx.y * a.max_pages + k0 + t] = (wave_part[0][t] + wave_part[1][t]) + (wave_part[2][t] + wave_part[3][t]);
+}
+
+constexpr int kFusedHeads = 16, kFusedThreads = 64 * kFusedHeads, kFusedPages = 16 * kFusedHeads;
+template <class F>
+__global__ __launch_bounds__(kFusedThreads) void k_select_fused(PagedArgs a, const float *__restrict__ weights,
+                                                                const int8_t *__restrict__ mean, int row0,
+                                                                double *__restrict__ part) {
+    constexpr int STEPS = 9, D = STEPS * kCodeStep;
+    __shared__ __attribute__((aligned(16))) int8_t codes[kFusedHeads][D + 16];  // 16 bytes more: other banks
+    __shared__ double share[kFusedHeads];
+    const int row = row0 + blockIdx.z, b = row / a.M, j = row - b * a.M, h0 = blockIdx.y * kFusedHeads;
+    const int w = threadIdx.x >> 6, l = threadIdx.x & 63, g = l >> 4;
+    const int32_t n = paged_len(a, b) - a.M + j + 1;
+    const int np = n > 0 ? ((n - 1) >> a.shift) + 1 : 0;
+    if ((int)blockIdx.x * kFusedPages >= np) return;
+    // a wave's 16 pages: their means come in while the codes are made
+    const int k0 = blockIdx.x * kFusedPages + 16 * w, k = k0 + (l & 15);
+    const int8_t *src = mean + (int64_t)paged_phys(a, b, k < np ? k : np - 1) * D;
+    si32x4 A[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) A[s] = *(const si32x4 *)(src + kCodeStep * s + 16 * g);
+    head_codes<F>(a, (int64_t)row * a.H + h0 + w, (int64_t)(row + 1) * a.H, weights, codes[w], &share[w]);
+    __syncthreads();
+    si32x4 c = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < STEPS; s++)
+        c = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[s], *(const si32x4 *)&codes[l & 15][kCodeStep * s + 16 * g], c, 0, 0, 0);
+    const double sh = share[l & 15];
+    double sum[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum[i] = sum16(sh * (double)(c[i] > 0 ? c[i] : 0));
+    const int i = l & 3;  // lane l: pages 4 g + i
+    const double mine = i == 0 ? sum[0] : i == 1 ? sum[1] : i == 2 ? sum[2] : sum[3];
+    if ((l & 15) < 4 && k0 + 4 * g + i < np)
+        part[((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * a.max_pages + k0 + 4 * g + i] = mine;
 }
 
 // The top_k pages of a row: the first keep_first, the last keep_last, then by
 // score, ties to the lower page; ascending, -1 behind them.  A workgroup per
-// row looks for the key of the last page to be taken: keys between the least
+// row adds the head groups' parts to the scores' keys and looks for the key of the last page to be taken: keys between the least
 // and the largest that are left fall into 256 bins by the first eight bits
 // in which those two differ; the bin that holds the one sought is looked
 // into further, until its keys are equal or at most 64, which one wave then
 // ranks.  One more pass writes the pages above that key and the first of
 // those equal to it.
 constexpr int kPickThreads = 512;
-__global__ __launch_bounds__(kPickThreads) void k_select_pick(PagedArgs a,
-                                                              const uint64_t *__restrict__ keys,
-                                                              int keep_first, int keep_last,
-                                                              int32_t *__restrict__ out) {
+__global__ __launch_bounds__(kPickThreads) void k_select_pick(PagedArgs a, const double *__restrict__ part,
+                                                              int tiles, const float *__restrict__ mean_scale,
+                                                              int row0, uint64_t *keys, int keep_first,
+                                                              int keep_last, int32_t *__restrict__ out) {
     constexpr int NW = kPickThreads / 64;
     __shared__ int hist[256], few_n, s_bin, s_above;
     __shared__ uint64_t ends[2][NW], few[64], s_key;
     __shared__ int scan[2][NW];
-    const int row = blockIdx.x, b = row / a.M, j = row - b * a.M, tid = threadIdx.x;
+    const int row = row0 + blockIdx.x, b = row / a.M, j = row - b * a.M, tid = threadIdx.x;
     const int lane = tid & 63, w = tid >> 6;
     const int32_t n = paged_len(a, b) - a.M + j + 1;
     const int np = n > 0 ? ((n - 1) >> a.shift) + 1 : 0;
@@ -338,7 +449,16 @@ __global__ __launch_bounds__(kPickThreads) void k_select_pick(PagedArgs a,
         for (int i = tid; i < a.top_k; i += kPickThreads) out[i] = i < np ? i : -1;
         return;
     }
-    keys += (int64_t)row * a.max_pages;
+    // thread tid makes and reads the keys of pages tid, tid + kPickThreads, ..
+    keys += (int64_t)blockIdx.x * a.max_pages;
+    part += (int64_t)blockIdx.x * tiles * a.max_pages;
+    for (int k = tid; k < np; k += kPickThreads) {
+        const float scale = mean_scale[paged_phys(a, b, k)];
+        double t = 0.0;
+#pragma unroll 8
+        for (int i = 0; i < tiles; i++) t += part[(int64_t)i * a.max_pages + k];
+        keys[k] = score_key(t * (double)scale);
+    }
     const int kept = keep_first + keep_last;  // of np > top_k >= kept pages
     auto scored = [&](int k) { return k >= keep_first && k < np - keep_last; };
     int need = a.top_k - kept;  // of the scored pages
@@ -653,35 +773,50 @@ extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const
     a.qabs = qabs_dev;
     a.qrope = q_rope_dev;
     a.top_k = (int32_t)top_k;
-    const int64_t R = batch * rows, D = a.L + a.P;
+    const int64_t R = batch * rows, D = a.L + a.P, tiles = (heads + kFusedHeads - 1) / kFusedHeads;
+    const bool fused = D == 9 * kCodeStep && R * tiles <= ctx->multiprocessors;
+    // slices of rows whose codes and parts take 64 MB at most
+    const int64_t parts = fused ? tiles : 1, row_bytes = parts * max_pages * 8 + (fused ? 0 : heads * code_row(D));
+    int64_t slice = (int64_t(64) << 20) / row_bytes;
+    slice = slice < 1 ? 1 : slice < R ? slice : R;
     ScratchPlan plan;
-    plan.add((size_t)(R * heads * code_row(D)));
-    plan.add((size_t)(R * heads) * 8);
-    plan.add((size_t)(R * max_pages) * 8);
+    plan.add((size_t)(slice * parts * max_pages) * 8);
+    plan.add((size_t)(slice * max_pages) * 8);
+    plan.add(fused ? 0 : (size_t)(slice * heads * code_row(D)));
+    plan.add(fused ? 0 : (size_t)(slice * heads) * 8);
     std::vector<void *> ptrs;
     UT_TRY(scratch_acquire(ctx, plan, ptrs));
-    int8_t *codes = (int8_t *)ptrs[0];
-    double *share = (double *)ptrs[1];
-    uint64_t *keys = (uint64_t *)ptrs[2];
-    int tok = timing_begin(ctx, "select_codes");
-    const dim3 four((unsigned)((R * heads + 3) / 4));
-    if (kv->fmt == UT_KV_BF16)
-        hipLaunchKernelGGL(k_select_codes<Bf16>, four, dim3(256), 0, ctx->stream, a, weights_dev, R * heads, codes, share);
-    else
-        hipLaunchKernelGGL(k_select_codes<F16x2>, four, dim3(256), 0, ctx->stream, a, weights_dev, R * heads, codes, share);
-    timing_end(ctx, tok);
-    UT_TRY(launch_check(ctx, "k_select_codes"));
-    tok = timing_begin(ctx, "select_score");
-    const dim3 grid((unsigned)((max_pages + kScorePages - 1) / kScorePages), (unsigned)R);
-    if (D == 9 * kCodeStep)
-        hipLaunchKernelGGL(k_select_score<true>, grid, dim3(256), 0, ctx->stream, a, codes, share, kv->mean, kv->mean_scale, keys);
-    else
-        hipLaunchKernelGGL(k_select_score<false>, grid, dim3(256), 0, ctx->stream, a, codes, share, kv->mean, kv->mean_scale, keys);
-    timing_end(ctx, tok);
-    UT_TRY(launch_check(ctx, "k_select_score"));
-    tok = timing_begin(ctx, "select_pick");
-    hipLaunchKernelGGL(k_select_pick, dim3((unsigned)R), dim3(kPickThreads), 0, ctx->stream, a, keys,
-                       (int)keep_first, (int)keep_last, sel_dev);
-    timing_end(ctx, tok);
-    return launch_check(ctx, "k_select_pick");
+    double *part = (double *)ptrs[0], *share = (double *)ptrs[3];
+    uint64_t *keys = (uint64_t *)ptrs[1];
+    int8_t *codes = (int8_t *)ptrs[2];
+    const bool bf16 = kv->fmt == UT_KV_BF16;
+    for (int64_t r0 = 0; r0 < R; r0 += slice) {
+        const int64_t n = R - r0 < slice ? R - r0 : slice;
+        if (fused) {
+            int tok = timing_begin(ctx, "select_fused");
+            hipLaunchKernelGGL((bf16 ? k_select_fused<Bf16> : k_select_fused<F16x2>),
+                               dim3((unsigned)((max_pages + kFusedPages - 1) / kFusedPages), (unsigned)tiles, (unsigned)n),
+                               dim3(kFusedThreads), 0, ctx->stream, a, weights_dev, kv->mean, (int)r0, part);
+            timing_end(ctx, tok);
+            UT_TRY(launch_check(ctx, "k_select_fused"));
+        } else {
+            int tok = timing_begin(ctx, "select_codes");
+            hipLaunchKernelGGL((bf16 ? k_select_codes<Bf16> : k_select_codes<F16x2>), dim3((unsigned)((n * heads + 3) / 4)),
+                               dim3(256), 0, ctx->stream, a, weights_dev, r0 * heads, n * heads, codes, share);
+            timing_end(ctx, tok);
+            UT_TRY(launch_check(ctx, "k_select_codes"));
+            tok = timing_begin(ctx, "select_score");
+            hipLaunchKernelGGL((D == 9 * kCodeStep ? k_select_score<true> : k_select_score<false>),
+                               dim3((unsigned)((max_pages + kScorePages - 1) / kScorePages), (unsigned)n), dim3(256), 0,
+                               ctx->stream, a, codes, share, kv->mean, (int)r0, part);
+            timing_end(ctx, tok);
+            UT_TRY(launch_check(ctx, "k_select_score"));
+        }
+        int tok = timing_begin(ctx, "select_pick");
+        hipLaunchKernelGGL(k_select_pick, dim3((unsigned)n), dim3(kPickThreads), 0, ctx->stream, a, part, (int)parts,
+                           kv->mean_scale, (int)r0, keys, (int)keep_first, (int)keep_last, sel_dev);
+        timing_end(ctx, tok);
+        UT_TRY(launch_check(ctx, "k_select_pick"));
+    }
+    return UT_OK;
 }

@@ -13,7 +13,6 @@ typedef _Float16 pf16x8 __attribute__((ext_vector_type(8)));
 typedef float pf32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t pu32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
-typedef const __attribute__((address_space(4))) int32_t const_i32;
 
 constexpr int kPT = 32;             // positions per tile
 constexpr int kPL = 512, kPD = 576;

@@ -549,6 +549,7 @@ class PagedCache:
             self._tensor("mean_scale", mean_scale, torch.float32, (n,))
         self._kv = MlaPages(_ptr(pages), _ptr(mean), _ptr(mean_scale), n, self.page, latent, rope,
                             self.fmt)
+        self._ref = C.byref(self._kv)
 
     @classmethod
     def empty(cls, ctx: Context, n_pages: int, page: int = 64, latent: int = 512, rope: int = 64,
@@ -563,25 +564,27 @@ class PagedCache:
         return cls(ctx, pages, latent, rope, torch.zeros((n_pages, D), dtype=torch.int8, device=d),
                    torch.zeros(n_pages, device=d))
 
-    def _tensor(self, name: str, t, dtype, shape) -> Optional[int]:
-        if tuple(t.shape) != tuple(shape):
+    def _tensor(self, name: str, t, dtype, shape) -> int:
+        if t.shape != shape:
             raise ShapeError(UT_ERR_SHAPE, f"PagedCache: {name} must be {list(shape)}, got {list(t.shape)}")
-        if t.dtype != dtype or not t.is_contiguous() or not t.is_cuda or t.device.index != self.ctx.device:
+        if t.dtype != dtype or not t.is_contiguous() or t.get_device() != self.ctx.device:
             raise UtError(UT_ERR_ARG, f"PagedCache: {name} must be a contiguous {dtype} tensor on "
                                       f"cuda:{self.ctx.device}")
         return t.data_ptr()
 
     def _batch(self, table, lens, rows: int):
         torch = _torch()
-        if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
+        if table.dim() != 2 or 0 in table.shape:
             raise ShapeError(UT_ERR_SHAPE, f"PagedCache: table must be [B, max_pages], got {list(table.shape)}")
         B, n = table.shape
-        stride = table.stride(0) if B > 1 else max(n, table.stride(0))
-        if (table.dtype != torch.int32 or not table.is_cuda or table.device.index != self.ctx.device
-                or (n > 1 and table.stride(1) != 1) or stride < n):
+        stride, step = table.stride()
+        if B == 1 and stride < n:
+            stride = n
+        if (table.dtype != torch.int32 or table.get_device() != self.ctx.device or stride < n
+                or (step != 1 and n > 1)):
             raise UtError(UT_ERR_ARG, f"PagedCache: table must be int32 rows of adjacent entries on "
                                       f"cuda:{self.ctx.device}")
-        return (self.ctx.handle, C.byref(self._kv), table.data_ptr(), stride, n,
+        return (self.ctx.handle, self._ref, table.data_ptr(), stride, n,
                 self._tensor("lens", lens, torch.int32, (B,)), B, rows)
 
     def _queries(self, table, lens, qabs, q_rope):
