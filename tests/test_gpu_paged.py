@@ -93,6 +93,15 @@ def test_attend_long(ctx, fmt, lens, M, H):
     attend_case(ctx, fmt, lens, M, H, 512, 64, 64)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("lens,M,H,L,P,page", [
+    ([5000], 1, 4, 64, 16, 16), ([3000, 1, 777, 0], 2, 5, 128, 32, 4), ([2500, 64], 1, 6, 136, 8, 64),
+    ([900] * 130, 1, 6, 72, 8, 32), ([65, 3, 200] * 200, 1, 5, 64, 16, 8), ([700, 130], 3, 7, 768, 256, 128)])
+def test_attend_other_widths_long(ctx, fmt, lens, M, H, L, P, page):
+    """Slices of a row joined, slices that are left empty, and none at all."""
+    attend_case(ctx, fmt, lens, M, H, L, P, page)
+
+
 @pytest.mark.parametrize("H", [16, 64, 128])
 def test_attend_many_sequences(ctx, H):
     """More sequences than workgroups look up at once, most of them short."""
@@ -435,7 +444,7 @@ def test_refusals(ctx):
     for k in (dict(B=70000), dict(M=2**31), dict(width=2**30, stride=2**30)):
         assert all(c == shape for c in calls(kv(), **k)), k
     assert list(calls(kv(), H=0))[:3] == [arg] * 3 and list(calls(kv(), H=70000))[:3] == [shape] * 3
-    assert list(calls(kv(), M=40000))[:3] == [shape] * 3
+    assert list(calls(kv(), M=40000))[:3] == [shape] * 3 and list(calls(kv(), M=40000, H=1))[:3] == [shape] * 3
     b = batch(kv())
     assert lib.ut_mla_sparse_attend(*b, 16, p, p, 0.1, None, 2, p) == arg
     assert lib.ut_mla_sparse_attend(*b, 16, p, p, 0.1, p, 0, p) == arg
@@ -448,7 +457,8 @@ def test_refusals(ctx):
 
 
 # ------------------------------------------------- streams, graphs, runs
-def test_captured_steps_follow_lengths(ctx):
+@pytest.mark.parametrize("H,L,P", [(128, 512, 64), (4, 64, 16)])
+def test_captured_steps_follow_lengths(ctx, H, L, P):
     """One step captured (append, select, attention over the selection and
     over everything), replayed as the lengths grow and a page is added, with
     eager calls of other sizes between: every replay gives the eager call's
@@ -459,13 +469,13 @@ def test_captured_steps_follow_lengths(ctx):
         c = U.Context(0)
         g = torch.Generator(device="cuda").manual_seed(3)
         rnd = lambda *d: torch.randn(d, device="cuda", generator=g)
-        B, M, H = 3, 2, 128
-        cache = U.PagedCache.empty(c, 60, page=16)
+        B, M = 3, 2
+        cache = U.PagedCache.empty(c, 60, page=16, latent=L, rope=P)
         table = torch.arange(60, dtype=torch.int32, device="cuda").reshape(3, 20)
         lens = torch.tensor([150, 17, 31], dtype=torch.int32, device="cuda")
-        cache.append(table, lens, rnd(B, 150, 512), rnd(B, 150, 64))
-        lat, kr = rnd(B, M, 512), rnd(B, M, 64)
-        q = rnd(B, M, H, 512).bfloat16(), rnd(B, M, H, 64).bfloat16()
+        cache.append(table, lens, rnd(B, 150, L), rnd(B, 150, P))
+        lat, kr = rnd(B, M, L), rnd(B, M, P)
+        q = rnd(B, M, H, L).bfloat16(), rnd(B, M, H, P).bfloat16()
 
         def step():
             cache.append(table, lens, lat, kr)
@@ -480,7 +490,7 @@ def test_captured_steps_follow_lengths(ctx):
             got = step()
         for k in range(4):
             lens += M
-            lat.copy_(rnd(B, M, 512))
+            lat.copy_(rnd(B, M, L))
             for t in got:
                 t.zero_()
             graph.replay()
@@ -490,9 +500,9 @@ def test_captured_steps_follow_lengths(ctx):
             want = step()  # writes the same rows again
             assert all(torch.equal(a, b) for a, b in zip(first, want))
             assert torch.equal(pages, cache.pages)
-            big = rnd(64, 1, H, 512).bfloat16()  # grows the arena past what the graph took
+            big = rnd(64, 1, H, L).bfloat16()  # grows the arena past what the graph took
             cache.attend(table[:1].expand(64, 20).contiguous(), lens[:1].expand(64).contiguous(), big,
-                         rnd(64, 1, H, 64).bfloat16(), SCALE)
+                         rnd(64, 1, H, P).bfloat16(), SCALE)
             c.synchronize()
 
 

@@ -137,73 +137,206 @@ __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__r
 }
 
 // ----------------------------------------------------------- attention ---
-// Any latent width: a workgroup takes one head of one row and goes over its
-// positions 64 at a time, four lanes to a position, with the running maximum
-// and sum of the softmax.  Only visible positions are read.
-constexpr int kGenChunk = 64;
+// Any latent width and page, in f32: a workgroup takes four heads of one row
+// and a slice of its positions, 64 at a time.  Scores: four lanes to a
+// position, which is read once for the four heads; then a wave to a head for
+// the maximum and the weights (one exponential each); context: a lane to a
+// dim, or 2 or 4 of them with part of the positions each where the latent has
+// at most 128 or 64 (with one, 3 lanes of 4 would idle at 64).  Only visible
+// positions are read.
+//
+// The chains of dependent loads bound it, not bytes: so a row is cut into
+// slices until four workgroups a CU run, and k_paged_generic_join joins them.
+// 1 row of 4 heads over 1459 positions of 64 + 16 takes 22 us a call, and
+// 337 with a whole row to a workgroup; 50 x 4 such rows in f16x2 48 and 431.
+constexpr int kGenChunk = 64, kGenHeads = 4, kGenSlices = 32;
+constexpr float kGenLow = -3.402823466e38f;  // the maximum before any score
+
+// Virtual positions of a row and how they are cut.
+struct GenCut {
+    int64_t total;
+    int32_t chunks, per;  // chunks of a slice
+};
+__device__ __forceinline__ GenCut gen_cut(const PagedArgs &a, int32_t n, int slices) {
+    GenCut c;
+    c.total = n <= 0 ? 0 : a.sel ? (int64_t)a.top_k << a.shift : n;
+    c.chunks = (int32_t)((c.total + kGenChunk - 1) / kGenChunk);
+    c.per = (c.chunks + slices - 1) / slices;
+    return c;
+}
+
+// part_ml [row][head][slice][2], part_o [row][head][slice][L]
 template <class F>
-__global__ __launch_bounds__(256) void k_paged_attend(PagedArgs a) {
+__global__ __launch_bounds__(256) void k_paged_generic(PagedArgs a, int slices, float *__restrict__ part_ml,
+                                                       float *__restrict__ part_o) {
     extern __shared__ float sm[];
-    const int h = blockIdx.x, j = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-    const int D = a.L + a.P;
-    float *q = sm, *o = q + D, *p = o + a.L;  // [D], [L], [kGenChunk]
+    constexpr int HG = kGenHeads;
+    const int h0 = blockIdx.x * HG, j = blockIdx.y / slices, sl = blockIdx.y - j * slices, b = blockIdx.z;
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, D = a.L + a.P;
+    float *q = sm;                                     // [HG][D], then the lanes' contexts
+    __shared__ alignas(16) float p[kGenChunk][HG];
+    __shared__ float s_m[HG], s_f[HG];
     __shared__ int64_t at[kGenChunk];
-    const int64_t r = ((int64_t)b * a.M + j) * a.H + h;
+    const int64_t r = (int64_t)b * a.M + j;
     const int32_t n = paged_len(a, b) - a.M + j + 1;
-    for (int d = tid; d < D; d += 256)
-        q[d] = d < a.L ? (float)((const typename F::q_t *)a.qabs)[r * a.L + d]
-                       : (float)((const typename F::q_t *)a.qrope)[r * a.P + (d - a.L)];
-    for (int d = tid; d < a.L; d += 256) o[d] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    const int64_t total = a.sel ? (int64_t)a.top_k << a.shift : (int64_t)(n > 0 ? n : 0);
+    const GenCut cut = gen_cut(a, n, slices);
+    const int32_t c0 = sl * cut.per, c1 = c0 + cut.per < cut.chunks ? c0 + cut.per : cut.chunks;
+    if (sl > 0 && c0 >= c1) return;  // slice 0 writes a row without positions
+    for (int i = tid; i < HG * D; i += 256) {
+        const int h = h0 + i / D < a.H ? h0 + i / D : a.H - 1, d = i % D;
+        q[i] = d < a.L ? (float)((const typename F::q_t *)a.qabs)[(r * a.H + h) * a.L + d]
+                       : (float)((const typename F::q_t *)a.qrope)[(r * a.H + h) * a.P + (d - a.L)];
+    }
+    // lanes of a dim: `ways`, over positions way, way + ways, ..
+    const int ways = a.L <= 64 ? 4 : a.L <= 128 ? 2 : 1, width = 256 / ways, way = tid / width, d0 = tid - way * width;
+    float o[HG][4];
+#pragma unroll
+    for (int h = 0; h < HG; h++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[h][i] = 0.0f;
+    float m = kGenLow, l = 0.0f;  // wave w: of head w
     const int64_t row16 = (int64_t)D * F::kPlanes;
-    for (int64_t t0 = 0; t0 < total; t0 += kGenChunk) {
-        __syncthreads();
+    for (int32_t c = c0; c < c1; c++) {
         if (tid < kGenChunk) {
-            const int64_t t = t0 + tid;
+            const int64_t t = (int64_t)c * kGenChunk + tid;
             int64_t row = -1;
-            if (t < total) {
+            if (t < cut.total) {
                 int64_t k = t >> a.shift;
-                if (a.sel) k = a.sel[((int64_t)b * a.M + j) * a.top_k + k];
-                const int64_t pos = (k << a.shift) + (t & ((1 << a.shift) - 1));
-                if (k >= 0 && pos < n)
-                    row = ((int64_t)paged_phys(a, b, (int)k) << a.shift) + (t & ((1 << a.shift) - 1));
+                if (a.sel) k = a.sel[r * a.top_k + k];
+                const int64_t in = t & ((1 << a.shift) - 1);
+                if (k >= 0 && (k << a.shift) + in < n) row = ((int64_t)paged_phys(a, b, (int)k) << a.shift) + in;
             }
             at[tid] = row;
         }
         __syncthreads();
-        const int t = tid >> 2, s = tid & 3;
-        float acc = 0.0f;
-        const int64_t row = at[t];
-        if (row >= 0) {
-            const uint16_t *src = (const uint16_t *)a.pages + row * row16;
-            for (int d = s; d < D; d += 4) acc = __builtin_fmaf(q[d], F::value(src, D, d), acc);
+        {
+            const int t = tid >> 2, s = tid & 3;
+            float acc[HG] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (at[t] >= 0) {
+                const uint16_t *src = (const uint16_t *)a.pages + at[t] * row16;
+#pragma unroll 4
+                for (int d = 4 * s; d < D; d += 16) {
+                    uint2 v[F::kPlanes];
+#pragma unroll
+                    for (int i = 0; i < F::kPlanes; i++) v[i] = *(const uint2 *)(src + i * D + d);
+#pragma unroll
+                    for (int h = 0; h < HG; h++) {
+                        const float4 x = *(const float4 *)(q + h * D + d);
+                        acc[h] = __builtin_fmaf(x.x, F::stored(v, 0), acc[h]);
+                        acc[h] = __builtin_fmaf(x.y, F::stored(v, 1), acc[h]);
+                        acc[h] = __builtin_fmaf(x.z, F::stored(v, 2), acc[h]);
+                        acc[h] = __builtin_fmaf(x.w, F::stored(v, 3), acc[h]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < HG; h++) {
+                acc[h] += __shfl_xor(acc[h], 1, 64);
+                acc[h] += __shfl_xor(acc[h], 2, 64);
+            }
+            p[t][s] = s == 0 ? acc[0] : s == 1 ? acc[1] : s == 2 ? acc[2] : acc[3];
         }
-        acc += __shfl_xor(acc, 1, 64);
-        acc += __shfl_xor(acc, 2, 64);
-        if (s == 0) p[t] = row >= 0 ? __fmul_rn(acc, a.scale) : -INFINITY;
         __syncthreads();
-        // NaN scores reach the output: a maximum that skips them, then e^NaN
-        float mn = m;
-        for (int i = 0; i < kGenChunk; i++) mn = fmaxf(mn, p[i]);
-        const float base = mn > -INFINITY ? mn : 0.0f, f = m > -INFINITY ? expf(m - base) : 0.0f;
-        float ls = 0.0f;
-        for (int i = 0; i < kGenChunk; i++)
-            if (at[i] >= 0) ls += expf(p[i] - base);
-        l = l * f + ls;
-        m = mn;
-        for (int d = tid; d < a.L; d += 256) {
-            float v = o[d] * f;
-            for (int i = 0; i < kGenChunk; i++)
-                if (at[i] >= 0)
-                    v = __builtin_fmaf(expf(p[i] - base),
-                                       F::value((const uint16_t *)a.pages + at[i] * row16, D, d), v);
-            o[d] = v;
+        {
+            // a maximum that skips NaN; the weight of a NaN score is NaN
+            const bool live = at[lane] >= 0;
+            const float v = live ? __fmul_rn(p[lane][w], a.scale) : -INFINITY;
+            float top = v;
+            for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+            const float mn = fmaxf(m, top), f = expf(m - mn), e = live ? expf(v - mn) : 0.0f;
+            float sum = e;
+            for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+            l = l * f + sum;
+            m = mn;
+            p[lane][w] = e;
+            if (lane == 0) s_f[w] = f;
         }
+        __syncthreads();
+        float f[HG];
+#pragma unroll
+        for (int h = 0; h < HG; h++) f[h] = s_f[h];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = d0 + width * i;
+            if (d >= a.L) break;
+            float x[HG];
+#pragma unroll
+            for (int h = 0; h < HG; h++) x[h] = o[h][i] * f[h];
+#pragma unroll 8
+            for (int t = way; t < kGenChunk; t += ways)
+                if (at[t] >= 0) {
+                    const float v = F::value((const uint16_t *)a.pages + at[t] * row16, D, d);
+                    const float4 e = *(const float4 *)p[t];
+                    x[0] = __builtin_fmaf(e.x, v, x[0]);
+                    x[1] = __builtin_fmaf(e.y, v, x[1]);
+                    x[2] = __builtin_fmaf(e.z, v, x[2]);
+                    x[3] = __builtin_fmaf(e.w, v, x[3]);
+                }
+#pragma unroll
+            for (int h = 0; h < HG; h++) o[h][i] = x[h];
+        }
+        __syncthreads();
+    }
+    if (lane == 0) {
+        s_m[w] = m;
+        s_f[w] = l;
+    }
+    if (ways > 1) {  // the lanes of a dim: one dim each (i = 0)
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < HG; h++) sm[h * 256 + tid] = o[h][0];
+        __syncthreads();
+        if (way == 0)
+#pragma unroll
+            for (int h = 0; h < HG; h++)
+                for (int y = 1; y < ways; y++) o[h][0] += sm[h * 256 + y * width + d0];
     }
     __syncthreads();
-    for (int d = tid; d < a.L; d += 256)
-        ((typename F::q_t *)a.out)[r * a.L + d] = (typename F::q_t)(l != 0.0f ? o[d] / l : 0.0f);
+#pragma unroll
+    for (int h = 0; h < HG; h++) {
+        if (h0 + h >= a.H) break;
+        const int64_t rh = r * a.H + h0 + h;
+        const float sum = s_f[h], inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+        if (slices > 1 && tid == 0) {
+            part_ml[(rh * slices + sl) * 2] = s_m[h];
+            part_ml[(rh * slices + sl) * 2 + 1] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = d0 + width * i;
+            if (way > 0 || d >= a.L) break;
+            if (slices > 1) part_o[(rh * slices + sl) * a.L + d] = o[h][i];
+            else ((typename F::q_t *)a.out)[rh * a.L + d] = (typename F::q_t)(o[h][i] * inv);
+        }
+    }
+}
+
+// out = sum_s o_s e^(m_s - M) / sum_s l_s e^(m_s - M) over a row's slices.
+template <class F>
+__global__ __launch_bounds__(256) void k_paged_generic_join(PagedArgs a, int slices, const float *__restrict__ part_ml,
+                                                            const float *__restrict__ part_o) {
+    const int64_t rh = blockIdx.x;
+    const int row = (int)(rh / a.H), b = row / a.M;
+    const GenCut cut = gen_cut(a, paged_len(a, b) - a.M + (row - b * a.M) + 1, slices);
+    const int used = cut.chunks > 0 ? (cut.chunks + cut.per - 1) / cut.per : 1;
+    float M = kGenLow, sum = 0.0f, w[kGenSlices];
+#pragma unroll
+    for (int s = 0; s < kGenSlices; s++)
+        if (s < used) M = fmaxf(M, part_ml[(rh * slices + s) * 2]);
+#pragma unroll
+    for (int s = 0; s < kGenSlices; s++)
+        if (s < used) {
+            w[s] = expf(part_ml[(rh * slices + s) * 2] - M);
+            sum = __builtin_fmaf(part_ml[(rh * slices + s) * 2 + 1], w[s], sum);
+        }
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+    for (int d = threadIdx.x; d < a.L; d += 256) {
+        float v = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kGenSlices; s++)
+            if (s < used) v = __builtin_fmaf(part_o[(rh * slices + s) * a.L + d], w[s], v);
+        ((typename F::q_t *)a.out)[rh * a.L + d] = (typename F::q_t)(v * inv);
+    }
 }
 
 // -------------------------------------------------------------- select ---
@@ -606,9 +739,11 @@ struct DeviceScope {
     }
 };
 
+constexpr int64_t kMostRows = 65535;  // query rows of a call
 static int32_t paged_args(ut_ctx *ctx, const char *what, const ut_mla_pages *kv,
                           const int32_t *table, int64_t stride, int64_t max_pages,
-                          const int32_t *lens, int64_t B, int64_t M, int64_t H, PagedArgs &a) {
+                          const int32_t *lens, int64_t B, int64_t M, int64_t H, int64_t most_rows,
+                          PagedArgs &a) {
     auto bad = [&](const char *why) {
         set_error(ctx, "%s: %s", what, why);
         return UT_ERR_ARG;
@@ -631,7 +766,7 @@ static int32_t paged_args(ut_ctx *ctx, const char *what, const ut_mla_pages *kv,
         return shape("latent and rope must be multiples of 8 that add up to at most 1024");
     if (kv->n_pages > INT32_MAX / page || max_pages > INT32_MAX / page)
         return shape("a pool and a sequence hold fewer than 2^31 positions");
-    if (B > 65535 || H > 65535 || M > INT32_MAX / B / H || (H > 1 && B * M > 65535))
+    if (B > 65535 || H > 65535 || M > INT32_MAX / B / H || B * M > most_rows)
         return shape("too many sequences, rows or heads");
     a = PagedArgs{};
     a.pages = kv->pages;
@@ -652,13 +787,37 @@ static int32_t paged_args(ut_ctx *ctx, const char *what, const ut_mla_pages *kv,
 }
 
 static int32_t launch_paged_generic(ut_ctx *ctx, const PagedArgs &a, int32_t fmt) {
-    const size_t lds = (size_t)(2 * a.L + a.P + kGenChunk) * 4;
-    const dim3 grid((unsigned)a.H, (unsigned)a.M, (unsigned)a.B);
-    int tok = timing_begin(ctx, "paged_attend");
-    if (fmt == UT_KV_BF16) hipLaunchKernelGGL(k_paged_attend<Bf16>, grid, dim3(256), lds, ctx->stream, a);
-    else hipLaunchKernelGGL(k_paged_attend<F16x2>, grid, dim3(256), lds, ctx->stream, a);
+    // slices: four workgroups a CU, partial results of 64 MB at most
+    const int64_t groups = (a.H + kGenHeads - 1) / kGenHeads, R = (int64_t)a.B * a.M;
+    const int64_t cap = (int64_t)(a.sel ? a.top_k : a.max_pages) << a.shift;
+    int64_t slices = 4 * ctx->multiprocessors / (R * groups);
+    const int64_t room = (int64_t(64) << 20) / (R * a.H * a.L * 4), chunks = (cap + kGenChunk - 1) / kGenChunk;
+    slices = slices < room ? slices : room;
+    slices = slices < chunks ? slices : chunks;
+    slices = slices < 1 ? 1 : slices < kGenSlices ? slices : kGenSlices;
+    float *ml = nullptr, *po = nullptr;
+    if (slices > 1) {
+        ScratchPlan plan;
+        plan.add((size_t)(R * a.H * slices) * 8);
+        plan.add((size_t)(R * a.H * slices * a.L) * 4);
+        std::vector<void *> ptrs;
+        UT_TRY(scratch_acquire(ctx, plan, ptrs));
+        ml = (float *)ptrs[0];
+        po = (float *)ptrs[1];
+    }
+    const size_t lds = (size_t)kGenHeads * (a.L + a.P < 256 ? 256 : a.L + a.P) * 4;
+    int tok = timing_begin(ctx, "paged_generic");
+    hipLaunchKernelGGL((fmt == UT_KV_BF16 ? k_paged_generic<Bf16> : k_paged_generic<F16x2>),
+                       dim3((unsigned)groups, (unsigned)(a.M * slices), (unsigned)a.B), dim3(256), lds, ctx->stream, a,
+                       (int)slices, ml, po);
     timing_end(ctx, tok);
-    return launch_check(ctx, "k_paged_attend");
+    UT_TRY(launch_check(ctx, "k_paged_generic"));
+    if (slices == 1) return UT_OK;
+    tok = timing_begin(ctx, "paged_generic_join");
+    hipLaunchKernelGGL((fmt == UT_KV_BF16 ? k_paged_generic_join<Bf16> : k_paged_generic_join<F16x2>),
+                       dim3((unsigned)(R * a.H)), dim3(256), 0, ctx->stream, a, (int)slices, ml, po);
+    timing_end(ctx, tok);
+    return launch_check(ctx, "k_paged_generic_join");
 }
 
 static int32_t paged_attend(ut_ctx *ctx, const char *what, const ut_mla_pages *kv,
@@ -668,7 +827,7 @@ static int32_t paged_attend(ut_ctx *ctx, const char *what, const ut_mla_pages *k
                             void *out) {
     DeviceScope dev(ctx->device);
     PagedArgs a;
-    UT_TRY(paged_args(ctx, what, kv, table, stride, max_pages, lens, B, M, H, a));
+    UT_TRY(paged_args(ctx, what, kv, table, stride, max_pages, lens, B, M, H, kMostRows, a));
     if (!qabs || !qrope || !out || ((uintptr_t)qabs & 15) != 0 || ((uintptr_t)qrope & 15) != 0 ||
         ((uintptr_t)out & 15) != 0) {
         set_error(ctx, "%s: queries and output must be 16-byte aligned device memory", what);
@@ -697,7 +856,7 @@ extern "C" int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv,
     DeviceScope dev(ctx->device);
     PagedArgs a;
     UT_TRY(paged_args(ctx, "ut_mla_paged_append", kv, table_dev, table_stride, max_pages, lens_dev,
-                      batch, rows, 1, a));
+                      batch, rows, 1, INT32_MAX, a));
     if (!latent_dev || !krot_dev || ((uintptr_t)latent_dev & 15) != 0 ||
         ((uintptr_t)krot_dev & 15) != 0 || !kv->mean != !kv->mean_scale) {
         set_error(ctx, "ut_mla_paged_append: rows must be 16-byte aligned device memory, and mean "
@@ -756,7 +915,7 @@ extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const
     DeviceScope dev(ctx->device);
     PagedArgs a;
     UT_TRY(paged_args(ctx, "ut_mla_page_select", kv, table_dev, table_stride, max_pages, lens_dev,
-                      batch, rows, heads, a));
+                      batch, rows, heads, kMostRows, a));
     if (!qabs_dev || !q_rope_dev || !sel_dev || !kv->mean || !kv->mean_scale ||
         ((uintptr_t)qabs_dev & 15) != 0 || ((uintptr_t)q_rope_dev & 15) != 0 ||
         ((uintptr_t)kv->mean & 15) != 0) {
