@@ -310,13 +310,15 @@ int32_t ut_mla_attend_split(ut_ctx *ctx, const float *qabs_dev, const float *q_r
  * included.  Row j of a sequence stands at position lens - rows + j and sees
  * the positions up to its own: lens - rows + j + 1 of them.  Where that is not
  * positive (a batch padded with lens 0, fewer new rows than `rows`, aligned
- * to the end) the row has no position and sees nothing.  Sequences may share pages; entries behind a
- * sequence's last page are not read.  Lengths and tables stay on the device
- * and may change between replays of a captured call.  A length that is
+ * to the end) the row has no position and sees nothing.  Sequences may share
+ * pages; entries behind a sequence's last page are not read.  Lengths and
+ * tables stay on the device and may change between replays of a captured call.  A length that is
  * negative or beyond its table is cut, a page id outside the pool reads page
  * 0 (an append writes nothing there), and the next ut_ctx_synchronize returns
  * UT_ERR_BAD_PAGE; the values of that sequence are then unspecified.  At most
- * 65535 sequences, and rows in all for the calls with queries.
+ * 65535 sequences, and rows in all for the calls with queries; a sequence (and
+ * what a row selects) spans at most 2^31 - 1024 positions, a pool fewer than
+ * 2^31.  What a call writes must not overlap what it reads.
  * All calls run on the context's device and stream; those that need working
  * memory take the context's arena. */
 enum { UT_KV_BF16 = 0, UT_KV_F16X2 = 1 };
@@ -331,7 +333,8 @@ typedef struct {
 /* Writes the rows latent [batch, rows, latent] and krot [batch, rows, rope]
  * (f32) to their positions, and the summary of every page they fall into
  * anew from its stored positions below lens.  A position before the cache's
- * start is not written.  Two rows must not fall on one place of the pool. */
+ * start is not written.  A page that new rows fall into must not stand in the
+ * call's table twice, by two sequences or in one. */
 int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
                             int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
                             int64_t batch, int64_t rows, const float *latent_dev,

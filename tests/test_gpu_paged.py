@@ -88,7 +88,8 @@ def test_attend_other_widths(ctx, fmt, lens, M, H, L, P, page):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("lens,M,H", [([9001], 1, 128), ([5000, 17, 3000], 2, 128), ([6001] * 5, 1, 16),
-                                      ([4000, 0, 2000, 1], 1, 64), ([12000], 4, 32)])
+                                      ([4000, 0, 2000, 1], 1, 64), ([12000], 4, 32), ([140, 200], 140, 128),
+                                      ([1000, 64, 30], 64, 16)])
 def test_attend_long(ctx, fmt, lens, M, H):
     attend_case(ctx, fmt, lens, M, H, 512, 64, 64)
 
@@ -194,7 +195,7 @@ def test_a_pool_past_32_bits(ctx):
 @pytest.mark.parametrize("lens,M,H,page,top_k", [
     ([400, 33, 0, 1], 2, 128, 16, 7), ([1000], 1, 128, 64, 5), ([700, 650], 3, 32, 32, 9),
     ([500, 20], 1, 16, 64, 3), ([300, 299], 1, 64, 8, 20), ([90, 200], 2, 4, 4, 11), ([2100, 70], 1, 48, 128, 4),
-    ([50, 61], 2, 32, 2, 13)])
+    ([50, 61], 2, 32, 2, 13), ([100, 900], 1, 128, 16, 300), ([1100, 5], 2, 16, 1024, 1)])
 def test_attend_selected_pages(ctx, fmt, lens, M, H, page, top_k):
     """Entries in any order, gaps among them, pages behind the row's end, one
     listed twice, a row with none; pages that no row lists hold NaN."""
@@ -441,13 +442,14 @@ def test_refusals(ctx):
     for k in (dict(table=None), dict(lens=None), dict(stride=3), dict(width=0), dict(B=0), dict(M=0), dict(q=None),
               dict(q=p + 4), dict(o=None)):
         assert all(c == arg for c in calls(kv(), **k)), k
-    for k in (dict(B=70000), dict(M=2**31), dict(width=2**30, stride=2**30)):
+    for k in (dict(B=70000), dict(M=2**31), dict(width=2**30, stride=2**30), dict(width=2**27 - 63, stride=2**27)):
         assert all(c == shape for c in calls(kv(), **k)), k
     assert list(calls(kv(), H=0))[:3] == [arg] * 3 and list(calls(kv(), H=70000))[:3] == [shape] * 3
     assert list(calls(kv(), M=40000))[:3] == [shape] * 3 and list(calls(kv(), M=40000, H=1))[:3] == [shape] * 3
     b = batch(kv())
     assert lib.ut_mla_sparse_attend(*b, 16, p, p, 0.1, None, 2, p) == arg
     assert lib.ut_mla_sparse_attend(*b, 16, p, p, 0.1, p, 0, p) == arg
+    assert lib.ut_mla_sparse_attend(*b, 16, p, p, 0.1, p, 2**27 - 63, p) == arg
     for first, last, k in ((-1, 1, 4), (1, -1, 4), (3, 2, 4), (0, 0, 0), (5, 0, 4), (2**62, 2**62, 4)):
         assert lib.ut_mla_page_select(*b, 16, p, p, None, first, last, k, p) == arg
     for k in (dict(mean=None), dict(mean_scale=None), dict(mean=None, mean_scale=None)):
@@ -591,3 +593,42 @@ def test_calls_on_a_stream_of_their_own(ctx):
             outs.append([c.attend(table, lens, qabs, qrope, SCALE) for _ in range(5)])
             c.ctx.synchronize()
     assert all(torch.equal(o, want) for v in outs for o in v)
+
+
+def test_two_contexts_at_once(ctx):
+    """Two contexts on streams of their own, over one pool, their calls under
+    way at the same time: each has the bits of its calls alone."""
+    import undertow_amd as U
+    g = torch.Generator(device="cuda").manual_seed(8)
+    rnd = lambda *d: torch.randn(d, device="cuda", generator=g)
+    cache = U.PagedCache.empty(ctx, 300, page=16)
+    table = torch.randperm(300, device="cuda", generator=g)[:264].reshape(3, 88).int()
+    lens = torch.tensor([700, 90, 1300], dtype=torch.int32, device="cuda")
+    cache.append(table, lens, rnd(3, 1300, 512), rnd(3, 1300, 64))
+    ctx.synchronize()
+    torch.cuda.synchronize()
+    runs = []
+    for k, M in enumerate((1, 4)):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            c = U.Context(0)
+            mine = U.PagedCache(c, cache.pages, 512, 64, cache.mean, cache.mean_scale)
+            q = rnd(3, M, 128, 512).bfloat16(), rnd(3, M, 128, 64).bfloat16()
+            s.synchronize()
+            runs.append((s, c, mine, q))
+
+    def turn(s, c, mine, q):
+        with torch.cuda.stream(s):
+            sel = mine.select(table, lens, *q, 9)
+            return sel, mine.attend(table, lens, *q, SCALE), mine.attend_pages(table, lens, *q, SCALE, sel)
+
+    alone = []
+    for x in runs:
+        alone.append(turn(*x))
+        x[1].synchronize()
+    both = [[turn(*x) for x in runs] for _ in range(10)]
+    for x in runs:
+        x[1].synchronize()
+    for pair in both:
+        for got, want in zip(pair, alone):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))

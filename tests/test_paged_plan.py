@@ -17,7 +17,7 @@ extern "C" {
 int64_t ranges(int64_t W, int64_t most, int64_t least) { return ut::plan_ranges(W, most, least); }
 int64_t begin(int64_t W, int64_t N, int64_t r) { return ut::plan_begin(W, N, r); }
 int64_t range_of(int64_t W, int64_t N, int64_t t) { return ut::plan_range_of(W, N, t); }
-int64_t slot(int64_t W, int64_t N, int64_t r, int64_t pre) { return ut::plan_slot(W, N, r, pre); }
+int64_t slot(int64_t r, int64_t begins) { return ut::plan_slot(r, begins != 0); }
 int len(int n, int64_t cap, int *bad) { bool b = false; int v = ut::plan_len(n, cap, b); *bad = b; return v; }
 int page(int p, int n, int *bad) { bool b = false; int v = ut::plan_page(p, n, b); *bad = b; return v; }
 }
@@ -32,7 +32,7 @@ def L(tmp_path_factory):
                     str(d / "p.so"), str(d / "p.cpp")], check=True)
     lib = C.CDLL(str(d / "p.so"))
     i = C.c_int64
-    for f, n in (("ranges", 3), ("begin", 3), ("range_of", 3), ("slot", 4)):
+    for f, n in (("ranges", 3), ("begin", 3), ("range_of", 3), ("slot", 2)):
         getattr(lib, f).restype, getattr(lib, f).argtypes = i, [i] * n
     lib.len.argtypes = [C.c_int, i, C.POINTER(C.c_int)]
     lib.page.argtypes = [C.c_int, C.c_int, C.POINTER(C.c_int)]
@@ -64,13 +64,13 @@ def test_every_tile_once_and_parts_meet(L, seed):
                 taken[k] += 1
                 assert L.range_of(W, N, k) == r
             if b - a < t:
-                parts.setdefault(L.slot(W, N, r, pre[u]), []).append((u, r))
+                parts.setdefault(L.slot(r, s <= pre[u]), []).append((u, r))
     assert taken == [1] * W
     assert all(len(v) == 1 for v in parts.values()) and all(0 <= k < 2 * N for k in parts)
     for u, t in enumerate(tiles):  # what joins the parts finds each of them
         if t:
             r0, r1 = L.range_of(W, N, pre[u]), L.range_of(W, N, pre[u] + t - 1)
-            got = [parts[L.slot(W, N, r, pre[u])][0] for r in range(r0, r1 + 1)] if r1 > r0 else []
+            got = [parts[L.slot(r, r == r0)][0] for r in range(r0, r1 + 1)] if r1 > r0 else []
             assert got == [(u, r) for r in range(r0, r1 + 1)] * (r1 > r0)
 
 

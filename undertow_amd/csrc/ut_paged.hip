@@ -725,13 +725,13 @@ __global__ __launch_bounds__(kPickThreads) void k_select_pick(PagedArgs a, const
 // there whichever device the caller has current.
 struct DeviceScope {
     int before = -1;
-    bool ok = true;
+    hipError_t err;
     explicit DeviceScope(int device) {
         int d = -1;
-        ok = hipGetDevice(&d) == hipSuccess;
-        if (ok && d != device) {
+        err = hipGetDevice(&d);
+        if (err == hipSuccess && d != device) {
             before = d;
-            ok = hipSetDevice(device) == hipSuccess;
+            err = hipSetDevice(device);
         }
     }
     ~DeviceScope() {
@@ -740,7 +740,7 @@ struct DeviceScope {
 };
 
 constexpr int64_t kMostRows = 65535;  // query rows of a call
-static int32_t paged_args(ut_ctx *ctx, const char *what, const ut_mla_pages *kv,
+static int32_t paged_args(ut_ctx *ctx, const DeviceScope &dev, const char *what, const ut_mla_pages *kv,
                           const int32_t *table, int64_t stride, int64_t max_pages,
                           const int32_t *lens, int64_t B, int64_t M, int64_t H, int64_t most_rows,
                           PagedArgs &a) {
@@ -753,6 +753,7 @@ static int32_t paged_args(ut_ctx *ctx, const char *what, const ut_mla_pages *kv,
     if (kv->n_pages <= 0 || max_pages <= 0 || B <= 0 || M <= 0 || H <= 0 || stride < max_pages)
         return bad("sizes must be positive and the table's stride cover its pages");
     if (((uintptr_t)kv->pages & 15) != 0) return bad("pages must be 16-byte aligned");
+    UT_CHECK_HIP(ctx, dev.err);
     const int64_t page = kv->page, L = kv->latent, P = kv->rope;
     auto shape = [&](const char *why) {
         set_error(ctx, "%s: %s (page %lld, latent %lld, rope %lld, sequences %lld, rows %lld, heads %lld)",
@@ -764,8 +765,8 @@ static int32_t paged_args(ut_ctx *ctx, const char *what, const ut_mla_pages *kv,
         return shape("a page is a power of two of at most 1024 positions");
     if (L <= 0 || P <= 0 || L % 8 != 0 || P % 8 != 0 || L + P > 1024)
         return shape("latent and rope must be multiples of 8 that add up to at most 1024");
-    if (kv->n_pages > INT32_MAX / page || max_pages > INT32_MAX / page)
-        return shape("a pool and a sequence hold fewer than 2^31 positions");
+    if (kv->n_pages > INT32_MAX / page || max_pages > kMostPositions / page)
+        return shape("a pool holds fewer than 2^31 positions, a sequence at most 2^31 - 1024");
     if (B > 65535 || H > 65535 || M > INT32_MAX / B / H || B * M > most_rows)
         return shape("too many sequences, rows or heads");
     a = PagedArgs{};
@@ -827,7 +828,7 @@ static int32_t paged_attend(ut_ctx *ctx, const char *what, const ut_mla_pages *k
                             void *out) {
     DeviceScope dev(ctx->device);
     PagedArgs a;
-    UT_TRY(paged_args(ctx, what, kv, table, stride, max_pages, lens, B, M, H, kMostRows, a));
+    UT_TRY(paged_args(ctx, dev, what, kv, table, stride, max_pages, lens, B, M, H, kMostRows, a));
     if (!qabs || !qrope || !out || ((uintptr_t)qabs & 15) != 0 || ((uintptr_t)qrope & 15) != 0 ||
         ((uintptr_t)out & 15) != 0) {
         set_error(ctx, "%s: queries and output must be 16-byte aligned device memory", what);
@@ -855,7 +856,7 @@ extern "C" int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv,
     if (!ctx) return UT_ERR_ARG;
     DeviceScope dev(ctx->device);
     PagedArgs a;
-    UT_TRY(paged_args(ctx, "ut_mla_paged_append", kv, table_dev, table_stride, max_pages, lens_dev,
+    UT_TRY(paged_args(ctx, dev, "ut_mla_paged_append", kv, table_dev, table_stride, max_pages, lens_dev,
                       batch, rows, 1, INT32_MAX, a));
     if (!latent_dev || !krot_dev || ((uintptr_t)latent_dev & 15) != 0 ||
         ((uintptr_t)krot_dev & 15) != 0 || !kv->mean != !kv->mean_scale) {
@@ -896,8 +897,8 @@ extern "C" int32_t ut_mla_sparse_attend(ut_ctx *ctx, const ut_mla_pages *kv,
                                         const void *q_rope_dev, float scale, const int32_t *sel_dev,
                                         int64_t top_k, void *clat_dev) {
     if (!ctx) return UT_ERR_ARG;
-    if (!sel_dev || top_k <= 0 || (kv && kv->page > 0 && top_k > INT32_MAX / kv->page)) {
-        set_error(ctx, "ut_mla_sparse_attend: a selection of at least one page is needed");
+    if (!sel_dev || top_k <= 0 || (kv && kv->page > 0 && top_k > kMostPositions / kv->page)) {
+        set_error(ctx, "ut_mla_sparse_attend: a selection of one page or more, 2^31 - 1024 positions at most, is needed");
         return UT_ERR_ARG;
     }
     return paged_attend(ctx, "ut_mla_sparse_attend", kv, table_dev, table_stride, max_pages,
@@ -914,7 +915,7 @@ extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const
     if (!ctx) return UT_ERR_ARG;
     DeviceScope dev(ctx->device);
     PagedArgs a;
-    UT_TRY(paged_args(ctx, "ut_mla_page_select", kv, table_dev, table_stride, max_pages, lens_dev,
+    UT_TRY(paged_args(ctx, dev, "ut_mla_page_select", kv, table_dev, table_stride, max_pages, lens_dev,
                       batch, rows, heads, kMostRows, a));
     if (!qabs_dev || !q_rope_dev || !sel_dev || !kv->mean || !kv->mean_scale ||
         ((uintptr_t)qabs_dev & 15) != 0 || ((uintptr_t)q_rope_dev & 15) != 0 ||

@@ -716,7 +716,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
                     *(o4 *)(out + 16 * mt) = v;
                 }
         } else if (active) {
-            const int64_t slot = (2 * r + (rg.s <= q.first ? 1 : 0)) * p.groups + grp;  // plan_slot
+            const int64_t slot = plan_slot(r, rg.s <= q.first) * p.groups + grp;
             pf32x4 *po = (pf32x4 *)p.part_o + slot * 128 * kCols + g * kCols + col;
 #pragma unroll
             for (int mt = 0; mt < 32; mt++) po[mt * 4 * kCols] = wv.o[mt];
@@ -755,7 +755,7 @@ template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_j
 #pragma unroll
         for (int i = 0; i < COUNT; i++) {
             const int x = r + 4 * i;
-            const int64_t slot = (2ll * x + (x == r0 ? 1 : 0)) * p.groups + grp;  // plan_slot
+            const int64_t slot = plan_slot(x, x == r0) * p.groups + grp;
             ml[i] = *(const float2 *)(p.part_ml + (slot * kCols + col) * 2);
 #pragma unroll
             for (int k = 0; k < 4; k++)
@@ -835,7 +835,7 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     const int64_t most = ctx->multiprocessors / p.chunks;
     p.least = kLeastTiles;
     p.most = (int32_t)plan_ranges(W, most < 1 ? 1 : most, p.least);
-    const int64_t slots = 2ll * p.most * p.groups;
+    const int64_t slots = p.most > 1 ? plan_slot(p.most, false) * p.groups : 0;
     ScratchPlan plan;
     plan.add((size_t)slots * kPL * kCols * 4);
     plan.add((size_t)slots * kCols * 8);

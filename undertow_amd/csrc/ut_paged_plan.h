@@ -30,10 +30,12 @@ UT_PLAN_FN int64_t plan_ranges(int64_t W, int64_t most, int64_t least) {
 UT_PLAN_FN int64_t plan_begin(int64_t W, int64_t N, int64_t r) { return W * r / N; }
 // The range that holds tile t.
 UT_PLAN_FN int64_t plan_range_of(int64_t W, int64_t N, int64_t t) { return ((t + 1) * N - 1) / W; }
-// Where range r leaves its part of the sequence whose first tile is `first`.
-UT_PLAN_FN int64_t plan_slot(int64_t W, int64_t N, int64_t r, int64_t first) {
-    return 2 * r + (plan_begin(W, N, r) <= first ? 1 : 0);
-}
+// Where range r leaves its part of a sequence that begins in it, or of the one
+// that began before it.
+UT_PLAN_FN int64_t plan_slot(int64_t r, bool begins) { return 2 * r + (begins ? 1 : 0); }
+// Positions of a sequence or a selection: tile and page counts may step past
+// the end by some tiles and stay in 32 bits.
+constexpr int64_t kMostPositions = INT32_MAX - 1023;
 // A length cut to what the table can hold; a page id cut to the pool.
 UT_PLAN_FN int32_t plan_len(int32_t n, int64_t cap, bool &bad) {
     if (n >= 0 && n <= cap) return n;
