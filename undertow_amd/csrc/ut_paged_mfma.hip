@@ -204,6 +204,10 @@ struct MfmaBf16 {
     static constexpr int kPlanes = 1, kWaves = 8;
     static constexpr bool kBetween = false;  // copies between the products (the branches cost registers)
     static constexpr int kDepth = 4;
+    // empty tiles that stand for the queries, first tiles and result of a
+    // sequence that begins in a range: 64 sequences of up to 8192 positions take
+    // 135 us with 0, 132 with 2, 126 with 4, 115 with 8, 117 with 16
+    static constexpr int kLead = 8;
     static constexpr float kRise = 11.5f;  // log2 units a score may exceed the offset (8 nats)
     typedef __bf16 out_t;
     struct Query {
@@ -286,6 +290,9 @@ struct MfmaF16x2 {
     static constexpr int kPlanes = 2, kWaves = 4;
     static constexpr bool kBetween = true;
     static constexpr int kDepth = 4;
+    // (a tile takes twice as long: 11 x 3 rows 103 us with 0, 96.1 with 2, 96.4
+    // with 4, 99.7 with 8)
+    static constexpr int kLead = 4;
     static constexpr float kRise = 1.0f;
     typedef float out_t;
     struct Query {
@@ -820,7 +827,10 @@ template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_j
 
 bool paged_mfma_ok(const PagedArgs &a) { return a.L == kPL && a.P == kPD - kPL && a.shift >= 3; }
 
-constexpr int kLeastTiles = 2, kLeadTiles = 4;
+// A range takes two tiles or more: with one a call of few positions splits
+// into more parts than it saves (one row over 2048 listed positions 28.2 us,
+// two 23.8, four 23.2; over 509 positions 18.4, 19.0, 22.0).
+constexpr int kLeastTiles = 2;
 
 template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const PagedArgs &a) {
     PagedMfmaArgs p{};
@@ -830,7 +840,7 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     p.chunks = (p.groups + F::kWaves - 1) / F::kWaves;
     p.per = (p.groups + p.chunks - 1) / p.chunks;
     const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
-    p.lead = kLeadTiles;
+    p.lead = F::kLead;
     const int64_t W = (int64_t)p.units * ((cap + kPT - 1) / kPT + p.lead);  // at most
     const int64_t most = ctx->multiprocessors / p.chunks;
     p.least = kLeastTiles;
