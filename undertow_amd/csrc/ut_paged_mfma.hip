@@ -1,5 +1,32 @@
 // ut_paged_mfma.hip -- attention over the paged latent cache on the matrix
 // cores, for latent 512 + rope 64 and pages of 8 positions and more.
+//
+// For a row's heads q_h and the positions t it sees, one pass over the cache:
+//   s_ht = scale (q_h . [latent_t | krot_t]),  out_h = sum_t e^(s_ht - m_h)
+//   latent_t / sum_t e^(s_ht - m_h), with m_h the largest score so far (or one
+// not far below it).
+//
+// Each position is 1152 bytes (f16x2: 2304) and costs 128 heads 2 * 128 *
+// (576 + 512) operations: at 5.1 TB/s and 1.2 PFLOP/s (a large copy's and a
+// large matrix product's rates) 0.23 ns against 0.23 ns, so memory and matrix
+// cores have to be busy all the time, and together.  Hence:
+// - 16 columns (heads of one row) a wave with the whole latent width in
+//   registers (128 of context, 72 of queries), so that scores, weights and
+//   contexts never leave the wave.  32 columns spill; two waves to a column
+//   group, each with half of the tiles, took 145 us instead of 130 (64
+//   sequences of up to 8192 positions).
+// - eight such waves over one tile of 32 positions in LDS: K is read from it
+//   as it lies, V transposed by the LDS reads, and three further tiles are on
+//   their way, straight to LDS.
+// - equal ranges of the whole batch's tiles, one workgroup a CU
+//   (ut_paged_plan.h), and a join of what the ranges leave (k_paged_join).
+//
+// A tile of 128 heads takes 1.95 us: 1.17 PFLOP/s and, with one row a sequence,
+// 4.8 TB/s over 256 CUs; the LDS reads alone would take 1.1 us of it (K 288 KB
+// at 558 B/ns, V 256 KB at 431, as measured by themselves).  64 ragged sequences of up to 8192
+// positions (329 MB): 115 us, of which products and copies 70, the start 9
+// (lengths 1.4, queries issued 4.6, first tiles 8.7 us from the start),
+// partial results written 5 to 10, their join 16 (82 MB each way).
 #include <type_traits>
 
 #include "ut_paged.h"
@@ -283,9 +310,11 @@ struct MfmaBf16 {
 // hi*hi + lo*hi + hi*lo (lo*lo lies 2^-22 below).  Stored low parts are
 // scaled by 2^11: the scores' sum with them is scaled back at its end, and in
 // the context such a part meets the weight's high part times 2^-11, so that
-// all three products add up in one accumulator.  Queries are scaled by a power of two to a maximum in [2^14, 2^15) and
-// weights by 2^14 (at most 2^15), so that neither their low parts nor the
-// scaled high parts fall out of f16's range where they matter.
+// all three products add up in one accumulator.  Queries are scaled by a power
+// of two to a maximum in [2^14, 2^15) and weights by 2^14 (at most 2^15), so
+// that neither their low parts nor the scaled high parts fall out of f16's
+// range where they matter.  Three products a score bound it: 33 rows of 128
+// heads over up to 4099 positions (61 GFLOP in f16) take 96 us, floor 52.
 struct MfmaF16x2 {
     static constexpr int kPlanes = 2, kWaves = 4;
     static constexpr bool kBetween = true;
@@ -737,11 +766,13 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
 
 // Joins the parts of a unit that lies in more than one range:
 // out = sum_r o_r 2^(m_r - M) / sum_r l_r 2^(m_r - M).  A workgroup takes one
-// column group and 64 dims, each of its waves every fourth part, as many
-// at a time as there are, with all their loads under way; the waves' results meet in LDS.
+// column group and 64 dims, each of its waves every fourth part, as many at a
+// time as there are, with all their loads under way; the waves' results meet
+// in LDS.  Bound by the parts' bytes: 82 MB in 16.9 us (4.9 TB/s); 8 parts of
+// one row take 4.2.
 template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_join(PagedMfmaArgs p) {
     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
-    __shared__ __attribute__((aligned(16))) pf32x4 so[4][16][kCols];
+    __shared__ __attribute__((aligned(16))) pf32x4 so[4][16][kCols + 1];  // one more: other banks
     __shared__ float2 sml[4][kCols];
     const PagedArgs &a = p.a;
     const int u = blockIdx.x / p.groups, grp = blockIdx.x - u * p.groups, tid = threadIdx.x;
