@@ -333,7 +333,8 @@ typedef struct {
 /* Writes the rows latent [batch, rows, latent] and krot [batch, rows, rope]
  * (f32) to their positions, and the summary of every page they fall into
  * anew from its stored positions below lens.  A position before the cache's
- * start is not written.  A page that new rows fall into must not stand in the
+ * start is not written.  A call writes at most 2^22 pages of a sequence.  A
+ * page that new rows fall into must not stand in the
  * call's table twice, by two sequences or in one. */
 int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
                             int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
@@ -358,7 +359,7 @@ int32_t ut_mla_paged_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *
  * with q_h = [qabs | q_rope] of head h and code(q) = rint(q * 127 / max|q|):
  * the products are exact in integers and the sum runs in 64 bits.  weights
  * [batch, rows, heads] f32 or NULL (all 1).  A head whose query is not finite
- * is left out; a NaN score ranks last. */
+ * is left out; a NaN score ranks last.  max_pages is at most 2^27 here. */
 int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
                            int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
                            int64_t batch, int64_t rows, int64_t heads, const void *qabs_dev,

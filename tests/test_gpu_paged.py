@@ -444,6 +444,10 @@ def test_refusals(ctx):
         assert all(c == arg for c in calls(kv(), **k)), k
     for k in (dict(B=70000), dict(M=2**31), dict(width=2**30, stride=2**30), dict(width=2**27 - 63, stride=2**27)):
         assert all(c == shape for c in calls(kv(), **k)), k
+    one = dict(page=1, pages=pages.data_ptr())  # within 32 bits, past what a launch spans
+    assert list(calls(kv(**one), M=2**28, width=2**28, stride=2**28, B=1))[3] == shape
+    assert list(calls(kv(**one), M=2**28, width=2**28, stride=2**28, B=1, H=1))[2] == shape
+    assert lib.ut_mla_page_select(*batch(kv(**one), width=2**28, stride=2**28), 16, p, p, None, 1, 1, 2, p) == shape
     assert list(calls(kv(), H=0))[:3] == [arg] * 3 and list(calls(kv(), H=70000))[:3] == [shape] * 3
     assert list(calls(kv(), M=40000))[:3] == [shape] * 3 and list(calls(kv(), M=40000, H=1))[:3] == [shape] * 3
     b = batch(kv())

@@ -50,6 +50,11 @@ def test_pools_that_are_none():
                                    mean_scale=dev(3))) == UT_ERR_SHAPE
 
 
+def test_a_format_that_is_none():
+    for fmt in (2, -1, "bf16", None):
+        assert code(lambda: PagedCache.empty(Ctx(), 4, fmt=fmt)) == UT_ERR_ARG
+
+
 def test_batches_that_do_not_fit(cache):
     i32 = lambda *s: dev(*s, dtype=torch.int32)
     bf = lambda *s: dev(*s, dtype=torch.bfloat16)

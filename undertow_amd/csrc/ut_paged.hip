@@ -747,7 +747,8 @@ struct DeviceScope {
     }
 };
 
-constexpr int64_t kMostRows = 65535;  // query rows of a call
+constexpr int64_t kMostRows = 65535;         // query rows of a call
+constexpr int64_t kMostGroups = 1ll << 22;   // workgroups along a grid's first axis, where pages set them
 static int32_t paged_args(ut_ctx *ctx, const DeviceScope &dev, const char *what, const ut_mla_pages *kv,
                           const int32_t *table, int64_t stride, int64_t max_pages,
                           const int32_t *lens, int64_t B, int64_t M, int64_t H, int64_t most_rows,
@@ -874,6 +875,10 @@ extern "C" int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv,
     }
     // pages that `rows` positions can fall into
     const int64_t page = kv->page, touched = (rows + page - 2) / page + 1;
+    if (touched > kMostGroups && max_pages > kMostGroups) {
+        set_error(ctx, "ut_mla_paged_append: rows of more than %lld pages in a call", (long long)kMostGroups);
+        return UT_ERR_SHAPE;
+    }
     const size_t lds = kv->mean ? (size_t)(a.L + a.P) * 4 * sizeof(double) : 0;
     const dim3 grid((unsigned)(touched < max_pages ? touched : max_pages), (unsigned)batch);
     int tok = timing_begin(ctx, "paged_append");
@@ -937,6 +942,11 @@ extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const
         set_error(ctx, "ut_mla_page_select: top_k %lld must hold the %lld first and %lld last pages",
                   (long long)top_k, (long long)keep_first, (long long)keep_last);
         return UT_ERR_ARG;
+    }
+    if (max_pages > kMostGroups * kScorePages) {
+        set_error(ctx, "ut_mla_page_select: a row chooses among at most %lld pages, the table holds %lld",
+                  (long long)(kMostGroups * kScorePages), (long long)max_pages);
+        return UT_ERR_SHAPE;
     }
     a.qabs = qabs_dev;
     a.qrope = q_rope_dev;

@@ -2,9 +2,9 @@
 // cores, for latent 512 + rope 64 and pages of 8 positions and more.
 //
 // For a row's heads q_h and the positions t it sees, one pass over the cache:
-//   s_ht = scale (q_h . [latent_t | krot_t]),  out_h = sum_t e^(s_ht - m_h)
-//   latent_t / sum_t e^(s_ht - m_h), with m_h the largest score so far (or one
-// not far below it).
+//   s_ht = scale (q_h . [latent_t | krot_t]),
+//   out_h = sum_t e^(s_ht - m_h) latent_t / sum_t e^(s_ht - m_h),
+// with m_h the largest score so far, or one not far below it.
 //
 // Each position is 1152 bytes (f16x2: 2304) and costs 128 heads 2 * 128 *
 // (576 + 512) operations: at 5.1 TB/s and 1.2 PFLOP/s (a large copy's and a
@@ -23,10 +23,11 @@
 //
 // A tile of 128 heads takes 1.95 us: 1.17 PFLOP/s and, with one row a sequence,
 // 4.8 TB/s over 256 CUs; the LDS reads alone would take 1.1 us of it (K 288 KB
-// at 558 B/ns, V 256 KB at 431, as measured by themselves).  64 ragged sequences of up to 8192
-// positions (329 MB): 115 us, of which products and copies 70, the start 9
-// (lengths 1.4, queries issued 4.6, first tiles 8.7 us from the start),
-// partial results written 5 to 10, their join 16 (82 MB each way).
+// at 558 B/ns, V 256 KB at 431, as measured by themselves).  64 ragged
+// sequences of up to 8192 positions (329 MB): 115 us, of which products and
+// copies 70, the start 9 (lengths 1.4, queries issued 4.6, first tiles 8.7 us
+// from the start), partial results written 5 to 10, their join 16 (82 MB each
+// way).
 #include <type_traits>
 
 #include "ut_paged.h"

@@ -556,6 +556,8 @@ class PagedCache:
               fmt: int = KV_BF16, summaries: bool = True) -> "PagedCache":
         """A cache over a pool of its own."""
         torch = _torch()
+        if fmt not in (KV_BF16, KV_F16X2):
+            raise UtError(UT_ERR_ARG, f"PagedCache: fmt is KV_BF16 or KV_F16X2, got {fmt!r}")
         d, D = f"cuda:{ctx.device}", latent + rope
         pages = (torch.zeros((n_pages, page, D), dtype=torch.bfloat16, device=d) if fmt == KV_BF16
                  else torch.zeros((n_pages, page, 2, D), dtype=torch.float16, device=d))
