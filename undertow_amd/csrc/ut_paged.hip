@@ -361,24 +361,40 @@ template <class T> __device__ __forceinline__ int code8(T q, T top, T f) {
     const bool next = e > top || -e > top || ((e == top || -e == top) && (k & 1));
     return next ? (e > 0 ? k + 1 : k - 1) : k;
 }
-// The codes of head r (none from `end` on), by a wave: code_row(D) bytes,
-// zeros behind the D; its share.
-template <class F>
-__device__ __forceinline__ void head_codes(const PagedArgs &a, int64_t r, int64_t end, const float *weights,
-                                           int8_t *codes, double *share) {
-    const int lane = threadIdx.x & 63, D = a.L + a.P, Dp = (int)code_row(D);
+// Head r's query (none from `end` on), over a wave: eight dims a lane, a
+// single one behind them, and (D is at most 1024) up to seven more, which are
+// read where they are used.
+template <class F> struct HeadQuery {
     typedef typename F::q_t q_t;
-    typedef typename F::code_t T;
     typedef q_t q8 __attribute__((ext_vector_type(8)));
-    const bool any = r < end;
-    if (!any) r = end - 1;
-    const q_t *qa = (const q_t *)a.qabs + r * a.L, *qr = (const q_t *)a.qrope + r * a.P;
-    auto at = [&](int d) { return (float)(d < a.L ? qa[d] : qr[d - a.L]); };
+    const q_t *qa, *qr;
+    q8 q;
+    q_t one;
+    float weight;
+    bool any;
+    __device__ __forceinline__ HeadQuery(const PagedArgs &a, int64_t r, int64_t end, const float *weights) {
+        const int lane = threadIdx.x & 63, D = a.L + a.P;
+        any = r < end;
+        if (!any) r = end - 1;
+        qa = (const q_t *)a.qabs + r * a.L;
+        qr = (const q_t *)a.qrope + r * a.P;
+        q = q8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (8 * lane < D) q = *(const q8 *)(8 * lane < a.L ? qa + 8 * lane : qr + (8 * lane - a.L));
+        one = 0;
+        if (512 + lane < D) one = 512 + lane < a.L ? qa[512 + lane] : qr[512 + lane - a.L];
+        weight = weights ? weights[r] : 1.0f;
+    }
+};
+// Its codes: code_row(D) bytes, zeros behind the D; its share.
+template <class F>
+__device__ __forceinline__ void head_codes(const PagedArgs &a, const HeadQuery<F> &x, int8_t *codes, double *share) {
+    const int lane = threadIdx.x & 63, D = a.L + a.P, Dp = (int)code_row(D);
+    typedef typename F::code_t T;
+    auto at = [&](int d) { return (float)(d < a.L ? x.qa[d] : x.qr[d - a.L]); };
     auto bits = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };  // NaN lies above infinity
-    // eight dims a lane, then (D is at most 1024) up to eight single ones
-    q8 q = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (8 * lane < D) q = *(const q8 *)(8 * lane < a.L ? qa + 8 * lane : qr + (8 * lane - a.L));
-    const float one = 512 + lane < D ? at(512 + lane) : 0.0f, weight = weights ? weights[r] : 1.0f;
+    const auto q = x.q;
+    const float one = (float)x.one, weight = x.weight;
+    const bool any = x.any;
     uint32_t top = bits(one);
 #pragma unroll
     for (int k = 0; k < 8; k++) {
@@ -428,7 +444,8 @@ template <int CTRL> __device__ __forceinline__ double dpp_double(double v) {
 //
 // many rows: a launch makes all codes; then a workgroup takes 32 pages of a
 // row, its waves every fourth tile of 16 heads, so that a page's mean is read
-// once for all heads;
+// once for all heads (48 rows of up to 625 pages: 27.3 us a call, with 16 pages
+// 28.5, with 64 29.8);
 // few rows (and rows of nine whole steps of 64): one launch, a workgroup takes
 // 16 heads, whose codes its waves make first, and 256 pages or more, and
 // leaves its heads' part of each sum.
@@ -452,10 +469,10 @@ __global__ __launch_bounds__(256) void k_select_codes(PagedArgs a, const float *
                                                       int64_t heads, int8_t *__restrict__ codes,
                                                       double *__restrict__ share) {
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i < heads) head_codes<F>(a, r0 + i, r0 + heads, weights, codes + i * code_row(a.L + a.P), share + i);
+    if (i < heads) head_codes<F>(a, HeadQuery<F>(a, r0 + i, r0 + heads, weights), codes + i * code_row(a.L + a.P), share + i);
 }
 
-constexpr int kScorePages = 32;
+constexpr int kScorePages = 32, kScoreTiles = kScorePages / 16;
 template <bool FULL>
 __global__ __launch_bounds__(256) void k_select_score(PagedArgs a, const int8_t *__restrict__ codes,
                                                       const double *__restrict__ share,
@@ -469,9 +486,22 @@ __global__ __launch_bounds__(256) void k_select_score(PagedArgs a, const int8_t 
     const int32_t n = paged_len(a, b) - a.M + j + 1;
     const int np = n > 0 ? ((n - 1) >> a.shift) + 1 : 0, k0 = blockIdx.x * kScorePages;
     if (k0 >= np) return;
-    si32x4 A[2][STEPS];
+    // a tile of heads is loaded under the products of the one before, the first
+    // beside the look-ups of the pages
+    si32x4 B[STEPS];
+    double sh = 0.0;
+    auto load = [&](int h0) {
+        const int h = h0 + (l & 15);
+        const int64_t r = (int64_t)blockIdx.y * a.H + (h < a.H ? h : a.H - 1);
+        sh = h < a.H ? share[r] : 0.0;
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
+        for (int s = 0; s < STEPS; s++)
+            if (FULL || s < steps) B[s] = *(const si32x4 *)(codes + r * Dp + kCodeStep * s + 16 * g);
+    };
+    if (16 * w < a.H) load(16 * w);
+    si32x4 A[kScoreTiles][STEPS];
+#pragma unroll
+    for (int t = 0; t < kScoreTiles; t++) {
         const int k = k0 + 16 * t + (l & 15);
         const int8_t *src = mean + (int64_t)paged_phys(a, b, k < np ? k : np - 1) * D;
 #pragma unroll
@@ -486,41 +516,29 @@ __global__ __launch_bounds__(256) void k_select_score(PagedArgs a, const int8_t 
             }
         }
     }
-    double sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    // the next tile of heads is loaded under this one's products
-    si32x4 B[STEPS];
-    double sh = 0.0;
-    auto load = [&](int h0) {
-        const int h = h0 + (l & 15);
-        const int64_t r = (int64_t)blockIdx.y * a.H + (h < a.H ? h : a.H - 1);
-        sh = h < a.H ? share[r] : 0.0;
-#pragma unroll
-        for (int s = 0; s < STEPS; s++)
-            if (FULL || s < steps) B[s] = *(const si32x4 *)(codes + r * Dp + kCodeStep * s + 16 * g);
-    };
-    if (16 * w < a.H) load(16 * w);
+    double sum[4 * kScoreTiles] = {};
     for (int h0 = 16 * w; h0 < a.H; h0 += 64) {
-        si32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        si32x4 c[kScoreTiles] = {};
         const double share_h = sh;
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
-            if (FULL || s < steps) {
-                c[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[0][s], B[s], c[0], 0, 0, 0);
-                c[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[1][s], B[s], c[1], 0, 0, 0);
-            }
+            if (FULL || s < steps)
+#pragma unroll
+                for (int t = 0; t < kScoreTiles; t++)
+                    c[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[t][s], B[s], c[t], 0, 0, 0);
         if (h0 + 64 < a.H) load(h0 + 64);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 4 * kScoreTiles; i++) {
             const int v = c[i >> 2][i & 3];
             sum[i] += share_h * (double)(v > 0 ? v : 0);
         }
     }
     // lane l: pages 16 (i >> 2) + 4 g + (i & 3) for its head column
 #pragma unroll
-    for (int i = 0; i < 8; i++) sum[i] = sum16(sum[i]);
+    for (int i = 0; i < 4 * kScoreTiles; i++) sum[i] = sum16(sum[i]);
     if ((l & 15) == 0)
 #pragma unroll
-        for (int i = 0; i < 8; i++) wave_part[w][16 * (i >> 2) + 4 * g + (i & 3)] = sum[i];
+        for (int i = 0; i < 4 * kScoreTiles; i++) wave_part[w][16 * (i >> 2) + 4 * g + (i & 3)] = sum[i];
     __syncthreads();
     const int t = threadIdx.x;
     if (t < kScorePages && k0 + t < np)
@@ -537,6 +555,8 @@ __global__ __launch_bounds__(kFusedThreads) void k_select_fused(PagedArgs a, con
     __shared__ double share[kFusedHeads];
     const int row = row0 + blockIdx.z, b = row / a.M, j = row - b * a.M, h0 = blockIdx.y * kFusedHeads;
     const int w = threadIdx.x >> 6, l = threadIdx.x & 63, g = l >> 4;
+    // the query is read beside the length and the table
+    const HeadQuery<F> query(a, (int64_t)row * a.H + h0 + w, (int64_t)(row + 1) * a.H, weights);
     const int32_t n = paged_len(a, b) - a.M + j + 1;
     const int np = n > 0 ? ((n - 1) >> a.shift) + 1 : 0;
     if ((int)blockIdx.x * kFusedPages >= np) return;
@@ -546,7 +566,7 @@ __global__ __launch_bounds__(kFusedThreads) void k_select_fused(PagedArgs a, con
     si32x4 A[STEPS];
 #pragma unroll
     for (int s = 0; s < STEPS; s++) A[s] = *(const si32x4 *)(src + kCodeStep * s + 16 * g);
-    head_codes<F>(a, (int64_t)row * a.H + h0 + w, (int64_t)(row + 1) * a.H, weights, codes[w], &share[w]);
+    head_codes<F>(a, query, codes[w], &share[w]);
     __syncthreads();
     si32x4 c = {0, 0, 0, 0};
 #pragma unroll
@@ -571,7 +591,7 @@ __global__ __launch_bounds__(kFusedThreads) void k_select_fused(PagedArgs a, con
 // equal or at most 64, which one wave then ranks.  One more pass writes the
 // pages above that key and the first of those equal to it.  Passes over a few
 // hundred keys, each a barrier apart: 512 pages 6.2 us, 48 rows of up to 625
-// pages 8.1 (codes 9.0 and scores 12.0 before it).
+// pages 8.0 (codes 9.0 and scores 11.7 before it).
 constexpr int kPickThreads = 512;
 __global__ __launch_bounds__(kPickThreads) void k_select_pick(PagedArgs a, const double *__restrict__ part,
                                                               int tiles, const float *__restrict__ mean_scale,
