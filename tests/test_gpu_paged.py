@@ -103,11 +103,11 @@ def test_attend_other_widths_long(ctx, fmt, lens, M, H, L, P, page):
     attend_case(ctx, fmt, lens, M, H, L, P, page)
 
 
-@pytest.mark.parametrize("H", [16, 64, 128])
-def test_attend_many_sequences(ctx, H):
+@pytest.mark.parametrize("fmt,H", [("bf16", 16), ("bf16", 64), ("bf16", 128), ("f16x2", 16)])
+def test_attend_many_sequences(ctx, fmt, H):
     """More sequences than workgroups look up at once, most of them short."""
     lens = [(37 * k) % 90 for k in range(700)]
-    attend_case(ctx, "bf16", lens, 1, H, 512, 64, 16)
+    attend_case(ctx, fmt, lens, 1, H, 512, 64, 16)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
