@@ -14,7 +14,7 @@ CSRC = Path(__file__).resolve().parents[1] / "undertow_amd" / "csrc"
 SRC = r"""
 #include "ut_paged_plan.h"
 extern "C" {
-int64_t ranges(int64_t W, int64_t most, int64_t least) { return ut::plan_ranges(W, most, least); }
+int64_t ranges(int64_t W, int64_t most, float spread) { return ut::plan_ranges(W, (int32_t)most, spread); }
 int64_t begin(int64_t W, int64_t N, int64_t r) { return ut::plan_begin(W, N, r); }
 int64_t range_of(int64_t W, int64_t N, int64_t t) { return ut::plan_range_of(W, N, t); }
 int64_t slot(int64_t r, int64_t begins) { return ut::plan_slot(r, begins != 0); }
@@ -34,6 +34,7 @@ def L(tmp_path_factory):
     i = C.c_int64
     for f, n in (("ranges", 3), ("begin", 3), ("range_of", 3), ("slot", 2)):
         getattr(lib, f).restype, getattr(lib, f).argtypes = i, [i] * n
+    lib.ranges.argtypes = [i, i, C.c_float]
     lib.len.argtypes = [C.c_int, i, C.POINTER(C.c_int)]
     lib.page.argtypes = [C.c_int, C.c_int, C.POINTER(C.c_int)]
     return lib
@@ -43,11 +44,12 @@ def L(tmp_path_factory):
 def test_every_tile_once_and_parts_meet(L, seed):
     rng = random.Random(seed)
     tiles = [rng.choice([0, 1, 2, rng.randint(0, 40), rng.randint(0, 1000)]) for _ in range(rng.randint(1, 70))]
-    W, most, least = sum(tiles), rng.choice([1, 7, 64, 256, 512]), rng.choice([1, 2, 4])
-    N = L.ranges(W, most, least)
-    assert 1 <= N <= most and (N == 1 or N <= max(1, -(-W // least)))
+    W, most, spread = sum(tiles), rng.choice([1, 7, 64, 256, 512]), rng.choice([0.5, 4, 16, 64 * 16])
+    N = L.ranges(W, most, spread)
+    assert 1 <= N <= most and (N == 1 or N <= W)
     if W == 0:
         return
+    assert N == min(most, W, max(1, int((W * spread) ** 0.5 + 0.5)))
     pre, at = [], 0
     for t in tiles:
         pre.append(at)

@@ -55,7 +55,7 @@ struct PagedMfmaArgs {
     int32_t chunks;   // workgroups that share a unit's positions
     int32_t per;      // column groups of a workgroup
     int32_t most;     // ranges at most
-    int32_t least;    // tiles a range at least
+    float spread;     // plan_ranges'
     float *part_o;    // [slot][group][128 quads][16 columns][4]
     float *part_ml;   // [slot][group][16 columns][2]
     int64_t *plan;    // [units] first tile of each, then W
@@ -96,7 +96,7 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 }
 
 struct Range {
-    int64_t W, N, s, e;  // the range takes tiles [s, e) of W
+    int64_t W, s, e;  // the range takes tiles [s, e) of W
     int u;               // the unit that holds tile s, and its first tile (behind its empty ones)
     int64_t first;
 };
@@ -123,10 +123,10 @@ __device__ bool find_range(const PagedMfmaArgs &p, int64_t r, bool leave, Range 
         if (leave && tid < p.units) p.plan[tid] = pre;
         if (leave && tid == 0) p.plan[p.units] = g.W;
         if (g.W == 0) return false;
-        g.N = plan_ranges(g.W, p.most, p.least);
-        if (r >= g.N) return false;
-        g.s = plan_begin(g.W, g.N, r);
-        g.e = plan_begin(g.W, g.N, r + 1);
+        const int64_t N = plan_ranges(g.W, p.most, p.spread);
+        if (r >= N) return false;
+        g.s = plan_begin(g.W, N, r);
+        g.e = plan_begin(g.W, N, r + 1);
         const int64_t at = g.s + p.lead;
         const int lead = __builtin_ctzll(__ballot(pre <= at && at < pre + t));
         g.u = __builtin_amdgcn_readfirstlane(lead);
@@ -149,10 +149,10 @@ __device__ bool find_range(const PagedMfmaArgs &p, int64_t r, bool leave, Range 
     if (leave && tid == 0) p.plan[p.units] = W;
     g.W = W = uniform(W);
     if (W == 0) return false;
-    g.N = plan_ranges(W, p.most, p.least);
-    if (r >= g.N) return false;
-    g.s = plan_begin(W, g.N, r);
-    g.e = plan_begin(W, g.N, r + 1);
+    const int64_t N = plan_ranges(W, p.most, p.spread);
+    if (r >= N) return false;
+    g.s = plan_begin(W, N, r);
+    g.e = plan_begin(W, N, r + 1);
     // unit u: [pre - lead, pre - lead + t), the first unit's lead before 0
     const int64_t at = g.s + p.lead;
     if (p.units <= NW * 64) {
@@ -236,6 +236,10 @@ struct MfmaBf16 {
     // sequence that begins in a range: 64 sequences of up to 8192 positions take
     // 135 us with 0, 132 with 2, 126 with 4, 115 with 8, 117 with 16
     static constexpr int kLead = 8;
+    // a tile's time to a part's in the join (plan_ranges): one row over 32768
+    // positions takes 48 us with 2, 44 with 3, 42 with 4, 41 with 8, and 59 in as
+    // many ranges as CUs; 4 rows over 500 positions 19.8, 20.8, 20.4, 24.3
+    static constexpr int kRatio = 4;
     static constexpr float kRise = 11.5f;  // log2 units a score may exceed the offset (8 nats)
     typedef __bf16 out_t;
     struct Query {
@@ -323,6 +327,9 @@ struct MfmaF16x2 {
     // (a tile takes twice as long: 11 x 3 rows 103 us with 0, 96.1 with 2, 96.4
     // with 4, 99.7 with 8)
     static constexpr int kLead = 4;
+    // one row over 500 positions 22.0 us with 4, 19.5 with 16; over 10000 43.2
+    // in as many ranges as CUs, 40.0 with 16, 40.6 with 32
+    static constexpr int kRatio = 16;
     static constexpr float kRise = 1.0f;
     typedef float out_t;
     struct Query {
@@ -781,7 +788,7 @@ template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_j
     const int64_t W = p.plan[p.units], first = p.plan[u];
     const int64_t tiles = unit_tiles<SPARSE>(a, u);
     if (tiles == 0) return;
-    const int64_t N = plan_ranges(W, p.most, p.least);
+    const int64_t N = plan_ranges(W, p.most, p.spread);
     const int r0 = (int)plan_range_of(W, N, first), r1 = (int)plan_range_of(W, N, first + tiles - 1);
     if (r0 == r1) return;
     float m = kLow, L = 0.0f;
@@ -859,24 +866,25 @@ template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_j
 
 bool paged_mfma_ok(const PagedArgs &a) { return a.L == kPL && a.P == kPD - kPL && a.shift >= 3; }
 
-// A range takes two tiles or more: with one a call of few positions splits
-// into more parts than it saves (one row over 2048 listed positions 28.2 us,
-// two 23.8, four 23.2; over 509 positions 18.4, 19.0, 22.0).
-constexpr int kLeastTiles = 2;
-
 template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const PagedArgs &a) {
     PagedMfmaArgs p{};
     p.a = a;
     p.units = SPARSE ? a.B * a.M : a.B;
     p.groups = (SPARSE ? 1 : a.M) * ((a.H + kCols - 1) / kCols);
-    p.chunks = (p.groups + F::kWaves - 1) / F::kWaves;
-    p.per = (p.groups + p.chunks - 1) / p.chunks;
     const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
     p.lead = F::kLead;
-    const int64_t W = (int64_t)p.units * ((cap + kPT - 1) / kPT + p.lead);  // at most
-    const int64_t most = ctx->multiprocessors / p.chunks;
-    p.least = kLeastTiles;
-    p.most = (int32_t)plan_ranges(W, most < 1 ? 1 : most, p.least);
+    p.spread = (float)p.units * F::kRatio;
+    const int64_t W = (int64_t)p.units * ((cap + kPT - 1) / kPT + p.lead) - p.lead;  // at most
+    // Where a call's ranges leave CUs free, its heads are spread over them: a
+    // workgroup of few columns issues its queries, tiles' products and results
+    // sooner (one row over 509 positions 18.9 us with 8 column groups a workgroup,
+    // 15.8 with one; one row over 32 listed pages of 64 23.7 and 21.1).
+    const int32_t cus = ctx->multiprocessors, free = cus / plan_ranges(W, cus, p.spread);
+    p.per = free < p.groups ? (p.groups + free - 1) / free : 1;
+    p.per = p.per < F::kWaves ? p.per : F::kWaves;
+    p.chunks = (p.groups + p.per - 1) / p.per;
+    p.per = (p.groups + p.chunks - 1) / p.chunks;
+    p.most = plan_ranges(W, p.chunks < cus ? cus / p.chunks : 1, p.spread);
     const int64_t slots = p.most > 1 ? plan_slot(p.most, false) * p.groups : 0;
     ScratchPlan plan;
     plan.add((size_t)slots * kPL * kCols * 4);

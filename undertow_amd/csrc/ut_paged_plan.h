@@ -12,6 +12,7 @@
 // each (plan_slot), every other sequence in it is whole.
 #pragma once
 
+#include <cmath>
 #include <cstdint>
 
 #if defined(__HIPCC__)
@@ -22,11 +23,27 @@
 
 namespace ut {
 
-// How many ranges: as many as may be, with `least` tiles in each.
-UT_PLAN_FN int64_t plan_ranges(int64_t W, int64_t most, int64_t least) {
-    const int64_t n = (W + least - 1) / least;
-    return n < 1 ? 1 : n < most ? n : most;
+// How many ranges.  A row of t tiles in x of them costs t / x tiles one after
+// another, and its x parts are joined one after another: least at x = sqrt(t
+// tile / join).  For `units` rows of W tiles together that is N = sqrt(W units
+// tile / join) in all; `most` at most, and one tile at least.
+// spread = units tile / join.
+UT_PLAN_FN int32_t plan_ranges(int64_t W, int32_t most, float spread) {
+    const float x = (float)W * spread, top = (float)most;
+    int32_t n = most;
+    if (x < top * top) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        n = (int32_t)(__builtin_amdgcn_sqrtf(x) + 0.5f);  // the nearest or the next one: no matter
+#else
+        n = (int32_t)(sqrtf(x) + 0.5f);
+#endif
+        n = n < most ? n : most;
+    }
+    n = (int64_t)n < W ? n : (int32_t)W;
+    return n < 1 ? 1 : n;
 }
+// (the longer ranges lie among the others: all in front, and so on the first
+// XCDs, costs 64 long sequences 1 %)
 UT_PLAN_FN int64_t plan_begin(int64_t W, int64_t N, int64_t r) { return W * r / N; }
 // The range that holds tile t.
 UT_PLAN_FN int64_t plan_range_of(int64_t W, int64_t N, int64_t t) { return ((t + 1) * N - 1) / W; }
