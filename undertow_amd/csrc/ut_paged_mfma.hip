@@ -240,6 +240,10 @@ struct MfmaBf16 {
     // positions takes 48 us with 2, 44 with 3, 42 with 4, 41 with 8, and 59 in as
     // many ranges as CUs; 4 rows over 500 positions 19.8, 20.8, 20.4, 24.3
     static constexpr int kRatio = 4;
+    // and to that of a column group's part's bytes, written and read (2 x 32 KB at
+    // a 5 TB/s that all share): 5 x 4 rows over up to 2083 positions 39.3 us
+    // without, 36.4 with 150, 35.3 with 75; 49 rows of up to 24 20.3, 18.5, 24.7
+    static constexpr int kBytesRatio = 150;
     static constexpr float kRise = 11.5f;  // log2 units a score may exceed the offset (8 nats)
     typedef __bf16 out_t;
     struct Query {
@@ -330,6 +334,8 @@ struct MfmaF16x2 {
     // one row over 500 positions 22.0 us with 4, 19.5 with 16; over 10000 43.2
     // in as many ranges as CUs, 40.0 with 16, 40.6 with 32
     static constexpr int kRatio = 16;
+    // 63 x 4 rows of up to 25 positions 66.5 us without and with 280, 80.4 with 140
+    static constexpr int kBytesRatio = 280;
     static constexpr float kRise = 1.0f;
     typedef float out_t;
     struct Query {
@@ -873,13 +879,14 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     p.groups = (SPARSE ? 1 : a.M) * ((a.H + kCols - 1) / kCols);
     const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
     p.lead = F::kLead;
-    p.spread = (float)p.units * F::kRatio;
-    const int64_t W = (int64_t)p.units * ((cap + kPT - 1) / kPT + p.lead) - p.lead;  // at most
-    // Where a call's ranges leave CUs free, its heads are spread over them: a
+    p.spread = fminf((float)p.units * F::kRatio, (float)F::kBytesRatio / (float)p.groups);
+    const int64_t tiles = (int64_t)p.units * ((cap + kPT - 1) / kPT);  // at most
+    const int64_t W = tiles + (int64_t)(p.units - 1) * p.lead;
+    // Where a call's tiles (the empty ones left out) leave CUs free, its heads are spread over them: a
     // workgroup of few columns issues its queries, tiles' products and results
     // sooner (one row over 509 positions 18.9 us with 8 column groups a workgroup,
     // 15.8 with one; one row over 32 listed pages of 64 23.7 and 21.1).
-    const int32_t cus = ctx->multiprocessors, free = cus / plan_ranges(W, cus, p.spread);
+    const int32_t cus = ctx->multiprocessors, free = cus / plan_ranges(tiles, cus, p.spread);
     p.per = free < p.groups ? (p.groups + free - 1) / free : 1;
     p.per = p.per < F::kWaves ? p.per : F::kWaves;
     p.chunks = (p.groups + p.per - 1) / p.per;

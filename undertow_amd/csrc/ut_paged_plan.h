@@ -26,8 +26,9 @@ namespace ut {
 // How many ranges.  A row of t tiles in x of them costs t / x tiles one after
 // another, and its x parts are joined one after another: least at x = sqrt(t
 // tile / join).  For `units` rows of W tiles together that is N = sqrt(W units
-// tile / join) in all; `most` at most, and one tile at least.
-// spread = units tile / join.
+// tile / join) in all.  All parts share the memory they pass through: joined
+// in `bytes` each at once, N = sqrt(W tile / bytes).  spread is the smaller of
+// units tile / join and tile / bytes; `most` ranges at most, of one tile at least.
 UT_PLAN_FN int32_t plan_ranges(int64_t W, int32_t most, float spread) {
     const float x = (float)W * spread, top = (float)most;
     int32_t n = most;
