@@ -103,6 +103,15 @@ def test_attend_other_widths_long(ctx, fmt, lens, M, H, L, P, page):
     attend_case(ctx, fmt, lens, M, H, L, P, page)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("lens,M,H,page", [
+    ([1, 0, 33, 64, 100, 0], 2, 32, 16), ([40], 1, 128, 64), ([0, 0, 7], 1, 48, 8), ([5, 90, 31] * 30, 1, 16, 32),
+    ([60, 1, 17], 4, 128, 128)])
+def test_attend_short_in_a_wide_table(ctx, fmt, lens, M, H, page):
+    """Lengths far below what the table holds: cut into ranges all the same."""
+    attend_case(ctx, fmt, lens, M, H, 512, 64, page, width=9000 // page)
+
+
 @pytest.mark.parametrize("fmt,H", [("bf16", 16), ("bf16", 64), ("bf16", 128), ("f16x2", 16)])
 def test_attend_many_sequences(ctx, fmt, H):
     """More sequences than workgroups look up at once, most of them short."""

@@ -56,6 +56,7 @@ struct PagedMfmaArgs {
     int32_t per;      // column groups of a workgroup
     int32_t most;     // ranges at most
     float spread;     // plan_ranges'
+    int32_t whole;    // a range is a unit (most: units), and there is no join
     float *part_o;    // [slot][group][128 quads][16 columns][4]
     float *part_ml;   // [slot][group][16 columns][2]
     int64_t *plan;    // [units] first tile of each, then W
@@ -108,6 +109,10 @@ __device__ bool find_range(const PagedMfmaArgs &p, int64_t r, bool leave, Range 
     __shared__ int64_t s[NW];
     __shared__ int64_t found[2];
     const int tid = threadIdx.x;
+    if (p.whole) {
+        g = {0, 0, __builtin_amdgcn_readfirstlane(unit_tiles<SPARSE>(p.a, (int)r)), (int)r, 0};
+        return g.e > 0;
+    }
     if (p.units <= 64) {
         // every wave by itself
         const int lane = tid & 63;
@@ -244,6 +249,7 @@ struct MfmaBf16 {
     // a 5 TB/s that all share): 5 x 4 rows over up to 2083 positions 39.3 us
     // without, 36.4 with 150, 35.3 with 75; 49 rows of up to 24 20.3, 18.5, 24.7
     static constexpr int kBytesRatio = 150;
+    static constexpr float kJoin = 2.5f;  // the join's launch, in tiles
     static constexpr float kRise = 11.5f;  // log2 units a score may exceed the offset (8 nats)
     typedef __bf16 out_t;
     struct Query {
@@ -336,6 +342,7 @@ struct MfmaF16x2 {
     static constexpr int kRatio = 16;
     // 63 x 4 rows of up to 25 positions 66.5 us without and with 280, 80.4 with 140
     static constexpr int kBytesRatio = 280;
+    static constexpr float kJoin = 1.3f;
     static constexpr float kRise = 1.0f;
     typedef float out_t;
     struct Query {
@@ -880,19 +887,43 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
     p.lead = F::kLead;
     p.spread = fminf((float)p.units * F::kRatio, (float)F::kBytesRatio / (float)p.groups);
-    const int64_t tiles = (int64_t)p.units * ((cap + kPT - 1) / kPT);  // at most
+    const int64_t each = (cap + kPT - 1) / kPT, tiles = p.units * each;  // at most
     const int64_t W = tiles + (int64_t)(p.units - 1) * p.lead;
-    // Where a call's tiles (the empty ones left out) leave CUs free, its heads are spread over them: a
+    // Where n ranges leave CUs free, a call's heads are spread over them: a
     // workgroup of few columns issues its queries, tiles' products and results
     // sooner (one row over 509 positions 18.9 us with 8 column groups a workgroup,
     // 15.8 with one; one row over 32 listed pages of 64 23.7 and 21.1).
-    const int32_t cus = ctx->multiprocessors, free = cus / plan_ranges(tiles, cus, p.spread);
-    p.per = free < p.groups ? (p.groups + free - 1) / free : 1;
-    p.per = p.per < F::kWaves ? p.per : F::kWaves;
-    p.chunks = (p.groups + p.per - 1) / p.per;
-    p.per = (p.groups + p.chunks - 1) / p.chunks;
+    const int32_t cus = ctx->multiprocessors;
+    auto spread_heads = [&](int32_t n) {
+        const int32_t free = n < cus ? cus / n : 1;
+        p.per = free < p.groups ? (p.groups + free - 1) / free : 1;
+        p.per = p.per < F::kWaves ? p.per : F::kWaves;
+        p.chunks = (p.groups + p.per - 1) / p.per;
+        p.per = (p.groups + p.chunks - 1) / p.chunks;
+    };
+    // Whole units, one or more after another on a CU, or equal ranges (the empty
+    // tiles do not count for the heads' spread) and their join, whichever takes
+    // fewer tiles' time by what the table holds at most.  Cut and whole: 49 rows of
+    // up to 24 positions 18.5 and 13.2 us, 54 x 2 of up to 365 44.5 and 30.1, 64 of
+    // up to 600 41.6 and 35.0, one of 200 15.6 and 17.5.
+    spread_heads(p.units);
+    const int64_t turns = ((int64_t)p.units * p.chunks + cus - 1) / cus, whole = turns * (each + p.lead) - p.lead;
+    spread_heads(plan_ranges(tiles, cus, p.spread));
     p.most = plan_ranges(W, p.chunks < cus ? cus / p.chunks : 1, p.spread);
-    const int64_t slots = p.most > 1 ? plan_slot(p.most, false) * p.groups : 0;
+    const float parts = (float)p.most * p.groups / F::kBytesRatio;
+    p.whole = (float)whole <= (float)W / p.most + F::kJoin + parts;
+    if (p.whole) {
+        spread_heads(p.units);
+        p.most = p.units;
+    }
+    const int64_t wgs = ((int64_t)p.most * p.chunks + 7) / 8 * 8;
+    if (p.whole) {
+        int tok = timing_begin(ctx, "paged_mfma");
+        hipLaunchKernelGGL((k_paged_mfma<F, SPARSE>), dim3((unsigned)wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
+        timing_end(ctx, tok);
+        return launch_check(ctx, "k_paged_mfma");
+    }
+    const int64_t slots = plan_slot(p.most, false) * p.groups;
     ScratchPlan plan;
     plan.add((size_t)slots * kPL * kCols * 4);
     plan.add((size_t)slots * kCols * 8);
@@ -902,12 +933,10 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     p.part_o = (float *)ptrs[0];
     p.part_ml = (float *)ptrs[1];
     p.plan = (int64_t *)ptrs[2];
-    const int64_t wgs = ((int64_t)p.most * p.chunks + 7) / 8 * 8;
     int tok = timing_begin(ctx, "paged_mfma");
     hipLaunchKernelGGL((k_paged_mfma<F, SPARSE>), dim3((unsigned)wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
     timing_end(ctx, tok);
     UT_TRY(launch_check(ctx, "k_paged_mfma"));
-    if (p.most == 1) return UT_OK;
     tok = timing_begin(ctx, "paged_join");
     hipLaunchKernelGGL((k_paged_join<F, SPARSE>), dim3((unsigned)((int64_t)p.units * p.groups), kPL / 64), dim3(256), 0,
                        ctx->stream, p);

@@ -1,6 +1,7 @@
 // ut_paged_plan.h -- how a batch over the paged cache is cut into equal
 // ranges of work, and the bounds of what its lengths and tables may say.
-// Plain arithmetic for the kernels and for the host.
+// Plain arithmetic for the kernels and for the host.  (Where every sequence is
+// short, a workgroup takes one whole, and there are no ranges.)
 //
 // The sequences' tiles stand in one row, one sequence after another, W in
 // all.  Range r of N takes the tiles [W r / N, W (r + 1) / N), so a ragged
