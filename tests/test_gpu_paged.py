@@ -204,7 +204,8 @@ def test_a_pool_past_32_bits(ctx):
 @pytest.mark.parametrize("lens,M,H,page,top_k", [
     ([400, 33, 0, 1], 2, 128, 16, 7), ([1000], 1, 128, 64, 5), ([700, 650], 3, 32, 32, 9),
     ([500, 20], 1, 16, 64, 3), ([300, 299], 1, 64, 8, 20), ([90, 200], 2, 4, 4, 11), ([2100, 70], 1, 48, 128, 4),
-    ([50, 61], 2, 32, 2, 13), ([100, 900], 1, 128, 16, 300), ([1100, 5], 2, 16, 1024, 1)])
+    ([50, 61], 2, 32, 2, 13), ([100, 900], 1, 128, 16, 300), ([1100, 5], 2, 16, 1024, 1),
+    ([20, 33, 0, 70], 1, 64, 32, 150), ([9, 16] * 40, 2, 32, 16, 3)])
 def test_attend_selected_pages(ctx, fmt, lens, M, H, page, top_k):
     """Entries in any order, gaps among them, pages behind the row's end, one
     listed twice, a row with none; pages that no row lists hold NaN."""

@@ -110,7 +110,21 @@ __device__ bool find_range(const PagedMfmaArgs &p, int64_t r, bool leave, Range 
     __shared__ int64_t found[2];
     const int tid = threadIdx.x;
     if (p.whole) {
-        g = {0, 0, __builtin_amdgcn_readfirstlane(unit_tiles<SPARSE>(p.a, (int)r)), (int)r, 0};
+        const PagedArgs &a = p.a;
+        const int u = (int)r;
+        g = {0, 0, __builtin_amdgcn_readfirstlane(unit_tiles<SPARSE>(a, u)), u, 0};
+        if (SPARSE && g.e > 0) {
+            // a list's tiles up to its last page that the row sees (one at least)
+            const int b = u / a.M, n = paged_len(a, b) - a.M + (u - b * a.M) + 1;
+            int64_t end = 0;
+            for (int32_t i = 0; i < a.top_k; i += 64) {
+                const int32_t at = i + (tid & 63), page = at < a.top_k ? a.sel[(int64_t)u * a.top_k + at] : -1;
+                const uint64_t seen = __ballot(page >= 0 && ((int64_t)page << a.shift) < n);
+                if (seen) end = i + 64 - __builtin_clzll(seen);
+            }
+            const int64_t tiles = ((end << a.shift) + kPT - 1) / kPT;
+            g.e = uniform(tiles > 0 ? tiles : 1);
+        }
         return g.e > 0;
     }
     if (p.units <= 64) {
@@ -760,7 +774,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
         if (more) start(nx);
         // ---- the unit's context, or this range's part of it
         const float sum = col_sum(wv.l);
-        if (active && q.b0 == 0 && q.b1 == q.tiles) {
+        if (active && ((SPARSE && p.whole) || (q.b0 == 0 && q.b1 == q.tiles))) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             typename F::out_t *out = (typename F::out_t *)a.out + row * kPL + 4 * g;
             if (q.h0 + col < a.H)
@@ -907,7 +921,11 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     // up to 24 positions 18.5 and 13.2 us, 54 x 2 of up to 365 44.5 and 30.1, 64 of
     // up to 600 41.6 and 35.0, one of 200 15.6 and 17.5.
     spread_heads(p.units);
-    const int64_t turns = ((int64_t)p.units * p.chunks + cus - 1) / cus, whole = turns * (each + p.lead) - p.lead;
+    // (no more pages are to be expected of a list than the table holds: 20 rows of
+    // one page and 12 places in f16 pairs 33.0 us cut, 18.6 whole)
+    const int64_t listed = (((int64_t)(a.top_k < a.max_pages ? a.top_k : a.max_pages) << a.shift) + kPT - 1) / kPT;
+    const int64_t turns = ((int64_t)p.units * p.chunks + cus - 1) / cus;
+    const int64_t whole = turns * ((SPARSE ? listed : each) + p.lead) - p.lead;
     spread_heads(plan_ranges(tiles, cus, p.spread));
     p.most = plan_ranges(W, p.chunks < cus ? cus / p.chunks : 1, p.spread);
     const float parts = (float)p.most * p.groups / F::kBytesRatio;
