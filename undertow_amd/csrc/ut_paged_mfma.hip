@@ -801,14 +801,14 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
 
 // Joins the parts of a unit that lies in more than one range:
 // out = sum_r o_r 2^(m_r - M) / sum_r l_r 2^(m_r - M).  A workgroup takes one
-// column group and 64 dims, each of its waves every fourth part, as many at a
+// column group and 64 dims, each of its NW waves every NW-th part, as many at a
 // time as there are, with all their loads under way; the waves' results meet
 // in LDS.  Bound by the parts' bytes: 82 MB in 16.9 us (4.9 TB/s); 8 parts of
 // one row take 4.2.
-template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_join(PagedMfmaArgs p) {
+template <class F, bool SPARSE, int NW> __global__ __launch_bounds__(NW * 64) void k_paged_join(PagedMfmaArgs p) {
     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
-    __shared__ __attribute__((aligned(16))) pf32x4 so[4][16][kCols + 1];  // one more: other banks
-    __shared__ float2 sml[4][kCols];
+    __shared__ __attribute__((aligned(16))) pf32x4 so[NW][16][kCols + 1];  // one more: other banks
+    __shared__ float2 sml[NW][kCols];
     const PagedArgs &a = p.a;
     const int u = blockIdx.x / p.groups, grp = blockIdx.x - u * p.groups, tid = threadIdx.x;
     const int w = tid >> 6, col = tid & 15, qd = (tid >> 4) & 3;
@@ -820,14 +820,14 @@ template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_j
     if (r0 == r1) return;
     float m = kLow, L = 0.0f;
     pf32x4 t[4] = {};
-    // N parts, r and every fourth behind it
+    // some parts: r and every NW-th behind it
     auto add = [&](int r, auto many) {
         constexpr int COUNT = decltype(many)::value;
         float2 ml[COUNT];
         pf32x4 v[COUNT][4];
 #pragma unroll
         for (int i = 0; i < COUNT; i++) {
-            const int x = r + 4 * i;
+            const int x = r + NW * i;
             const int64_t slot = plan_slot(x, x == r0) * p.groups + grp;
             ml[i] = *(const float2 *)(p.part_ml + (slot * kCols + col) * 2);
 #pragma unroll
@@ -853,14 +853,14 @@ template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_j
         m = mn;
     };
     int r = r0 + w;
-    for (; r + 28 <= r1; r += 32) add(r, std::integral_constant<int, 8>());
-    if (r + 12 <= r1) {
+    for (; r + 7 * NW <= r1; r += 8 * NW) add(r, std::integral_constant<int, 8>());
+    if (r + 3 * NW <= r1) {
         add(r, std::integral_constant<int, 4>());
-        r += 16;
+        r += 4 * NW;
     }
-    if (r + 4 <= r1) {
+    if (r + NW <= r1) {
         add(r, std::integral_constant<int, 2>());
-        r += 8;
+        r += 2 * NW;
     }
     if (r <= r1) add(r, std::integral_constant<int, 1>());
     if (qd == 0) sml[w][col] = make_float2(m, L);
@@ -868,13 +868,14 @@ template <class F, bool SPARSE> __global__ __launch_bounds__(256) void k_paged_j
     for (int k = 0; k < 4; k++) so[w][qd + 4 * k][col] = t[k];
     __syncthreads();
     // thread: four dims (tid & 15) of column tid >> 4
+    if (tid >= 256) return;
     const int c = tid >> 4, d = tid & 15;
     float M = kLow, sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) M = fmaxf(M, sml[i][c].x);
+    for (int i = 0; i < NW; i++) M = fmaxf(M, sml[i][c].x);
     pf32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < NW; i++) {
         const float f = __builtin_amdgcn_exp2f(sml[i][c].x - M);
         const pf32x4 v = so[i][d][c];
         sum = __builtin_fmaf(sml[i][c].y, f, sum);
@@ -900,7 +901,6 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     p.groups = (SPARSE ? 1 : a.M) * ((a.H + kCols - 1) / kCols);
     const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
     p.lead = F::kLead;
-    p.spread = fminf((float)p.units * F::kRatio, (float)F::kBytesRatio / (float)p.groups);
     const int64_t each = (cap + kPT - 1) / kPT, tiles = p.units * each;  // at most
     const int64_t W = tiles + (int64_t)(p.units - 1) * p.lead;
     // Where n ranges leave CUs free, a call's heads are spread over them: a
@@ -926,21 +926,32 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     const int64_t listed = (((int64_t)(a.top_k < a.max_pages ? a.top_k : a.max_pages) << a.shift) + kPT - 1) / kPT;
     const int64_t turns = ((int64_t)p.units * p.chunks + cus - 1) / cus;
     const int64_t whole = turns * ((SPARSE ? listed : each) + p.lead) - p.lead;
-    spread_heads(plan_ranges(tiles, cus, p.spread));
-    p.most = plan_ranges(W, p.chunks < cus ? cus / p.chunks : 1, p.spread);
+    auto cut = [&](int32_t ratio) {
+        p.spread = fminf((float)p.units * ratio, (float)F::kBytesRatio / (float)p.groups);
+        spread_heads(plan_ranges(tiles, cus, p.spread));
+        p.most = plan_ranges(W, p.chunks < cus ? cus / p.chunks : 1, p.spread);
+    };
+    cut(F::kRatio);
     const float parts = (float)p.most * p.groups / F::kBytesRatio;
     p.whole = (float)whole <= (float)W / p.most + F::kJoin + parts;
-    if (p.whole) {
-        spread_heads(p.units);
-        p.most = p.units;
-    }
-    const int64_t wgs = ((int64_t)p.most * p.chunks + 7) / 8 * 8;
-    if (p.whole) {
+    auto launch = [&]() -> int32_t {
+        const int64_t wgs = ((int64_t)p.most * p.chunks + 7) / 8 * 8;
         int tok = timing_begin(ctx, "paged_mfma");
         hipLaunchKernelGGL((k_paged_mfma<F, SPARSE>), dim3((unsigned)wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
         timing_end(ctx, tok);
         return launch_check(ctx, "k_paged_mfma");
+    };
+    if (p.whole) {
+        spread_heads(p.units);
+        p.most = p.units;
+        return launch();
     }
+    // The join takes 16 waves a workgroup, and twice the ranges pay, where there
+    // are few units of many parts: one row over 32768 positions 42.8 us with 4 waves,
+    // 39.5 with 16, 37.2 with the ranges (over 509, 8 parts, 15.5 and 15.9).
+    const dim3 grid((unsigned)((int64_t)p.units * p.groups), kPL / 64);
+    const bool wide = (int64_t)grid.x * grid.y <= cus && p.most > 16 * p.units;
+    if (wide) cut(2 * F::kRatio);
     const int64_t slots = plan_slot(p.most, false) * p.groups;
     ScratchPlan plan;
     plan.add((size_t)slots * kPL * kCols * 4);
@@ -951,13 +962,12 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     p.part_o = (float *)ptrs[0];
     p.part_ml = (float *)ptrs[1];
     p.plan = (int64_t *)ptrs[2];
-    int tok = timing_begin(ctx, "paged_mfma");
-    hipLaunchKernelGGL((k_paged_mfma<F, SPARSE>), dim3((unsigned)wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
-    timing_end(ctx, tok);
-    UT_TRY(launch_check(ctx, "k_paged_mfma"));
-    tok = timing_begin(ctx, "paged_join");
-    hipLaunchKernelGGL((k_paged_join<F, SPARSE>), dim3((unsigned)((int64_t)p.units * p.groups), kPL / 64), dim3(256), 0,
-                       ctx->stream, p);
+    UT_TRY(launch());
+    int tok = timing_begin(ctx, "paged_join");
+    if (wide)
+        hipLaunchKernelGGL((k_paged_join<F, SPARSE, 16>), grid, dim3(1024), 0, ctx->stream, p);
+    else
+        hipLaunchKernelGGL((k_paged_join<F, SPARSE, 4>), grid, dim3(256), 0, ctx->stream, p);
     timing_end(ctx, tok);
     return launch_check(ctx, "k_paged_join");
 }
