@@ -344,8 +344,8 @@ int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *
  * heads, latent], q_rope [batch, rows, heads, rope], clat like qabs, in the
  * cache format's type.  A row that sees nothing gets zeros.  What a row does
  * not see does not reach it, NaN and infinities included.  Equal calls give
- * equal bits; a row's rounding may depend on the lengths of the batch (the
- * work is cut evenly over the device). */
+ * equal bits; a row's rounding may depend on the sizes of the call and the
+ * lengths of its batch (the work is cut evenly over the device). */
 int32_t ut_mla_paged_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
                             int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
                             int64_t batch, int64_t rows, int64_t heads, const void *qabs_dev,

@@ -646,3 +646,39 @@ def test_two_contexts_at_once(ctx):
     for pair in both:
         for got, want in zip(pair, alone):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_captured_calls_share_the_arena(ctx):
+    """Two graphs of one context, the second captured with more working memory
+    than the first, replayed in turn with eager calls between: each replay has
+    the eager call's bits."""
+    import undertow_amd as U
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rnd = lambda *d: torch.randn(d, device="cuda", generator=g)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        c = U.Context(0)
+        cache = U.PagedCache.empty(c, 400, page=16)
+        table = torch.randperm(400, device="cuda", generator=g).reshape(4, 100).int()
+        lens = torch.tensor([1600, 3, 700, 1111], dtype=torch.int32, device="cuda")
+        cache.append(table, lens, rnd(4, 1600, 512), rnd(4, 1600, 64))
+        calls = []
+        for rows, n in ((1, 1), (3, 4)):
+            q = rnd(n, rows, 128, 512).bfloat16(), rnd(n, rows, 128, 64).bfloat16()
+            calls.append((lambda t, x, q: lambda: cache.attend(t, x, *q, SCALE))(table[:n], lens[:n], q))
+        graphs = []
+        for f in calls:
+            f()
+            s.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                out = f()
+            graphs.append((graph, out))
+        for turn in range(4):
+            lens -= turn
+            want = [f().clone() for f in calls]
+            for (graph, out), w in list(zip(graphs, want))[::1 if turn % 2 else -1]:
+                out.zero_()
+                graph.replay()
+                s.synchronize()
+                assert torch.equal(out, w)

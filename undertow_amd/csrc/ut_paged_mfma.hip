@@ -903,10 +903,11 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     p.lead = F::kLead;
     const int64_t each = (cap + kPT - 1) / kPT, tiles = p.units * each;  // at most
     const int64_t W = tiles + (int64_t)(p.units - 1) * p.lead;
-    // Where n ranges leave CUs free, a call's heads are spread over them: a
-    // workgroup of few columns issues its queries, tiles' products and results
-    // sooner (one row over 509 positions 18.9 us with 8 column groups a workgroup,
-    // 15.8 with one; one row over 32 listed pages of 64 23.7 and 21.1).
+    // Where n ranges (or whole units) leave CUs free, a call's heads are
+    // spread over them: a workgroup of few columns issues its queries, tiles'
+    // products and results sooner (one row over 509 positions 18.9 us with 8
+    // column groups a workgroup, 15.8 with one; one row over 32 listed pages
+    // of 64 23.7 and 21.1).
     const int32_t cus = ctx->multiprocessors;
     auto spread_heads = [&](int32_t n) {
         const int32_t free = n < cus ? cus / n : 1;
