@@ -1,0 +1,91 @@
+"""How a call of paged attention is cut (plan_call in
+undertow_amd/csrc/ut_paged_plan.h), on the CPU, for both cache
+formats: what it launches covers the call, and it reserves no more than the
+parts that can be made."""
+import ctypes as C
+import random
+import subprocess
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "undertow_amd" / "csrc"
+CUS = 256
+
+SRC = r"""
+#include "ut_paged_plan.h"
+extern "C" {
+void costs(int bf16, ut::PlanCosts *c) { *c = bf16 ? ut::kCostsBf16 : ut::kCostsF16x2; }
+void cut(const ut::PlanCosts *c, int cus, int units, int groups, int64_t each, int64_t listed, ut::PlanCall *out) {
+    *out = ut::plan_call(*c, cus, units, groups, each, listed);
+}
+}
+"""
+
+
+class Costs(C.Structure):
+    _fields_ = [("waves", C.c_int32), ("lead", C.c_int32), ("ratio", C.c_int32), ("bytes_ratio", C.c_int32),
+                ("join", C.c_float)]
+
+
+class Call(C.Structure):
+    _fields_ = [("whole", C.c_int32), ("most", C.c_int32), ("per", C.c_int32), ("chunks", C.c_int32),
+                ("wide", C.c_int32), ("spread", C.c_float), ("slots", C.c_int64)]
+
+
+
+@pytest.fixture(scope="module")
+def cut(tmp_path_factory):
+    d = tmp_path_factory.mktemp("cut")
+    (d / "c.cpp").write_text(SRC)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", str(CSRC), "-o", str(d / "c.so"),
+                    str(d / "c.cpp")], check=True)
+    lib = C.CDLL(str(d / "c.so"))
+    f, costs = lib.cut, {}
+    f.restype, f.argtypes = None, [C.POINTER(Costs), C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int64, C.POINTER(Call)]
+    lib.costs.restype, lib.costs.argtypes = None, [C.c_int, C.POINTER(Costs)]
+    for fmt in ("bf16", "f16x2"):
+        costs[fmt] = Costs()
+        lib.costs(fmt == "bf16", C.byref(costs[fmt]))
+
+    def call(fmt, sequences, rows, heads, positions):
+        out, each = Call(), -(-positions // 32)
+        f(costs[fmt], CUS, sequences, rows * -(-heads // 16), each, each, out)
+        return out
+    call.waves = {k: c.waves for k, c in costs.items()}
+    return call
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f16x2"])
+@pytest.mark.parametrize("seed", range(20))
+def test_a_call_is_covered_and_reserves_what_its_parts_take(cut, fmt, seed):
+    rng = random.Random(seed)
+    log = lambda lo, hi: round(lo * (hi / lo) ** rng.random())
+    for _ in range(200):
+        B = log(1, 65535)
+        M = log(1, max(1, 65535 // B))
+        H = rng.choice([1, 16, 20, 64, 128, 160, 1000])
+        p = cut(fmt, B, M, H, log(1, 2**31 - 1024))
+        groups, waves = M * -(-H // 16), cut.waves[fmt]
+        assert 1 <= p.per <= waves and p.per * p.chunks >= groups and p.per * (p.chunks - 1) < groups
+        if p.whole:
+            assert p.most == B and p.slots == 0
+        elif p.most == 1:
+            assert p.slots == 0
+        else:  # ranges that run at once, two places each
+            assert p.most * p.chunks <= CUS and p.slots == 2 * p.most * groups <= 2 * CUS * waves
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f16x2"])
+@pytest.mark.parametrize("B,M", [(1, 512), (1, 2048), (1, 8192), (1, 65535), (3, 777), (4, 256), (2, 20000)])
+@pytest.mark.parametrize("positions", [100, 2000, 32768, 1 << 20])
+def test_prompt_rows_leave_no_parts(cut, fmt, B, M, positions):
+    p = cut(fmt, B, M, 128, max(M, positions))
+    assert p.slots == 0 and (p.whole or p.most == 1)
+
+
+def test_one_range_counts_its_rounds_over_the_cus(cut):
+    """777 workgroups take four rounds over all sequences, 3 x 777 ten over one."""
+    assert cut("bf16", 3, 777, 128, 1900).whole
+    p = cut("bf16", 4, 256, 128, 4096)  # four rounds of one, or one of four: equal shares
+    assert not p.whole and p.most == 1

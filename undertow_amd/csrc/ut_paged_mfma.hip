@@ -19,7 +19,8 @@
 //   as it lies, V transposed by the LDS reads, and three further tiles are on
 //   their way, straight to LDS.
 // - equal ranges of the whole batch's tiles, one workgroup a CU
-//   (ut_paged_plan.h), and a join of what the ranges leave (k_paged_join).
+//   (ut_paged_plan.h), and a join of what the ranges leave (k_paged_join); whole
+//   sequences, or one range, where there is nothing to join.
 //
 // A tile of 128 heads takes 1.95 us: 1.17 PFLOP/s and, with one row a sequence,
 // 4.8 TB/s over 256 CUs; the LDS reads alone would take 1.1 us of it (K 288 KB
@@ -45,6 +46,7 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 constexpr int kPT = 32;             // positions per tile
 constexpr int kPL = 512, kPD = 576;
 constexpr int kCols = 16;           // heads per column group (a wave's)
+static_assert(kPlanJoinSlices * 64 == kPL, "a workgroup of the join takes 64 dims");
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLow = -3.402823466e38f;  // the offset before any score
 
@@ -59,7 +61,7 @@ struct PagedMfmaArgs {
     int32_t whole;    // a range is a unit (most: units), and there is no join
     float *part_o;    // [slot][group][128 quads][16 columns][4]
     float *part_ml;   // [slot][group][16 columns][2]
-    int64_t *plan;    // [units] first tile of each, then W
+    int64_t *plan;    // [units] first tile of each, then W (where there is more than one range)
     int32_t lead;     // empty tiles before every unit with tiles but the first
 };
 
@@ -248,22 +250,10 @@ template <int PLANES> __device__ __forceinline__ LaneAddr lane_addr(int l) {
 
 // bf16 pages: queries and weights in bf16.
 struct MfmaBf16 {
-    static constexpr int kPlanes = 1, kWaves = 8;
+    static constexpr PlanCosts kCosts = kCostsBf16;
+    static constexpr int kPlanes = 1, kWaves = kCosts.waves;
     static constexpr bool kBetween = false;  // copies between the products (the branches cost registers)
     static constexpr int kDepth = 4;
-    // empty tiles that stand for the queries, first tiles and result of a
-    // sequence that begins in a range: 64 sequences of up to 8192 positions take
-    // 135 us with 0, 132 with 2, 126 with 4, 115 with 8, 117 with 16
-    static constexpr int kLead = 8;
-    // a tile's time to a part's in the join (plan_ranges): one row over 32768
-    // positions takes 48 us with 2, 44 with 3, 42 with 4, 41 with 8, and 59 in as
-    // many ranges as CUs; 4 rows over 500 positions 19.8, 20.8, 20.4, 24.3
-    static constexpr int kRatio = 4;
-    // and to that of a column group's part's bytes, written and read (2 x 32 KB at
-    // a 5 TB/s that all share): 5 x 4 rows over up to 2083 positions 39.3 us
-    // without, 36.4 with 150, 35.3 with 75; 49 rows of up to 24 20.3, 18.5, 24.7
-    static constexpr int kBytesRatio = 150;
-    static constexpr float kJoin = 2.5f;  // the join's launch, in tiles
     static constexpr float kRise = 11.5f;  // log2 units a score may exceed the offset (8 nats)
     typedef __bf16 out_t;
     struct Query {
@@ -345,18 +335,10 @@ struct MfmaBf16 {
 // range where they matter.  Three products a score bound it: 33 rows of 128
 // heads over up to 4099 positions (61 GFLOP in f16) take 96 us, floor 52.
 struct MfmaF16x2 {
-    static constexpr int kPlanes = 2, kWaves = 4;
+    static constexpr PlanCosts kCosts = kCostsF16x2;
+    static constexpr int kPlanes = 2, kWaves = kCosts.waves;
     static constexpr bool kBetween = true;
     static constexpr int kDepth = 4;
-    // (a tile takes twice as long: 11 x 3 rows 103 us with 0, 96.1 with 2, 96.4
-    // with 4, 99.7 with 8)
-    static constexpr int kLead = 4;
-    // one row over 500 positions 22.0 us with 4, 19.5 with 16; over 10000 43.2
-    // in as many ranges as CUs, 40.0 with 16, 40.6 with 32
-    static constexpr int kRatio = 16;
-    // 63 x 4 rows of up to 25 positions 66.5 us without and with 280, 80.4 with 140
-    static constexpr int kBytesRatio = 280;
-    static constexpr float kJoin = 1.3f;
     static constexpr float kRise = 1.0f;
     typedef float out_t;
     struct Query {
@@ -658,7 +640,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
         if (unit_tiles<SPARSE>(a, u) == 0)
             for (int64_t i = tid; i < vec; i += NW * 64) ((pu32x4 *)a.out)[u * vec + i] = pu32x4{0, 0, 0, 0};
     Range rg;
-    if (r >= p.most || !find_range<SPARSE, NW>(p, r, r == 0 && chunk == 0, rg)) return;
+    if (r >= p.most || !find_range<SPARSE, NW>(p, r, p.most > 1 && r == 0 && chunk == 0, rg)) return;
     const int grp = chunk * p.per + w;
     const bool active = w < p.per && grp < p.groups;
     const int gr = active ? grp : 0;
@@ -900,41 +882,17 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     p.units = SPARSE ? a.B * a.M : a.B;
     p.groups = (SPARSE ? 1 : a.M) * ((a.H + kCols - 1) / kCols);
     const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
-    p.lead = F::kLead;
-    const int64_t each = (cap + kPT - 1) / kPT, tiles = p.units * each;  // at most
-    const int64_t W = tiles + (int64_t)(p.units - 1) * p.lead;
-    // Where n ranges (or whole units) leave CUs free, a call's heads are
-    // spread over them: a workgroup of few columns issues its queries, tiles'
-    // products and results sooner (one row over 509 positions 18.9 us with 8
-    // column groups a workgroup, 15.8 with one; one row over 32 listed pages
-    // of 64 23.7 and 21.1).
-    const int32_t cus = ctx->multiprocessors;
-    auto spread_heads = [&](int32_t n) {
-        const int32_t free = n < cus ? cus / n : 1;
-        p.per = free < p.groups ? (p.groups + free - 1) / free : 1;
-        p.per = p.per < F::kWaves ? p.per : F::kWaves;
-        p.chunks = (p.groups + p.per - 1) / p.per;
-        p.per = (p.groups + p.chunks - 1) / p.chunks;
-    };
-    // Whole units, one or more after another on a CU, or equal ranges (the empty
-    // tiles do not count for the heads' spread) and their join, whichever takes
-    // fewer tiles' time by what the table holds at most.  Cut and whole: 49 rows of
-    // up to 24 positions 18.5 and 13.2 us, 54 x 2 of up to 365 44.5 and 30.1, 64 of
-    // up to 600 41.6 and 35.0, one of 200 15.6 and 17.5.
-    spread_heads(p.units);
+    p.lead = F::kCosts.lead;
+    const int64_t each = (cap + kPT - 1) / kPT;
     // (no more pages are to be expected of a list than the table holds: 20 rows of
     // one page and 12 places in f16 pairs 33.0 us cut, 18.6 whole)
     const int64_t listed = (((int64_t)(a.top_k < a.max_pages ? a.top_k : a.max_pages) << a.shift) + kPT - 1) / kPT;
-    const int64_t turns = ((int64_t)p.units * p.chunks + cus - 1) / cus;
-    const int64_t whole = turns * ((SPARSE ? listed : each) + p.lead) - p.lead;
-    auto cut = [&](int32_t ratio) {
-        p.spread = fminf((float)p.units * ratio, (float)F::kBytesRatio / (float)p.groups);
-        spread_heads(plan_ranges(tiles, cus, p.spread));
-        p.most = plan_ranges(W, p.chunks < cus ? cus / p.chunks : 1, p.spread);
-    };
-    cut(F::kRatio);
-    const float parts = (float)p.most * p.groups / F::kBytesRatio;
-    p.whole = (float)whole <= (float)W / p.most + F::kJoin + parts;
+    const PlanCall plan = plan_call(F::kCosts, ctx->multiprocessors, p.units, p.groups, each, SPARSE ? listed : each);
+    p.whole = plan.whole;
+    p.most = plan.most;
+    p.per = plan.per;
+    p.chunks = plan.chunks;
+    p.spread = plan.spread;
     auto launch = [&]() -> int32_t {
         const int64_t wgs = ((int64_t)p.most * p.chunks + 7) / 8 * 8;
         int tok = timing_begin(ctx, "paged_mfma");
@@ -942,30 +900,20 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
         timing_end(ctx, tok);
         return launch_check(ctx, "k_paged_mfma");
     };
-    if (p.whole) {
-        spread_heads(p.units);
-        p.most = p.units;
-        return launch();
-    }
-    // The join takes 16 waves a workgroup, and twice the ranges pay, where there
-    // are few units of many parts: one row over 32768 positions 42.8 us with 4 waves,
-    // 39.5 with 16, 37.2 with the ranges (over 509, 8 parts, 15.5 and 15.9).
-    const dim3 grid((unsigned)((int64_t)p.units * p.groups), kPL / 64);
-    const bool wide = (int64_t)grid.x * grid.y <= cus && p.most > 16 * p.units;
-    if (wide) cut(2 * F::kRatio);
-    const int64_t slots = plan_slot(p.most, false) * p.groups;
-    ScratchPlan plan;
-    plan.add((size_t)slots * kPL * kCols * 4);
-    plan.add((size_t)slots * kCols * 8);
-    plan.add((size_t)(p.units + 1) * 8);
+    if (plan.slots == 0) return launch();  // nothing is left to join
+    ScratchPlan scratch;
+    scratch.add((size_t)plan.slots * kPL * kCols * 4);
+    scratch.add((size_t)plan.slots * kCols * 8);
+    scratch.add((size_t)(p.units + 1) * 8);
     std::vector<void *> ptrs;
-    UT_TRY(scratch_acquire(ctx, plan, ptrs));
+    UT_TRY(scratch_acquire(ctx, scratch, ptrs));
     p.part_o = (float *)ptrs[0];
     p.part_ml = (float *)ptrs[1];
     p.plan = (int64_t *)ptrs[2];
     UT_TRY(launch());
+    const dim3 grid((unsigned)((int64_t)p.units * p.groups), kPlanJoinSlices);
     int tok = timing_begin(ctx, "paged_join");
-    if (wide)
+    if (plan.wide)
         hipLaunchKernelGGL((k_paged_join<F, SPARSE, 16>), grid, dim3(1024), 0, ctx->stream, p);
     else
         hipLaunchKernelGGL((k_paged_join<F, SPARSE, 4>), grid, dim3(256), 0, ctx->stream, p);
