@@ -16,8 +16,9 @@ SRC = r"""
 #include "ut_paged_plan.h"
 extern "C" {
 void costs(int bf16, ut::PlanCosts *c) { *c = bf16 ? ut::kCostsBf16 : ut::kCostsF16x2; }
-void cut(const ut::PlanCosts *c, int cus, int units, int groups, int64_t each, int64_t listed, ut::PlanCall *out) {
-    *out = ut::plan_call(*c, cus, units, groups, each, listed);
+void cut(const ut::PlanCosts *c, int cus, int units, int groups, int64_t each, int64_t listed, int lists,
+         ut::PlanCall *out) {
+    *out = ut::plan_call(*c, cus, units, groups, each, listed, lists);
 }
 }
 """
@@ -25,7 +26,7 @@ void cut(const ut::PlanCosts *c, int cus, int units, int groups, int64_t each, i
 
 class Costs(C.Structure):
     _fields_ = [("waves", C.c_int32), ("lead", C.c_int32), ("ratio", C.c_int32), ("bytes_ratio", C.c_int32),
-                ("join", C.c_float)]
+                ("join", C.c_float), ("brief", C.c_int32)]
 
 
 class Call(C.Structure):
@@ -42,15 +43,16 @@ def cut(tmp_path_factory):
                     str(d / "c.cpp")], check=True)
     lib = C.CDLL(str(d / "c.so"))
     f, costs = lib.cut, {}
-    f.restype, f.argtypes = None, [C.POINTER(Costs), C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int64, C.POINTER(Call)]
+    f.restype, f.argtypes = None, [C.POINTER(Costs), C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int,
+                                   C.POINTER(Call)]
     lib.costs.restype, lib.costs.argtypes = None, [C.c_int, C.POINTER(Costs)]
     for fmt in ("bf16", "f16x2"):
         costs[fmt] = Costs()
         lib.costs(fmt == "bf16", C.byref(costs[fmt]))
 
-    def call(fmt, sequences, rows, heads, positions):
+    def call(fmt, sequences, rows, heads, positions, lists=False):
         out, each = Call(), -(-positions // 32)
-        f(costs[fmt], CUS, sequences, rows * -(-heads // 16), each, each, out)
+        f(costs[fmt], CUS, sequences, rows * -(-heads // 16), each, each, lists, out)
         return out
     call.waves = {k: c.waves for k, c in costs.items()}
     return call
@@ -89,3 +91,22 @@ def test_one_range_counts_its_rounds_over_the_cus(cut):
     assert cut("bf16", 3, 777, 128, 1900).whole
     p = cut("bf16", 4, 256, 128, 4096)  # four rounds of one, or one of four: equal shares
     assert not p.whole and p.most == 1
+
+
+@pytest.mark.parametrize("fmt,B,M,H,whole_at,cut_at", [
+    ("bf16", 64, 1, 128, 600, 1024), ("bf16", 64, 4, 128, 1024, 4096), ("bf16", 256, 1, 128, 1024, 2048),
+    ("bf16", 128, 2, 128, 1024, 4096), ("bf16", 32, 8, 128, 1024, 4096), ("bf16", 200, 1, 16, 300, 1000),
+    ("bf16", 500, 1, 128, 500, 2000), ("f16x2", 128, 1, 128, 300, 600), ("f16x2", 64, 2, 128, 100, 600)])
+def test_long_sequences_of_differing_lengths_are_cut(cut, fmt, B, M, H, whole_at, cut_at):
+    """As measured on lengths spread evenly up to the table's width: whole
+    sequences while they are short, ranges from there on at any length, also
+    where the workgroups of whole sequences fill the device to the last CU."""
+    assert cut(fmt, B, M, H, whole_at).whole and cut(fmt, B, M, H, whole_at // 4).whole
+    for n in (cut_at, 2 * cut_at, 4 * cut_at, 32 * cut_at):
+        assert not cut(fmt, B, M, H, n).whole, n
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f16x2"])
+def test_a_list_counts_in_full(cut, fmt):
+    """Rows of a batch choose as many pages each: 256 lists of 16 pages of 64."""
+    assert cut(fmt, 256, 1, 128, 1024, lists=True).whole

@@ -887,7 +887,8 @@ template <class F, bool SPARSE> static int32_t launch_fmt(ut_ctx *ctx, const Pag
     // (no more pages are to be expected of a list than the table holds: 20 rows of
     // one page and 12 places in f16 pairs 33.0 us cut, 18.6 whole)
     const int64_t listed = (((int64_t)(a.top_k < a.max_pages ? a.top_k : a.max_pages) << a.shift) + kPT - 1) / kPT;
-    const PlanCall plan = plan_call(F::kCosts, ctx->multiprocessors, p.units, p.groups, each, SPARSE ? listed : each);
+    const PlanCall plan =
+        plan_call(F::kCosts, ctx->multiprocessors, p.units, p.groups, each, SPARSE ? listed : each, SPARSE);
     p.whole = plan.whole;
     p.most = plan.most;
     p.per = plan.per;

@@ -1,7 +1,8 @@
 // ut_paged_plan.h -- how a batch over the paged cache is cut into equal
 // ranges of work, and the bounds of what its lengths and tables may say.
 // Plain arithmetic for the kernels and for the host.  (Where every sequence is
-// short, a workgroup takes one whole, and there are no ranges.)
+// short by what the table holds, a workgroup takes one whole, and there are no
+// ranges: plan_call.)
 //
 // The sequences' tiles stand in one row, one sequence after another, W in
 // all.  Range r of N takes the tiles [W r / N, W (r + 1) / N), so a ragged
@@ -64,6 +65,7 @@ struct PlanCosts {  // of a cache format
     int32_t ratio;        // a tile's time to a part's in the join (plan_ranges)
     int32_t bytes_ratio;  // and to that of a column group's part's bytes, written and read
     float join;           // the join's launch, in tiles
+    int32_t brief;        // a sequence of so few tiles does not pay for the cut (plan_call)
 };
 // lead: 64 sequences of up to 8192 positions take 135 us with 0, 132 with 2, 126
 // with 4, 115 with 8, 117 with 16.  ratio: one row over 32768 positions 48 us
@@ -71,13 +73,13 @@ struct PlanCosts {  // of a cache format
 // rows over 500 positions 19.8, 20.8, 20.4, 24.3.  bytes_ratio (2 x 32 KB at a 5
 // TB/s that all share): 5 x 4 rows over up to 2083 positions 39.3 us without,
 // 36.4 with 150, 35.3 with 75; 49 rows of up to 24 20.3, 18.5, 24.7.
-constexpr PlanCosts kCostsBf16 = {8, 8, 4, 150, 2.5f};
+constexpr PlanCosts kCostsBf16 = {8, 8, 4, 150, 2.5f, 20};
 // (a tile takes twice as long) lead: 11 x 3 rows 103 us with 0, 96.1 with 2, 96.4
 // with 4, 99.7 with 8.  ratio: one row over 500 positions 22.0 us with 4, 19.5
 // with 16; over 10000 43.2 in as many ranges as CUs, 40.0 with 16, 40.6 with 32.
 // bytes_ratio: 63 x 4 rows of up to 25 positions 66.5 us without and with 280,
 // 80.4 with 140.
-constexpr PlanCosts kCostsF16x2 = {4, 4, 16, 280, 1.3f};
+constexpr PlanCosts kCostsF16x2 = {4, 4, 16, 280, 1.3f, 10};
 struct PlanCall {
     int32_t whole;        // a range is a unit: no parts, no join
     int32_t most;         // ranges at most (whole: units)
@@ -97,14 +99,23 @@ inline void plan_heads(PlanCall &p, const PlanCosts &c, int32_t cus, int32_t gro
     p.chunks = (groups + p.per - 1) / p.per;
     p.per = (groups + p.chunks - 1) / p.chunks;
 }
-// `units` units of `groups` column groups and of `each` tiles at most, of which
-// `listed` are to be expected of a list.
+// `units` units of `groups` column groups and of `each` tiles at most; of a list
+// (`lists`) `listed` are to be expected, of a table half: a batch's lengths
+// differ, and its longest sequence sets the table's width.
 //
 // Whole units, one or more after another on a CU, or equal ranges (the empty
 // tiles do not count for the heads' spread) and their join, whichever takes
-// fewer tiles' time.  Cut and whole: 49 rows of up to 24 positions 18.5 and 13.2
-// us, 54 x 2 of up to 365 44.5 and 30.1, 64 of up to 600 41.6 and 35.0, one of
-// 200 15.6 and 17.5.
+// fewer tiles' time: whole units that of the longest one, ranges that of the
+// tiles there are.  Cut and whole, lengths spread evenly up to the longest: 64
+// sequences of up to 1024 positions 45 and 48 us, of up to 8192 113 and 313; 256
+// of up to 1024 105 and 85, of up to 4096 218 and 264; 64 x 4 of up to 1024 94 and
+// 78, of up to 4096 189 and 245.  All of them that long: 256 of 2048 204 and 177,
+// 64 x 4 of 4096 309 and 291; one of them, the others a sixteenth: 65 and 127, 75
+// and 229; none of them, all a sixteenth of the table: 66 and 32, 55 and 38 (a
+// table cut to the pages in use is cheaper).
+// Up to `brief` tiles a sequence the ranges' tiles count in full: they save
+// little where one is long, and cost more where all are.  64 of up to 600
+// positions 40 and 34 us, all of them that long 47 and 36, one of them 32 and 34.
 //
 // Where a unit's column groups alone fill the CUs (prompt rows), there is one
 // range: its workgroups each go through all units, in rounds over the CUs,
@@ -115,9 +126,9 @@ inline void plan_heads(PlanCall &p, const PlanCosts &c, int32_t cus, int32_t gro
 // with equal ones; 3 x 777 over up to 1900 (whole 0.86 of the range) 1249 and 1368,
 // 1341 and 1781; in f16 pairs (0.92) 5.35 ms and 4.63, 5.33 and 5.93.
 inline PlanCall plan_call(const PlanCosts &c, int32_t cus, int32_t units, int32_t groups, int64_t each,
-                          int64_t listed) {
+                          int64_t listed, bool lists) {
     PlanCall p{};
-    const int64_t tiles = units * each, W = tiles + (int64_t)(units - 1) * c.lead;
+    const int64_t tiles = units * each, empty = (int64_t)(units - 1) * c.lead, W = tiles + empty;
     plan_heads(p, c, cus, groups, units);
     const int64_t turns = ((int64_t)units * p.chunks + cus - 1) / cus;
     const float whole = (float)(turns * (listed + c.lead) - c.lead);
@@ -127,12 +138,13 @@ inline PlanCall plan_call(const PlanCosts &c, int32_t cus, int32_t units, int32_
         p.most = plan_ranges(W, p.chunks < cus ? cus / p.chunks : 1, p.spread);
     };
     cut(c.ratio);
-    const int64_t rounds = ((int64_t)p.most * p.chunks + cus - 1) / cus;
-    const float ranges = (float)rounds * ((float)W / p.most);
-    if (p.most == 1)
-        p.whole = units == 1 || whole < 0.9f * ranges;
-    else
-        p.whole = whole <= ranges + c.join + (float)p.most * groups / c.bytes_ratio;
+    if (p.most == 1) {
+        const int64_t rounds = ((int64_t)p.chunks + cus - 1) / cus;
+        p.whole = units == 1 || whole < 0.9f * (float)(rounds * W);
+    } else {
+        const float there = lists || each <= c.brief ? (float)W : 0.5f * (float)tiles + (float)empty;
+        p.whole = whole <= there / p.most + c.join + (float)p.most * groups / c.bytes_ratio;
+    }
     if (p.whole) {
         plan_heads(p, c, cus, groups, units);
         p.most = units;
