@@ -312,10 +312,11 @@ int32_t ut_mla_attend_split(ut_ctx *ctx, const float *qabs_dev, const float *q_r
  * positive (a batch padded with lens 0, fewer new rows than `rows`, aligned
  * to the end) the row has no position and sees nothing.  Sequences may share
  * pages; entries behind a sequence's last page are not read.  Lengths and
- * tables stay on the device and may change between replays of a captured call.  A length that is
- * negative or beyond its table is cut, a page id outside the pool reads page
- * 0 (an append writes nothing there), and the next ut_ctx_synchronize returns
- * UT_ERR_BAD_PAGE; the values of that sequence are then unspecified.  At most
+ * tables stay on the device and may change between replays of a captured call.
+ * A length that is negative or beyond its table is cut, a page id outside the
+ * pool reads page 0, and the next ut_ctx_synchronize returns UT_ERR_BAD_PAGE;
+ * the values of that sequence are then unspecified.  An append writes nothing
+ * for such a length, and nothing to such a page.  At most
  * 65535 sequences, and rows in all for the calls with queries; a sequence (and
  * what a row selects) spans at most 2^31 - 1024 positions, a pool fewer than
  * 2^31.  What a call writes must not overlap what it reads.

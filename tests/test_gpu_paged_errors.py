@@ -1,0 +1,47 @@
+"""Bad lengths and pages of the paged calls on the GPU: what is left alone and
+what is reported."""
+import pytest
+import torch
+
+import paged_ref as R
+from test_gpu_paged import pages_in_order
+
+pytestmark = pytest.mark.gpu
+FMTS = ["bf16", "f16x2"]
+
+
+def bad_page(ctx):
+    import undertow_amd as U
+    with pytest.raises(U.UtError) as e:
+        ctx.synchronize()
+    assert e.value.code == U.runtime.UT_ERR_BAD_PAGE
+    ctx.synchronize()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("summaries", [True, False])
+@pytest.mark.parametrize("rows,over", [(1, 1), (4, 1), (4, 3), (40, 7), (2, 1000), (3, 2**31 - 113)])
+def test_append_past_the_table_writes_nothing(ctx, fmt, summaries, rows, over):
+    """A sequence one position (and more) longer than its table: its pages and
+    their summaries stay as they are to the bit, and the others' rows are
+    written."""
+    cap = 7 * 16
+    pool = R.Pool(43, fmt, [100, cap, 80], 16, 512, 64)
+    mean, scale = pages_in_order(pool)
+    more = dict(mean=mean.cuda(), mean_scale=scale.cuda()) if summaries else {}
+    cache = pool.cuda(ctx=ctx, **more)
+    table, lens = pool.table.cuda(), pool.lens32().cuda()
+    lens[1] = cap + over
+    x = pool.randn(3, rows, 576)
+    cache.append(table, lens, x[..., :512].contiguous().cuda(), x[..., 512:].contiguous().cuda())
+    bad_page(ctx)
+    for b in (0, 2):
+        n = pool.lens[b]
+        pool.put(b, n - rows, x[b])
+        for k in range((n - rows) // 16, -(-n // 16)):
+            at = pool.table[b, k].long()
+            mean[at], scale[at] = R.summary(pool.rows(b, torch.arange(k * 16, min(n, (k + 1) * 16))))
+    assert torch.equal(cache.pages.cpu().view(torch.int16), pool.pages.view(torch.int16))
+    if summaries:
+        assert torch.equal(cache.mean.cpu(), mean)
+        assert torch.equal(cache.mean_scale.cpu().view(torch.int32), scale.view(torch.int32))

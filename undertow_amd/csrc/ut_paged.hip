@@ -67,13 +67,14 @@ __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__r
     extern __shared__ double sum[];  // [4][D]
     __shared__ double red[16];
     const int b = blockIdx.y, tid = threadIdx.x, D = a.L + a.P, nq = D / 4;
-    const int32_t len = paged_len(a, b);
+    bool bad = false;
+    const int32_t len = paged_len(a, b, bad);
+    if (bad) return;  // cut to the table's end, the new rows would take the place of older ones
     const int32_t from = len > a.M ? len - a.M : 0;  // the first new position
     const int k = (from >> a.shift) + (int)blockIdx.x;
     const int32_t page = 1 << a.shift;
     const int64_t p0 = (int64_t)k << a.shift;
     if (p0 >= len) return;
-    bool bad = false;
     const int32_t phys = paged_phys(a, b, k, bad);
     if (bad) return;
     const int live = len - p0 < page ? (int)(len - p0) : page;

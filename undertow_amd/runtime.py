@@ -607,7 +607,8 @@ class PagedCache:
 
     def append(self, table, lens, latent, krot) -> None:
         """Writes latent [B, M, latent] and krot [B, M, rope] (f32) to each
-        sequence's last M positions, and their pages' summaries anew."""
+        sequence's last M positions, and their pages' summaries anew; nothing
+        for a sequence whose length is negative or beyond its table."""
         torch = _torch()
         if latent.dim() != 3:
             raise ShapeError(UT_ERR_SHAPE, f"PagedCache: latent must be [B, rows, latent], got {list(latent.shape)}")
