@@ -78,7 +78,8 @@ const char *ut_last_error(const ut_ctx *ctx);
 int32_t     ut_ctx_set_stream(ut_ctx *ctx, void *stream);
 void       *ut_ctx_stream(ut_ctx *ctx);
 /* Waits for the context's stream; also reports errors detected on device
- * since the last call (UT_ERR_BAD_EXPERT, UT_ERR_BAD_PAGE). */
+ * since the last call (UT_ERR_BAD_EXPERT, UT_ERR_BAD_PAGE; where there are
+ * both, the second is reported by the call after it). */
 int32_t     ut_ctx_synchronize(ut_ctx *ctx);
 /* Per-kernel timing with HIP events on the context stream (bench tooling):
  * while enabled, every kernel the library launches is bracketed by events;

@@ -45,3 +45,30 @@ def test_append_past_the_table_writes_nothing(ctx, fmt, summaries, rows, over):
     if summaries:
         assert torch.equal(cache.mean.cpu(), mean)
         assert torch.equal(cache.mean_scale.cpu().view(torch.int32), scale.view(torch.int32))
+
+
+def test_an_expert_error_does_not_hide_a_page_error(ctx):
+    """Both found before one synchronize: one each from two of them."""
+    import undertow_amd as U
+    c = U.Context(0)
+    H = 64
+    w = lambda o, i: U.QTensor(c, U.INT8, torch.ones((o, i), dtype=torch.int8).numpy(), torch.ones(o).numpy(), o, i)
+    experts = U.ExpertTable(c, 1, H, 32)
+    experts.set(0, w(32, H), w(32, H), w(H, 32))
+    x, one = torch.ones((1, H), device="cuda"), torch.ones((1, 1), device="cuda")
+    pool = R.Pool(47, "bf16", [20], 16, 64, 16)
+    q = [t.cuda() for t in pool.queries(1, 4)]
+    cache, table = pool.cuda(ctx=c), pool.table.cuda()
+    for order in ((0, 1), (1, 0)):
+        for k in order:
+            if k == 0:
+                experts.moe_experts(torch.tensor([[9]], dtype=torch.int32, device="cuda"), one, x)
+            else:
+                cache.attend(table, torch.tensor([33], dtype=torch.int32, device="cuda"), *q, 0.1)
+        codes = []
+        for _ in range(2):
+            with pytest.raises(U.UtError) as e:
+                c.synchronize()
+            codes.append(e.value.code)
+        assert sorted(codes) == sorted([U.runtime.UT_ERR_BAD_EXPERT, U.runtime.UT_ERR_BAD_PAGE])
+        c.synchronize()

@@ -178,8 +178,10 @@ int32_t check_device_error(ut_ctx *ctx) {
     int32_t f[2] = {0, 0};
     UT_CHECK_HIP(ctx, hipMemcpy(f, ctx->dev_err, 8, hipMemcpyDeviceToHost));
     if (!f[0] && !f[1]) return UT_OK;
-    UT_CHECK_HIP(ctx, hipMemset(ctx->dev_err, 0, 8));
-    if (!f[0]) {
+    // one error a call: the other word stays for the next
+    const int word = f[0] ? 0 : 1;
+    UT_CHECK_HIP(ctx, hipMemset(ctx->dev_err + word, 0, 4));
+    if (word == 1) {
         set_error(ctx, "a paged call met a length beyond its table or a page outside its pool "
                        "(reported by a kernel)");
         return UT_ERR_BAD_PAGE;
