@@ -369,7 +369,8 @@ int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *t
                            int64_t keep_last, int64_t top_k, int32_t *sel_dev);
 /* ut_mla_paged_attend over the listed pages only: sel [batch, rows, top_k]
  * sequence page numbers in any order.  Negative entries and pages behind the
- * row's end are skipped; a page listed twice counts twice. */
+ * row's end are skipped; a page listed twice counts twice.  Of the table only
+ * the listed pages' entries have to name a page. */
 int32_t ut_mla_sparse_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
                              int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
                              int64_t batch, int64_t rows, int64_t heads, const void *qabs_dev,

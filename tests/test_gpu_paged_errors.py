@@ -72,3 +72,29 @@ def test_an_expert_error_does_not_hide_a_page_error(ctx):
             codes.append(e.value.code)
         assert sorted(codes) == sorted([U.runtime.UT_ERR_BAD_EXPERT, U.runtime.UT_ERR_BAD_PAGE])
         c.synchronize()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("lens,M,H,L,P,page,top_k,width", [
+    ([400, 333, 100], 2, 32, 512, 64, 16, 6, 25), ([900], 1, 128, 512, 64, 64, 40, 20),
+    ([500, 480] * 20, 1, 16, 512, 64, 8, 300, 63), ([300, 200], 2, 4, 64, 16, 8, 5, 38)])
+def test_pages_that_no_row_lists_need_not_be_there(ctx, fmt, lens, M, H, L, P, page, top_k, width):
+    """A window's old pages given back, their entries made invalid: lists of
+    later pages, with empty places and pages behind the row's end among them,
+    read as with a whole table and report nothing."""
+    pool = R.Pool(53, fmt, lens, page, L, P, width=width)
+    qabs, qrope = [t.cuda() for t in pool.queries(M, H)]
+    sel = torch.full((len(lens), M, top_k), -1, dtype=torch.int32)
+    table = torch.full_like(pool.table, -1)
+    for b, n in enumerate(lens):
+        last = (n - M) // page
+        ids = range(max(1, last - 3), last + 1)
+        sel[b, :, 1:1 + len(ids)] = torch.tensor(ids, dtype=torch.int32)
+        sel[b, :, -1] = width + 5
+        table[b, list(ids)] = pool.table[b, list(ids)]
+    cache, n = pool.cuda(ctx=ctx), pool.lens32().cuda()
+    want = cache.attend_pages(pool.table.cuda(), n, qabs, qrope, 0.07, sel.cuda())
+    ctx.synchronize()
+    got = cache.attend_pages(table.cuda(), n, qabs, qrope, 0.07, sel.cuda())
+    ctx.synchronize()
+    assert torch.equal(got, want) and torch.isfinite(want).all()

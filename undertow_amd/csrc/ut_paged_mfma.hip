@@ -529,8 +529,11 @@ template <bool SPARSE> __device__ __forceinline__ int32_t page_of(const Lookup &
     return (v0 < k.n ? v0 : k.n - 1) >> k.shift;
 }
 template <bool SPARSE> __device__ __forceinline__ int32_t page_entry(const Lookup &k, int32_t page) {
-    if (SPARSE && (page < 0 || ((int64_t)page << k.shift) >= k.n)) page = 0;
-    return k.table[page];
+    // the pool's first page stands in for one that is not listed or not seen: the
+    // table need not name any but the listed ones
+    const bool none = SPARSE && (page < 0 || ((int64_t)page << k.shift) >= k.n);
+    const int32_t entry = k.table[none ? 0 : page];
+    return none ? 0 : entry;
 }
 // The visible positions of the tile at v0 for a row that sees n.
 template <bool SPARSE>
