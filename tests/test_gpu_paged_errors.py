@@ -98,3 +98,25 @@ def test_pages_that_no_row_lists_need_not_be_there(ctx, fmt, lens, M, H, L, P, p
     got = cache.attend_pages(table.cuda(), n, qabs, qrope, 0.07, sel.cuda())
     ctx.synchronize()
     assert torch.equal(got, want) and torch.isfinite(want).all()
+
+
+def test_a_new_cache_is_zero_before_the_context_writes_to_it(ctx):
+    """Made on torch's stream, behind work that it still has to do, for a
+    context on a stream of its own: what the context appends stays."""
+    import undertow_amd as U
+    c = U.Context(0, bind_torch_stream=False)
+    lat, kr = torch.randn((1, 40, 512), device="cuda"), torch.randn((1, 40, 64), device="cuda")
+    table = torch.arange(3, dtype=torch.int32, device="cuda")[None]
+    lens = torch.tensor([40], dtype=torch.int32, device="cuda")
+    U.PagedCache.empty(c, 3, 16).append(table, lens, lat, kr)  # the first call's set-up
+    c.synchronize()
+    x = torch.randn((8192, 8192), device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(4):
+        x = (x @ x) * 1e-4
+    cache = U.PagedCache.empty(c, 3, 16)
+    cache.append(table, lens, lat, kr)
+    c.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(cache.pages.flatten(0, 1)[:40], torch.cat([lat, kr], -1)[0].bfloat16())
+    assert (cache.mean_scale > 0).all()

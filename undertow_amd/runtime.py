@@ -561,10 +561,15 @@ class PagedCache:
         d, D = f"cuda:{ctx.device}", latent + rope
         pages = (torch.zeros((n_pages, page, D), dtype=torch.bfloat16, device=d) if fmt == KV_BF16
                  else torch.zeros((n_pages, page, 2, D), dtype=torch.float16, device=d))
-        if not summaries:
-            return cls(ctx, pages, latent, rope)
-        return cls(ctx, pages, latent, rope, torch.zeros((n_pages, D), dtype=torch.int8, device=d),
-                   torch.zeros(n_pages, device=d))
+        mean = scale = None
+        if summaries:
+            mean = torch.zeros((n_pages, D), dtype=torch.int8, device=d)
+            scale = torch.zeros(n_pages, device=d)
+        # the zeros are there before a call on the context's stream
+        torch_stream = torch.cuda.current_stream(ctx.device)
+        if torch_stream.cuda_stream != (lib().ut_ctx_stream(ctx.handle) or 0):
+            torch_stream.synchronize()
+        return cls(ctx, pages, latent, rope, mean, scale)
 
     def _tensor(self, name: str, t, dtype, shape) -> int:
         if t.shape != shape:
