@@ -559,7 +559,8 @@ __device__ __forceinline__ uint32_t visible(const Lookup &k, int32_t v0, int32_t
 // steps by the rest.  Written out, since the compiler would have every later
 // LDS read wait for every copy under way: the kernel waits itself.  Nothing
 // is loaded into a register, and the address is read when the instruction
-// issues.
+// issues.  (m0 is reserved: the compiler takes no clobber of it and sets it anew
+// where it needs it, which it does nowhere in these kernels.)
 template <int I> __device__ __forceinline__ void copy_block(uint32_t off, const uint8_t *src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3"
                  :
