@@ -20,6 +20,10 @@ void cut(const ut::PlanCosts *c, int cus, int units, int groups, int64_t each, i
          ut::PlanCall *out) {
     *out = ut::plan_call(*c, cus, units, groups, each, listed, lists);
 }
+int64_t ranges(int64_t W, int64_t most, float spread) { return ut::plan_ranges(W, (int32_t)most, spread); }
+int64_t begin(int64_t W, int64_t N, int64_t r) { return ut::plan_begin(W, N, r); }
+int64_t range_of(int64_t W, int64_t N, int64_t t) { return ut::plan_range_of(W, N, t); }
+int64_t slot(int64_t r, int64_t begins) { return ut::plan_slot(r, begins != 0); }
 }
 """
 
@@ -54,7 +58,13 @@ def cut(tmp_path_factory):
         out, each = Call(), -(-positions // 32)
         f(costs[fmt], CUS, sequences, rows * -(-heads // 16), each, each, lists, out)
         return out
+    call.costs = costs
     call.waves = {k: c.waves for k, c in costs.items()}
+    for name in ("ranges", "begin", "range_of", "slot"):
+        g = getattr(lib, name)
+        g.restype, g.argtypes = C.c_int64, [C.c_int64, C.c_int64] + [C.c_int64] * (name in ("begin", "range_of"))
+        setattr(call, name, g)
+    lib.ranges.argtypes = [C.c_int64, C.c_int64, C.c_float]
     return call
 
 
@@ -110,3 +120,54 @@ def test_long_sequences_of_differing_lengths_are_cut(cut, fmt, B, M, H, whole_at
 def test_a_list_counts_in_full(cut, fmt):
     """Rows of a batch choose as many pages each: 256 lists of 16 pages of 64."""
     assert cut(fmt, 256, 1, 128, 1024, lists=True).whole
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f16x2"])
+@pytest.mark.parametrize("seed", range(30))
+def test_every_tile_once_behind_the_empty_ones(cut, fmt, seed):
+    """The row of tiles with empty ones before every unit but the first: each
+    range finds the unit that it begins in, goes on from there and takes every
+    tile once, and what joins a unit's parts finds each of them."""
+    rng = random.Random(seed)
+    lead = cut.costs[fmt].lead
+    tiles = [rng.choice([0, 0, 1, 2, rng.randint(0, 40), rng.randint(0, 1000)]) for _ in range(rng.randint(1, 900))]
+    total = [t + lead if t else 0 for t in tiles]  # a unit with its empty tiles
+    if not any(tiles):
+        return
+    W = sum(total) - lead
+    N = cut.ranges(W, rng.choice([2, 7, 64, 256]), rng.choice([0.5, 4.0, 64.0, 1e6]))
+    first, at = [], 0  # first tile of each: `lead` tiles of the first one would stand before 0
+    for t in total:
+        first.append(at)
+        at += t
+    taken, parts = [[0] * t for t in tiles], {}
+    for r in range(N):
+        s, e = cut.begin(W, N, r), cut.begin(W, N, r + 1)
+        assert s < e
+        found = [u for u, t in enumerate(total) if first[u] <= s + lead < first[u] + t]
+        assert len(found) == 1
+        u, f, at = found[0], first[found[0]], s
+        while True:  # the parts of a range, as the kernel walks them
+            while at < e and u < len(tiles) and not tiles[u]:
+                u += 1
+            if at >= e or u == len(tiles):
+                break
+            b0, b1 = max(at - f, 0), min(e - f, tiles[u])
+            if b0 >= b1:
+                break
+            for x in range(b0, b1):
+                taken[u][x] += 1
+            if (b0, b1) != (0, tiles[u]):
+                assert parts.setdefault(cut.slot(r, s <= f), (u, r)) == (u, r)
+            f += tiles[u] + lead
+            at = f
+            u += 1
+    assert all(x == 1 for t in taken for x in t)
+    assert all(0 <= k < 2 * N for k in parts)
+    joined = []
+    for u, t in enumerate(tiles):
+        if t:
+            r0, r1 = cut.range_of(W, N, first[u]), cut.range_of(W, N, first[u] + t - 1)
+            if r1 > r0:
+                joined += [(parts[cut.slot(r, r == r0)], (u, r)) for r in range(r0, r1 + 1)]
+    assert all(a == b for a, b in joined) and len(joined) == len(parts)
