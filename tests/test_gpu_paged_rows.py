@@ -1,10 +1,10 @@
-"""Prompt-sized calls of the paged latent cache's attention on the GPU: their
-values against 64 bits, and what they reserve."""
+"""Prompt-sized calls of the paged latent cache on the GPU: attention and page
+selection against 64 bits, and what attention reserves."""
 import pytest
 import torch
 
 import paged_ref as R
-from test_gpu_paged import SCALE, close
+from test_gpu_paged import SCALE, close, pages_in_order
 
 pytestmark = pytest.mark.gpu
 FMTS = ["bf16", "f16x2"]
@@ -67,3 +67,52 @@ def test_attend_prompt_rows(ctx, fmt, lens, M, H, width):
     got = pool.cuda(ctx=ctx).attend(pool.table.cuda(), pool.lens32().cuda(), qabs.cuda(), qrope.cuda(), SCALE)
     ctx.synchronize()
     check(pool, fmt, got, qabs, qrope)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("lens,M,H,width,at", [
+    ([97, 64, 130], 40, 128, 192, 5), ([97, 64, 130], 64, 32, 4096, 33), ([300, 500, 20], 150, 128, 512, 70),
+    ([600, 100], 128, 256, 4096, 100)])
+def test_a_later_prompt_row_does_not_reach_an_earlier_one(ctx, fmt, lens, M, H, width, at):
+    """NaN and infinities in one row of a prompt: that row and those behind it
+    are NaN, the rows before it are as without."""
+    pool = R.Pool(67, fmt, lens, 64, 512, 64, width=width // 64)
+    qabs, qrope = pool.queries(M, H)
+    args = pool.table.cuda(), pool.lens32().cuda(), qabs.cuda(), qrope.cuda(), SCALE
+    clean = pool.cuda(ctx=ctx).attend(*args)
+    for b, n in enumerate(lens):
+        x = torch.full((1, 576), float("nan"))
+        x[:, 1::2] = float("inf")
+        if n - M + at >= 0:
+            pool.put(b, n - M + at, x)
+    got = pool.cuda(ctx=ctx).attend(*args)
+    ctx.synchronize()
+    for b, n in enumerate(lens):
+        if n - M + at >= 0:
+            assert torch.equal(got[b, :at], clean[b, :at]) and torch.isfinite(clean[b]).all()
+            assert not torch.isfinite(got[b, at:]).any()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("lens,M,H,page,top_k", [
+    ([700, 90], 130, 32, 64, 6), ([500], 300, 128, 16, 20), ([300, 40, 111], 100, 16, 8, 9), ([400, 399], 60, 64, 128, 3)])
+def test_selected_pages_of_prompt_rows(ctx, fmt, lens, M, H, page, top_k):
+    """Many rows of a sequence choose, with head weights, and attend to their
+    choice: the choice as defined, the rest against 64 bits."""
+    pool = R.Pool(71, fmt, lens, page, 512, 64)
+    mean, scale = pages_in_order(pool)
+    qabs, qrope = pool.queries(M, H)
+    w = pool.randn(len(lens), M, H)
+    cache = pool.cuda(ctx=ctx, mean=mean.cuda(), mean_scale=scale.cuda())
+    where = pool.table.cuda(), pool.lens32().cuda(), qabs.cuda(), qrope.cuda()
+    sel = cache.select(*where, top_k, 1, 1, weights=w.cuda())
+    got = cache.attend_pages(*where, SCALE, sel)
+    ctx.synchronize()
+    q = torch.cat([qabs, qrope], -1).double()
+    for b, n in enumerate(lens):
+        for j in list(range(0, M, 17)) + [M - 1]:
+            k = -(-max(0, n - M + j + 1) // page)
+            at = pool.table[b, :k].long()
+            want = R.select(q[b, j], mean[at], scale[at], k, 1, 1, top_k, w[b, j])
+            assert sel[b, j].tolist() == want, (b, j)
+    check(pool, fmt, got, qabs, qrope, sel.cpu())
