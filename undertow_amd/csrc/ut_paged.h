@@ -27,14 +27,11 @@ struct PagedArgs {
 typedef const __attribute__((address_space(4))) int32_t const_i32;
 
 // Positions of sequence b, bounded by what its row of the table can hold.
-__device__ __forceinline__ int32_t paged_len(const PagedArgs &a, int b, bool &bad) {
+__device__ __forceinline__ int32_t paged_len(const PagedArgs &a, int b) {
+    bool bad = false;
     const int32_t n = plan_len(((const_i32 *)a.lens)[b], (int64_t)a.max_pages << a.shift, bad);
     if (bad) *a.err = 1;
     return n;
-}
-__device__ __forceinline__ int32_t paged_len(const PagedArgs &a, int b) {
-    bool bad = false;
-    return paged_len(a, b, bad);
 }
 // The physical page of a sequence's k-th page (k < max_pages); an id outside
 // the pool is reported and page 0 stands in for it.

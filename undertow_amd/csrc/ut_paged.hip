@@ -68,8 +68,11 @@ __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__r
     __shared__ double red[16];
     const int b = blockIdx.y, tid = threadIdx.x, D = a.L + a.P, nq = D / 4;
     bool bad = false;
-    const int32_t len = paged_len(a, b, bad);
-    if (bad) return;  // cut to the table's end, the new rows would take the place of older ones
+    const int32_t len = plan_len(((const_i32 *)a.lens)[b], (int64_t)a.max_pages << a.shift, bad);
+    if (bad) {  // cut to the table's end, the new rows would take the place of older ones
+        *a.err = 1;
+        return;
+    }
     const int32_t from = len > a.M ? len - a.M : 0;  // the first new position
     const int k = (from >> a.shift) + (int)blockIdx.x;
     const int32_t page = 1 << a.shift;
