@@ -345,9 +345,16 @@ int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *
 /* ut_mla_attend for each row over its sequence's pages: qabs [batch, rows,
  * heads, latent], q_rope [batch, rows, heads, rope], clat like qabs, in the
  * cache format's type.  A row that sees nothing gets zeros.  What a row does
- * not see does not reach it, NaN and infinities included.  Equal calls give
- * equal bits; a row's rounding may depend on the sizes of the call and the
- * lengths of its batch (the work is cut evenly over the device). */
+ * not see does not reach it, NaN and infinities included; one that it sees may
+ * make its whole context NaN.  Scores and sums are f32.  With bf16 pages of
+ * 8 positions and more at latent 512 + rope 64 the softmax weights are rounded
+ * to bf16 before they meet the values, in numerator and denominator alike (the
+ * matrix cores take both operands in one type): a context is off by at most
+ * 2^-8 of its values' weighted spread for that, and by its own rounding.  f16x2
+ * pages keep the weights to 22 bits.  Equal calls give equal bits; a row's
+ * rounding may depend on the sizes of the call and the lengths of its batch
+ * (the work is cut evenly over the device).  Working memory: some 135 MB of the
+ * arena at most; none where the rows alone fill the device (prompts). */
 int32_t ut_mla_paged_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
                             int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
                             int64_t batch, int64_t rows, int64_t heads, const void *qabs_dev,
@@ -359,7 +366,9 @@ int32_t ut_mla_paged_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *
  * them.  The score of a page is
  *   mean_scale * sum_h weight_h * max|q_h| / 127 * max(0, code(q_h) . mean)
  * with q_h = [qabs | q_rope] of head h and code(q) = rint(q * 127 / max|q|):
- * the products are exact in integers and the sum runs in 64 bits.  weights
+ * the products are exact in integers and the sum runs in 64 bits, in the same
+ * order for every page of a call: equal pages tie exactly, while pages whose
+ * sums are equal in real numbers only may fall either way.  weights
  * [batch, rows, heads] f32 or NULL (all 1).  A head whose query is not finite
  * is left out; a NaN score ranks last.  max_pages is at most 2^27 here. */
 int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
