@@ -116,3 +116,35 @@ def test_selected_pages_of_prompt_rows(ctx, fmt, lens, M, H, page, top_k):
             want = R.select(q[b, j], mean[at], scale[at], k, 1, 1, top_k, w[b, j])
             assert sel[b, j].tolist() == want, (b, j)
     check(pool, fmt, got, qabs, qrope, sel.cpu())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("lens,M,H,width,warm", [
+    ([600, 200], 128, 256, 4096, False), ([700], 300, 128, 8192, False), ([900, 30, 400], 2, 128, 4096, True)])
+def test_captured_prompt_rows_follow_lengths(fmt, lens, M, H, width, warm):
+    """One range, whole sequences (both captured at once: they reserve nothing)
+    and ranges with their join, replayed as lengths shrink and grow again, with
+    eager calls between: every replay has the eager call's bits."""
+    import undertow_amd as U
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        c = U.Context(0)
+        pool = R.Pool(73, fmt, lens, 64, 512, 64, width=width // 64)
+        q = [t.cuda() for t in pool.queries(M, H)]
+        cache, table, n = pool.cuda(ctx=c), pool.table.cuda(), pool.lens32().cuda()
+        out = torch.empty_like(q[0])
+        if warm:
+            cache.attend(table, n, *q, SCALE, out=out)
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            cache.attend(table, n, *q, SCALE, out=out)
+        for less in (0, 25, 125, 0, 500):
+            n.copy_((pool.lens32().cuda() - less).clamp(min=0))
+            out.fill_(7.0)
+            graph.replay()
+            s.synchronize()
+            got = out.clone()
+            assert torch.equal(got, cache.attend(table, n, *q, SCALE))
+            c.synchronize()
+            assert torch.isfinite(got).all()
