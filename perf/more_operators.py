@@ -142,7 +142,7 @@ def _quantised(x, L):
 
 
 def _values(pool, rows, scales=None):
-    """The values that stored rows stand for, in f32."""
+    """The values that stored rows stand for, in f32 (in 64 bits where the scales are)."""
     if pool["fmt"] == "bf16":
         return rows.float()
     if pool["fmt"] == "f16x2":
@@ -156,9 +156,10 @@ def _at(pool, *index):
     return _values(pool, pool["pages"][index], pool["scales"][index] if "scales" in pool else None)
 
 
-def _summary(values, live):
-    """Codes and scales of the mean rows of pages [..., page, row], over the live positions [..., page]."""
-    s = (values.double() * live[..., None]).sum(-2)
+def _summary(st, pages, live):
+    """Codes and scales of the mean rows of pages, over the live positions [..., page]; in 64 bits,
+    since a mean next to a border between two codes takes one or the other."""
+    s = (_values(st, st["pages"][pages], st["scales"][pages].double()) * live[..., None]).sum(-2)
     top = s.abs().amax(-1)
     codes = torch.round(s * 127.0 / torch.where(top > 0, top, 1.0)[..., None])
     return codes.to(torch.int8), (top / (127.0 * live.sum(-1).clamp(min=1))).float()
@@ -209,7 +210,7 @@ def prepare(case, seed):
     B, M = case["batch"], case["rows"]
     rnd = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
     if case["kind"] == "append":
-        st["mean"], st["mean_scale"] = _summary(_at(st), torch.ones(st["pages"].shape[:2], dtype=torch.float64, device="cuda"))
+        st["mean"], st["mean_scale"] = _summary(st, slice(None), torch.ones(st["pages"].shape[:2], dtype=torch.float64, device="cuda"))
         st["latent"], st["krot"] = rnd(B, M, st["L"]), rnd(B, M, st["P"])
     elif case["kind"] == "read":  # the last rows of each sequence, or all of a shorter one
         st["starts"] = (st["lens"] - M).clamp(min=0).int()
@@ -311,7 +312,7 @@ def _append(st):
     at = torch.minimum(first + torch.arange((M + page - 2) // page + 1, device=lens.device), last)
     touched = table.gather(1, at)
     live = (at[..., None] * page + torch.arange(page, device=lens.device) < lens[:, None, None]).double()
-    st["mean"][touched], st["mean_scale"][touched] = _summary(_at(st, touched), live)
+    st["mean"][touched], st["mean_scale"][touched] = _summary(st, touched, live)
 
 
 def run(st):
