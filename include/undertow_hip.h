@@ -299,11 +299,16 @@ int32_t ut_mla_attend_split(ut_ctx *ctx, const float *qabs_dev, const float *q_r
  *   UT_KV_BF16   [n_pages][page][D] bf16; queries and contexts are bf16 too;
  *   UT_KV_F16X2  [n_pages][page][2][D] f16, x = hi + lo / 2048 to 2^-23 |x|
  *                (|x| up to 65504; finite values beyond take that), the bytes
- *                of f32 rows; queries and contexts are f32.
+ *                of f32 rows; queries and contexts are f32;
+ *   UT_KV_I8     [n_pages][page][D] 8-bit codes and scales [n_pages][page][2]
+ *                f32, of a position's latent and of its krot: x = code * scale
+ *                to 1/254 of the part's largest (a part with a value that is
+ *                not finite is NaN); queries and contexts are bf16.
  * mean / mean_scale (both or neither NULL) summarise each page for
  * ut_mla_page_select: the mean row is mean_scale[p] * mean[p][d] to 1/254 of
- * its largest value.  pages and mean are 16-byte aligned.  The struct is
- * read during the call only; the memory is the caller's.
+ * its largest value.  pages, mean and scales are 16-byte aligned; scales is
+ * read for UT_KV_I8 only.  The struct is read during the call only; the memory
+ * is the caller's.
  *
  * A batch: table_dev holds `batch` rows, table_stride entries apart, each of
  * max_pages physical page ids in the sequence's order; lens_dev [batch]
@@ -323,13 +328,14 @@ int32_t ut_mla_attend_split(ut_ctx *ctx, const float *qabs_dev, const float *q_r
  * 2^31.  What a call writes must not overlap what it reads.
  * All calls run on the context's device and stream; those that need working
  * memory take the context's arena. */
-enum { UT_KV_BF16 = 0, UT_KV_F16X2 = 1 };
+enum { UT_KV_BF16 = 0, UT_KV_F16X2 = 1, UT_KV_I8 = 8 };
 typedef struct {
     void *pages;
     int8_t *mean;      /* [n_pages][D] or NULL */
     float *mean_scale; /* [n_pages] or NULL */
     int64_t n_pages, page, latent, rope;
     int32_t fmt;
+    float *scales;     /* [n_pages][page][2], UT_KV_I8 only */
 } ut_mla_pages;
 
 /* Writes the rows latent [batch, rows, latent] and krot [batch, rows, rope]
@@ -342,6 +348,15 @@ int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *
                             int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
                             int64_t batch, int64_t rows, const float *latent_dev,
                             const float *krot_dev);
+/* Rows read back: row j of sequence b is position starts_dev[b] + j (starts_dev
+ * NULL: j), as latent [batch, rows, latent] and krot [batch, rows, rope] in f32
+ * or bf16 (the f32 value rounded once more).  Rows outside the sequence are
+ * zeros. */
+enum { UT_ROWS_F32 = 0, UT_ROWS_BF16 = 1 };
+int32_t ut_mla_paged_read(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
+                          int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
+                          int64_t batch, int64_t rows, const int32_t *starts_dev, int32_t type,
+                          void *latent_dev, void *krot_dev);
 /* ut_mla_attend for each row over its sequence's pages: qabs [batch, rows,
  * heads, latent], q_rope [batch, rows, heads, rope], clat like qabs, in the
  * cache format's type.  A row that sees nothing gets zeros.  What a row does
@@ -385,6 +400,17 @@ int32_t ut_mla_sparse_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t 
                              int64_t batch, int64_t rows, int64_t heads, const void *qabs_dev,
                              const void *q_rope_dev, float scale, const int32_t *sel_dev,
                              int64_t top_k, void *clat_dev);
+
+/* ut_mla_paged_attend where a row at position p sees, of the positions up to
+ * p, the last `window` (p - window + 1 .. p, one at least) and the sequence's
+ * first `sinks` (0 and more).  Of the table only the pages that hold a position
+ * which some row of the call sees have to name a page: a server may give the
+ * others back. */
+int32_t ut_mla_window_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
+                             int64_t table_stride, int64_t max_pages, const int32_t *lens_dev,
+                             int64_t batch, int64_t rows, int64_t heads, const void *qabs_dev,
+                             const void *q_rope_dev, float scale, int64_t window, int64_t sinks,
+                             void *clat_dev);
 
 /* ---------------------------------------------------------------- model */
 /* DeepseekConfig fields the forward pass reads (adapters/undertow-deepseek-

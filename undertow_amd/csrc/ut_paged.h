@@ -9,6 +9,7 @@ namespace ut {
 // What the kernels read of a paged cache and a batch over it.
 struct PagedArgs {
     const void *pages;     // [n_pages][page][row]
+    const float2 *scales;  // [n_pages][page] of the latent codes and of the rotary ones (8-bit pages)
     const int32_t *table;  // [B][stride]: physical page of a sequence's k-th page
     int64_t stride;        // entries from one sequence's row of the table to the next
     const int32_t *lens;   // [B]
@@ -17,6 +18,7 @@ struct PagedArgs {
     int32_t B, M, H, L, P;
     const int32_t *sel;    // [B][M][top_k] pages of the sequence, or nullptr: all
     int32_t top_k;
+    int32_t window, sinks;  // positions that a row sees before its end and from the start; window 0: all
     float scale;
     const void *qabs, *qrope;
     void *out;

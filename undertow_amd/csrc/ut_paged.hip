@@ -1,15 +1,23 @@
-// ut_paged.hip -- the paged MLA latent cache: appending a step's rows, the
-// score that selects pages, and attention for any latent width.
+// ut_paged.hip -- the paged MLA latent cache: appending a step's rows, reading
+// them back, the score that selects pages, and attention for any latent width.
+#include <type_traits>
+
 #include "ut_paged.h"
 
 namespace ut {
 
+// quad: the values d .. d + 3 of the row at a position of the pool (d a
+// multiple of 4: in one part); value: one of them.
 struct Bf16 {
     static constexpr int kPlanes = 1;
     typedef __bf16 q_t;
     typedef float code_t;
-    __device__ static float value(const uint16_t *row, int D, int d) {
-        return __uint_as_float((uint32_t)row[d] << 16);
+    __device__ static float value(const PagedArgs &a, int64_t pos, int d) {
+        return __uint_as_float((uint32_t)((const uint16_t *)a.pages)[pos * (a.L + a.P) + d] << 16);
+    }
+    __device__ static float4 quad(const PagedArgs &a, int64_t pos, int d) {
+        const uint2 h[1] = {*(const uint2 *)((const uint16_t *)a.pages + pos * (a.L + a.P) + d)};
+        return make_float4(stored(h, 0), stored(h, 1), stored(h, 2), stored(h, 3));
     }
     // four values as a row holds them, and back
     __device__ static void store(const float (&x)[4], uint2 (&h)[1]) {
@@ -27,9 +35,16 @@ struct F16x2 {
     static constexpr int kPlanes = 2;
     typedef float q_t;
     typedef double code_t;
-    __device__ static float value(const uint16_t *row, int D, int d) {
-        const _Float16 *h = (const _Float16 *)row;
+    __device__ static float value(const PagedArgs &a, int64_t pos, int d) {
+        const int D = a.L + a.P;
+        const _Float16 *h = (const _Float16 *)a.pages + pos * 2 * D;
         return __fadd_rn((float)h[d], __fmul_rn((float)h[D + d], 1.0f / kF16x2Step));
+    }
+    __device__ static float4 quad(const PagedArgs &a, int64_t pos, int d) {
+        const int D = a.L + a.P;
+        const uint16_t *row = (const uint16_t *)a.pages + pos * 2 * D + d;
+        const uint2 h[2] = {*(const uint2 *)row, *(const uint2 *)(row + D)};
+        return make_float4(stored(h, 0), stored(h, 1), stored(h, 2), stored(h, 3));
     }
     __device__ static void store(const float (&x)[4], uint2 (&h)[2]) {
         _Float16 v[2][4];
@@ -41,6 +56,26 @@ struct F16x2 {
     __device__ static float stored(const uint2 (&h)[2], int i) {
         const _Float16 *hi = (const _Float16 *)&h[0], *lo = (const _Float16 *)&h[1];
         return __fadd_rn((float)hi[i], __fmul_rn((float)lo[i], 1.0f / kF16x2Step));
+    }
+};
+
+// 8 bits: a position's latent part and its rotary part each by a scale of its
+// own, x = code scale to 1/254 of the part's largest.
+__device__ __forceinline__ float code_byte(uint32_t w, int i) { return (float)((int32_t)(w << (24 - 8 * i)) >> 24); }
+struct I8 {
+    typedef __bf16 q_t;
+    typedef float code_t;
+    __device__ static float scale(const PagedArgs &a, int64_t pos, int d) {
+        return ((const float *)a.scales)[2 * pos + (d < a.L ? 0 : 1)];
+    }
+    __device__ static float value(const PagedArgs &a, int64_t pos, int d) {
+        return __fmul_rn((float)((const int8_t *)a.pages)[pos * (a.L + a.P) + d], scale(a, pos, d));
+    }
+    __device__ static float4 quad(const PagedArgs &a, int64_t pos, int d) {
+        const uint32_t w = *(const uint32_t *)((const int8_t *)a.pages + pos * (a.L + a.P) + d);
+        const float s = scale(a, pos, d);
+        return make_float4(__fmul_rn(code_byte(w, 0), s), __fmul_rn(code_byte(w, 1), s), __fmul_rn(code_byte(w, 2), s),
+                           __fmul_rn(code_byte(w, 3), s));
     }
 };
 
@@ -58,6 +93,28 @@ struct F16x2 {
 // 16 new rows of a thread under way at a time change nothing there; the dims
 // cut over workgroups, sums and then codes in two launches, took 10.8 us, but
 // the call 18.2 against 16.2.
+// A page's summary from the sums of its rows, four a dim in LDS.
+__device__ __forceinline__ void write_summary(double *sum, int D, int live, int8_t *mean, float *mean_scale) {
+    __shared__ double red[16];
+    const int tid = threadIdx.x;
+    __syncthreads();
+    double top = 0.0;
+    for (int d = tid; d < D; d += blockDim.x) {
+        const double t = (sum[d] + sum[D + d]) + (sum[2 * D + d] + sum[3 * D + d]);
+        sum[d] = t;
+        top = fmax(top, fabs(t));
+    }
+    for (int off = 32; off >= 1; off >>= 1) top = fmax(top, __shfl_xor(top, off, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+    __syncthreads();
+    for (int w = 0; w < (int)(blockDim.x >> 6); w++) top = fmax(top, red[w]);
+    for (int d = tid; d < D; d += blockDim.x) {
+        const double c = top > 0.0 ? rint(sum[d] * 127.0 / top) : 0.0;
+        mean[d] = (int8_t)(c >= -127.0 && c <= 127.0 ? (int)c : 0);
+    }
+    if (tid == 0) *mean_scale = (float)(top / (127.0 * live));
+}
+
 template <class F>
 __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__restrict__ pages,
                                                       const float *__restrict__ latent,
@@ -65,7 +122,6 @@ __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__r
                                                       int8_t *__restrict__ mean,
                                                       float *__restrict__ mean_scale) {
     extern __shared__ double sum[];  // [4][D]
-    __shared__ double red[16];
     const int b = blockIdx.y, tid = threadIdx.x, D = a.L + a.P, nq = D / 4;
     bool bad = false;
     const int32_t len = plan_len(((const_i32 *)a.lens)[b], (int64_t)a.max_pages << a.shift, bad);
@@ -127,23 +183,160 @@ __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__r
 #pragma unroll
             for (int i = 0; i < 4; i++) sum[s * D + d + i] = t[i];
     }
+    if (mean) write_summary(sum, D, live, mean + (int64_t)phys * D, mean_scale + phys);
+}
+
+// code = rint(q 127 / top) of the real quotient, |q| <= top, f about 127 / top.
+// c = rint(q f) may miss by one next to a half; q 127 - c top is exact and
+// tells: a bf16 query's numbers fit f32 (15 bits), a f32 value's take 64 bits.
+__device__ __forceinline__ float exact_fma(float x, float y, float z) { return __builtin_fmaf(x, y, z); }
+__device__ __forceinline__ double exact_fma(double x, double y, double z) { return __builtin_fma(x, y, z); }
+template <class T> __device__ __forceinline__ int code8(T q, T top, T f) {
+    const T c = rint(q * f), e = exact_fma(c, -2 * top, q * 254);  // twice the rest
+    const int k = (int)c;
+    const bool next = e > top || -e > top || ((e == top || -e == top) && (k & 1));
+    return next ? (e > 0 ? k + 1 : k - 1) : k;
+}
+
+// The same for 8-bit pages: a wave takes a new row at a time, its quads in
+// registers (D is at most 1024), for the largest magnitude A of each part,
+//   scale = fl32(A / 127), code = rint(127 x / A)
+// of the real quotient (64 bits: the codes are a value that a test can demand
+// exactly).  A part with a value that is not finite gets codes 0 and the scale
+// NaN: it is NaN read back.  The summary's sums take code * scale, exact in 64
+// bits, from the rows as they are then stored.
+__global__ __launch_bounds__(576) void k_paged_append_i8(PagedArgs a, int8_t *pages, float2 *scales,
+                                                         const float *__restrict__ latent,
+                                                         const float *__restrict__ krot,
+                                                         int8_t *__restrict__ mean,
+                                                         float *__restrict__ mean_scale) {
+    extern __shared__ double sum[];  // [4][D]
+    constexpr int NW = 9;
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, D = a.L + a.P, nq = D / 4;
+    bool bad = false;
+    const int32_t len = plan_len(((const_i32 *)a.lens)[b], (int64_t)a.max_pages << a.shift, bad);
+    if (bad) {  // cut to the table's end, the new rows would take the place of older ones
+        *a.err = 1;
+        return;
+    }
+    const int32_t from = len > a.M ? len - a.M : 0;  // the first new position
+    const int k = (from >> a.shift) + (int)blockIdx.x;
+    const int32_t page = 1 << a.shift;
+    const int64_t p0 = (int64_t)k << a.shift;
+    if (p0 >= len) return;
+    const int32_t phys = paged_phys(a, b, k, bad);
+    if (bad) return;
+    const int live = len - p0 < page ? (int)(len - p0) : page;
+    const int first = from > p0 ? (int)(from - p0) : 0;  // the page's first new row
+    const int64_t at0 = (int64_t)phys << a.shift, r0 = (int64_t)b * a.M + (p0 - (len - a.M));
+    for (int o = first + w; o < live; o += NW) {
+        float4 x[4];
+        uint32_t top[2] = {0, 0};  // bits of |x|: NaN lies above infinity
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = 4 * (lane + 64 * i);
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (d < D) x[i] = *(const float4 *)(d < a.L ? latent + (r0 + o) * a.L + d : krot + (r0 + o) * a.P + (d - a.L));
+            const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
+                if (d < a.L) top[0] = m > top[0] ? m : top[0];
+                else top[1] = m > top[1] ? m : top[1];
+            }
+        }
+        for (int off = 32; off >= 1; off >>= 1)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                const uint32_t y = __shfl_xor(top[p], off, 64);
+                top[p] = y > top[p] ? y : top[p];
+            }
+        double m[2], f[2];
+        float sc[2];
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            const bool fits = top[p] < 0x7f800000u;
+            m[p] = fits ? (double)__uint_as_float(top[p]) : 0.0;
+            f[p] = m[p] > 0.0 ? 127.0 / m[p] : 0.0;
+            sc[p] = fits ? (float)(m[p] / 127.0) : __uint_as_float(0x7fc00000u);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = 4 * (lane + 64 * i), p = d < a.L ? 0 : 1;
+            const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            uint32_t c = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                c |= (uint32_t)((m[p] > 0.0 ? code8<double>((double)v[e], m[p], f[p]) : 0) & 255) << (8 * e);
+            if (d < D) *(uint32_t *)(pages + (at0 + o) * D + d) = c;
+        }
+        if (lane == 0) scales[at0 + o] = make_float2(sc[0], sc[1]);
+    }
     if (!mean) return;
     __syncthreads();
-    double top = 0.0;
-    for (int d = tid; d < D; d += blockDim.x) {
-        const double t = (sum[d] + sum[D + d]) + (sum[2 * D + d] + sum[3 * D + d]);
-        sum[d] = t;
-        top = fmax(top, fabs(t));
+    for (int u = tid; u < 4 * nq; u += blockDim.x) {
+        const int s = u / nq, d = (u - s * nq) * 4;
+        double t[4] = {0.0, 0.0, 0.0, 0.0};
+        constexpr int kRows = 16;  // at a time, so that as many loads are under way
+        for (int o0 = s; o0 < live; o0 += 4 * kRows) {
+            uint32_t v[kRows];
+            float sc[kRows];
+#pragma unroll
+            for (int i = 0; i < kRows; i++) {
+                const int64_t o = at0 + (o0 + 4 * i < live ? o0 + 4 * i : o0);
+                v[i] = *(const uint32_t *)(pages + o * D + d);
+                sc[i] = ((const float *)scales)[2 * o + (d < a.L ? 0 : 1)];
+            }
+#pragma unroll
+            for (int i = 0; i < kRows; i++)
+                if (o0 + 4 * i < live)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) t[e] += (double)code_byte(v[i], e) * (double)sc[i];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[s * D + d + e] = t[e];
     }
-    for (int off = 32; off >= 1; off >>= 1) top = fmax(top, __shfl_xor(top, off, 64));
-    if ((tid & 63) == 0) red[tid >> 6] = top;
-    __syncthreads();
-    for (int w = 0; w < (int)(blockDim.x >> 6); w++) top = fmax(top, red[w]);
-    for (int d = tid; d < D; d += blockDim.x) {
-        const double c = top > 0.0 ? rint(sum[d] * 127.0 / top) : 0.0;
-        mean[(int64_t)phys * D + d] = (int8_t)(c >= -127.0 && c <= 127.0 ? (int)c : 0);
+    write_summary(sum, D, live, mean + (int64_t)phys * D, mean_scale + phys);
+}
+
+// ---------------------------------------------------------------- read ---
+// Rows start_b + j of each sequence as f32 or bf16: value(x) rounded once more
+// where that is bf16; zeros for rows outside the sequence.  A thread takes
+// eight values of a row, a workgroup as many whole rows as it has room for.
+template <class T> __device__ __forceinline__ void put8(T *dst, const float4 &x, const float4 &y) {
+    if constexpr (sizeof(T) == 4) {
+        ((float4 *)dst)[0] = x;
+        ((float4 *)dst)[1] = y;
+    } else {
+        typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+        *(b8 *)dst = b8{(__bf16)x.x, (__bf16)x.y, (__bf16)x.z, (__bf16)x.w, (__bf16)y.x, (__bf16)y.y, (__bf16)y.z, (__bf16)y.w};
     }
-    if (tid == 0) mean_scale[phys] = (float)(top / (127.0 * live));
+}
+constexpr int kReadThreads = 512, kReadTurns = 4;
+template <class F, class T>
+__global__ __launch_bounds__(kReadThreads) void k_paged_read(PagedArgs a, const int32_t *__restrict__ starts, int rows,
+                                                             T *__restrict__ latent, T *__restrict__ krot) {
+    const int b = blockIdx.y, G = (a.L + a.P) / 8, in = threadIdx.x / G, d = 8 * (threadIdx.x - in * G);
+    const int32_t len = paged_len(a, b);
+    const int64_t start = starts ? starts[b] : 0;
+    if (in >= rows) return;
+    float4 x[kReadTurns], y[kReadTurns];
+#pragma unroll
+    for (int i = 0; i < kReadTurns; i++) {
+        const int64_t j = ((int64_t)blockIdx.x * kReadTurns + i) * rows + in, t = start + j;
+        x[i] = y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (j < a.M && t >= 0 && t < len) {
+            const int32_t phys = paged_phys(a, b, (int)(t >> a.shift));
+            const int64_t pos = ((int64_t)phys << a.shift) + (t & ((1 << a.shift) - 1));
+            x[i] = F::quad(a, pos, d);
+            y[i] = F::quad(a, pos, d + 4);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kReadTurns; i++) {
+        const int64_t j = ((int64_t)blockIdx.x * kReadTurns + i) * rows + in, r = (int64_t)b * a.M + j;
+        if (j < a.M) put8(d < a.L ? latent + r * a.L + d : krot + r * a.P + (d - a.L), x[i], y[i]);
+    }
 }
 
 // ----------------------------------------------------------- attention ---
@@ -162,14 +355,18 @@ __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__r
 constexpr int kGenChunk = 64, kGenHeads = 4, kGenSlices = 32;
 constexpr float kGenLow = -3.402823466e38f;  // the maximum before any score
 
-// Virtual positions of a row and how they are cut.
+// Virtual positions of a row and how they are cut.  With a window these are
+// the `first` first ones and then those from `from` on.
 struct GenCut {
     int64_t total;
     int32_t chunks, per;  // chunks of a slice
+    int32_t first, from;
 };
 __device__ __forceinline__ GenCut gen_cut(const PagedArgs &a, int32_t n, int slices) {
     GenCut c;
-    c.total = n <= 0 ? 0 : a.sel ? (int64_t)a.top_k << a.shift : n;
+    c.from = a.window && n > a.window ? n - a.window : 0;
+    c.first = a.sinks < c.from ? a.sinks : c.from;
+    c.total = n <= 0 ? 0 : a.sel ? (int64_t)a.top_k << a.shift : n - c.from + c.first;
     c.chunks = (int32_t)((c.total + kGenChunk - 1) / kGenChunk);
     c.per = (c.chunks + slices - 1) / slices;
     return c;
@@ -205,12 +402,12 @@ __global__ __launch_bounds__(256) void k_paged_generic(PagedArgs a, int slices, 
 #pragma unroll
         for (int i = 0; i < 4; i++) o[h][i] = 0.0f;
     float m = kGenLow, l = 0.0f;  // wave w: of head w
-    const int64_t row16 = (int64_t)D * F::kPlanes;
     for (int32_t c = c0; c < c1; c++) {
         if (tid < kGenChunk) {
-            const int64_t t = (int64_t)c * kGenChunk + tid;
+            int64_t t = (int64_t)c * kGenChunk + tid;
             int64_t row = -1;
             if (t < cut.total) {
+                t += t >= cut.first ? cut.from - cut.first : 0;
                 int64_t k = t >> a.shift;
                 if (a.sel) k = a.sel[r * a.top_k + k];
                 const int64_t in = t & ((1 << a.shift) - 1);
@@ -223,19 +420,16 @@ __global__ __launch_bounds__(256) void k_paged_generic(PagedArgs a, int slices, 
             const int t = tid >> 2, s = tid & 3;
             float acc[HG] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (at[t] >= 0) {
-                const uint16_t *src = (const uint16_t *)a.pages + at[t] * row16;
 #pragma unroll 4
                 for (int d = 4 * s; d < D; d += 16) {
-                    uint2 v[F::kPlanes];
-#pragma unroll
-                    for (int i = 0; i < F::kPlanes; i++) v[i] = *(const uint2 *)(src + i * D + d);
+                    const float4 v = F::quad(a, at[t], d);
 #pragma unroll
                     for (int h = 0; h < HG; h++) {
                         const float4 x = *(const float4 *)(q + h * D + d);
-                        acc[h] = __builtin_fmaf(x.x, F::stored(v, 0), acc[h]);
-                        acc[h] = __builtin_fmaf(x.y, F::stored(v, 1), acc[h]);
-                        acc[h] = __builtin_fmaf(x.z, F::stored(v, 2), acc[h]);
-                        acc[h] = __builtin_fmaf(x.w, F::stored(v, 3), acc[h]);
+                        acc[h] = __builtin_fmaf(x.x, v.x, acc[h]);
+                        acc[h] = __builtin_fmaf(x.y, v.y, acc[h]);
+                        acc[h] = __builtin_fmaf(x.z, v.z, acc[h]);
+                        acc[h] = __builtin_fmaf(x.w, v.w, acc[h]);
                     }
                 }
             }
@@ -275,7 +469,7 @@ __global__ __launch_bounds__(256) void k_paged_generic(PagedArgs a, int slices, 
 #pragma unroll 8
             for (int t = way; t < kGenChunk; t += ways)
                 if (at[t] >= 0) {
-                    const float v = F::value((const uint16_t *)a.pages + at[t] * row16, D, d);
+                    const float v = F::value(a, at[t], d);
                     const float4 e = *(const float4 *)p[t];
                     x[0] = __builtin_fmaf(e.x, v, x[0]);
                     x[1] = __builtin_fmaf(e.y, v, x[1]);
@@ -350,21 +544,11 @@ __global__ __launch_bounds__(256) void k_paged_generic_join(PagedArgs a, int sli
 }
 
 // -------------------------------------------------------------- select ---
-// A head's query in 8 bits: code = rint(q 127 / max|q|) of the real quotient;
-// its share of a score is weight max|q| / 127.  A head with a value that is
-// not finite has none.  c = rint(q (127 / max)) may miss by one next to a
-// half; q 127 - c max is exact and tells: a bf16 query's numbers fit f32 (15
-// bits), a f32 one's take 64 bits.
+// A head's query in 8 bits: code = rint(q 127 / max|q|) of the real quotient
+// (code8); its share of a score is weight max|q| / 127.  A head with a value
+// that is not finite has none.
 constexpr int kCodeStep = 64;
 __host__ __device__ inline int64_t code_row(int64_t D) { return (D + kCodeStep - 1) / kCodeStep * kCodeStep; }
-__device__ __forceinline__ float exact_fma(float x, float y, float z) { return __builtin_fmaf(x, y, z); }
-__device__ __forceinline__ double exact_fma(double x, double y, double z) { return __builtin_fma(x, y, z); }
-template <class T> __device__ __forceinline__ int code8(T q, T top, T f) {
-    const T c = rint(q * f), e = exact_fma(c, -2 * top, q * 254);  // twice the rest
-    const int k = (int)c;
-    const bool next = e > top || -e > top || ((e == top || -e == top) && (k & 1));
-    return next ? (e > 0 ? k + 1 : k - 1) : k;
-}
 // Head r's query (none from `end` on), over a wave: eight dims a lane, a
 // single one behind them, and (D is at most 1024) up to seven more, which are
 // read where they are used.
@@ -782,7 +966,9 @@ static int32_t paged_args(ut_ctx *ctx, const DeviceScope &dev, const char *what,
         return UT_ERR_ARG;
     };
     if (!kv || !kv->pages || !table || !lens) return bad("null pointer");
-    if (kv->fmt != UT_KV_BF16 && kv->fmt != UT_KV_F16X2) return bad("unknown cache format");
+    if (kv->fmt != UT_KV_BF16 && kv->fmt != UT_KV_F16X2 && kv->fmt != UT_KV_I8) return bad("unknown cache format");
+    if (kv->fmt == UT_KV_I8 && (!kv->scales || ((uintptr_t)kv->scales & 15) != 0))
+        return bad("8-bit pages need their scales, 16-byte aligned");
     if (kv->n_pages <= 0 || max_pages <= 0 || B <= 0 || M <= 0 || H <= 0 || stride < max_pages)
         return bad("sizes must be positive and the table's stride cover its pages");
     if (((uintptr_t)kv->pages & 15) != 0) return bad("pages must be 16-byte aligned");
@@ -804,6 +990,7 @@ static int32_t paged_args(ut_ctx *ctx, const DeviceScope &dev, const char *what,
         return shape("too many sequences, rows or heads");
     a = PagedArgs{};
     a.pages = kv->pages;
+    a.scales = kv->fmt == UT_KV_I8 ? (const float2 *)kv->scales : nullptr;
     a.table = table;
     a.stride = stride;
     a.lens = lens;
@@ -823,7 +1010,8 @@ static int32_t paged_args(ut_ctx *ctx, const DeviceScope &dev, const char *what,
 static int32_t launch_paged_generic(ut_ctx *ctx, const PagedArgs &a, int32_t fmt) {
     // slices: four workgroups a CU, partial results of 64 MB at most
     const int64_t groups = (a.H + kGenHeads - 1) / kGenHeads, R = (int64_t)a.B * a.M;
-    const int64_t cap = (int64_t)(a.sel ? a.top_k : a.max_pages) << a.shift;
+    const int64_t held = (int64_t)(a.sel ? a.top_k : a.max_pages) << a.shift, near = (int64_t)a.window + a.sinks;
+    const int64_t cap = a.window && near < held ? near : held;
     int64_t slices = 4 * ctx->multiprocessors / (R * groups);
     const int64_t room = (int64_t(64) << 20) / (R * a.H * a.L * 4), chunks = (cap + kGenChunk - 1) / kGenChunk;
     slices = slices < room ? slices : room;
@@ -841,14 +1029,16 @@ static int32_t launch_paged_generic(ut_ctx *ctx, const PagedArgs &a, int32_t fmt
     }
     const size_t lds = (size_t)kGenHeads * (a.L + a.P < 256 ? 256 : a.L + a.P) * 4;
     int tok = timing_begin(ctx, "paged_generic");
-    hipLaunchKernelGGL((fmt == UT_KV_BF16 ? k_paged_generic<Bf16> : k_paged_generic<F16x2>),
+    hipLaunchKernelGGL((fmt == UT_KV_BF16 ? k_paged_generic<Bf16>
+                        : fmt == UT_KV_I8 ? k_paged_generic<I8>
+                                          : k_paged_generic<F16x2>),
                        dim3((unsigned)groups, (unsigned)(a.M * slices), (unsigned)a.B), dim3(256), lds, ctx->stream, a,
                        (int)slices, ml, po);
     timing_end(ctx, tok);
     UT_TRY(launch_check(ctx, "k_paged_generic"));
     if (slices == 1) return UT_OK;
     tok = timing_begin(ctx, "paged_generic_join");
-    hipLaunchKernelGGL((fmt == UT_KV_BF16 ? k_paged_generic_join<Bf16> : k_paged_generic_join<F16x2>),
+    hipLaunchKernelGGL((fmt == UT_KV_F16X2 ? k_paged_generic_join<F16x2> : k_paged_generic_join<Bf16>),
                        dim3((unsigned)(R * a.H)), dim3(256), 0, ctx->stream, a, (int)slices, ml, po);
     timing_end(ctx, tok);
     return launch_check(ctx, "k_paged_generic_join");
@@ -858,7 +1048,7 @@ static int32_t paged_attend(ut_ctx *ctx, const char *what, const ut_mla_pages *k
                             const int32_t *table, int64_t stride, int64_t max_pages,
                             const int32_t *lens, int64_t B, int64_t M, int64_t H, const void *qabs,
                             const void *qrope, float scale, const int32_t *sel, int64_t top_k,
-                            void *out) {
+                            int64_t window, int64_t sinks, void *out) {
     DeviceScope dev(ctx->device);
     PagedArgs a;
     UT_TRY(paged_args(ctx, dev, what, kv, table, stride, max_pages, lens, B, M, H, kMostRows, a));
@@ -872,8 +1062,11 @@ static int32_t paged_attend(ut_ctx *ctx, const char *what, const ut_mla_pages *k
     a.scale = scale;
     a.sel = sel;
     a.top_k = (int32_t)top_k;
+    // (no sequence is longer than kMostPositions)
+    a.window = (int32_t)(window < kMostPositions ? window : kMostPositions);
+    a.sinks = (int32_t)(sinks < kMostPositions ? sinks : kMostPositions);
     a.out = out;
-    if (paged_mfma_ok(a)) return launch_paged_mfma(ctx, a, kv->fmt);
+    if (paged_mfma_ok(a) && kv->fmt != UT_KV_I8 && !window) return launch_paged_mfma(ctx, a, kv->fmt);
     return launch_paged_generic(ctx, a, kv->fmt);
 }
 
@@ -909,11 +1102,51 @@ extern "C" int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv,
     if (kv->fmt == UT_KV_BF16)
         hipLaunchKernelGGL(k_paged_append<Bf16>, grid, dim3(576), lds, ctx->stream, a,
                            (uint16_t *)kv->pages, latent_dev, krot_dev, kv->mean, kv->mean_scale);
+    else if (kv->fmt == UT_KV_I8)
+        hipLaunchKernelGGL(k_paged_append_i8, grid, dim3(576), lds, ctx->stream, a, (int8_t *)kv->pages,
+                           (float2 *)kv->scales, latent_dev, krot_dev, kv->mean, kv->mean_scale);
     else
         hipLaunchKernelGGL(k_paged_append<F16x2>, grid, dim3(576), lds, ctx->stream, a,
                            (uint16_t *)kv->pages, latent_dev, krot_dev, kv->mean, kv->mean_scale);
     timing_end(ctx, tok);
     return launch_check(ctx, "k_paged_append");
+}
+
+extern "C" int32_t ut_mla_paged_read(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
+                                     int64_t table_stride, int64_t max_pages,
+                                     const int32_t *lens_dev, int64_t batch, int64_t rows,
+                                     const int32_t *starts_dev, int32_t type, void *latent_dev,
+                                     void *krot_dev) {
+    if (!ctx) return UT_ERR_ARG;
+    DeviceScope dev(ctx->device);
+    PagedArgs a;
+    UT_TRY(paged_args(ctx, dev, "ut_mla_paged_read", kv, table_dev, table_stride, max_pages, lens_dev,
+                      batch, rows, 1, INT32_MAX, a));
+    if (!latent_dev || !krot_dev || ((uintptr_t)latent_dev & 15) != 0 || ((uintptr_t)krot_dev & 15) != 0 ||
+        (type != UT_ROWS_F32 && type != UT_ROWS_BF16)) {
+        set_error(ctx, "ut_mla_paged_read: rows are f32 or bf16 in 16-byte aligned device memory");
+        return UT_ERR_ARG;
+    }
+    const int per = kReadThreads / ((a.L + a.P) / 8);  // rows of a workgroup at a time
+    const int64_t groups = (rows + per * kReadTurns - 1) / (per * kReadTurns);
+    if (groups > kMostGroups) {
+        set_error(ctx, "ut_mla_paged_read: more than %lld rows of a sequence in a call",
+                  (long long)(kMostGroups * per * kReadTurns));
+        return UT_ERR_SHAPE;
+    }
+    const dim3 grid((unsigned)groups, (unsigned)batch);
+    int tok = timing_begin(ctx, "paged_read");
+    auto launch = [&](auto *out) {
+        typedef std::remove_pointer_t<decltype(out)> T;
+        hipLaunchKernelGGL((kv->fmt == UT_KV_BF16 ? k_paged_read<Bf16, T>
+                            : kv->fmt == UT_KV_I8 ? k_paged_read<I8, T>
+                                                  : k_paged_read<F16x2, T>),
+                           grid, dim3(kReadThreads), 0, ctx->stream, a, starts_dev, per, out, (T *)krot_dev);
+    };
+    if (type == UT_ROWS_F32) launch((float *)latent_dev);
+    else launch((__bf16 *)latent_dev);
+    timing_end(ctx, tok);
+    return launch_check(ctx, "k_paged_read");
 }
 
 extern "C" int32_t ut_mla_paged_attend(ut_ctx *ctx, const ut_mla_pages *kv,
@@ -924,7 +1157,24 @@ extern "C" int32_t ut_mla_paged_attend(ut_ctx *ctx, const ut_mla_pages *kv,
     if (!ctx) return UT_ERR_ARG;
     return paged_attend(ctx, "ut_mla_paged_attend", kv, table_dev, table_stride, max_pages,
                         lens_dev, batch, rows, heads, qabs_dev, q_rope_dev, scale, nullptr, 0,
-                        clat_dev);
+                        0, 0, clat_dev);
+}
+
+extern "C" int32_t ut_mla_window_attend(ut_ctx *ctx, const ut_mla_pages *kv,
+                                        const int32_t *table_dev, int64_t table_stride,
+                                        int64_t max_pages, const int32_t *lens_dev, int64_t batch,
+                                        int64_t rows, int64_t heads, const void *qabs_dev,
+                                        const void *q_rope_dev, float scale, int64_t window,
+                                        int64_t sinks, void *clat_dev) {
+    if (!ctx) return UT_ERR_ARG;
+    if (window < 1 || sinks < 0) {
+        set_error(ctx, "ut_mla_window_attend: a window of one position or more and no fewer than 0 first ones are "
+                       "needed, not %lld and %lld", (long long)window, (long long)sinks);
+        return UT_ERR_ARG;
+    }
+    return paged_attend(ctx, "ut_mla_window_attend", kv, table_dev, table_stride, max_pages,
+                        lens_dev, batch, rows, heads, qabs_dev, q_rope_dev, scale, nullptr, 0,
+                        window, sinks, clat_dev);
 }
 
 extern "C" int32_t ut_mla_sparse_attend(ut_ctx *ctx, const ut_mla_pages *kv,
@@ -940,7 +1190,7 @@ extern "C" int32_t ut_mla_sparse_attend(ut_ctx *ctx, const ut_mla_pages *kv,
     }
     return paged_attend(ctx, "ut_mla_sparse_attend", kv, table_dev, table_stride, max_pages,
                         lens_dev, batch, rows, heads, qabs_dev, q_rope_dev, scale, sel_dev, top_k,
-                        clat_dev);
+                        0, 0, clat_dev);
 }
 
 extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,
@@ -991,7 +1241,7 @@ extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const
     double *part = (double *)ptrs[0], *share = (double *)ptrs[3];
     uint64_t *keys = (uint64_t *)ptrs[1];
     int8_t *codes = (int8_t *)ptrs[2];
-    const bool bf16 = kv->fmt == UT_KV_BF16;
+    const bool bf16 = kv->fmt != UT_KV_F16X2;  // queries
     for (int64_t r0 = 0; r0 < R; r0 += slice) {
         const int64_t n = R - r0 < slice ? R - r0 : slice;
         if (fused) {

@@ -40,7 +40,8 @@ UT_ERR_STATE = -10
 UT_ERR_IO = -11
 UT_ERR_BAD_PAGE = -12
 
-KV_BF16, KV_F16X2 = 0, 1
+KV_BF16, KV_F16X2, KV_I8 = 0, 1, 8
+ROWS_F32, ROWS_BF16 = 0, 1
 
 
 class UtError(RuntimeError):
@@ -104,12 +105,15 @@ _SIGS = [
     ("ut_mla_cache_split", _i32, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     ("ut_mla_attend_split", _i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp]),
     ("ut_mla_paged_append", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp]),
+    ("ut_mla_paged_read", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _vp]),
     ("ut_mla_paged_attend", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _f32,
                                    _vp]),
     ("ut_mla_page_select", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp,
                                   _i64, _i64, _i64, _vp]),
     ("ut_mla_sparse_attend", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _f32,
                                     _vp, _i64, _vp]),
+    ("ut_mla_window_attend", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _f32,
+                                    _i64, _i64, _vp]),
     ("ut_model_create", _i32, [_vp, _vp, C.POINTER(_vp)]),
     ("ut_model_set_tensor", _i32, [_vp, C.c_char_p, _i32, _vp, _i64, _vp, _i64, _i64]),
     ("ut_model_finalize", _i32, [_vp]),
@@ -196,7 +200,7 @@ class ModelConfig(C.Structure):
 class MlaPages(C.Structure):
     """ut_mla_pages: a pool of pages and their summaries."""
     _fields_ = [("pages", _vp), ("mean", _vp), ("mean_scale", _vp), ("n_pages", _i64),
-                ("page", _i64), ("latent", _i64), ("rope", _i64), ("fmt", _i32)]
+                ("page", _i64), ("latent", _i64), ("rope", _i64), ("fmt", _i32), ("scales", _vp)]
 
 
 class StoreConfig(C.Structure):
@@ -515,10 +519,11 @@ class PagedCache:
     """One layer's latent cache of many sequences in a pool of pages.
 
     pages: bfloat16 [n_pages, page, latent + rope], or float16 [n_pages, page,
-    2, latent + rope] whose two planes stand for f32 values hi + lo / 2048;
-    mean (int8 [n_pages, latent + rope]) and mean_scale (float32 [n_pages])
+    2, latent + rope] whose two planes stand for f32 values hi + lo / 2048, or
+    int8 [n_pages, page, latent + rope] codes with scales float32 [n_pages,
+    page, 2] of a position's latent and of its rotated key.  mean (int8 [n_pages, latent + rope]) and mean_scale (float32 [n_pages])
     hold a summary per page for ``select``.  The tensors are the caller's and
-    stay theirs.
+    stay theirs.  Queries and contexts are bfloat16, with float16 pages float32.
 
     Every call takes a batch: table [B, max_pages] int32 (physical pages in a
     sequence's order; the rows may be slices of a wider table) and lens [B]
@@ -527,28 +532,34 @@ class PagedCache:
     page out of range is reported by the context's next ``synchronize``."""
 
     def __init__(self, ctx: Context, pages, latent: int = 512, rope: int = 64, mean=None,
-                 mean_scale=None):
+                 mean_scale=None, scales=None):
         torch = _torch()
         D = latent + rope
-        if pages.dtype == torch.bfloat16:
+        if pages.dtype == torch.int8:
+            self.fmt, self.dtype, shape = KV_I8, torch.bfloat16, tuple(pages.shape[:2]) + (D,)
+        elif pages.dtype == torch.bfloat16:
             self.fmt, self.dtype, shape = KV_BF16, torch.bfloat16, tuple(pages.shape[:2]) + (D,)
         elif pages.dtype == torch.float16:
             self.fmt, self.dtype, shape = KV_F16X2, torch.float32, tuple(pages.shape[:2]) + (2, D)
         else:
-            raise UtError(UT_ERR_ARG, f"PagedCache: pages are bfloat16 or float16, got {pages.dtype}")
+            raise UtError(UT_ERR_ARG, f"PagedCache: pages are bfloat16, float16 or int8, got {pages.dtype}")
         if len(pages.shape) < 2:
             raise ShapeError(UT_ERR_SHAPE, "PagedCache: pages must have a page and a position axis")
         if (mean is None) != (mean_scale is None):
             raise UtError(UT_ERR_ARG, "PagedCache: mean and mean_scale are given together")
+        if (self.fmt == KV_I8) != (scales is not None):
+            raise UtError(UT_ERR_ARG, "PagedCache: int8 pages, and no others, are given with scales")
         self.ctx, self.latent, self.rope = ctx, latent, rope
-        self.pages, self.mean, self.mean_scale = pages, mean, mean_scale
+        self.pages, self.mean, self.mean_scale, self.scales = pages, mean, mean_scale, scales
         n, self.page = int(pages.shape[0]), int(pages.shape[1])
         self._tensor("pages", pages, pages.dtype, shape)
         if mean is not None:
             self._tensor("mean", mean, torch.int8, (n, D))
             self._tensor("mean_scale", mean_scale, torch.float32, (n,))
+        if scales is not None:
+            self._tensor("scales", scales, torch.float32, (n, self.page, 2))
         self._kv = MlaPages(_ptr(pages), _ptr(mean), _ptr(mean_scale), n, self.page, latent, rope,
-                            self.fmt)
+                            self.fmt, _ptr(scales))
         self._ref = C.byref(self._kv)
 
     @classmethod
@@ -556,11 +567,14 @@ class PagedCache:
               fmt: int = KV_BF16, summaries: bool = True) -> "PagedCache":
         """A cache over a pool of its own."""
         torch = _torch()
-        if fmt not in (KV_BF16, KV_F16X2):
-            raise UtError(UT_ERR_ARG, f"PagedCache: fmt is KV_BF16 or KV_F16X2, got {fmt!r}")
+        if fmt not in (KV_BF16, KV_F16X2, KV_I8):
+            raise UtError(UT_ERR_ARG, f"PagedCache: fmt is KV_BF16, KV_F16X2 or KV_I8, got {fmt!r}")
         d, D = f"cuda:{ctx.device}", latent + rope
-        pages = (torch.zeros((n_pages, page, D), dtype=torch.bfloat16, device=d) if fmt == KV_BF16
-                 else torch.zeros((n_pages, page, 2, D), dtype=torch.float16, device=d))
+        if fmt == KV_F16X2:
+            pages = torch.zeros((n_pages, page, 2, D), dtype=torch.float16, device=d)
+        else:
+            pages = torch.zeros((n_pages, page, D), dtype=torch.bfloat16 if fmt == KV_BF16 else torch.int8, device=d)
+        scales = torch.zeros((n_pages, page, 2), device=d) if fmt == KV_I8 else None
         mean = scale = None
         if summaries:
             mean = torch.zeros((n_pages, D), dtype=torch.int8, device=d)
@@ -569,7 +583,7 @@ class PagedCache:
         torch_stream = torch.cuda.current_stream(ctx.device)
         if torch_stream.cuda_stream != (lib().ut_ctx_stream(ctx.handle) or 0):
             torch_stream.synchronize()
-        return cls(ctx, pages, latent, rope, mean, scale)
+        return cls(ctx, pages, latent, rope, mean, scale, scales)
 
     def _tensor(self, name: str, t, dtype, shape) -> int:
         if t.shape != shape:
@@ -623,12 +637,43 @@ class PagedCache:
             *batch, self._tensor("latent", latent, torch.float32, (B, M, self.latent)),
             self._tensor("krot", krot, torch.float32, (B, M, self.rope))))
 
+    def read(self, table, lens, rows: int, starts=None, dtype=None, out=None):
+        """The rows at positions starts[b] + [0, rows) of each sequence (starts
+        [B] int32; None: from its first) -> (latent [B, rows, latent], krot [B,
+        rows, rope]) in dtype, float32 (None) or bfloat16; zeros where the
+        sequence has no such position.  out: the two tensors to write."""
+        torch = _torch()
+        dtype = torch.float32 if dtype is None else dtype
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise UtError(UT_ERR_ARG, f"PagedCache: rows are read as float32 or bfloat16, got {dtype}")
+        batch = self._batch(table, lens, rows)
+        B = batch[6]
+        s = None if starts is None else self._tensor("starts", starts, torch.int32, (B,))
+        shapes = (B, max(rows, 0), self.latent), (B, max(rows, 0), self.rope)
+        if out is None:
+            out = tuple(torch.empty(x, dtype=dtype, device=table.device) for x in shapes)
+        elif len(out) != 2:
+            raise ShapeError(UT_ERR_SHAPE, "PagedCache: out must be two tensors")
+        self.ctx.check(lib().ut_mla_paged_read(
+            *batch, s, ROWS_F32 if dtype == torch.float32 else ROWS_BF16,
+            self._tensor("out[0]", out[0], dtype, shapes[0]), self._tensor("out[1]", out[1], dtype, shapes[1])))
+        return tuple(out)
+
     def attend(self, table, lens, qabs, q_rope, scale: float, out=None):
         """Absorbed attention of qabs [B, M, H, latent] and q_rope [B, M, H,
         rope] over each row's positions -> [B, M, H, latent]."""
         q = self._queries(table, lens, qabs, q_rope)
         out = self._context(qabs, out)
         self.ctx.check(lib().ut_mla_paged_attend(*q, scale, _ptr(out)))
+        return out
+
+    def attend_window(self, table, lens, qabs, q_rope, scale: float, window: int, sinks: int = 0, out=None):
+        """``attend`` where each row sees the last `window` of the positions up
+        to its own and the sequence's first `sinks`.  Pages that hold none of
+        them for any row need not stand in the table."""
+        q = self._queries(table, lens, qabs, q_rope)
+        out = self._context(qabs, out)
+        self.ctx.check(lib().ut_mla_window_attend(*q, scale, window, sinks, _ptr(out)))
         return out
 
     def select(self, table, lens, qabs, q_rope, top_k: int, keep_first: int = 1, keep_last: int = 1,
