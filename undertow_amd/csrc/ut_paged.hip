@@ -1066,7 +1066,7 @@ static int32_t paged_attend(ut_ctx *ctx, const char *what, const ut_mla_pages *k
     a.window = (int32_t)(window < kMostPositions ? window : kMostPositions);
     a.sinks = (int32_t)(sinks < kMostPositions ? sinks : kMostPositions);
     a.out = out;
-    if (paged_mfma_ok(a) && kv->fmt != UT_KV_I8 && !window) return launch_paged_mfma(ctx, a, kv->fmt);
+    if (paged_mfma_ok(a)) return launch_paged_mfma(ctx, a, kv->fmt);
     return launch_paged_generic(ctx, a, kv->fmt);
 }
 
