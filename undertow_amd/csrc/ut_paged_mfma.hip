@@ -336,7 +336,7 @@ struct MfmaBf16 {
         }
         return sum;
     }
-    template <bool HIDE> __device__ __forceinline__ static void context(const Weights &x, uint32_t T, pf32x4 (&o)[32], pu32x4 keep) {
+    __device__ __forceinline__ static void context(const Weights &x, uint32_t T, pf32x4 (&o)[32]) {
         pu32x4 v[32];
         auto read = [&](int i) {
             const uint32_t b = (T ^ ((i & 3) << 5)) + (i >> 2) * 1024;
@@ -347,7 +347,6 @@ struct MfmaBf16 {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 32; i++) {
-            if (HIDE) v[i] &= keep;
             o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pbf16x8, v[i]), x.p, o[i], 0, 0, 0);
             if (i + kDepth < 32) read(i + kDepth);
             __builtin_amdgcn_sched_barrier(0);
@@ -450,7 +449,7 @@ struct MfmaF16x2 {
         x.d = x.h * (_Float16)(1.0f / kF16x2Step);
         return sum;
     }
-    template <bool HIDE> __device__ __forceinline__ static void context(const Weights &x, uint32_t T, pf32x4 (&o)[32], pu32x4 keep) {
+    __device__ __forceinline__ static void context(const Weights &x, uint32_t T, pf32x4 (&o)[32]) {
         pu32x4 h[32], d[32];
         auto read = [&](int i) {
             const uint32_t b = (T ^ ((i & 3) << 5)) + (i >> 2) * 1024;
@@ -462,12 +461,6 @@ struct MfmaF16x2 {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-            if (HIDE)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    h[i + e] &= keep;
-                    d[i + e] &= keep;
-                }
 #pragma unroll
             for (int e = 0; e < 2; e++) o[i + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pf16x8, h[i + e]), x.l, o[i + e], 0, 0, 0);
 #pragma unroll
@@ -504,7 +497,7 @@ struct MfmaI8 {
     static constexpr PlanCosts kCosts = kCostsI8;
     static constexpr int kPlanes = 1, kWaves = kCosts.waves;
     static constexpr bool kBetween = false;
-    static constexpr int kDepth = 4;
+    static constexpr int kDepth = 4, kAhead = 2;
     static constexpr float kRise = 11.5f;
     typedef __bf16 out_t;
     // The rotary codes of row r, 64 bytes: chunks of 16 XORed with (r >> 2) & 3, so
@@ -519,7 +512,9 @@ struct MfmaI8 {
                 (uint32_t)((r >> 3) * 8 * 1024 + (r & 7) * 128 + ((((j & 3) >> 1) ^ tile_swz(r)) << 4) + 8 * (j & 1)),
                 (uint32_t)(kRope + row * 64 + ((g ^ (row >> 2)) << 4)), (uint32_t)(kScales + 32 * g)};
     }
-    // 16 dims of a step of 64 in two registers quads: bf16, then high and low digits
+    // Of a power of two.
+    __device__ __forceinline__ static float inverse(float g) { return __uint_as_float((254u << 23) - __float_as_uint(g)); }
+    // 16 dims of a step of 64 in two register quads: bf16, then high and low digits
     struct Query {
         pu32x4 w[18];
         float lat, rope;  // a digit's worth in each part, times the scores' scale
@@ -592,45 +587,51 @@ struct MfmaI8 {
     __device__ __forceinline__ static void arrive(Query &x, float c) {
         x.lat = __fmul_rn(digits<0, 16>(x), c);
         x.rope = __fmul_rn(digits<16, 18>(x), c);
+#pragma unroll
+        for (int i = 0; i < 18; i++) asm volatile("" : "+v"(x.w[i]));
     }
-    template <class W> __device__ __forceinline__ static float unit(const W &w) { return 1.0f / w.g; }
-    // Both halves of the tile in turn, the rotary part first; between(i) behind step i of 18.
-    template <class B> __device__ __forceinline__ static void scores(const Query &x, uint32_t T, const LaneAddr &ad, float (&t)[8], B &&between) {
+    template <class W> __device__ __forceinline__ static float unit(const W &w) { return inverse(w.g); }
+    // The tile's halves one after the other (their sums together would not fit
+    // the registers, and a reload would wait for the copies), the rotary part first.
+    __device__ __forceinline__ static void scores(const Query &x, uint32_t T, const LaneAddr &ad, float (&t)[8]) {
         const pi32x4 zero = {0, 0, 0, 0};
-        pi32x4 h[2] = {zero, zero}, d[2] = {zero, zero}, rh[2], rd[2], k[18];
-        auto read = [&](int i) {
-            if (i < 2) k[i] = lds_read<pi32x4>(T + ad.r + i * 1024);
-            else k[i] = lds_read<pi32x4>(((T + ad.k) ^ ((((i - 2) >> 1) & 1) << 6)) + ((i - 2) >> 2) * 1024 + (i & 1) * 2 * kBlocks * 1024);
-        };
 #pragma unroll
-        for (int i = 0; i < kDepth; i++) read(i);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int half = 0; half < 2; half++) {
+            pi32x4 h = zero, d = zero, rh, rd, k[9];
+            auto read = [&](int i) {
+                if (i == 0) k[i] = lds_read<pi32x4>(T + ad.r + half * 1024);
+                else k[i] = lds_read<pi32x4>(((T + ad.k) ^ (((i - 1) & 1) << 6)) + ((i - 1) >> 1) * 1024 + half * 2 * kBlocks * 1024);
+            };
 #pragma unroll
-        for (int i = 0; i < 18; i++) {
-            const int q = i < 2 ? 16 : (i - 2) & ~1;
-            const pi32x4 qh = __builtin_bit_cast(pi32x4, x.w[q]), qd = __builtin_bit_cast(pi32x4, x.w[q + 1]);
-            if (i < 2) {
-                rh[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i], qh, zero, 0, 0, 0);
-                rd[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i], qd, zero, 0, 0, 0);
-            } else {
-                h[i & 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i], qh, h[i & 1], 0, 0, 0);
-                d[i & 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i], qd, d[i & 1], 0, 0, 0);
-            }
-            if (i + kDepth < 18) read(i + kDepth);
-            if (i == 4)
-#pragma unroll
-                for (int e = 0; e < 8; e++) t[e] = __fmul_rn((float)((rh[e >> 2][e & 3] << 8) + rd[e >> 2][e & 3]), x.rope);
-            between(i);
+            for (int i = 0; i < kAhead; i++) read(i);
             __builtin_amdgcn_sched_barrier(0);
-        }
-        // (a tile's scales: latent and rotary by turns)
-        pf32x4 s[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = lds_read<pf32x4>(T + ad.s + (i >> 1) * 128 + (i & 1) * 16);
+            for (int i = 0; i < 9; i++) {
+                const int q = i == 0 ? 16 : 2 * (i - 1);
+                const pi32x4 qh = __builtin_bit_cast(pi32x4, x.w[q]), qd = __builtin_bit_cast(pi32x4, x.w[q + 1]);
+                if (i == 0) {
+                    rh = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i], qh, zero, 0, 0, 0);
+                    rd = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i], qd, zero, 0, 0, 0);
+                } else {
+                    h = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i], qh, h, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i], qd, d, 0, 0, 0);
+                }
+                if (i + kAhead < 9) read(i + kAhead);
+                if (i == 2)
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float lat = __fmul_rn((float)((h[e >> 2][e & 3] << 8) + d[e >> 2][e & 3]), x.lat);
-            t[e] = __builtin_fmaf(lat, s[e >> 1][2 * (e & 1)], __fmul_rn(t[e], s[e >> 1][2 * (e & 1) + 1]));
+                    for (int e = 0; e < 4; e++) t[4 * half + e] = __fmul_rn((float)((rh[e] << 8) + rd[e]), x.rope);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // (a tile's scales: latent and rotary by turns)
+            pf32x4 s[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) s[i] = lds_read<pf32x4>(T + ad.s + half * 128 + i * 16);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float lat = __fmul_rn((float)((h[e] << 8) + d[e]), x.lat);
+                t[4 * half + e] = __builtin_fmaf(lat, s[e >> 1][2 * (e & 1)], __fmul_rn(t[4 * half + e], s[e >> 1][2 * (e & 1) + 1]));
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     // The latent scales of a lane's positions.
@@ -678,8 +679,16 @@ template <int PART> __device__ __forceinline__ void convert_block(const pu32x4 &
     const uint32_t at = to + ((block >> 2) * 8 + 2 * (block & 3) + (in >> 2)) * 1024 + row * 128 + (((2 * (in & 3) + e) ^ tile_swz(row)) << 4);
     *(__attribute__((address_space(3))) pu32x4 *)at = v;
 }
+// The lane, as if not known yet: what is worked out of it is worked out anew for
+// each tile, since the products need the registers that it would be kept in.
+__device__ __forceinline__ int lane_anew() {
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    return l;
+}
 __device__ __forceinline__ pu32x4 codes_of(uint32_t from, int block, int l) { return lds_read<pu32x4>(from + block * 1024 + l * 16); }
-__device__ __forceinline__ void convert_tile(uint32_t from, uint32_t to, int w, int l) {
+__device__ __forceinline__ void convert_tile(uint32_t from, uint32_t to, int w) {
+    const int l = lane_anew();
     const pu32x4 a = codes_of(from, w, l), b = codes_of(from, w + 8, l);
     convert_block<0>(a, to, w, l);
     convert_block<1>(a, to, w, l);
@@ -703,10 +712,8 @@ template <class F> struct Wave {
 // other without leaving the lane.  The offset m moves only where a score
 // exceeds it by more than kRise.
 // seen: the tile's visible positions.  A hidden position's score is replaced,
-// whatever it is; what V holds there must be finite (tile_clear), or HIDE: it
-// is set to zero as it is read, since rows with windows of their own do not see
-// ever fewer of a tile's positions, one row after another.
-template <class F, bool HIDE, class B>
+// whatever it is; what V holds there must be finite (tile_clear).
+template <class F, class B>
 __device__ __forceinline__ void tile_step(Wave<F> &w, const LaneAddr &ad, uint32_t T, uint32_t seen, float c, int g, B &&between) {
     pf32x4 s[2];
     F::scores(w.q, T + ad.k, s, between);
@@ -734,46 +741,21 @@ __device__ __forceinline__ void tile_step(Wave<F> &w, const LaneAddr &ad, uint32
     for (int i = 0; i < 8; i++) t[i] = __builtin_amdgcn_exp2f(t[i] - w.m);
     typename F::Weights p;
     w.l = __fadd_rn(w.l, F::weigh(p, t));
-    if (HIDE && seen != ~0u) {
-        pu32x4 keep;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t two = mine >> ((i >> 1) * 16 + (i & 1) * 2);
-            keep[i] = (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
-        }
-        F::template context<true>(p, T + ad.v, w.o, keep);
-    } else {
-        F::template context<false>(p, T + ad.v, w.o, pu32x4{});
-    }
+    F::context(p, T + ad.v, w.o);
 }
 
-// The same with 8-bit pages: T's codes and scales, V's values; `more`: the next
-// tile's values are made of its codes meanwhile.
-__device__ __forceinline__ void tile_codes(Wave<MfmaI8> &w, const LaneAddr &ad, uint32_t T, uint32_t V, uint32_t seen, int g,
-                                           bool more, uint32_t from, uint32_t to, int wave, int l) {
+// The same with 8-bit pages: T's codes and scales, V's values.
+__device__ __forceinline__ void tile_codes(Wave<MfmaI8> &w, uint32_t T, uint32_t V, uint32_t seen) {
     typedef MfmaI8 F;
+    const int l = lane_anew(), g = l >> 4;
+    const LaneAddr ad = F::addr(l);
     float t[8];
-    pu32x4 a;
-    F::scores(w.q, T, ad, t, [&](int i) {
-        if (!more) return;
-        if (i == 3) a = codes_of(from, wave, l);
-        if (i == 6) convert_block<0>(a, to, wave, l);
-        if (i == 8) convert_block<1>(a, to, wave, l);
-        if (i == 9) a = codes_of(from, wave + 8, l);
-        if (i == 12) convert_block<0>(a, to, wave + 8, l);
-        if (i == 14) convert_block<1>(a, to, wave + 8, l);
-    });
-    float s[8];
-    F::scales(T, ad, s);
-    if (seen != ~0u) {
-        const uint32_t mine = seen >> (4 * g);
+    F::scores(w.q, T, ad, t);
+    const uint32_t mine = seen >> (4 * g);
+    if (seen != ~0u)
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (!((mine >> ((i >> 2) * 16 + (i & 3))) & 1)) {
-                t[i] = -INFINITY;
-                s[i] = 0.0f;
-            }
-    }
+            if (!((mine >> ((i >> 2) * 16 + (i & 3))) & 1)) t[i] = -INFINITY;
     auto most = [](const float (&v)[8]) {
         return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
     };
@@ -790,6 +772,14 @@ __device__ __forceinline__ void tile_codes(Wave<MfmaI8> &w, const LaneAddr &ad, 
     float e[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(t[i] - w.m);
+    __builtin_amdgcn_sched_barrier(0);
+    float s[8];
+    F::scales(T, ad, s);
+    // (a hidden position's scale is any)
+    if (seen != ~0u)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (!((mine >> ((i >> 2) * 16 + (i & 3))) & 1)) s[i] = 0.0f;
     w.l = __fadd_rn(w.l, __fadd_rn(__fadd_rn(__fadd_rn(e[0], e[1]), __fadd_rn(e[2], e[3])), __fadd_rn(__fadd_rn(e[4], e[5]), __fadd_rn(e[6], e[7]))));
 #pragma unroll
     for (int i = 0; i < 8; i++) e[i] = __fmul_rn(e[i], s[i]);
@@ -800,7 +790,7 @@ __device__ __forceinline__ void tile_codes(Wave<MfmaI8> &w, const LaneAddr &ad, 
         w.top = col_max(w.top);
         const int up = (int)(__float_as_uint(w.top) >> 23) - 127;
         const float gn = w.top > 0.0f ? __uint_as_float((uint32_t)(127 + (10 - up < 120 ? 10 - up : 120)) << 23) : w.g;
-        const float by = __fmul_rn(__fmul_rn(f, gn), 1.0f / w.g);
+        const float by = __fmul_rn(__fmul_rn(f, gn), F::inverse(w.g));
         w.g = gn;
 #pragma unroll
         for (int mt = 0; mt < 32; mt++) w.o[mt] *= by;
@@ -887,6 +877,18 @@ __device__ __forceinline__ uint32_t visible(const Lookup &k, int32_t v0, int32_t
         m |= ones << i;
     }
     return m;
+}
+
+// What some row of a unit sees of tile x, and what each of the M rows does.
+// (Windows follow on one another: what some row sees is one run, too.)
+template <int KIND> __device__ __forceinline__ uint32_t some_see(const Lookup &k, int32_t x, int32_t len) {
+    const int32_t v0 = tile_at<KIND>(k, x), lo = KIND == kNear ? k.cut.start - v0 : 0;
+    return low_bits(len - v0) & (lo <= 0 ? ~0u : (lo >= 32 ? 0u : ~0u << lo) | low_bits(k.sinks - v0));
+}
+template <int KIND> __device__ __forceinline__ uint32_t all_see(const Lookup &k, int32_t x, int32_t len, int32_t M) {
+    const int32_t v0 = tile_at<KIND>(k, x);
+    const uint32_t last = KIND == kNear ? visible<KIND>(k, v0, len) : ~0u;
+    return last & low_bits(len - M + 1 - v0);
 }
 
 // Column block I of a lane's row, 128 bytes apart there and 1 KiB apart in
@@ -1045,6 +1047,11 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
         if (CODES && l < (w < 4 ? 32 : 4)) copy_block<0>(off3, src3, dst3);
     };
     auto entry_of = [&](const Seg &q, int32_t x) { return page_entry<KIND>(q.lk, page_of<KIND>(q.lk, tile_at<KIND>(q.lk, x) + 8 * rb)); };
+    // the row of a wave's column group (kNear: a unit is a sequence)
+    auto row_of = [&](int wave) {
+        const int grp = chunk * p.per + wave, last = p.groups - 1;
+        return (grp < last ? grp : last) / ((a.H + kCols - 1) / kCols);
+    };
     auto start = [&](const Seg &q) {
         for (int32_t x = q.b0; x < q.b1 && x < q.b0 + STAGES - 1; x++) {
             entry = entry_of(q, x);
@@ -1071,7 +1078,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
             wv.g = 0x1p120f;
             // the first tile's values
             wait_tiles<F>(q.b1 - 1 - q.b0, STAGES - 2);
-            convert_tile(stage0, stage0 + STAGES * TILE, w, l);
+            convert_tile(stage0, stage0 + STAGES * TILE, w);
         }
 #pragma unroll
         for (int mt = 0; mt < 32; mt++) wv.o[mt] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1097,19 +1104,19 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
                 const uint32_t V = stage0 + STAGES * TILE, par = (uint32_t)(x - q.b0) & 1;
                 const bool more = x + 1 < q.b1;
                 const uint32_t from = stage0 + (uint32_t)(x + 1 - q.b0) % STAGES * TILE, to = V + (par ^ 1) * HALF;
-                if (active && seen) tile_codes(wv, ad, stage0 + ps, V + par * HALF, seen, g, more, from, to, w, l);
-                else if (more) convert_tile(from, to, w, l);
+                if (more) convert_tile(from, to, w);
+                if (active && seen) tile_codes(wv, stage0 + ps, V + par * HALF, seen);
                 entry = page_entry<KIND>(q.lk, page);
                 seen = visible<KIND>(q.lk, tile_at<KIND>(q.lk, x + 1), q.n);
             } else {
-            // what the unit's last row sees, and its first one (with a window
-            // values that a row does not see are left out as they are read)
-            const uint32_t most = KIND != kAll ? seen : visible<kAll>(q.lk, x * kPT, q.len);
-            const uint32_t least = KIND != kAll ? seen : visible<kAll>(q.lk, x * kPT, q.len - a.M + 1);
+            // what some row of the unit sees, and what every one does
+            const uint32_t most = SPARSE ? seen : some_see<KIND>(q.lk, x, q.len);
+            const uint32_t least = SPARSE ? seen : all_see<KIND>(q.lk, x, q.len, a.M);
             bool odd = false;
-            if (KIND != kNear && least != ~0u) {
+            if (least != ~0u) {
                 // a value that is not finite where only later rows look: those
-                // rows first, then it is cleared for the rows before
+                // rows first, then it is cleared for the rows before (with a
+                // window: each wave's row by itself)
                 if (most != ~0u) tile_clear<F>(T, ~most);
                 if (least != most) {
                     if (tid == 0) s_odd = 0;
@@ -1121,9 +1128,14 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
             }
             const int32_t page = page_of<KIND>(q.lk, tile_at<KIND>(q.lk, x + STAGES) + 8 * rb);
             uint32_t now = most;
+            int turn = 0;  // a wave
+            if (KIND == kNear && odd) {
+                tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), q.len - a.M + row_of(0) + 1));
+                __syncthreads();
+            }
             do {
-                if (active && seen && (!odd || seen == now))
-                    tile_step<F, KIND == kNear>(wv, ad, stage0 + ps, seen, c, g, [&](int i) {
+                if (active && seen && (!odd || (KIND == kNear ? q.j == row_of(turn) : seen == now)))
+                    tile_step<F>(wv, ad, stage0 + ps, seen, c, g, [&](int i) {
                         // a copy every few products
                         constexpr int EVERY = 36 / COPIES;
                         if (F::kBetween && i % EVERY == 0 && due) copy_nth<0, COPIES>(i / EVERY, off, src, dst);
@@ -1131,7 +1143,23 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
                 else if (F::kBetween && due)
                     copy_blocks<0, COPIES>(off, src, dst);
                 due = false;
-                if (!odd || now == least) break;
+                if (!odd) break;
+                if constexpr (KIND == kNear) {
+                    // the tile anew, for the next row that a wave has
+                    while (++turn < p.per && row_of(turn) == row_of(turn - 1)) {}
+                    if (turn >= p.per) break;
+                    __syncthreads();
+                    entry = entry_of(q, x);
+                    aim(q, x);
+                    copy_blocks<0, COPIES>(off, src, dst);
+                    fifth();
+                    __builtin_amdgcn_s_waitcnt(kWaitVm0);
+                    __syncthreads();
+                    tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), q.len - a.M + row_of(turn) + 1));
+                    __syncthreads();
+                    continue;
+                }
+                if (now == least) break;
                 __syncthreads();
                 tile_clear<F>(T, now & ~(now >> 1));
                 __syncthreads();
@@ -1149,8 +1177,9 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
         const float sum = col_sum(wv.l);
         if (active && ((SPARSE && p.whole) || (q.b0 == 0 && q.b1 == q.tiles))) {
             const float inv = (sum == 0.0f ? 0.0f : 1.0f / sum) * F::unit(wv);
-            typename F::out_t *out = (typename F::out_t *)a.out + row * kPL + 4 * g;
-            if (q.h0 + col < a.H)
+            const int lo = CODES ? lane_anew() : l, ho = q.h0 + (lo & 15);
+            typename F::out_t *out = (typename F::out_t *)a.out + (CODES ? q.row + (ho < a.H ? ho : a.H - 1) : row) * kPL + 4 * (lo >> 4);
+            if (ho < a.H)
 #pragma unroll
                 for (int mt = 0; mt < 32; mt++) {
                     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
