@@ -80,7 +80,7 @@ constexpr PlanCosts kCostsBf16 = {8, 8, 4, 150, 2.5f, 20};
 // bytes_ratio: 63 x 4 rows of up to 25 positions 66.5 us without and with 280,
 // 80.4 with 140.
 constexpr PlanCosts kCostsF16x2 = {4, 4, 16, 280, 1.3f, 10};
-constexpr PlanCosts kCostsI8 = kCostsBf16;
+constexpr PlanCosts kCostsI8 = {4, 8, 4, 150, 2.5f, 20};
 struct PlanCall {
     int32_t whole;        // a range is a unit: no parts, no join
     int32_t most;         // ranges at most (whole: units)
