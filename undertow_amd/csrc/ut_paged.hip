@@ -93,28 +93,6 @@ struct I8 {
 // 16 new rows of a thread under way at a time change nothing there; the dims
 // cut over workgroups, sums and then codes in two launches, took 10.8 us, but
 // the call 18.2 against 16.2.
-// A page's summary from the sums of its rows, four a dim in LDS.
-__device__ __forceinline__ void write_summary(double *sum, int D, int live, int8_t *mean, float *mean_scale) {
-    __shared__ double red[16];
-    const int tid = threadIdx.x;
-    __syncthreads();
-    double top = 0.0;
-    for (int d = tid; d < D; d += blockDim.x) {
-        const double t = (sum[d] + sum[D + d]) + (sum[2 * D + d] + sum[3 * D + d]);
-        sum[d] = t;
-        top = fmax(top, fabs(t));
-    }
-    for (int off = 32; off >= 1; off >>= 1) top = fmax(top, __shfl_xor(top, off, 64));
-    if ((tid & 63) == 0) red[tid >> 6] = top;
-    __syncthreads();
-    for (int w = 0; w < (int)(blockDim.x >> 6); w++) top = fmax(top, red[w]);
-    for (int d = tid; d < D; d += blockDim.x) {
-        const double c = top > 0.0 ? rint(sum[d] * 127.0 / top) : 0.0;
-        mean[d] = (int8_t)(c >= -127.0 && c <= 127.0 ? (int)c : 0);
-    }
-    if (tid == 0) *mean_scale = (float)(top / (127.0 * live));
-}
-
 template <class F>
 __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__restrict__ pages,
                                                       const float *__restrict__ latent,
@@ -122,6 +100,7 @@ __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__r
                                                       int8_t *__restrict__ mean,
                                                       float *__restrict__ mean_scale) {
     extern __shared__ double sum[];  // [4][D]
+    __shared__ double red[16];
     const int b = blockIdx.y, tid = threadIdx.x, D = a.L + a.P, nq = D / 4;
     bool bad = false;
     const int32_t len = plan_len(((const_i32 *)a.lens)[b], (int64_t)a.max_pages << a.shift, bad);
@@ -183,7 +162,23 @@ __global__ __launch_bounds__(576) void k_paged_append(PagedArgs a, uint16_t *__r
 #pragma unroll
             for (int i = 0; i < 4; i++) sum[s * D + d + i] = t[i];
     }
-    if (mean) write_summary(sum, D, live, mean + (int64_t)phys * D, mean_scale + phys);
+    if (!mean) return;
+    __syncthreads();
+    double top = 0.0;
+    for (int d = tid; d < D; d += blockDim.x) {
+        const double t = (sum[d] + sum[D + d]) + (sum[2 * D + d] + sum[3 * D + d]);
+        sum[d] = t;
+        top = fmax(top, fabs(t));
+    }
+    for (int off = 32; off >= 1; off >>= 1) top = fmax(top, __shfl_xor(top, off, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+    __syncthreads();
+    for (int w = 0; w < (int)(blockDim.x >> 6); w++) top = fmax(top, red[w]);
+    for (int d = tid; d < D; d += blockDim.x) {
+        const double c = top > 0.0 ? rint(sum[d] * 127.0 / top) : 0.0;
+        mean[(int64_t)phys * D + d] = (int8_t)(c >= -127.0 && c <= 127.0 ? (int)c : 0);
+    }
+    if (tid == 0) mean_scale[phys] = (float)(top / (127.0 * live));
 }
 
 // code = rint(q 127 / top) of the real quotient, |q| <= top, f about 127 / top.
@@ -198,21 +193,96 @@ template <class T> __device__ __forceinline__ int code8(T q, T top, T f) {
     return next ? (e > 0 ? k + 1 : k - 1) : k;
 }
 
-// The same for 8-bit pages: a wave takes a new row at a time, its quads in
-// registers (D is at most 1024), for the largest magnitude A of each part,
+// The same for 8-bit pages: a wave takes a page's row at a time, in registers.
+// A new row: for the largest magnitude A of each part,
 //   scale = fl32(A / 127), code = rint(127 x / A)
-// of the real quotient (64 bits: the codes are a value that a test can demand
-// exactly).  A part with a value that is not finite gets codes 0 and the scale
-// NaN: it is NaN read back.  The summary's sums take code * scale, exact in 64
-// bits, from the rows as they are then stored.
-__global__ __launch_bounds__(576) void k_paged_append_i8(PagedArgs a, int8_t *pages, float2 *scales,
-                                                         const float *__restrict__ latent,
-                                                         const float *__restrict__ krot,
-                                                         int8_t *__restrict__ mean,
-                                                         float *__restrict__ mean_scale) {
-    extern __shared__ double sum[];  // [4][D]
-    constexpr int NW = 9;
-    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, D = a.L + a.P, nq = D / 4;
+// of the real quotient (codes are a value that a test can demand exactly: next to
+// a half the rest in 64 bits tells).  A part with a value that is not finite gets
+// codes 0 and the scale NaN: it is NaN read back.  Every row, the older ones read
+// back, is added to the wave's sums of code * scale, exact products in 64 bits,
+// and the waves' sums meet in LDS.  Latency bounds a step (length, table, rows, one
+// reduction over the waves), a page of new rows its CU's arithmetic: sixteen
+// waves, the next row loaded under the present one's, older rows four at a time.
+constexpr int kAppendWaves = 16, kAppendOld = 4;
+struct PartQuant {
+    float m, f, scale;  // the part's largest, about 127 / m, what is stored
+    __device__ __forceinline__ explicit PartQuant(uint32_t top) {
+        const bool fits = top < 0x7f800000u;
+        m = fits ? __uint_as_float(top) : 0.0f;
+        f = m >= 0x1p-100f ? 127.0f / m : 0.0f;
+        scale = fits ? (float)((double)m / 127.0) : __uint_as_float(0x7fc00000u);
+    }
+};
+// How a row lies in a wave.  512 + 64: eight latent values a lane and a rotary one.
+struct RowWide {
+    static constexpr int N = 9, kSlots = 8;  // values of a lane; waves' sums that fit LDS
+    const int lane, D;
+    __device__ __forceinline__ RowWide(const PagedArgs &a, int lane) : lane(lane), D(576) {}
+    __device__ __forceinline__ int dim(int v, int l) const { return v < 8 ? 8 * l + v : 512 + l; }
+    __device__ __forceinline__ bool latent(int v) const { return v < 8; }
+    __device__ __forceinline__ void load(float (&x)[N], const float *lat, const float *rope) const {
+        const float4 y = ((const float4 *)lat)[2 * lane], z = ((const float4 *)lat)[2 * lane + 1];
+        x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w, x[4] = z.x, x[5] = z.y, x[6] = z.z, x[7] = z.w;
+        x[8] = rope[lane];
+    }
+    __device__ __forceinline__ void read(int32_t (&c)[N], const int8_t *row) const {
+        const uint2 w = ((const uint2 *)row)[lane];
+#pragma unroll
+        for (int v = 0; v < 8; v++) c[v] = (int32_t)((v < 4 ? w.x : w.y) << (24 - 8 * (v & 3))) >> 24;
+        c[8] = row[512 + lane];
+    }
+    __device__ __forceinline__ void write(const int32_t (&c)[N], int8_t *row) const {
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int v = 0; v < 8; v++) w[v >> 2] |= (uint32_t)(c[v] & 255) << (8 * (v & 3));
+        ((uint2 *)row)[lane] = make_uint2(w[0], w[1]);
+        row[512 + lane] = (int8_t)c[8];
+    }
+};
+// Any widths (D at most 1024): quads lane, lane + 64, ..
+struct RowAny {
+    static constexpr int N = 16, kSlots = 4;
+    const int lane, D, L;
+    __device__ __forceinline__ RowAny(const PagedArgs &a, int lane) : lane(lane), D(a.L + a.P), L(a.L) {}
+    __device__ __forceinline__ int dim(int v, int l) const { return 4 * (l + 64 * (v >> 2)) + (v & 3); }
+    __device__ __forceinline__ bool latent(int v) const { return dim(v, lane) < L; }
+    __device__ __forceinline__ void load(float (&x)[N], const float *lat, const float *rope) const {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const int d = dim(i, lane);
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (d < D) y = *(const float4 *)(d < L ? lat + d : rope + (d - L));
+            x[i] = y.x, x[i + 1] = y.y, x[i + 2] = y.z, x[i + 3] = y.w;
+        }
+    }
+    __device__ __forceinline__ void read(int32_t (&c)[N], const int8_t *row) const {
+#pragma unroll
+        for (int v = 0; v < N; v += 4) {
+            const uint32_t w = dim(v, lane) < D ? *(const uint32_t *)(row + dim(v, lane)) : 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) c[v + e] = (int32_t)(w << (24 - 8 * e)) >> 24;
+        }
+    }
+    __device__ __forceinline__ void write(const int32_t (&c)[N], int8_t *row) const {
+#pragma unroll
+        for (int v = 0; v < N; v += 4)
+            if (dim(v, lane) < D)
+                *(uint32_t *)(row + dim(v, lane)) = (uint32_t)(c[v] & 255) | (uint32_t)(c[v + 1] & 255) << 8 |
+                                                    (uint32_t)(c[v + 2] & 255) << 16 | (uint32_t)(c[v + 3] & 255) << 24;
+    }
+};
+template <class Row>
+__global__ __launch_bounds__(kAppendWaves * 64) void k_paged_append_i8(PagedArgs a, int8_t *__restrict__ pages,
+                                                                       float2 *__restrict__ scales,
+                                                                       const float *__restrict__ latent,
+                                                                       const float *__restrict__ krot,
+                                                                       int8_t *__restrict__ mean,
+                                                                       float *__restrict__ mean_scale) {
+    constexpr int NW = kAppendWaves, N = Row::N, SLOTS = Row::kSlots;
+    __shared__ double sum[SLOTS][N * 64];
+    __shared__ double red[NW];
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), D = a.L + a.P;
+    const Row row(a, lane);
     bool bad = false;
     const int32_t len = plan_len(((const_i32 *)a.lens)[b], (int64_t)a.max_pages << a.shift, bad);
     if (bad) {  // cut to the table's end, the new rows would take the place of older ones
@@ -229,113 +299,139 @@ __global__ __launch_bounds__(576) void k_paged_append_i8(PagedArgs a, int8_t *pa
     const int live = len - p0 < page ? (int)(len - p0) : page;
     const int first = from > p0 ? (int)(from - p0) : 0;  // the page's first new row
     const int64_t at0 = (int64_t)phys << a.shift, r0 = (int64_t)b * a.M + (p0 - (len - a.M));
+    double t[N] = {};
+    auto add = [&](const int32_t (&c)[N], float2 sc) {
+#pragma unroll
+        for (int v = 0; v < N; v++) t[v] = __builtin_fma((double)c[v], (double)(row.latent(v) ? sc.x : sc.y), t[v]);
+    };
+    float next[N];
+    auto load = [&](int o) {
+        if (o < live) row.load(next, latent + (r0 + o) * a.L, krot + (r0 + o) * a.P);
+    };
+    load(first + w);
+    if (mean)
+        for (int o0 = w; o0 < first; o0 += kAppendOld * NW) {
+            int32_t c[kAppendOld][N];
+            float2 sc[kAppendOld];
+#pragma unroll
+            for (int n = 0; n < kAppendOld; n++) {
+                const int64_t at = at0 + (o0 + n * NW < first ? o0 + n * NW : o0);
+                sc[n] = scales[at];
+                row.read(c[n], pages + at * D);
+            }
+#pragma unroll
+            for (int n = 0; n < kAppendOld; n++)
+                if (o0 + n * NW < first) add(c[n], sc[n]);
+        }
+#pragma unroll 1
     for (int o = first + w; o < live; o += NW) {
-        float4 x[4];
+        float x[N];
         uint32_t top[2] = {0, 0};  // bits of |x|: NaN lies above infinity
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int d = 4 * (lane + 64 * i);
-            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (d < D) x[i] = *(const float4 *)(d < a.L ? latent + (r0 + o) * a.L + d : krot + (r0 + o) * a.P + (d - a.L));
-            const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
-                if (d < a.L) top[0] = m > top[0] ? m : top[0];
-                else top[1] = m > top[1] ? m : top[1];
-            }
+        for (int v = 0; v < N; v++) {
+            x[v] = next[v];
+            const uint32_t u = __float_as_uint(x[v]) & 0x7fffffffu;
+            const bool lat = row.latent(v);
+            top[0] = lat && u > top[0] ? u : top[0];
+            top[1] = !lat && u > top[1] ? u : top[1];
         }
+        load(o + NW);
+#pragma unroll
         for (int off = 32; off >= 1; off >>= 1)
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 const uint32_t y = __shfl_xor(top[p], off, 64);
                 top[p] = y > top[p] ? y : top[p];
             }
-        double m[2], f[2];
-        float sc[2];
+        const PartQuant lat(top[0]), rope(top[1]);
+        // x f is off by 1.6e-5 at most; f = 0 where the part has no codes, or is too small for it
+        bool near = (lat.m > 0.0f && lat.f == 0.0f) || (rope.m > 0.0f && rope.f == 0.0f);
+        int32_t c[N];
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
-            const bool fits = top[p] < 0x7f800000u;
-            m[p] = fits ? (double)__uint_as_float(top[p]) : 0.0;
-            f[p] = m[p] > 0.0 ? 127.0 / m[p] : 0.0;
-            sc[p] = fits ? (float)(m[p] / 127.0) : __uint_as_float(0x7fc00000u);
+        for (int v = 0; v < N; v++) {
+            const float f = row.latent(v) ? lat.f : rope.f, q = f > 0.0f ? __fmul_rn(x[v], f) : 0.0f, k = rintf(q);
+            near = near || fabsf(q - k) > 0.49995f;
+            c[v] = (int32_t)k;
         }
+        if (__any(near)) {
+            const double fl = lat.m > 0.0f ? 127.0 / (double)lat.m : 0.0, fr = rope.m > 0.0f ? 127.0 / (double)rope.m : 0.0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int d = 4 * (lane + 64 * i), p = d < a.L ? 0 : 1;
-            const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            uint32_t c = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                c |= (uint32_t)((m[p] > 0.0 ? code8<double>((double)v[e], m[p], f[p]) : 0) & 255) << (8 * e);
-            if (d < D) *(uint32_t *)(pages + (at0 + o) * D + d) = c;
+            for (int v = 0; v < N; v++) {
+                const double m = row.latent(v) ? lat.m : rope.m, f = row.latent(v) ? fl : fr;
+                c[v] = m > 0.0 ? code8<double>((double)x[v], m, f) : 0;
+            }
         }
-        if (lane == 0) scales[at0 + o] = make_float2(sc[0], sc[1]);
+        row.write(c, pages + (at0 + o) * D);
+        const float2 sc = make_float2(lat.scale, rope.scale);
+        if (lane == 0) scales[at0 + o] = sc;
+        if (mean) add(c, sc);
     }
     if (!mean) return;
-    __syncthreads();
-    for (int u = tid; u < 4 * nq; u += blockDim.x) {
-        const int s = u / nq, d = (u - s * nq) * 4;
-        double t[4] = {0.0, 0.0, 0.0, 0.0};
-        constexpr int kRows = 16;  // at a time, so that as many loads are under way
-        for (int o0 = s; o0 < live; o0 += 4 * kRows) {
-            uint32_t v[kRows];
-            float sc[kRows];
+    // as many waves at a time as have room add theirs
+#pragma unroll 1
+    for (int turn = 0; turn < NW / SLOTS; turn++) {
+        if (w / SLOTS == turn)
 #pragma unroll
-            for (int i = 0; i < kRows; i++) {
-                const int64_t o = at0 + (o0 + 4 * i < live ? o0 + 4 * i : o0);
-                v[i] = *(const uint32_t *)(pages + o * D + d);
-                sc[i] = ((const float *)scales)[2 * o + (d < a.L ? 0 : 1)];
+            for (int v = 0; v < N; v++) {
+                double &s = sum[w % SLOTS][v * 64 + lane];
+                s = turn ? s + t[v] : t[v];
             }
-#pragma unroll
-            for (int i = 0; i < kRows; i++)
-                if (o0 + 4 * i < live)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) t[e] += (double)code_byte(v[i], e) * (double)sc[i];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) sum[s * D + d + e] = t[e];
+        __syncthreads();
     }
-    write_summary(sum, D, live, mean + (int64_t)phys * D, mean_scale + phys);
+    double all = 0.0, top = 0.0;  // (a thread has one dim)
+    const int d = tid < N * 64 ? row.dim(tid >> 6, lane) : D;
+    if (d < D) {
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) all += sum[i][tid];
+        top = fabs(all);
+    }
+    for (int off = 32; off >= 1; off >>= 1) top = fmax(top, __shfl_xor(top, off, 64));
+    if (lane == 0) red[w] = top;
+    __syncthreads();
+    for (int i = 0; i < NW; i++) top = fmax(top, red[i]);
+    if (d < D) {
+        const double c = top > 0.0 ? rint(all * 127.0 / top) : 0.0;
+        mean[(int64_t)phys * D + d] = (int8_t)(c >= -127.0 && c <= 127.0 ? (int)c : 0);
+    }
+    if (tid == 0) mean_scale[phys] = (float)(top / (127.0 * live));
 }
 
 // ---------------------------------------------------------------- read ---
-// Rows start_b + j of each sequence as f32 or bf16: value(x) rounded once more
-// where that is bf16; zeros for rows outside the sequence.  A thread takes
-// eight values of a row, a workgroup as many whole rows as it has room for.
-template <class T> __device__ __forceinline__ void put8(T *dst, const float4 &x, const float4 &y) {
-    if constexpr (sizeof(T) == 4) {
-        ((float4 *)dst)[0] = x;
-        ((float4 *)dst)[1] = y;
-    } else {
-        typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-        *(b8 *)dst = b8{(__bf16)x.x, (__bf16)x.y, (__bf16)x.z, (__bf16)x.w, (__bf16)y.x, (__bf16)y.y, (__bf16)y.z, (__bf16)y.w};
-    }
+// Rows start_b + j of each sequence as f32 or bf16: value(x), rounded once more
+// where that is bf16; zeros for rows outside the sequence.  A thread takes four
+// values of a row, so that a wave's stores are whole lines, a workgroup as many
+// whole rows as it has room for, kReadTurns of them at a time, all looked up and
+// loaded before the first is stored.
+template <bool PAST, class T> __device__ __forceinline__ void put4(T *dst, const float4 &x) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    const t4 v = {(T)x.x, (T)x.y, (T)x.z, (T)x.w};
+    if constexpr (PAST) __builtin_nontemporal_store(v, (t4 *)dst);
+    else *(t4 *)dst = v;
 }
-constexpr int kReadThreads = 512, kReadTurns = 4;
-template <class F, class T>
+constexpr int kReadThreads = 576, kReadTurns = 4;
+// Rows of more bytes than this go past the L2s, which hold 32 MB together.
+constexpr int64_t kReadPast = int64_t(32) << 20;
+template <class F, bool PAST, class T>
 __global__ __launch_bounds__(kReadThreads) void k_paged_read(PagedArgs a, const int32_t *__restrict__ starts, int rows,
                                                              T *__restrict__ latent, T *__restrict__ krot) {
-    const int b = blockIdx.y, G = (a.L + a.P) / 8, in = threadIdx.x / G, d = 8 * (threadIdx.x - in * G);
+    const int b = blockIdx.y, G = (a.L + a.P) / 4, in = threadIdx.x / G, d = 4 * (threadIdx.x - in * G);
     const int32_t len = paged_len(a, b);
     const int64_t start = starts ? starts[b] : 0;
     if (in >= rows) return;
-    float4 x[kReadTurns], y[kReadTurns];
+    float4 x[kReadTurns];
 #pragma unroll
     for (int i = 0; i < kReadTurns; i++) {
         const int64_t j = ((int64_t)blockIdx.x * kReadTurns + i) * rows + in, t = start + j;
-        x[i] = y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (j < a.M && t >= 0 && t < len) {
             const int32_t phys = paged_phys(a, b, (int)(t >> a.shift));
-            const int64_t pos = ((int64_t)phys << a.shift) + (t & ((1 << a.shift) - 1));
-            x[i] = F::quad(a, pos, d);
-            y[i] = F::quad(a, pos, d + 4);
+            x[i] = F::quad(a, ((int64_t)phys << a.shift) + (t & ((1 << a.shift) - 1)), d);
         }
     }
 #pragma unroll
     for (int i = 0; i < kReadTurns; i++) {
         const int64_t j = ((int64_t)blockIdx.x * kReadTurns + i) * rows + in, r = (int64_t)b * a.M + j;
-        if (j < a.M) put8(d < a.L ? latent + r * a.L + d : krot + r * a.P + (d - a.L), x[i], y[i]);
+        if (j < a.M) put4<PAST>(d < a.L ? latent + r * a.L + d : krot + r * a.P + (d - a.L), x[i]);
     }
 }
 
@@ -1103,8 +1199,9 @@ extern "C" int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv,
         hipLaunchKernelGGL(k_paged_append<Bf16>, grid, dim3(576), lds, ctx->stream, a,
                            (uint16_t *)kv->pages, latent_dev, krot_dev, kv->mean, kv->mean_scale);
     else if (kv->fmt == UT_KV_I8)
-        hipLaunchKernelGGL(k_paged_append_i8, grid, dim3(576), lds, ctx->stream, a, (int8_t *)kv->pages,
-                           (float2 *)kv->scales, latent_dev, krot_dev, kv->mean, kv->mean_scale);
+        hipLaunchKernelGGL((a.L == 512 && a.P == 64 ? k_paged_append_i8<RowWide> : k_paged_append_i8<RowAny>), grid,
+                           dim3(kAppendWaves * 64), 0, ctx->stream, a, (int8_t *)kv->pages, (float2 *)kv->scales,
+                           latent_dev, krot_dev, kv->mean, kv->mean_scale);
     else
         hipLaunchKernelGGL(k_paged_append<F16x2>, grid, dim3(576), lds, ctx->stream, a,
                            (uint16_t *)kv->pages, latent_dev, krot_dev, kv->mean, kv->mean_scale);
@@ -1127,7 +1224,7 @@ extern "C" int32_t ut_mla_paged_read(ut_ctx *ctx, const ut_mla_pages *kv, const 
         set_error(ctx, "ut_mla_paged_read: rows are f32 or bf16 in 16-byte aligned device memory");
         return UT_ERR_ARG;
     }
-    const int per = kReadThreads / ((a.L + a.P) / 8);  // rows of a workgroup at a time
+    const int per = kReadThreads / ((a.L + a.P) / 4);  // rows of a workgroup at a time
     const int64_t groups = (rows + per * kReadTurns - 1) / (per * kReadTurns);
     if (groups > kMostGroups) {
         set_error(ctx, "ut_mla_paged_read: more than %lld rows of a sequence in a call",
@@ -1138,10 +1235,13 @@ extern "C" int32_t ut_mla_paged_read(ut_ctx *ctx, const ut_mla_pages *kv, const 
     int tok = timing_begin(ctx, "paged_read");
     auto launch = [&](auto *out) {
         typedef std::remove_pointer_t<decltype(out)> T;
-        hipLaunchKernelGGL((kv->fmt == UT_KV_BF16 ? k_paged_read<Bf16, T>
-                            : kv->fmt == UT_KV_I8 ? k_paged_read<I8, T>
-                                                  : k_paged_read<F16x2, T>),
-                           grid, dim3(kReadThreads), 0, ctx->stream, a, starts_dev, per, out, (T *)krot_dev);
+        const bool past = batch * rows * (a.L + a.P) * (int64_t)sizeof(T) > kReadPast;
+        auto go = [&](auto f) {
+            typedef decltype(f) F;
+            hipLaunchKernelGGL((past ? k_paged_read<F, true, T> : k_paged_read<F, false, T>), grid, dim3(kReadThreads), 0,
+                               ctx->stream, a, starts_dev, per, out, (T *)krot_dev);
+        };
+        kv->fmt == UT_KV_BF16 ? go(Bf16()) : kv->fmt == UT_KV_I8 ? go(I8()) : go(F16x2());
     };
     if (type == UT_ROWS_F32) launch((float *)latent_dev);
     else launch((__bf16 *)latent_dev);

@@ -649,15 +649,20 @@ class PagedCache:
         batch = self._batch(table, lens, rows)
         B = batch[6]
         s = None if starts is None else self._tensor("starts", starts, torch.int32, (B,))
-        shapes = (B, max(rows, 0), self.latent), (B, max(rows, 0), self.rope)
+        shapes = (B, rows, self.latent), (B, rows, self.rope)
         if out is None:
-            out = tuple(torch.empty(x, dtype=dtype, device=table.device) for x in shapes)
+            n = max(rows, 0)  # (the library turns down a count that is not positive)
+            out = (torch.empty((B, n, self.latent), dtype=dtype, device=table.device),
+                   torch.empty((B, n, self.rope), dtype=dtype, device=table.device))
         elif len(out) != 2:
             raise ShapeError(UT_ERR_SHAPE, "PagedCache: out must be two tensors")
-        self.ctx.check(lib().ut_mla_paged_read(
-            *batch, s, ROWS_F32 if dtype == torch.float32 else ROWS_BF16,
-            self._tensor("out[0]", out[0], dtype, shapes[0]), self._tensor("out[1]", out[1], dtype, shapes[1])))
-        return tuple(out)
+        else:
+            for i, shape in enumerate(shapes):
+                self._tensor(f"out[{i}]", out[i], dtype, shape)
+        lat, kr = out
+        self.ctx.check(lib().ut_mla_paged_read(*batch, s, ROWS_F32 if dtype == torch.float32 else ROWS_BF16,
+                                               lat.data_ptr(), kr.data_ptr()))
+        return lat, kr
 
     def attend(self, table, lens, qabs, q_rope, scale: float, out=None):
         """Absorbed attention of qabs [B, M, H, latent] and q_rope [B, M, H,
