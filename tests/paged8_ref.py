@@ -81,10 +81,12 @@ def largest(kv, q, L, scale):
 
 def close(fmt, got, want, spread, mass, step=0.0, top=0.0):
     """As the attention tests of the other formats; 8 bits: an output is
-    rounded once (2^-8 of it), a weight times its position's scale to 11 bits
+    rounded once (2^-8 of it); a weight times its position's scale to 11 bits
     in the numerator alone (2^-11 sum_t p_t |v_t|; one below 2^-24 of the
-    largest by 2^-35 of that: `top`), a score is off by `step`, which moves the
-    context by that times its spread, and what is left is f32 arithmetic."""
+    largest by 2^-35 of that: `top`); where a row's positions are cut, each
+    part's context to 11 bits (2^-11 of its share, and those add up to no more
+    than sum_t p_t |v_t|); a score is off by `step`, which moves the context by
+    that times its spread; and what is left is f32 arithmetic."""
     got = got.double().cpu()
     want, spread, mass = want.cpu(), spread.cpu(), mass.cpu()
     assert torch.isfinite(got).all()
@@ -93,16 +95,18 @@ def close(fmt, got, want, spread, mass, step=0.0, top=0.0):
     elif fmt == "f16x2":
         tol = 5.2e-5 * spread + 2.0 ** -20 * (mass + want.abs()) + 1e-30
     else:
-        tol = 2.0 ** -8 * want.abs() + (6e-5 + 1.05 * step) * spread + 2.0 ** -11 * mass + 2.0 ** -35 * top + 1e-30
+        tol = 2.0 ** -8 * want.abs() + (6e-5 + 1.05 * step) * spread + 2 * 2.0 ** -11 * mass + 2.0 ** -35 * top + 1e-30
     err = (got - want).abs()
     assert (err <= tol).all(), float((err / tol).max())
 
 
-def check(pool, fmt, got, qabs, qrope, scale, sel=None, window=None, sinks=0):
-    """Every row of `got` against 64 bits (on the device that `got` is on);
-    rows that see nothing are zeros."""
+def check(pool, fmt, got, qabs, qrope, scale, sel=None, window=None, sinks=0, only=None):
+    """Every row of `got` (of the sequences `only`) against 64 bits (on the
+    device that `got` is on); rows that see nothing are zeros."""
     B, M, H, L = qabs.shape
     for b, n in enumerate(pool.lens):
+        if only is not None and b not in only:
+            continue
         for j in range(M):
             at = positions(n - M + j + 1, window, sinks)
             if sel is not None:

@@ -251,7 +251,7 @@ def test_bad_lengths_and_pages_are_reported(ctx, bad_page):
     pool = R8.Pool8(31, [100, 90, 80], 16, 512, 64, width=7)
     qabs, qrope = [t.cuda() for t in pool.queries(1, 16)]
     cache, lens, table = pool.cuda(ctx=ctx), pool.lens32().cuda(), pool.table.cuda()
-    good = [cache.attend(table, lens, qabs, qrope, SCALE), *cache.read(table, lens, 80)]
+    good = cache.read(table, lens, 80)
     ctx.synchronize()
     if bad_page:
         table[1, 4] = pool.n_pages
@@ -265,9 +265,12 @@ def test_bad_lengths_and_pages_are_reported(ctx, bad_page):
         with pytest.raises(U.UtError) as e:
             ctx.synchronize()
         assert e.value.code == U.runtime.UT_ERR_BAD_PAGE
-        if got:
-            want = good[:1] if len(got) == 1 else good[1:]
-            assert all(torch.equal(a[::2], b[::2]) for a, b in zip(got, want))
+        # the other sequences are as they should be: rows read back to the bit; contexts,
+        # whose sums a length may cut elsewhere, in their tolerance
+        if got and len(got) == 1:
+            R8.check(pool, "i8", got[0], qabs.cpu(), qrope.cpu(), SCALE, only=(0, 2))
+        elif got:
+            assert all(torch.equal(a[::2], b[::2]) for a, b in zip(got, good))
     for b in (0, 2):
         n = pool.lens[b]
         at = tuple(t.cuda() for t in pool.where(b, torch.arange(n - 40, n)))

@@ -12,6 +12,7 @@ typedef __bf16 pbf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 pbf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 pbf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 pf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pf16x4 __attribute__((ext_vector_type(4)));
 typedef float pf32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t pu32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
@@ -32,7 +33,7 @@ struct PagedMfmaArgs {
     int32_t most;     // ranges at most
     float spread;     // plan_ranges'
     int32_t whole;    // a range is a unit (most: units), and there is no join
-    float *part_o;    // [slot][group][128 quads][16 columns][4]
+    void *part_o;     // [slot][group][128 quads][16 columns][4], f32 or (8-bit pages) f16
     float *part_ml;   // [slot][group][16 columns][2]
     int64_t *plan;    // [units] first tile of each, then W (where there is more than one range)
     int32_t lead;     // empty tiles before every unit with tiles but the first
@@ -42,18 +43,7 @@ struct PagedMfmaArgs {
 // the first ones and a window.
 enum { kAll, kListed, kNear };
 
-// With a window a sequence's tiles are its first `ts`, which hold the first
-// positions, and those from the one on where the first row's window begins;
-// `skip` tiles between them are left out.
-struct NearCut {
-    int32_t start;  // the first row's window
-    int32_t ts, skip;
-};
-__device__ __forceinline__ NearCut near_cut(const PagedArgs &a, int32_t n) {
-    const int32_t end = n - a.M + 1, start = end > a.window ? end - a.window : 0, from = start / kPT;
-    const int32_t s = a.sinks < n ? a.sinks : n, ts = (int32_t)(((int64_t)s + kPT - 1) / kPT);
-    return {start, ts < from ? ts : from, ts < from ? from - ts : 0};
-}
+__device__ __forceinline__ NearCut near_cut(const PagedArgs &a, int32_t n) { return near_cut(n, a.M, a.window, a.sinks, kPT); }
 
 // Tiles of a unit.
 template <int KIND> __device__ __forceinline__ int32_t unit_tiles(const PagedArgs &a, int u) {
@@ -237,7 +227,7 @@ struct Lookup {
 };
 // The first position of the unit's tile x.
 template <int KIND> __device__ __forceinline__ int32_t tile_at(const Lookup &k, int32_t x) {
-    return (KIND == kNear && x >= k.cut.ts ? x + k.cut.skip : x) * kPT;
+    return KIND == kNear ? near_tile(k.cut, x, kPT) : x * kPT;
 }
 // The page of the sequence that holds the unit's position v0; one that it
 // does have, where there is none or it lies behind the end.
@@ -247,7 +237,7 @@ template <int KIND> __device__ __forceinline__ int32_t page_of(const Lookup &k, 
         return i < k.top_k ? k.sel[i] : 0;
     }
     // (eight positions that no row sees: their page need not be named)
-    if (KIND == kNear && v0 >= k.sinks && v0 + 8 <= k.cut.start) return -1;
+    if (KIND == kNear && near_hidden(k.cut, k.sinks, v0, 8)) return -1;
     return (v0 < k.n ? v0 : k.n - 1) >> k.shift;
 }
 template <int KIND> __device__ __forceinline__ int32_t page_entry(const Lookup &k, int32_t page) {
@@ -257,17 +247,11 @@ template <int KIND> __device__ __forceinline__ int32_t page_entry(const Lookup &
     const int32_t entry = k.table[none ? 0 : page];
     return none ? 0 : entry;
 }
-__device__ __forceinline__ uint32_t low_bits(int32_t c) { return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u; }
 // The visible positions of the tile at v0 for a row that sees n.
 template <int KIND>
 __device__ __forceinline__ uint32_t visible(const Lookup &k, int32_t v0, int32_t n) {
     if (KIND == kAll) return low_bits(n - v0);
-    if (KIND == kNear) {
-        // the window's positions from `lo` on
-        const int32_t lo = n > k.window ? n - k.window - v0 : 0;
-        const uint32_t near = lo <= 0 ? ~0u : lo >= 32 ? 0u : ~0u << lo;
-        return low_bits(n - v0) & (near | low_bits(k.sinks - v0));
-    }
+    if (KIND == kNear) return near_seen(v0, n, k.window, k.sinks);
     const int per = k.shift >= 5 ? 32 : 1 << k.shift;
     uint32_t m = 0;
     for (int i = 0; i < 32; i += per) {
@@ -281,15 +265,13 @@ __device__ __forceinline__ uint32_t visible(const Lookup &k, int32_t v0, int32_t
 }
 
 // What some row of a unit sees of tile x, and what each of the M rows does.
-// (Windows follow on one another: what some row sees is one run, too.)
 template <int KIND> __device__ __forceinline__ uint32_t some_see(const Lookup &k, int32_t x, int32_t len) {
-    const int32_t v0 = tile_at<KIND>(k, x), lo = KIND == kNear ? k.cut.start - v0 : 0;
-    return low_bits(len - v0) & (lo <= 0 ? ~0u : (lo >= 32 ? 0u : ~0u << lo) | low_bits(k.sinks - v0));
+    const int32_t v0 = tile_at<KIND>(k, x);
+    return KIND == kNear ? near_some(k.cut, v0, len, k.sinks) : low_bits(len - v0);
 }
 template <int KIND> __device__ __forceinline__ uint32_t all_see(const Lookup &k, int32_t x, int32_t len, int32_t M) {
     const int32_t v0 = tile_at<KIND>(k, x);
-    const uint32_t last = KIND == kNear ? visible<KIND>(k, v0, len) : ~0u;
-    return last & low_bits(len - M + 1 - v0);
+    return KIND == kNear ? near_every(v0, len, M, k.window, k.sinks) : low_bits(len - M + 1 - v0);
 }
 
 // Column block I of a lane's row, 128 bytes apart there and 1 KiB apart in
@@ -366,13 +348,12 @@ template <int KIND> struct Walk {
     }
 };
 
-// The kernel of 8-bit pages (ut_paged_codes.hip), `wgs` workgroups, so many of
-// which run on a CU at a time.
-constexpr int kCodesPerCu = 2;
+// The kernel of 8-bit pages (ut_paged_codes.hip), `wgs` workgroups.
 struct CodesI8 {
     static constexpr bool kCodes = true;
     static constexpr PlanCosts kCosts = kCostsI8;
     typedef __bf16 out_t;
+    typedef _Float16 part_t;
 };
 void launch_codes(ut_ctx *ctx, const PagedMfmaArgs &p, int kind, unsigned wgs);
 

@@ -32,7 +32,7 @@ typedef int pi32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 pf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t pu32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kCW = kCostsI8.waves;
+constexpr int kCW = kCostsI8.waves, kCodesPerCu = kCostsI8.slots;
 // LDS: two tiles of codes (32 x 512 latent ones in 16 blocks of 8 rows and 128
 // bytes, 32 x 64 rotary ones), the scales of four tiles, one tile's values.
 constexpr int kCBlocks = 4, kCRope = 16 * 1024, kCTile = 18 * 1024, kCStages = 2;
@@ -306,11 +306,27 @@ __device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, 
                 *(pbf16x4 *)(out + 16 * mt) = v;
             }
     } else if (active) {
-        const int64_t slot = plan_slot(r, rg.s <= q.first) * p.groups + grp;
-        pf32x4 *po = (pf32x4 *)p.part_o + slot * 128 * kCols + g * kCols + col;
+        // a part's context in f16, which is 1/8 of what the output's own rounding to
+        // bf16 may take, times a power of two of the column that puts the largest at
+        // 2^13 to 2^14; the sum goes with it, and the offset back
+        float top = 0.0f;
 #pragma unroll
-        for (int mt = 0; mt < 32; mt++) po[mt * 4 * kCols] = w.o[mt];
-        if (g == 0) *(float2 *)(p.part_ml + (slot * kCols + col) * 2) = make_float2(w.m, sum);
+        for (int mt = 0; mt < 32; mt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(w.o[mt][i]));
+        top = col_max(top);
+        const int e = (int)(__float_as_uint(top) >> 23) - 127, up = top > 0.0f && top < INFINITY ? (13 - e < 120 ? 13 - e : 120) : 0;
+        const float f = ldexpf(1.0f, up);
+        const int64_t slot = plan_slot(r, rg.s <= q.first) * p.groups + grp;
+        pf16x4 *po = (pf16x4 *)p.part_o + slot * 128 * kCols + g * kCols + col;
+#pragma unroll
+        for (int mt = 0; mt < 32; mt++) {
+            pf16x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = (_Float16)__fmul_rn(w.o[mt][i], f);
+            po[mt * 4 * kCols] = v;
+        }
+        if (g == 0) *(float2 *)(p.part_ml + (slot * kCols + col) * 2) = make_float2(w.m - (float)up, __fmul_rn(sum, f));
     }
 }
 
@@ -381,11 +397,16 @@ template <int KIND> __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4
                 tile_scores(wv, T, stage0 + kCScales + (n & 3) * 256, wv.m, t, s);
             }
             meet<-1>();
+            // the wave that is through with its scores goes first, so that the other of its SIMD
+            // is at its own scores under these products (512 prompt rows over 8192 positions 1327
+            // us without, 1227 with; at the scores 1290, at the context's products 1255)
+            __builtin_amdgcn_s_setprio(1);
             if (x + kCStages < q.b1) {
                 copy(q, x + kCStages);
                 entry = entry_of(q, x + kCStages + 1);
             }
             if (some) tile_context(wv, tile_weights(wv, seen, fresh, t, s), V);
+            __builtin_amdgcn_s_setprio(0);
         }
         __syncthreads();  // the stages may be filled again: with the next part's first tiles
         Seg nx;

@@ -57,6 +57,7 @@ struct MfmaBf16 {
     static constexpr int kDepth = 4;
     static constexpr float kRise = 11.5f;  // log2 units a score may exceed the offset (8 nats)
     typedef __bf16 out_t;
+    typedef float part_t;
     struct Query {
         pbf16x8 q[18];
     };
@@ -147,6 +148,7 @@ struct MfmaF16x2 {
     static constexpr int kDepth = 4;
     static constexpr float kRise = 1.0f;
     typedef float out_t;
+    typedef float part_t;
     struct Query {
         pf16x8 h[18], l[18];
     };
@@ -519,6 +521,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
 // one row take 4.2.
 template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void k_paged_join(PagedMfmaArgs p) {
     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
+    typedef typename F::part_t p4 __attribute__((ext_vector_type(4)));
     __shared__ __attribute__((aligned(16))) pf32x4 so[NW][16][kCols + 1];  // one more: other banks
     __shared__ float2 sml[NW][kCols];
     const PagedArgs &a = p.a;
@@ -536,7 +539,7 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
     auto add = [&](int r, auto many) {
         constexpr int COUNT = decltype(many)::value;
         float2 ml[COUNT];
-        pf32x4 v[COUNT][4];
+        p4 v[COUNT][4];
 #pragma unroll
         for (int i = 0; i < COUNT; i++) {
             const int x = r + NW * i;
@@ -544,7 +547,7 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
             ml[i] = *(const float2 *)(p.part_ml + (slot * kCols + col) * 2);
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                v[i][k] = ((const pf32x4 *)p.part_o)[(slot * 128 + blockIdx.y * 16 + qd + 4 * k) * kCols + col];
+                v[i][k] = ((const p4 *)p.part_o)[(slot * 128 + blockIdx.y * 16 + qd + 4 * k) * kCols + col];
         }
         float mn = m;
 #pragma unroll
@@ -560,7 +563,7 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
 #pragma unroll
             for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) t[k][e] = __builtin_fmaf(v[i][k][e], f, t[k][e]);
+                for (int e = 0; e < 4; e++) t[k][e] = __builtin_fmaf((float)v[i][k][e], f, t[k][e]);
         }
         m = mn;
     };
@@ -615,15 +618,13 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
     p.groups = (SPARSE ? 1 : a.M) * ((a.H + kCols - 1) / kCols);
     const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
     p.lead = F::kCosts.lead;
-    // (a window's rows see the window and up to M - 1 positions more, which may
-    // begin and end inside a tile, and so may the first positions)
-    const int64_t near = ((int64_t)a.window + a.M - 1 + kPT - 1) / kPT + 1 + ((int64_t)a.sinks + kPT - 1) / kPT;
+    const int64_t near = near_most(a.M, a.window, a.sinks, kPT);
     const int64_t held = (cap + kPT - 1) / kPT, each = KIND == kNear && near < held ? near : held;
     // (no more pages are to be expected of a list than the table holds: 20 rows of
     // one page and 12 places in f16 pairs 33.0 us cut, 18.6 whole)
     const int64_t listed = (((int64_t)(a.top_k < a.max_pages ? a.top_k : a.max_pages) << a.shift) + kPT - 1) / kPT;
     const PlanCall plan =
-        plan_call(F::kCosts, ctx->multiprocessors * (F::kCodes ? kCodesPerCu : 1), p.units, p.groups, each, SPARSE ? listed : each, SPARSE || each < held);
+        plan_call(F::kCosts, ctx->multiprocessors, p.units, p.groups, each, SPARSE ? listed : each, SPARSE || each < held);
     p.whole = plan.whole;
     p.most = plan.most;
     p.per = plan.per;
@@ -631,20 +632,20 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
     p.spread = plan.spread;
     auto launch = [&]() -> int32_t {
         const unsigned wgs = (unsigned)(((int64_t)p.most * p.chunks + 7) / 8 * 8);
-        int tok = timing_begin(ctx, "paged_mfma");
+        int tok = timing_begin(ctx, F::kCodes ? "paged_codes" : "paged_mfma");
         if constexpr (F::kCodes) launch_codes(ctx, p, KIND, wgs);
         else hipLaunchKernelGGL((k_paged_mfma<F, KIND>), dim3(wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
         timing_end(ctx, tok);
-        return launch_check(ctx, "k_paged_mfma");
+        return launch_check(ctx, F::kCodes ? "k_paged_codes" : "k_paged_mfma");
     };
     if (plan.slots == 0) return launch();  // nothing is left to join
     ScratchPlan scratch;
-    scratch.add((size_t)plan.slots * kPL * kCols * 4);
+    scratch.add((size_t)plan.slots * kPL * kCols * sizeof(typename F::part_t));
     scratch.add((size_t)plan.slots * kCols * 8);
     scratch.add((size_t)(p.units + 1) * 8);
     std::vector<void *> ptrs;
     UT_TRY(scratch_acquire(ctx, scratch, ptrs));
-    p.part_o = (float *)ptrs[0];
+    p.part_o = ptrs[0];
     p.part_ml = (float *)ptrs[1];
     p.plan = (int64_t *)ptrs[2];
     UT_TRY(launch());

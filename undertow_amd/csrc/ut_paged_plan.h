@@ -66,6 +66,7 @@ struct PlanCosts {  // of a cache format
     int32_t bytes_ratio;  // and to that of a column group's part's bytes, written and read
     float join;           // the join's launch, in tiles
     int32_t brief;        // a sequence of so few tiles does not pay for the cut (plan_call)
+    int32_t slots = 1;    // workgroups that run on a CU at a time
 };
 // lead: 64 sequences of up to 8192 positions take 135 us with 0, 132 with 2, 126
 // with 4, 115 with 8, 117 with 16.  ratio: one row over 32768 positions 48 us
@@ -80,7 +81,7 @@ constexpr PlanCosts kCostsBf16 = {8, 8, 4, 150, 2.5f, 20};
 // bytes_ratio: 63 x 4 rows of up to 25 positions 66.5 us without and with 280,
 // 80.4 with 140.
 constexpr PlanCosts kCostsF16x2 = {4, 4, 16, 280, 1.3f, 10};
-constexpr PlanCosts kCostsI8 = {4, 8, 4, 150, 2.5f, 20};
+constexpr PlanCosts kCostsI8 = {4, 8, 8, 300, 2.5f, 20, 2};
 struct PlanCall {
     int32_t whole;        // a range is a unit: no parts, no join
     int32_t most;         // ranges at most (whole: units)
@@ -131,16 +132,17 @@ inline PlanCall plan_call(const PlanCosts &c, int32_t cus, int32_t units, int32_
     PlanCall p{};
     const int64_t tiles = units * each, empty = (int64_t)(units - 1) * c.lead, W = tiles + empty;
     plan_heads(p, c, cus, groups, units);
-    const int64_t turns = ((int64_t)units * p.chunks + cus - 1) / cus;
+    const int32_t places = cus * c.slots;
+    const int64_t turns = ((int64_t)units * p.chunks + places - 1) / places;
     const float whole = (float)(turns * (listed + c.lead) - c.lead);
     auto cut = [&](int32_t ratio) {
         p.spread = fminf((float)units * ratio, (float)c.bytes_ratio / (float)groups);
-        plan_heads(p, c, cus, groups, plan_ranges(tiles, cus, p.spread));
-        p.most = plan_ranges(W, p.chunks < cus ? cus / p.chunks : 1, p.spread);
+        plan_heads(p, c, cus, groups, plan_ranges(tiles, places, p.spread));
+        p.most = plan_ranges(W, p.chunks < places ? places / p.chunks : 1, p.spread);
     };
     cut(c.ratio);
     if (p.most == 1) {
-        const int64_t rounds = ((int64_t)p.chunks + cus - 1) / cus;
+        const int64_t rounds = ((int64_t)p.chunks + places - 1) / places;
         p.whole = units == 1 || whole < 0.9f * (float)(rounds * W);
     } else {
         const float there = lists || each <= c.brief ? (float)W : 0.5f * (float)tiles + (float)empty;
@@ -159,6 +161,44 @@ inline PlanCall plan_call(const PlanCosts &c, int32_t cus, int32_t units, int32_
     if (p.wide) cut(2 * c.ratio);
     p.slots = plan_slot(p.most, false) * groups;
     return p;
+}
+// Rows with a window: of the positions before its end a row sees the last
+// `window` and the first `sinks`.  A sequence's rows end at n - M + 1 .. n.  Its
+// tiles are the first `ts`, which hold the first positions, and those from the one
+// on where the first row's window begins; `skip` tiles between them are left out.
+struct NearCut {
+    int32_t start;  // the first row's window
+    int32_t ts, skip;
+};
+UT_PLAN_FN NearCut near_cut(int32_t n, int32_t M, int32_t window, int32_t sinks, int32_t tile) {
+    const int32_t end = n - M + 1, start = end > window ? end - window : 0, from = start / tile;
+    const int32_t s = sinks < n ? sinks : n, ts = (int32_t)(((int64_t)s + tile - 1) / tile);
+    return {start, ts < from ? ts : from, ts < from ? from - ts : 0};
+}
+// The first position of tile x.
+UT_PLAN_FN int32_t near_tile(const NearCut &c, int32_t x, int32_t tile) { return (x >= c.ts ? x + c.skip : x) * tile; }
+// Tiles of a sequence at most.  (The windows may begin and end inside a tile, and
+// so may the first positions.)
+UT_PLAN_FN int64_t near_most(int64_t M, int64_t window, int64_t sinks, int64_t tile) {
+    return (window + M - 1 + tile - 1) / tile + 1 + (sinks + tile - 1) / tile;
+}
+// No row sees any of the `count` positions from v0 on.
+UT_PLAN_FN bool near_hidden(const NearCut &c, int32_t sinks, int32_t v0, int32_t count) {
+    return v0 >= sinks && v0 + count <= c.start;
+}
+// The visible positions of the 32 from v0 on: for a row that ends at n, for some
+// row of a sequence (windows follow on one another: together they are one run), and
+// for every row.
+UT_PLAN_FN uint32_t low_bits(int32_t c) { return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u; }
+UT_PLAN_FN uint32_t near_seen(int32_t v0, int32_t n, int32_t window, int32_t sinks) {
+    const int32_t from = n > window ? n - window - v0 : 0;
+    return low_bits(n - v0) & (~low_bits(from) | low_bits(sinks - v0));
+}
+UT_PLAN_FN uint32_t near_some(const NearCut &c, int32_t v0, int32_t n, int32_t sinks) {
+    return low_bits(n - v0) & (~low_bits(c.start - v0) | low_bits(sinks - v0));
+}
+UT_PLAN_FN uint32_t near_every(int32_t v0, int32_t n, int32_t M, int32_t window, int32_t sinks) {
+    return near_seen(v0, n, window, sinks) & low_bits(n - M + 1 - v0);
 }
 // Positions of a sequence or a selection: tile and page counts may step past
 // the end by some tiles and stay in 32 bits.
