@@ -61,11 +61,37 @@ def test_attend_prompt_rows(ctx, lens, M, H, width):
     attend_case(ctx, lens, M, H, width=width // 64)
 
 
+@pytest.mark.parametrize("lens", [[300, 64, 5], [5000, 64]])
 @pytest.mark.parametrize("H,L,P,spread", [(128, 512, 64, 3), (16, 512, 64, 12), (128, 512, 64, 20), (4, 64, 16, 12)])
-def test_attend_positions_of_very_different_sizes(ctx, H, L, P, spread):
+def test_attend_positions_of_very_different_sizes(ctx, lens, H, L, P, spread):
     """Scales up to 2^40 apart: a large position of small weight does not
     drown the small ones that have it, nor the other way round."""
-    attend_case(ctx, [300, 64, 5], 2, H, L, P, spread=spread)
+    attend_case(ctx, lens, 2, H, L, P, spread=spread)
+
+
+@pytest.mark.parametrize("lens", [[300, 40], [6000, 700, 3]])  # whole, and cut into ranges
+@pytest.mark.parametrize("size", [-100, -60, 60, 100])
+@pytest.mark.parametrize("H,L,P", [(128, 512, 64), (4, 64, 16)])
+def test_attend_tiny_and_huge_values(ctx, lens, size, H, L, P):
+    """Latent values of 2^size and queries of 2^-size: the context has the
+    values' size whatever that is."""
+    pool = R8.Pool8(41, lens, 64, L, P)
+    for b, n in enumerate(lens):
+        x = pool.randn(n, L + P)
+        x[:, :L] *= 2.0 ** size
+        pool.put(b, 0, x)
+    qabs, qrope = pool.queries(1, H)
+    qabs *= 2.0 ** -size
+    got = pool.cuda(ctx=ctx).attend(pool.table.cuda(), pool.lens32().cuda(), qabs.cuda(), qrope.cuda(), SCALE)
+    ctx.synchronize()
+    # tolerances relative to the values' size: everything is taken times 2^-size
+    for b, n in enumerate(lens):
+        kv = pool.rows(b, torch.arange(n)).cuda()
+        q = torch.cat([qabs[b, 0], qrope[b, 0]], -1).double().cuda()
+        out, spread, mass = R.attend(kv, q, L, SCALE)
+        down = 2.0 ** -size
+        R8.close("i8", (got[b, 0].double() * down), out * down, spread * down, mass * down,
+                 R8.score_step(kv, q, L, SCALE)[:, None].cpu(), R8.largest(kv, q, L, SCALE).cpu() * down)
 
 
 @pytest.mark.parametrize("H,L,P", [(128, 512, 64), (16, 512, 64), (4, 64, 16)])

@@ -14,8 +14,11 @@
 // rounded to f16, w = e^(s - m) a.  Scales may be of any size: m is a column's
 // offset that puts the largest such product so far at 2^10 to 2^15, so that one
 // loses bits from 2^-24 of the largest down; the sum of the weights themselves,
-// in f32, takes the size that they have then.  (m leaves the largest weight at
-// 2^60 or below: with scales below 2^-74 products lose bits.)
+// in f32, takes the size that they have then.  m leaves the largest weight at
+// 2^60 or below, and where the first scales that a column meets are so small that
+// this is not enough, they and all behind them are taken times a power of two.
+// (A column loses bits where its largest products are below 2^-74 of that first
+// scale's size, and come with scores that let all before them vanish.)
 //
 // A position is 584 bytes, half a bf16 one, for the same products at the same
 // rate, so that up to some 64 heads memory bounds it and with 128 the matrix
@@ -47,7 +50,7 @@ struct CodesWave {
     pu32x4 w[18];
     float lat, rope;  // what a digit is worth in each part, times the scores' scale
     pf32x4 o[32];     // context^T: dim 16 mt + 4 (l >> 4) + i, column l & 15
-    float m, l;       // offset (log2 units) and sum
+    float m, l, up;   // offset (log2 units) and sum; the power of two that values are taken times
 };
 
 // The lane, as if not known yet: what is worked out of it is worked out anew for
@@ -204,6 +207,9 @@ __device__ __forceinline__ pf16x8 tile_weights(CodesWave &w, uint32_t seen, bool
                 s[i] = 0.0f;
             }
     }
+    if (__any(w.up != 1.0f))
+#pragma unroll
+        for (int i = 0; i < 8; i++) s[i] = __fmul_rn(s[i], w.up);
     float e[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(t[i]);
@@ -221,6 +227,12 @@ __device__ __forceinline__ pf16x8 tile_weights(CodesWave &w, uint32_t seen, bool
         const float top = col_max(most(t)), to = fmaxf(u - 10.0f, top - kCMost);
         const bool move = (fresh || u > 15.0f || top > kCMost + kCRise) && fabsf(to) < INFINITY;
         const float by = move ? to : 0.0f, f = fresh ? 0.0f : __builtin_amdgcn_exp2f(-by);
+        if (fresh) {
+            const float low = top - kCMost - (u - 10.0f);  // (log2) too small for m alone
+            w.up = move && low > 0.0f && low < INFINITY ? ldexpf(1.0f, low < 120.0f ? (int)low : 120) : 1.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i] = __fmul_rn(s[i], w.up);
+        }
         w.m += by;
         w.l *= f;
 #pragma unroll
@@ -285,6 +297,7 @@ template <class B> __device__ __forceinline__ void load_queries(const PagedArgs 
     for (int i = 0; i < 18; i++) asm volatile("" : "+v"(w.w[i]));
     w.m = kLow;
     w.l = 0.0f;
+    w.up = 1.0f;
 #pragma unroll
     for (int mt = 0; mt < 32; mt++) w.o[mt] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
@@ -295,7 +308,7 @@ __device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, 
     const float sum = col_sum(w.l);
     const int l = lane_anew(), g = l >> 4, col = l & 15, h = q.h0 + col;
     if (active && ((KIND == kListed && p.whole) || (q.b0 == 0 && q.b1 == q.tiles))) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = sum == 0.0f ? 0.0f : __fmul_rn(1.0f / sum, 1.0f / w.up);
         __bf16 *out = (__bf16 *)a.out + (q.row + h) * kPL + 4 * g;
         if (h < a.H)
 #pragma unroll
@@ -308,7 +321,7 @@ __device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, 
     } else if (active) {
         // a part's context in f16, which is 1/8 of what the output's own rounding to
         // bf16 may take, times a power of two of the column that puts the largest at
-        // 2^13 to 2^14; the sum goes with it, and the offset back
+        // 2^13 to 2^14
         float top = 0.0f;
 #pragma unroll
         for (int mt = 0; mt < 32; mt++)
@@ -326,7 +339,7 @@ __device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, 
             for (int i = 0; i < 4; i++) v[i] = (_Float16)__fmul_rn(w.o[mt][i], f);
             po[mt * 4 * kCols] = v;
         }
-        if (g == 0) *(float2 *)(p.part_ml + (slot * kCols + col) * 2) = make_float2(w.m - (float)up, __fmul_rn(sum, f));
+        if (g == 0) *(float4 *)(p.part_ml + (slot * kCols + col) * 4) = make_float4(w.m, sum, __fmul_rn(ldexpf(1.0f, -up), 1.0f / w.up), 0.0f);
     }
 }
 

@@ -539,12 +539,20 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
     auto add = [&](int r, auto many) {
         constexpr int COUNT = decltype(many)::value;
         float2 ml[COUNT];
+        float unit[COUNT];  // of the part's context
         p4 v[COUNT][4];
 #pragma unroll
         for (int i = 0; i < COUNT; i++) {
             const int x = r + NW * i;
             const int64_t slot = plan_slot(x, x == r0) * p.groups + grp;
-            ml[i] = *(const float2 *)(p.part_ml + (slot * kCols + col) * 2);
+            if constexpr (F::kCodes) {
+                const float4 x = *(const float4 *)(p.part_ml + (slot * kCols + col) * 4);
+                ml[i] = make_float2(x.x, x.y);
+                unit[i] = x.z;
+            } else {
+                ml[i] = *(const float2 *)(p.part_ml + (slot * kCols + col) * 2);
+                unit[i] = 1.0f;
+            }
 #pragma unroll
             for (int k = 0; k < 4; k++)
                 v[i][k] = ((const p4 *)p.part_o)[(slot * 128 + blockIdx.y * 16 + qd + 4 * k) * kCols + col];
@@ -560,10 +568,11 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
         for (int i = 0; i < COUNT; i++) {
             const float f = __builtin_amdgcn_exp2f(ml[i].x - mn);
             L = __builtin_fmaf(ml[i].y, f, L);
+            const float fo = F::kCodes ? __fmul_rn(f, unit[i]) : f;
 #pragma unroll
             for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) t[k][e] = __builtin_fmaf((float)v[i][k][e], f, t[k][e]);
+                for (int e = 0; e < 4; e++) t[k][e] = __builtin_fmaf((float)v[i][k][e], fo, t[k][e]);
         }
         m = mn;
     };
@@ -641,7 +650,7 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
     if (plan.slots == 0) return launch();  // nothing is left to join
     ScratchPlan scratch;
     scratch.add((size_t)plan.slots * kPL * kCols * sizeof(typename F::part_t));
-    scratch.add((size_t)plan.slots * kCols * 8);
+    scratch.add((size_t)plan.slots * kCols * (F::kCodes ? 16 : 8));
     scratch.add((size_t)(p.units + 1) * 8);
     std::vector<void *> ptrs;
     UT_TRY(scratch_acquire(ctx, scratch, ptrs));
