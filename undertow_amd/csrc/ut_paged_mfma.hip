@@ -591,30 +591,31 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
 #pragma unroll
     for (int k = 0; k < 4; k++) so[w][qd + 4 * k][col] = t[k];
     __syncthreads();
-    // thread: four dims (tid & 15) of column tid >> 4
-    if (tid >= 256) return;
-    const int c = tid >> 4, d = tid & 15;
-    float M = kLow, sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NW; i++) M = fmaxf(M, sml[i][c].x);
-    pf32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < NW; i++) {
-        const float f = __builtin_amdgcn_exp2f(sml[i][c].x - M);
-        const pf32x4 v = so[i][d][c];
-        sum = __builtin_fmaf(sml[i][c].y, f, sum);
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(v[e], f, o[e]);
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    o4 v;
-#pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = (typename F::out_t)__fmul_rn(o[e], inv);
+    // thread: four dims (tid & 15) of column tid >> 4 (and every 4 NW-th)
     constexpr bool SPARSE = KIND == kListed;
-    const int per_row = (a.H + kCols - 1) / kCols;
+    const int per_row = (a.H + kCols - 1) / kCols, d = tid & 15;
     const int64_t row = SPARSE ? u : (int64_t)u * a.M + grp / per_row;
-    const int h = (SPARSE ? grp : grp % per_row) * kCols + c;
-    if (h < a.H) *(o4 *)((typename F::out_t *)a.out + (row * a.H + h) * kPL + blockIdx.y * 64 + 4 * d) = v;
+#pragma unroll
+    for (int c = tid >> 4; c < kCols; c += 4 * NW) {
+        float M = kLow, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; i++) M = fmaxf(M, sml[i][c].x);
+        pf32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            const float f = __builtin_amdgcn_exp2f(sml[i][c].x - M);
+            const pf32x4 v = so[i][d][c];
+            sum = __builtin_fmaf(sml[i][c].y, f, sum);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(v[e], f, o[e]);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        o4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = (typename F::out_t)__fmul_rn(o[e], inv);
+        const int h = (SPARSE ? grp : grp % per_row) * kCols + c;
+        if (h < a.H) *(o4 *)((typename F::out_t *)a.out + (row * a.H + h) * kPL + blockIdx.y * 64 + 4 * d) = v;
+    }
 }
 
 bool paged_mfma_ok(const PagedArgs &a) { return a.L == kPL && a.P == kPD - kPL && a.shift >= 3; }
@@ -660,7 +661,11 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
     UT_TRY(launch());
     const dim3 grid((unsigned)((int64_t)p.units * p.groups), kPlanJoinSlices);
     int tok = timing_begin(ctx, "paged_join");
-    if (plan.wide)
+    // (8-bit pages: one wave where a unit has few parts, so that more workgroups run at a time: 256
+    // sequences of up to 2048 positions 158 us with four, 147 with two, 143 with one)
+    if (F::kCodes && p.most <= 8 * p.units)
+        hipLaunchKernelGGL((k_paged_join<F, KIND, 1>), grid, dim3(64), 0, ctx->stream, p);
+    else if (plan.wide)
         hipLaunchKernelGGL((k_paged_join<F, KIND, 16>), grid, dim3(1024), 0, ctx->stream, p);
     else
         hipLaunchKernelGGL((k_paged_join<F, KIND, 4>), grid, dim3(256), 0, ctx->stream, p);
