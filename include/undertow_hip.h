@@ -366,7 +366,10 @@ int32_t ut_mla_paged_read(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *ta
  * to bf16 before they meet the values, in numerator and denominator alike (the
  * matrix cores take both operands in one type): a context is off by at most
  * 2^-8 of its values' weighted spread for that, and by its own rounding.  f16x2
- * pages keep the weights to 22 bits.  Equal calls give equal bits; a row's
+ * pages keep the weights to 22 bits.  With 8-bit pages of 8 positions and more at
+ * those widths each part of a query is rounded to 2^-16 of its largest value, a
+ * weight times its position's scale to 2^-11, and so is the context of each part
+ * of a sequence that is cut; others compute in f32.  Equal calls give equal bits; a row's
  * rounding may depend on the sizes of the call and the lengths of its batch
  * (the work is cut evenly over the device).  Working memory: some 135 MB of the
  * arena at most; none where the rows alone fill the device (prompts). */

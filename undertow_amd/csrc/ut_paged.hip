@@ -203,6 +203,8 @@ template <class T> __device__ __forceinline__ int code8(T q, T top, T f) {
 // and the waves' sums meet in LDS.  Latency bounds a step (length, table, rows, one
 // reduction over the waves), a page of new rows its CU's arithmetic: sixteen
 // waves, the next row loaded under the present one's, older rows four at a time.
+// 48 rows into pages of 64 7.9 us (1.1 MB), 3 x 777 rows 13.4 (6.8 MB); with the
+// rows written first and the page then summed from memory 10.2 and 36.
 constexpr int kAppendWaves = 16, kAppendOld = 4;
 struct PartQuant {
     float m, f, scale;  // the part's largest, about 127 / m, what is stored
@@ -401,7 +403,8 @@ __global__ __launch_bounds__(kAppendWaves * 64) void k_paged_append_i8(PagedArgs
 // where that is bf16; zeros for rows outside the sequence.  A thread takes four
 // values of a row, so that a wave's stores are whole lines, a workgroup as many
 // whole rows as it has room for, kReadTurns of them at a time, all looked up and
-// loaded before the first is stored.
+// loaded before the first is stored (131072 rows in f32 with 1, 2, 4 and 8 at a time
+// 96, 92, 90 and 100 us).
 template <bool PAST, class T> __device__ __forceinline__ void put4(T *dst, const float4 &x) {
     typedef T t4 __attribute__((ext_vector_type(4)));
     const t4 v = {(T)x.x, (T)x.y, (T)x.z, (T)x.w};
@@ -409,7 +412,9 @@ template <bool PAST, class T> __device__ __forceinline__ void put4(T *dst, const
     else *(t4 *)dst = v;
 }
 constexpr int kReadThreads = 576, kReadTurns = 4;
-// Rows of more bytes than this go past the L2s, which hold 32 MB together.
+// Rows of more bytes than this go past the L2s, which hold 32 MB together: 302 MB
+// in f32 52 us past them (6.5 TB/s with what is read) and 90 through them, 75 MB in
+// f32 15.4 and 15.8; what fits stays there for its reader.
 constexpr int64_t kReadPast = int64_t(32) << 20;
 template <class F, bool PAST, class T>
 __global__ __launch_bounds__(kReadThreads) void k_paged_read(PagedArgs a, const int32_t *__restrict__ starts, int rows,

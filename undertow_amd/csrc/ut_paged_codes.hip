@@ -21,12 +21,22 @@
 // scale's size, and come with scores that let all before them vanish.)
 //
 // A position is 584 bytes, half a bf16 one, for the same products at the same
-// rate, so that up to some 64 heads memory bounds it and with 128 the matrix
-// cores.  A wave has its columns' whole context and queries in registers (two
-// waves a SIMD); what a wave does between products (conversion, scales, softmax,
-// look-ups) takes as long as they do, so the two waves of a SIMD must not do it at
-// the same time.  Hence two workgroups a CU, four waves each, that know nothing of
-// one another: with eight waves in step a tile of 128 heads took 2.7 us.
+// rate, so that memory bounds up to some 64 heads and the matrix cores 128.  A
+// wave has its columns' whole context and queries in registers (two waves a SIMD),
+// and what it does between products (conversion, scales, softmax, look-ups) takes
+// as long as they do: the two waves of a SIMD must not do that at the same time.
+// Hence two workgroups a CU, four waves each, that know nothing of one another, and
+// a higher priority for the one that is past its scores.  What bounds it now, with
+// tiles of 32 positions:
+// - 128 heads: instructions.  A tile takes 2.4 us a CU where its data come from L2
+//   (512 prompt rows over 8192 positions 1215 us, 0.93 PFLOP/s; without the priority
+//   1327; bf16 pages, which need no conversion, 1030), 2.6 to 2.9 with the traffic
+//   of decoding: 64 sequences of up to 8192 119 us (bf16 115).
+// - 16 heads: memory, 1.03 us a tile and CU (4.7 TB/s), once it runs: 37 sequences
+//   of up to 12001 51 us in all (132 MB), of which its start, the ranges' ends and
+//   the join are half.
+// - few rows: latency.  A call over one tile takes 9.7 us, 1.7 of them that tile's,
+//   over four 15.5.
 #include "ut_paged_attend.h"
 
 namespace ut {

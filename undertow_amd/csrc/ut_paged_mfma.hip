@@ -29,6 +29,10 @@
 // copies 70, the start 9 (lengths 1.4, queries issued 4.6, first tiles 8.7 us
 // from the start), partial results written 5 to 10, their join 16 (82 MB each
 // way).
+//
+// With a window a unit is a sequence's tiles that some row sees, first ones and
+// window, numbered without those between: one row over 1024 of 16384 positions
+// 18.8 us in all, 13 x 3 rows of 64 heads over 777 of up to 5003 in f16x2 45.8.
 #include <type_traits>
 
 #include "ut_paged_attend.h"

@@ -81,6 +81,12 @@ constexpr PlanCosts kCostsBf16 = {8, 8, 4, 150, 2.5f, 20};
 // bytes_ratio: 63 x 4 rows of up to 25 positions 66.5 us without and with 280,
 // 80.4 with 140.
 constexpr PlanCosts kCostsF16x2 = {4, 4, 16, 280, 1.3f, 10};
+// (two workgroups of four waves a CU; a part in f16 is half as many bytes)  ratio:
+// one row over 32768 positions 47.8 us with 4, 43.4 with 8, 46.4 with 12.
+// bytes_ratio: 64 sequences of up to 600 47 us with 150, 41.5 with 300; 256 of up to
+// 1024 97 with 300, 110 with 600.  lead: those 256 109 us with 4, 97 with 8, 98 with
+// 14.  One row over 32768 with its heads spread over the CUs' places 54 us, over the
+// CUs alone, which then take two ranges each, 47.8.
 constexpr PlanCosts kCostsI8 = {4, 8, 8, 300, 2.5f, 20, 2};
 struct PlanCall {
     int32_t whole;        // a range is a unit: no parts, no join
