@@ -55,6 +55,29 @@ def test_attend_cut_into_ranges(ctx, lens, M, H, width):
     attend_case(ctx, lens, M, H, width=None if width is None else width // 64)
 
 
+@pytest.mark.parametrize("units", [60, 200, 600])  # each is found in another way
+@pytest.mark.parametrize("kind", ["all", "window", "listed"])
+def test_attend_of_many_sequences_in_a_wide_table(ctx, units, kind):
+    M = 1 if kind != "listed" else 2
+    lens = [(97 * k) % 331 if k % 7 else 0 for k in range(units // M)]
+    pool = R8.Pool8(17, lens, 64, 512, 64, 128)
+    qabs, qrope = pool.queries(M, 16)
+    where = pool.table.cuda(), pool.lens32().cuda(), qabs.cuda(), qrope.cuda(), SCALE
+    cache, more = pool.cuda(ctx=ctx), {}
+    if kind == "all":
+        got = cache.attend(*where)
+    elif kind == "window":
+        more = dict(window=150, sinks=33)
+        got = cache.attend_window(*where, **more)
+    else:
+        sel = torch.stack([torch.randperm(8, generator=pool.g)[:5] - 1 for _ in range(units)]).int().view(-1, M, 5)
+        # places that lists are seldom filled to
+        more = dict(sel=torch.cat([sel, torch.full((len(lens), M, 35), -1, dtype=torch.int32)], -1))
+        got = cache.attend_pages(*where, more["sel"].cuda())
+    ctx.synchronize()
+    R8.check(pool, "i8", got, qabs, qrope, SCALE, **more)
+
+
 @pytest.mark.parametrize("lens,M,H,width", [
     ([600, 40, 333], 128, 256, 4096), ([700], 300, 128, 8192), ([1500, 700], 40, 128, 2048), ([140, 200], 140, 16, 300)])
 def test_attend_prompt_rows(ctx, lens, M, H, width):

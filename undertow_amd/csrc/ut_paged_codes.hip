@@ -18,7 +18,9 @@
 // 2^60 or below, and where the first scales that a column meets are so small that
 // this is not enough, they and all behind them are taken times a power of two.
 // (A column loses bits where its largest products are below 2^-74 of that first
-// scale's size, and come with scores that let all before them vanish.)
+// scale's size, and come with scores that let all before them vanish; and its sum
+// those weights that are below 2^-36 of the largest at scales of 2^100, 2^-15 at the
+// largest number's.)
 //
 // A position is 584 bytes, half a bf16 one, for the same products at the same
 // rate, so that memory bounds up to some 64 heads and the matrix cores 128.  A
