@@ -30,6 +30,7 @@ void plan(int cus, int units, int groups, int64_t each, int64_t listed, int list
     out[0] = p.whole; out[1] = p.most; out[2] = p.per; out[3] = p.chunks; out[4] = p.slots;
 }
 int waves(void) { return ut::kCostsI8.waves; }
+int size(int call) { return call ? sizeof(ut::PlanCall) : sizeof(ut::PlanCosts); }
 int places(int cus) { return cus * ut::kCostsI8.slots; }
 }
 """
@@ -119,3 +120,8 @@ def test_calls_over_8_bit_pages_are_cut(L, seed):
         else:
             assert 1 <= most and (most == 1 or most * chunks <= L.places(cus))
             assert slots == (0 if most == 1 else 2 * most * groups)
+
+
+def test_what_other_tests_hold_of_a_plan_has_its_size(L):
+    import test_paged_cut as cut
+    assert [L.size(0), L.size(1)] == [C.sizeof(cut.Costs), C.sizeof(cut.Call)]

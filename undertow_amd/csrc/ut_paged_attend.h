@@ -351,7 +351,7 @@ template <int KIND> struct Walk {
 // The kernel of 8-bit pages (ut_paged_codes.hip), `wgs` workgroups.
 struct CodesI8 {
     static constexpr bool kCodes = true;
-    static constexpr PlanCosts kCosts = kCostsI8;
+    static constexpr PlanCostsMany kCosts = kCostsI8;
     typedef __bf16 out_t;
     typedef _Float16 part_t;
 };

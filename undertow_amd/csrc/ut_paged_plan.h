@@ -66,8 +66,12 @@ struct PlanCosts {  // of a cache format
     int32_t bytes_ratio;  // and to that of a column group's part's bytes, written and read
     float join;           // the join's launch, in tiles
     int32_t brief;        // a sequence of so few tiles does not pay for the cut (plan_call)
-    int32_t slots = 1;    // workgroups that run on a CU at a time
 };
+struct PlanCostsMany : PlanCosts {
+    int32_t slots;  // workgroups that run on a CU at a time
+};
+inline int32_t plan_places(const PlanCosts &, int32_t cus) { return cus; }
+inline int32_t plan_places(const PlanCostsMany &c, int32_t cus) { return cus * c.slots; }
 // lead: 64 sequences of up to 8192 positions take 135 us with 0, 132 with 2, 126
 // with 4, 115 with 8, 117 with 16.  ratio: one row over 32768 positions 48 us
 // with 2, 44 with 3, 42 with 4, 41 with 8, and 59 in as many ranges as CUs; 4
@@ -87,7 +91,7 @@ constexpr PlanCosts kCostsF16x2 = {4, 4, 16, 280, 1.3f, 10};
 // 1024 97 with 300, 110 with 600.  lead: those 256 109 us with 4, 97 with 8, 98 with
 // 14.  One row over 32768 with its heads spread over the CUs' places 54 us, over the
 // CUs alone, which then take two ranges each, 47.8.
-constexpr PlanCosts kCostsI8 = {4, 8, 8, 300, 2.5f, 20, 2};
+constexpr PlanCostsMany kCostsI8 = {{4, 8, 8, 300, 2.5f, 20}, 2};
 struct PlanCall {
     int32_t whole;        // a range is a unit: no parts, no join
     int32_t most;         // ranges at most (whole: units)
@@ -133,12 +137,13 @@ inline void plan_heads(PlanCall &p, const PlanCosts &c, int32_t cus, int32_t gro
 // 1034 us whole and 741 as one range with lengths spread evenly, 1055 and 1048
 // with equal ones; 3 x 777 over up to 1900 (whole 0.86 of the range) 1249 and 1368,
 // 1341 and 1781; in f16 pairs (0.92) 5.35 ms and 4.63, 5.33 and 5.93.
-inline PlanCall plan_call(const PlanCosts &c, int32_t cus, int32_t units, int32_t groups, int64_t each,
-                          int64_t listed, bool lists) {
+template <class Costs>
+PlanCall plan_call(const Costs &c, int32_t cus, int32_t units, int32_t groups, int64_t each, int64_t listed,
+                   bool lists) {
     PlanCall p{};
     const int64_t tiles = units * each, empty = (int64_t)(units - 1) * c.lead, W = tiles + empty;
     plan_heads(p, c, cus, groups, units);
-    const int32_t places = cus * c.slots;
+    const int32_t places = plan_places(c, cus);
     const int64_t turns = ((int64_t)units * p.chunks + places - 1) / places;
     const float whole = (float)(turns * (listed + c.lead) - c.lead);
     auto cut = [&](int32_t ratio) {
