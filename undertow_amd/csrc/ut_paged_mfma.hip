@@ -631,7 +631,7 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
     p.units = SPARSE ? a.B * a.M : a.B;
     p.groups = (SPARSE ? 1 : a.M) * ((a.H + kCols - 1) / kCols);
     const int64_t cap = (int64_t)(SPARSE ? a.top_k : a.max_pages) << a.shift;
-    p.lead = F::kCosts.lead;
+    p.lead = plan_lead(F::kCosts, p.groups);
     const int64_t near = near_most(a.M, a.window, a.sinks, kPT);
     const int64_t held = (cap + kPT - 1) / kPT, each = KIND == kNear && near < held ? near : held;
     // (no more pages are to be expected of a list than the table holds: 20 rows of

@@ -69,9 +69,12 @@ struct PlanCosts {  // of a cache format
 };
 struct PlanCostsMany : PlanCosts {
     int32_t slots;  // workgroups that run on a CU at a time
+    int32_t few;    // lead where a workgroup has all of a unit's heads
 };
 inline int32_t plan_places(const PlanCosts &, int32_t cus) { return cus; }
 inline int32_t plan_places(const PlanCostsMany &c, int32_t cus) { return cus * c.slots; }
+inline int32_t plan_lead(const PlanCosts &c, int32_t) { return c.lead; }
+inline int32_t plan_lead(const PlanCostsMany &c, int32_t groups) { return groups <= c.waves ? c.few : c.lead; }
 // lead: 64 sequences of up to 8192 positions take 135 us with 0, 132 with 2, 126
 // with 4, 115 with 8, 117 with 16.  ratio: one row over 32768 positions 48 us
 // with 2, 44 with 3, 42 with 4, 41 with 8, and 59 in as many ranges as CUs; 4
@@ -89,9 +92,10 @@ constexpr PlanCosts kCostsF16x2 = {4, 4, 16, 280, 1.3f, 10};
 // one row over 32768 positions 47.8 us with 4, 43.4 with 8, 46.4 with 12.
 // bytes_ratio: 64 sequences of up to 600 47 us with 150, 41.5 with 300; 256 of up to
 // 1024 97 with 300, 110 with 600.  lead: those 256 109 us with 4, 97 with 8, 98 with
-// 14.  One row over 32768 with its heads spread over the CUs' places 54 us, over the
+// 14; with 64 heads 77 with 0, 64 with 2, 60 with 4, 64 with 8, with 16 heads 53, 44,
+// 43.5 and 46.  One row over 32768 with its heads spread over the CUs' places 54 us, over the
 // CUs alone, which then take two ranges each, 47.8.
-constexpr PlanCostsMany kCostsI8 = {{4, 8, 8, 300, 2.5f, 20}, 2};
+constexpr PlanCostsMany kCostsI8 = {{4, 8, 8, 300, 2.5f, 20}, 2, 4};
 struct PlanCall {
     int32_t whole;        // a range is a unit: no parts, no join
     int32_t most;         // ranges at most (whole: units)
@@ -141,11 +145,12 @@ template <class Costs>
 PlanCall plan_call(const Costs &c, int32_t cus, int32_t units, int32_t groups, int64_t each, int64_t listed,
                    bool lists) {
     PlanCall p{};
-    const int64_t tiles = units * each, empty = (int64_t)(units - 1) * c.lead, W = tiles + empty;
+    const int32_t lead = plan_lead(c, groups);
+    const int64_t tiles = units * each, empty = (int64_t)(units - 1) * lead, W = tiles + empty;
     plan_heads(p, c, cus, groups, units);
     const int32_t places = plan_places(c, cus);
     const int64_t turns = ((int64_t)units * p.chunks + places - 1) / places;
-    const float whole = (float)(turns * (listed + c.lead) - c.lead);
+    const float whole = (float)(turns * (listed + lead) - lead);
     auto cut = [&](int32_t ratio) {
         p.spread = fminf((float)units * ratio, (float)c.bytes_ratio / (float)groups);
         plan_heads(p, c, cus, groups, plan_ranges(tiles, places, p.spread));
