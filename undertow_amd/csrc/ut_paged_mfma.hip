@@ -519,14 +519,16 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
 
 // Joins the parts of a unit that lies in more than one range:
 // out = sum_r o_r 2^(m_r - M) / sum_r l_r 2^(m_r - M).  A workgroup takes one
-// column group and 64 dims, each of its NW waves every NW-th part, as many at a
-// time as there are, with all their loads under way; the waves' results meet
+// column group and 16 NQ dims, each of its NW waves every NW-th part, as many at
+// a time as there are, with all their loads under way; the waves' results meet
 // in LDS.  Bound by the parts' bytes: 82 MB in 16.9 us (4.9 TB/s); 8 parts of
-// one row take 4.2.
-template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void k_paged_join(PagedMfmaArgs p) {
+// one row take 4.2.  NQ = 1 where that gives no more workgroups than CUs: one row
+// over 32768 positions in 8 bits 41.7 us with 4, 38.9 with 1 (bf16 37.4 and 36.0,
+// f16x2 59.1 and 56.8); two such rows, on 512 workgroups, 47.0 and 49.4.
+template <class F, int KIND, int NW, int NQ> __global__ __launch_bounds__(NW * 64) void k_paged_join(PagedMfmaArgs p) {
     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
     typedef typename F::part_t p4 __attribute__((ext_vector_type(4)));
-    __shared__ __attribute__((aligned(16))) pf32x4 so[NW][16][kCols + 1];  // one more: other banks
+    __shared__ __attribute__((aligned(16))) pf32x4 so[NW][4 * NQ][kCols + 1];  // one more: other banks
     __shared__ float2 sml[NW][kCols];
     const PagedArgs &a = p.a;
     const int u = blockIdx.x / p.groups, grp = blockIdx.x - u * p.groups, tid = threadIdx.x;
@@ -538,13 +540,13 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
     const int r0 = (int)plan_range_of(W, N, first), r1 = (int)plan_range_of(W, N, first + tiles - 1);
     if (r0 == r1) return;
     float m = kLow, L = 0.0f;
-    pf32x4 t[4] = {};
+    pf32x4 t[NQ] = {};
     // some parts: r and every NW-th behind it
     auto add = [&](int r, auto many) {
         constexpr int COUNT = decltype(many)::value;
         float2 ml[COUNT];
         float unit[COUNT];  // of the part's context
-        p4 v[COUNT][4];
+        p4 v[COUNT][NQ];
 #pragma unroll
         for (int i = 0; i < COUNT; i++) {
             const int x = r + NW * i;
@@ -558,8 +560,8 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
                 unit[i] = 1.0f;
             }
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                v[i][k] = ((const p4 *)p.part_o)[(slot * 128 + blockIdx.y * 16 + qd + 4 * k) * kCols + col];
+            for (int k = 0; k < NQ; k++)
+                v[i][k] = ((const p4 *)p.part_o)[(slot * 128 + blockIdx.y * 4 * NQ + qd + 4 * k) * kCols + col];
         }
         float mn = m;
 #pragma unroll
@@ -567,14 +569,14 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
         const float f0 = __builtin_amdgcn_exp2f(m - mn);
         L *= f0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) t[k] *= f0;
+        for (int k = 0; k < NQ; k++) t[k] *= f0;
 #pragma unroll
         for (int i = 0; i < COUNT; i++) {
             const float f = __builtin_amdgcn_exp2f(ml[i].x - mn);
             L = __builtin_fmaf(ml[i].y, f, L);
             const float fo = F::kCodes ? __fmul_rn(f, unit[i]) : f;
 #pragma unroll
-            for (int k = 0; k < 4; k++)
+            for (int k = 0; k < NQ; k++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) t[k][e] = __builtin_fmaf((float)v[i][k][e], fo, t[k][e]);
         }
@@ -593,14 +595,14 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
     if (r <= r1) add(r, std::integral_constant<int, 1>());
     if (qd == 0) sml[w][col] = make_float2(m, L);
 #pragma unroll
-    for (int k = 0; k < 4; k++) so[w][qd + 4 * k][col] = t[k];
+    for (int k = 0; k < NQ; k++) so[w][qd + 4 * k][col] = t[k];
     __syncthreads();
-    // thread: four dims (tid & 15) of column tid >> 4 (and every 4 NW-th)
+    // thread: four dims of a column (and of those behind it that have no thread)
     constexpr bool SPARSE = KIND == kListed;
-    const int per_row = (a.H + kCols - 1) / kCols, d = tid & 15;
+    const int per_row = (a.H + kCols - 1) / kCols, d = tid % (4 * NQ);
     const int64_t row = SPARSE ? u : (int64_t)u * a.M + grp / per_row;
 #pragma unroll
-    for (int c = tid >> 4; c < kCols; c += 4 * NW) {
+    for (int c = tid / (4 * NQ); c < kCols; c += 16 * NW / NQ) {
         float M = kLow, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < NW; i++) M = fmaxf(M, sml[i][c].x);
@@ -618,7 +620,7 @@ template <class F, int KIND, int NW> __global__ __launch_bounds__(NW * 64) void 
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = (typename F::out_t)__fmul_rn(o[e], inv);
         const int h = (SPARSE ? grp : grp % per_row) * kCols + c;
-        if (h < a.H) *(o4 *)((typename F::out_t *)a.out + (row * a.H + h) * kPL + blockIdx.y * 64 + 4 * d) = v;
+        if (h < a.H) *(o4 *)((typename F::out_t *)a.out + (row * a.H + h) * kPL + blockIdx.y * 16 * NQ + 4 * d) = v;
     }
 }
 
@@ -668,11 +670,13 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
     // (8-bit pages: one wave where a unit has few parts, so that more workgroups run at a time: 256
     // sequences of up to 2048 positions 158 us with four, 147 with two, 143 with one)
     if (F::kCodes && p.most <= 8 * p.units)
-        hipLaunchKernelGGL((k_paged_join<F, KIND, 1>), grid, dim3(64), 0, ctx->stream, p);
+        hipLaunchKernelGGL((k_paged_join<F, KIND, 1, 4>), grid, dim3(64), 0, ctx->stream, p);
+    else if (plan.wide && (int64_t)grid.x * 4 * kPlanJoinSlices <= ctx->multiprocessors)
+        hipLaunchKernelGGL((k_paged_join<F, KIND, 16, 1>), dim3(grid.x, 4 * kPlanJoinSlices), dim3(1024), 0, ctx->stream, p);
     else if (plan.wide)
-        hipLaunchKernelGGL((k_paged_join<F, KIND, 16>), grid, dim3(1024), 0, ctx->stream, p);
+        hipLaunchKernelGGL((k_paged_join<F, KIND, 16, 4>), grid, dim3(1024), 0, ctx->stream, p);
     else
-        hipLaunchKernelGGL((k_paged_join<F, KIND, 4>), grid, dim3(256), 0, ctx->stream, p);
+        hipLaunchKernelGGL((k_paged_join<F, KIND, 4, 4>), grid, dim3(256), 0, ctx->stream, p);
     timing_end(ctx, tok);
     return launch_check(ctx, "k_paged_join");
 }
