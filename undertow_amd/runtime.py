@@ -521,9 +521,10 @@ class PagedCache:
     pages: bfloat16 [n_pages, page, latent + rope], or float16 [n_pages, page,
     2, latent + rope] whose two planes stand for f32 values hi + lo / 2048, or
     int8 [n_pages, page, latent + rope] codes with scales float32 [n_pages,
-    page, 2] of a position's latent and of its rotated key.  mean (int8 [n_pages, latent + rope]) and mean_scale (float32 [n_pages])
-    hold a summary per page for ``select``.  The tensors are the caller's and
-    stay theirs.  Queries and contexts are bfloat16, with float16 pages float32.
+    page, 2] of a position's latent and of its rotated key.  mean (int8
+    [n_pages, latent + rope]) and mean_scale (float32 [n_pages]) hold a summary
+    per page for ``select``.  The tensors are the caller's and stay theirs.
+    Queries and contexts are bfloat16, with float16 pages float32.
 
     Every call takes a batch: table [B, max_pages] int32 (physical pages in a
     sequence's order; the rows may be slices of a wider table) and lens [B]
@@ -652,8 +653,8 @@ class PagedCache:
         shapes = (B, rows, self.latent), (B, rows, self.rope)
         if out is None:
             n = max(rows, 0)  # (the library turns down a count that is not positive)
-            out = (torch.empty((B, n, self.latent), dtype=dtype, device=table.device),
-                   torch.empty((B, n, self.rope), dtype=dtype, device=table.device))
+            out = (torch.empty(B, n, self.latent, dtype=dtype, device=table.device),
+                   torch.empty(B, n, self.rope, dtype=dtype, device=table.device))
         elif len(out) != 2:
             raise ShapeError(UT_ERR_SHAPE, "PagedCache: out must be two tensors")
         else:
