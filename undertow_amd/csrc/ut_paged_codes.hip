@@ -35,7 +35,7 @@
 //   1327; bf16 pages, which need no conversion, 1030), 2.6 to 2.9 with the traffic
 //   of decoding: 64 sequences of up to 8192 119 us (bf16 115).
 // - 16 heads: memory, 1.03 us a tile and CU (4.7 TB/s), once it runs: 37 sequences
-//   of up to 12001 51 us in all (132 MB), of which its start, the ranges' ends and
+//   of up to 12001 50 us in all (132 MB), of which its start, the ranges' ends and
 //   the join are half.
 // - few rows: latency.  A call over one tile takes 9.7 us, 1.7 of them that tile's,
 //   over four 15.5.

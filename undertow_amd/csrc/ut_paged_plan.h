@@ -74,10 +74,12 @@ struct PlanCostsMany : PlanCosts {
 inline int32_t plan_places(const PlanCosts &, int32_t cus) { return cus; }
 inline int32_t plan_places(const PlanCostsMany &c, int32_t cus) { return cus * c.slots; }
 inline int32_t plan_lead(const PlanCosts &c, int32_t) { return c.lead; }
-// How many times the ratio a wide join lets pay (plan_call).
-inline int32_t plan_wide(const PlanCosts &, int32_t) { return 2; }
+// How many units' ranges pay with a wide join (plan_call).
+inline int32_t plan_wide(const PlanCosts &, int32_t units, int32_t) { return 2 * units; }
 inline int32_t plan_lead(const PlanCostsMany &c, int32_t groups) { return groups <= c.waves ? c.few : c.lead; }
-inline int32_t plan_wide(const PlanCostsMany &c, int32_t groups) { return groups <= c.waves ? 8 : 2; }
+inline int32_t plan_wide(const PlanCostsMany &c, int32_t units, int32_t groups) {
+    return groups <= c.waves && units < 4 ? 8 : 2 * units;
+}
 // lead: 64 sequences of up to 8192 positions take 135 us with 0, 132 with 2, 126
 // with 4, 115 with 8, 117 with 16.  ratio: one row over 32768 positions 48 us
 // with 2, 44 with 3, 42 with 4, 41 with 8, and 59 in as many ranges as CUs; 4
@@ -154,12 +156,12 @@ PlanCall plan_call(const Costs &c, int32_t cus, int32_t units, int32_t groups, i
     const int32_t places = plan_places(c, cus);
     const int64_t turns = ((int64_t)units * p.chunks + places - 1) / places;
     const float whole = (float)(turns * (listed + lead) - lead);
-    auto cut = [&](int32_t ratio) {
-        p.spread = fminf((float)units * ratio, (float)c.bytes_ratio / (float)groups);
+    auto cut = [&](int32_t times) {
+        p.spread = fminf((float)times * (float)c.ratio, (float)c.bytes_ratio / (float)groups);
         plan_heads(p, c, cus, groups, plan_ranges(tiles, places, p.spread));
         p.most = plan_ranges(W, p.chunks < places ? places / p.chunks : 1, p.spread);
     };
-    cut(c.ratio);
+    cut(units);
     if (p.most == 1) {
         const int64_t rounds = ((int64_t)p.chunks + places - 1) / places;
         p.whole = units == 1 || whole < 0.9f * (float)(rounds * W);
@@ -176,12 +178,13 @@ PlanCall plan_call(const Costs &c, int32_t cus, int32_t units, int32_t groups, i
     // The join takes 16 waves a workgroup, and twice the ranges pay, where there
     // are few units of many parts: one row over 32768 positions 42.8 us with 4
     // waves, 39.5 with 16, 37.2 with the ranges (over 509, 8 parts, 15.5 and 15.9).
-    // Eight times where a workgroup of 8-bit pages has all heads, since then few
-    // places are taken: 64 heads over 32768 positions 35.0 us with twice, 34.6 with
-    // four times, 31.7 with eight, 16 heads 30.4, 28.6 and 25.9; 128 heads 38.6,
-    // 40.4 and 39.6.
+    // A few units of 8-bit pages whose heads a workgroup has all take few places, so
+    // that they get eight units' in all: 64 heads over 32768 positions 35.0 us with
+    // twice, 34.6 with four times, 31.3 with eight times the ranges, 16 heads 30.5,
+    // 28.7 and 26.0, two rows of 16 heads over up to 4096 19.8, 18.2 and 19.0, four
+    // 20.6, 21.3 and 22.8; 128 heads over 32768 38.6, 40.4 and 39.6.
     p.wide = (int64_t)units * groups * kPlanJoinSlices <= cus && p.most > 16 * units;
-    if (p.wide) cut(plan_wide(c, groups) * c.ratio);
+    if (p.wide) cut(plan_wide(c, units, groups));
     p.slots = plan_slot(p.most, false) * groups;
     return p;
 }
