@@ -55,6 +55,12 @@ def test_attend_cut_into_ranges(ctx, lens, M, H, width):
     attend_case(ctx, lens, M, H, width=None if width is None else width // 64)
 
 
+@pytest.mark.parametrize("units", [1, 2, 3, 4])
+@pytest.mark.parametrize("M,H", [(1, 16), (1, 50), (1, 64), (2, 16), (1, 128), (2, 128)])
+def test_attend_of_a_few_long_sequences(ctx, units, M, H):
+    attend_case(ctx, [7001, 3100, 9, 5000][:units], M, H)
+
+
 @pytest.mark.parametrize("units", [60, 200, 600])  # each is found in another way
 @pytest.mark.parametrize("kind", ["all", "window", "listed"])
 def test_attend_of_many_sequences_in_a_wide_table(ctx, units, kind):
@@ -291,6 +297,42 @@ def test_read_writes_its_rows_alone(ctx):
                             out=[x[:2 * 13 * w].view(2, 13, w) for x, w in zip(buf, (512, 64))])
     ctx.synchronize()
     assert all((x[-64:] == 7.0).all() for x in buf)
+
+
+def test_read_of_more_than_the_caches_hold(ctx):
+    """Rows that go past the L2s: the bits that they have a few at a time."""
+    pool = R8.Pool8(41, [4300, 17, 4100, 2500], 64, 512, 64)
+    cache, table, lens = pool.cuda(ctx=ctx), pool.table.cuda(), pool.lens32().cuda()
+    for t in (torch.float32, torch.bfloat16):
+        rows = 4200 if t == torch.float32 else 8400
+        assert 4 * rows * 576 * t.itemsize > 2**25
+        got = torch.cat(cache.read(table, lens, rows, dtype=t), -1)
+        for at in range(0, rows, 1400):
+            few = cache.read(table, lens, 1400, starts=torch.full((4,), at, dtype=torch.int32, device="cuda"), dtype=t)
+            ctx.synchronize()
+            assert torch.equal(got[:, at:at + 1400], torch.cat(few, -1))
+        assert torch.equal(got[1, :17].cpu(), pool.rows(1, torch.arange(17)).float().to(t))
+
+
+def test_positions_far_into_a_pool(ctx):
+    """Pages beyond 2^32 bytes: the bits that the same rows have in a small pool."""
+    import undertow_amd as U
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rnd = lambda *d: torch.randn(d, device="cuda", generator=g)
+    n, page, far = 700, 64, 2**33 // (64 * 576) + 30
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    new, q = (rnd(1, n, 512), rnd(1, n, 64)), (rnd(1, 2, 32, 512).bfloat16(), rnd(1, 2, 32, 64).bfloat16())
+    sel = torch.tensor([[[0, 9, 3], [10, 2, 1]]], dtype=torch.int32, device="cuda")
+    got = []
+    for pages, first in ((30, 0), (far, far - 30)):
+        cache = U.PagedCache.empty(ctx, pages, page, fmt=U.KV_I8)
+        table = (first + 29 - torch.arange(11, dtype=torch.int32, device="cuda"))[None].contiguous()
+        cache.append(table, lens, *new)
+        got.append((*cache.read(table, lens, n), cache.attend(table, lens, *q, SCALE), cache.attend_pages(table, lens, *q, SCALE, sel),
+                    cache.attend_window(table, lens, *q, SCALE, 100, 5), cache.mean[table[0].long()], cache.mean_scale[table[0].long()]))
+        ctx.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert torch.equal(got[0][0][0].cpu(), R8.values8(*R8.quantised(torch.cat(new, -1)[0].cpu(), 512), 512)[:, :512].float())
 
 
 # ------------------------------------------------- errors, streams, runs
