@@ -31,7 +31,7 @@
 // a higher priority for the one that is past its scores.  What bounds it now, with
 // tiles of 32 positions:
 // - 128 heads: instructions.  A tile takes 2.4 us a CU where its data come from L2
-//   (512 prompt rows over 8192 positions 1215 us, 0.93 PFLOP/s; without the priority
+//   (512 prompt rows over 8192 positions 1192 us, 0.95 PFLOP/s; without the priority
 //   1327; bf16 pages, which need no conversion, 1030), 2.6 to 2.9 with the traffic
 //   of decoding: 64 sequences of up to 8192 119 us (bf16 115).
 // - 16 heads: memory, 1.03 us a tile and CU (4.7 TB/s), once it runs: 37 sequences
@@ -72,9 +72,10 @@ __device__ __forceinline__ int lane_anew() {
     asm volatile("" : "+v"(l));
     return l;
 }
-// The rotary codes of row r, 64 bytes: chunks of 16 XORed with this, so that 16
-// rows' chunks meet the LDS's 16 slots once.
-__device__ __forceinline__ int rope_swz(int row) { return (row >> 2) & 3; }
+// The rotary codes of row r, 64 bytes: chunks of 16 XORed with 0, 2, 3 and 1 for the
+// rows 0 to 3, .. 12 to 15, so that the 16 lanes that a read takes at a time (0 to 3
+// with 12 to 15 and 20 to 27, the others likewise) meet the LDS's 16 slots once.
+__device__ __forceinline__ int rope_swz(int row) { return (0x78 >> ((row >> 1) & 6)) & 3; }
 
 // Part [I0, I1) of the words, bf16, to digits; what a digit is worth.
 template <int I0, int I1> __device__ __forceinline__ float query_digits(pu32x4 (&w)[18]) {
@@ -136,23 +137,25 @@ template <int I0, int I1> __device__ __forceinline__ float query_digits(pu32x4 (
 
 // A tile's latent codes (LDS address T) to f16 values (V), in blocks of 8 rows
 // and 64 values that the transposing reads take; wave w: row block w.  A lane
-// takes a row's 16 codes in two halves; which one first depends on its row and
-// column, so that neither the reads nor the writes of a turn meet in a slot.
+// takes 16 codes of a row, which become two of a block's eight chunks of a row:
+// those of odd blocks are XORed with one more, so that the eight lanes of a row
+// write to different slots (1192 us for 512 prompt rows over 8192 positions; with
+// reads of 8 codes, in halves by turns, that met in slots, 1230).
 //   f16(code) = (1024 + (code + 128)) - 1152, each step exact.
 __device__ __forceinline__ void convert_tile(uint32_t T, uint32_t V, int w) {
     const pf16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    const int l = lane_anew(), row = l >> 3, in = (l & 7) ^ row, half = ((in >> 2) ^ (row >> 1)) & 1;
-    const uint32_t src = T + w * kCBlocks * 1024 + l * 16 + half * 8;
-    const uint32_t dst = V + (w * 8 + (in >> 2)) * 1024 + row * 128 + (((2 * (in & 3) + half) ^ row) << 4);
-    pu32x2 c[8];
+    const int l = lane_anew(), row = l >> 3, in = (l & 7) ^ row;
+    const uint32_t src = T + w * kCBlocks * 1024 + l * 16;
+    const uint32_t dst = V + (w * 8 + (in >> 2)) * 1024 + row * 128 + (((2 * (in & 3)) ^ (in >> 2) ^ row) << 4);
+    pu32x4 c[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) c[i] = lds_read<pu32x2>((src ^ (i & 1 ? 8 : 0)) + (i >> 1) * 1024);
+    for (int i = 0; i < 4; i++) c[i] = lds_read<pu32x4>(src + i * 1024);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         pu32x4 v;
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            v[k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(pf16x2, __builtin_amdgcn_perm(0x64646464u, c[i][k >> 1] ^ 0x80808080u,
+            v[k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(pf16x2, __builtin_amdgcn_perm(0x64646464u, c[i >> 1][2 * (i & 1) + (k >> 1)] ^ 0x80808080u,
                                                                                                 k & 1 ? 0x04030402u : 0x04010400u)) + off);
         *(__attribute__((address_space(3))) pu32x4 *)((dst ^ (i & 1 ? 16 : 0)) + (i >> 1) * 2 * 1024) = v;
     }
@@ -267,7 +270,7 @@ __device__ __forceinline__ void tile_context(CodesWave &w, const pf16x8 &p, uint
     const uint32_t at = V + (r >> 3) * 8 * 1024 + (r & 7) * 128 + ((((j & 3) >> 1) ^ tile_swz(r)) << 4) + 8 * (j & 1);
     pu32x4 v[32];
     auto read = [&](int i) {
-        const uint32_t b = (at ^ ((i & 3) << 5)) + (i >> 2) * 1024;
+        const uint32_t b = (at ^ ((i & 3) << 5) ^ ((i & 4) << 2)) + (i >> 2) * 1024;
         v[i] = tr_read(b, b + 16 * 1024);
     };
 #pragma unroll
