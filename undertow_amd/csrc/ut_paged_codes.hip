@@ -30,12 +30,12 @@
 // Hence two workgroups a CU, four waves each, that know nothing of one another, and
 // a higher priority for the one that is past its scores.  What bounds it now, with
 // tiles of 32 positions:
-// - 128 heads: instructions.  A tile takes 2.4 us a CU where its data come from L2
+// - 128 heads: instructions.  A tile takes 2.35 us a CU where its data come from L2
 //   (512 prompt rows over 8192 positions 1192 us, 0.95 PFLOP/s; without the priority
-//   1327; bf16 pages, which need no conversion, 1030), 2.6 to 2.9 with the traffic
-//   of decoding: 64 sequences of up to 8192 119 us (bf16 115).
+//   1327; bf16 pages, which need no conversion, 1030), 2.6 to 2.8 with the traffic
+//   of decoding: 64 sequences of up to 8192 117 us (bf16 117).
 // - 16 heads: memory, 1.03 us a tile and CU (4.7 TB/s), once it runs: 37 sequences
-//   of up to 12001 50 us in all (132 MB), of which its start, the ranges' ends and
+//   of up to 12001 48 us in all (132 MB), of which its start, the ranges' ends and
 //   the join are half.
 // - few rows: latency.  A call over one tile takes 9.7 us, 1.7 of them that tile's,
 //   over four 15.5.
