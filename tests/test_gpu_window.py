@@ -166,3 +166,30 @@ def test_a_captured_window_slides(ctx):
             first, want = got.clone(), call()
             c.synchronize()
             assert torch.equal(first, want)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("H", [16, 50, 128])
+@pytest.mark.parametrize("window", [None, 60])
+def test_prompt_rows_end_where_each_does(ctx, fmt, H, window):
+    """Rows of a prompt before a value that is not finite have the bits that
+    they have without it, and are right; rows from it on are not finite."""
+    lens, M = [390, 70, 300], 300
+    pool = R8.pool(fmt, 43, lens, 64, 512, 64, 128)
+    qabs, qrope = pool.queries(M, H)
+    args = pool.table.cuda(), pool.lens32().cuda(), qabs.cuda(), qrope.cuda(), SCALE
+
+    def run():
+        cache = pool.cuda(ctx=ctx)
+        got = cache.attend(*args) if window is None else cache.attend_window(*args, window, 3)
+        ctx.synchronize()
+        return got
+
+    good = run()
+    R8.check(pool, fmt, good, qabs, qrope, SCALE, window=window, sinks=3 if window else 0)
+    for b, n in enumerate(lens):
+        at = pool.where(b, torch.tensor([n - 33]))
+        (pool.scales if fmt == "i8" else pool.pages)[at] = math.nan
+    bad = run()
+    assert torch.equal(bad[:, :M - 33], good[:, :M - 33])
+    assert bad[:, M - 33:].isnan().any(-1).all()

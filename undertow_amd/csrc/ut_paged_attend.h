@@ -33,6 +33,7 @@ struct PagedMfmaArgs {
     int32_t most;     // ranges at most
     float spread;     // plan_ranges'
     int32_t whole;    // a range is a unit (most: units), and there is no join
+    int32_t alone;    // no workgroup shares its tiles' count with another: each ends at the last one that its rows see
     void *part_o;     // [slot][group][128 quads][16 columns][4], f32 or (8-bit pages) f16
     float *part_ml;   // [slot][group][16 columns][2]; with f16 [4], the third what part_o is to be taken times
     int64_t *plan;    // [units] first tile of each, then W (where there is more than one range)
@@ -306,13 +307,14 @@ constexpr int wait_vm(int n) { return 0x0f70 | n; }
 
 // The part of a range that lies in one unit.
 struct Seg {
-    int32_t u, j, h0, b0, b1, tiles, len, n;
+    int32_t u, j, h0, b0, b1, tiles, n;
+    int32_t base, len, rows;  // row j sees the positions before base + j; the workgroup's rows end at len, so many
     int64_t first, row;
     Lookup lk;
 };
 // Goes over a range's parts.
 template <int KIND> struct Walk {
-    int32_t u;
+    int32_t u, j0, j1;  // j0 .. j1: the workgroup's rows
     int64_t first, at;
     __device__ __forceinline__ bool next(const PagedMfmaArgs &p, const Range &rg, int gr, Seg &q) {
         const PagedArgs &a = p.a;
@@ -327,8 +329,10 @@ template <int KIND> struct Walk {
         q.j = SPARSE ? u - b * a.M : gr / per_row;
         q.h0 = (SPARSE ? gr : gr % per_row) * kCols;
         q.tiles = tiles;
-        q.len = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-        q.n = q.len - a.M + q.j + 1;
+        q.base = __builtin_amdgcn_readfirstlane(paged_len(a, b)) - a.M + 1;
+        q.n = q.base + q.j;
+        q.len = q.base + j1 > 1 ? q.base + j1 : 1;  // (rows that see nothing go over one tile)
+        q.rows = j1 - j0 + 1;
         q.first = first;
         q.row = ((int64_t)b * a.M + q.j) * a.H;
         q.lk.table = (const_i32 *)(a.table + (int64_t)b * a.stride);
@@ -339,14 +343,31 @@ template <int KIND> struct Walk {
         if (KIND == kNear) {
             q.lk.window = a.window;
             q.lk.sinks = a.sinks;
-            q.lk.cut = near_cut(a, q.len);
+            q.lk.cut = near_cut(q.len, q.rows, a.window, a.sinks, kPT);
         }
+        if (KIND != kListed && p.alone) q.tiles = q.b1 = (q.len - 1) / kPT + 1 - (KIND == kNear ? q.lk.cut.skip : 0);
         first += tiles + p.lead;
         at = first;
         u++;
         return true;
     }
 };
+
+// Which range and which of its workgroups this one is.  Neighbours are on one XCD;
+// rows of very different ends (prompts) go from the last one to the first, over all
+// XCDs.
+__device__ __forceinline__ void place(const PagedMfmaArgs &p, int &id, int &r, int &chunk) {
+    const bool spread = p.alone && p.a.M > kPT;
+    id = spread ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    r = id / p.chunks;
+    chunk = id - r * p.chunks;
+    if (spread) chunk = p.chunks - 1 - chunk;
+}
+template <int KIND> __device__ __forceinline__ Walk<KIND> walk_of(const PagedMfmaArgs &p, const Range &rg, int chunk) {
+    const int per_row = (p.a.H + kCols - 1) / kCols, g0 = chunk * p.per, g1 = g0 + p.per < p.groups ? g0 + p.per : p.groups;
+    const bool own = KIND != kListed && p.alone;
+    return {rg.u, own ? g0 / per_row : 0, own ? (g1 - 1) / per_row : p.a.M - 1, rg.first, rg.s};
+}
 
 // The kernel of 8-bit pages (ut_paged_codes.hip), `wgs` workgroups.
 struct CodesI8 {

@@ -31,8 +31,8 @@
 // a higher priority for the one that is past its scores.  What bounds it now, with
 // tiles of 32 positions:
 // - 128 heads: instructions.  A tile takes 2.35 us a CU where its data come from L2
-//   (512 prompt rows over 8192 positions 1192 us, 0.95 PFLOP/s; without the priority
-//   1327; bf16 pages, which need no conversion, 1030), 2.6 to 2.8 with the traffic
+//   (512 prompt rows over 8192 positions 1177 us, 0.96 PFLOP/s; without the priority
+//   8 % more; bf16 pages, which need no conversion, 984), 2.6 to 2.8 with the traffic
 //   of decoding: 64 sequences of up to 8192 117 us (bf16 117).
 // - 16 heads: memory, 1.03 us a tile and CU (4.7 TB/s), once it runs: 37 sequences
 //   of up to 12001 48 us in all (132 MB), of which its start, the ranges' ends and
@@ -366,9 +366,8 @@ template <int KIND> __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4
     __shared__ __attribute__((aligned(1024))) uint8_t stage[kCLds];
     const PagedArgs &a = p.a;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int share = gridDim.x >> 3;
-    const int id = (blockIdx.x & 7) * share + (blockIdx.x >> 3);  // neighbours on one XCD
-    const int r = id / p.chunks, chunk = id - r * p.chunks;
+    int id, r, chunk;
+    place(p, id, r, chunk);
     // units without positions: zeros
     const int64_t vec = (int64_t)(SPARSE ? 1 : a.M) * a.H * kPL * 2 / 16;
     for (int u = id; u < p.units; u += gridDim.x)
@@ -401,7 +400,7 @@ template <int KIND> __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4
         }
         entry = entry_of(q, q.b0 + kCStages);
     };
-    Walk<KIND> walk = {rg.u, rg.first, rg.s};
+    Walk<KIND> walk = walk_of<KIND>(p, rg, chunk);
     Seg q;
     if (!walk.next(p, rg, gr, q)) return;
     bool begun = false;

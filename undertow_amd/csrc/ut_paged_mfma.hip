@@ -338,9 +338,8 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
     __shared__ int s_odd;
     const PagedArgs &a = p.a;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, col = l & 15;
-    const int share = gridDim.x >> 3;
-    const int id = (blockIdx.x & 7) * share + (blockIdx.x >> 3);  // neighbours on one XCD
-    const int r = id / p.chunks, chunk = id - r * p.chunks;
+    int id, r, chunk;
+    place(p, id, r, chunk);
     // units without positions: zeros
     const int64_t vec = (int64_t)(SPARSE ? 1 : a.M) * a.H * kPL * (int)sizeof(typename F::out_t) / 16;
     for (int u = id; u < p.units; u += gridDim.x)
@@ -391,7 +390,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
         }
         entry = entry_of(q, q.b0 + STAGES - 1);
     };
-    Walk<KIND> walk = {rg.u, rg.first, rg.s};
+    Walk<KIND> walk = walk_of<KIND>(p, rg, chunk);
     Seg q;
     if (!walk.next(p, rg, gr, q)) return;
     bool begun = false;
@@ -429,7 +428,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
             }
             // what some row of the unit sees, and what every one does
             const uint32_t most = SPARSE ? seen : some_see<KIND>(q.lk, x, q.len);
-            const uint32_t least = SPARSE ? seen : all_see<KIND>(q.lk, x, q.len, a.M);
+            const uint32_t least = SPARSE ? seen : all_see<KIND>(q.lk, x, q.len, q.rows);
             bool odd = false;
             if (least != ~0u) {
                 // a value that is not finite where only later rows look: those
@@ -448,7 +447,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
             uint32_t now = most;
             int turn = 0;  // a wave
             if (KIND == kNear && odd) {
-                tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), q.len - a.M + row_of(0) + 1));
+                tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), q.base + row_of(0)));
                 __syncthreads();
             }
             do {
@@ -473,7 +472,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
                     fifth();
                     __builtin_amdgcn_s_waitcnt(wait_vm(0));
                     __syncthreads();
-                    tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), q.len - a.M + row_of(turn) + 1));
+                    tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), q.base + row_of(turn)));
                     __syncthreads();
                     continue;
                 }
@@ -646,6 +645,7 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
     p.per = plan.per;
     p.chunks = plan.chunks;
     p.spread = plan.spread;
+    p.alone = plan.slots == 0;
     auto launch = [&]() -> int32_t {
         const unsigned wgs = (unsigned)(((int64_t)p.most * p.chunks + 7) / 8 * 8);
         int tok = timing_begin(ctx, F::kCodes ? "paged_codes" : "paged_mfma");

@@ -140,12 +140,12 @@ inline void plan_heads(PlanCall &p, const PlanCosts &c, int32_t cus, int32_t gro
 //
 // Where a unit's column groups alone fill the CUs (prompt rows), there is one
 // range: its workgroups each go through all units, in rounds over the CUs,
-// leave no parts and need no join.  They have the same tiles each, where whole
-// units of differing lengths leave CUs idle, so these have to be fewer by a
-// tenth.  4 x 256 rows of 128 heads over up to 4096 positions (equal counts) take
-// 1034 us whole and 741 as one range with lengths spread evenly, 1055 and 1048
-// with equal ones; 3 x 777 over up to 1900 (whole 0.86 of the range) 1249 and 1368,
-// 1341 and 1781; in f16 pairs (0.92) 5.35 ms and 4.63, 5.33 and 5.93.
+// leave no parts and need no join.  Their tiles differ only by their rows' place
+// in a unit, where whole units of differing lengths may leave CUs idle, so these
+// have to be fewer by a tenth.  Of 128 heads, whole and as one range: 4 x 256 rows
+// over up to 4096 positions 705 and 711 us, 3 x 777 over up to 1900 710 and 735 (in
+// f16 pairs 2131 and 2220, in 8 bits 805 and 832), 5 x 300 over up to 300 177 and
+// 201, 2 x 512 over up to 1024 212 and 207.
 template <class Costs>
 PlanCall plan_call(const Costs &c, int32_t cus, int32_t units, int32_t groups, int64_t each, int64_t listed,
                    bool lists) {
