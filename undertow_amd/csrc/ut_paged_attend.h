@@ -4,6 +4,8 @@
 // up, and copies straight to LDS.
 #pragma once
 
+#include <type_traits>
+
 #include "ut_paged.h"
 
 namespace ut {
@@ -33,7 +35,6 @@ struct PagedMfmaArgs {
     int32_t most;     // ranges at most
     float spread;     // plan_ranges'
     int32_t whole;    // a range is a unit (most: units), and there is no join
-    int32_t alone;    // no workgroup shares its tiles' count with another: each ends at the last one that its rows see
     void *part_o;     // [slot][group][128 quads][16 columns][4], f32 or (8-bit pages) f16
     float *part_ml;   // [slot][group][16 columns][2]; with f16 [4], the third what part_o is to be taken times
     int64_t *plan;    // [units] first tile of each, then W (where there is more than one range)
@@ -312,10 +313,13 @@ struct Seg {
     int64_t first, row;
     Lookup lk;
 };
-// Goes over a range's parts.
-template <int KIND> struct Walk {
-    int32_t u, j0, j1;  // j0 .. j1: the workgroup's rows
+// Goes over a range's parts.  OWN (prompts, where there are no parts to join): the
+// tiles of a unit are those that the workgroup's rows j0 .. j1 see, from the first
+// to the last.
+template <int KIND, bool OWN> struct Walk {
+    int32_t u;
     int64_t first, at;
+    int32_t j0, j1;
     __device__ __forceinline__ bool next(const PagedMfmaArgs &p, const Range &rg, int gr, Seg &q) {
         const PagedArgs &a = p.a;
         int32_t tiles = 0;
@@ -329,10 +333,14 @@ template <int KIND> struct Walk {
         q.j = SPARSE ? u - b * a.M : gr / per_row;
         q.h0 = (SPARSE ? gr : gr % per_row) * kCols;
         q.tiles = tiles;
-        q.base = __builtin_amdgcn_readfirstlane(paged_len(a, b)) - a.M + 1;
-        q.n = q.base + q.j;
-        q.len = q.base + j1 > 1 ? q.base + j1 : 1;  // (rows that see nothing go over one tile)
-        q.rows = j1 - j0 + 1;
+        q.len = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+        q.base = q.len - a.M + 1;
+        q.rows = a.M;
+        q.n = q.len - a.M + q.j + 1;
+        if (OWN) {
+            q.len = q.base + j1 > 1 ? q.base + j1 : 1;  // (rows that see nothing go over one tile)
+            q.rows = j1 - j0 + 1;
+        }
         q.first = first;
         q.row = ((int64_t)b * a.M + q.j) * a.H;
         q.lk.table = (const_i32 *)(a.table + (int64_t)b * a.stride);
@@ -345,7 +353,7 @@ template <int KIND> struct Walk {
             q.lk.sinks = a.sinks;
             q.lk.cut = near_cut(q.len, q.rows, a.window, a.sinks, kPT);
         }
-        if (KIND != kListed && p.alone) q.tiles = q.b1 = (q.len - 1) / kPT + 1 - (KIND == kNear ? q.lk.cut.skip : 0);
+        if (OWN) q.tiles = q.b1 = (q.len - 1) / kPT + 1 - (KIND == kNear ? q.lk.cut.skip : 0);
         first += tiles + p.lead;
         at = first;
         u++;
@@ -354,19 +362,26 @@ template <int KIND> struct Walk {
 };
 
 // Which range and which of its workgroups this one is.  Neighbours are on one XCD;
-// rows of very different ends (prompts) go from the last one to the first, over all
-// XCDs.
-__device__ __forceinline__ void place(const PagedMfmaArgs &p, int &id, int &r, int &chunk) {
-    const bool spread = p.alone && p.a.M > kPT;
-    id = spread ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    r = id / p.chunks;
-    chunk = id - r * p.chunks;
-    if (spread) chunk = p.chunks - 1 - chunk;
+// prompts' rows, whose ends differ, go from the last one to the first, over all XCDs.
+template <bool OWN> __device__ __forceinline__ int place(int chunks, int &r, int &chunk) {
+    const int id = OWN ? blockIdx.x : (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    r = id / chunks;
+    chunk = id - r * chunks;
+    if (OWN) chunk = chunks - 1 - chunk;
+    return id;
 }
-template <int KIND> __device__ __forceinline__ Walk<KIND> walk_of(const PagedMfmaArgs &p, const Range &rg, int chunk) {
+template <int KIND, bool OWN> __device__ __forceinline__ Walk<KIND, OWN> walk_of(const PagedMfmaArgs &p, const Range &rg, int chunk) {
+    if (!OWN) return {rg.u, rg.first, rg.s, 0, 0};
     const int per_row = (p.a.H + kCols - 1) / kCols, g0 = chunk * p.per, g1 = g0 + p.per < p.groups ? g0 + p.per : p.groups;
-    const bool own = KIND != kListed && p.alone;
-    return {rg.u, own ? g0 / per_row : 0, own ? (g1 - 1) / per_row : p.a.M - 1, rg.first, rg.s};
+    return {rg.u, rg.first, rg.s, g0 / per_row, (g1 - 1) / per_row};
+}
+// A call's kernel: f(KIND, OWN).
+template <class F> void with_kind(int kind, bool own, F &&f) {
+    typedef std::integral_constant<bool, true> yes;
+    typedef std::integral_constant<bool, false> no;
+    if (kind == kListed) f(std::integral_constant<int, kListed>(), no());
+    else if (kind == kAll) own ? f(std::integral_constant<int, kAll>(), yes()) : f(std::integral_constant<int, kAll>(), no());
+    else own ? f(std::integral_constant<int, kNear>(), yes()) : f(std::integral_constant<int, kNear>(), no());
 }
 
 // The kernel of 8-bit pages (ut_paged_codes.hip), `wgs` workgroups.
@@ -376,6 +391,6 @@ struct CodesI8 {
     typedef __bf16 out_t;
     typedef _Float16 part_t;
 };
-void launch_codes(ut_ctx *ctx, const PagedMfmaArgs &p, int kind, unsigned wgs);
+void launch_codes(ut_ctx *ctx, const PagedMfmaArgs &p, int kind, bool own, unsigned wgs);
 
 }  // namespace ut

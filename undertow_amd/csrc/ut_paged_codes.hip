@@ -361,13 +361,14 @@ __device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, 
 // As k_paged_mfma: a workgroup's waves have a column group each, over the same
 // tiles.  While a tile is worked on the next one is on its way; the one after it
 // takes its place as soon as its scores and values are made.
-template <int KIND> __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4) void k_paged_codes(PagedMfmaArgs p) {
+template <int KIND, bool OWN>
+__global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4) void k_paged_codes(PagedMfmaArgs p) {
     constexpr bool SPARSE = KIND == kListed;
     __shared__ __attribute__((aligned(1024))) uint8_t stage[kCLds];
     const PagedArgs &a = p.a;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int id, r, chunk;
-    place(p, id, r, chunk);
+    int r, chunk;
+    const int id = place<OWN>(p.chunks, r, chunk);
     // units without positions: zeros
     const int64_t vec = (int64_t)(SPARSE ? 1 : a.M) * a.H * kPL * 2 / 16;
     for (int u = id; u < p.units; u += gridDim.x)
@@ -400,7 +401,7 @@ template <int KIND> __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4
         }
         entry = entry_of(q, q.b0 + kCStages);
     };
-    Walk<KIND> walk = walk_of<KIND>(p, rg, chunk);
+    Walk<KIND, OWN> walk = walk_of<KIND, OWN>(p, rg, chunk);
     Seg q;
     if (!walk.next(p, rg, gr, q)) return;
     bool begun = false;
@@ -446,9 +447,10 @@ template <int KIND> __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4
     if (bad && (threadIdx.x & 63) == 0) *a.err = 1;
 }
 
-void launch_codes(ut_ctx *ctx, const PagedMfmaArgs &p, int kind, unsigned wgs) {
-    hipLaunchKernelGGL((kind == kAll ? k_paged_codes<kAll> : kind == kListed ? k_paged_codes<kListed> : k_paged_codes<kNear>),
-                       dim3(wgs), dim3(kCW * 64), 0, ctx->stream, p);
+void launch_codes(ut_ctx *ctx, const PagedMfmaArgs &p, int kind, bool own, unsigned wgs) {
+    with_kind(kind, own, [&](auto k, auto o) {
+        hipLaunchKernelGGL((k_paged_codes<decltype(k)::value, decltype(o)::value>), dim3(wgs), dim3(kCW * 64), 0, ctx->stream, p);
+    });
 }
 
 }  // namespace ut

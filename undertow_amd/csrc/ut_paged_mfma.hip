@@ -330,7 +330,7 @@ template <class F> __device__ __forceinline__ bool tile_odd(uint8_t *T, uint32_t
 // the same tiles.  Four (f16x2: two) tiles fit the LDS: the products of one
 // run while the next three (one) are on their way.  A table entry is read a
 // tile before its copy, and the copies issue between the products.
-template <class F, int KIND>
+template <class F, int KIND, bool OWN>
 __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(PagedMfmaArgs p) {
     constexpr bool SPARSE = KIND == kListed;
     constexpr int NW = F::kWaves, PL = F::kPlanes, STAGES = 4 / PL, ROW = kPD * 2 * PL, TILE = 36 * PL * 1024;
@@ -338,8 +338,8 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
     __shared__ int s_odd;
     const PagedArgs &a = p.a;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, col = l & 15;
-    int id, r, chunk;
-    place(p, id, r, chunk);
+    int r, chunk;
+    const int id = place<OWN>(p.chunks, r, chunk);
     // units without positions: zeros
     const int64_t vec = (int64_t)(SPARSE ? 1 : a.M) * a.H * kPL * (int)sizeof(typename F::out_t) / 16;
     for (int u = id; u < p.units; u += gridDim.x)
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
         }
         entry = entry_of(q, q.b0 + STAGES - 1);
     };
-    Walk<KIND> walk = walk_of<KIND>(p, rg, chunk);
+    Walk<KIND, OWN> walk = walk_of<KIND, OWN>(p, rg, chunk);
     Seg q;
     if (!walk.next(p, rg, gr, q)) return;
     bool begun = false;
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
             }
             // what some row of the unit sees, and what every one does
             const uint32_t most = SPARSE ? seen : some_see<KIND>(q.lk, x, q.len);
-            const uint32_t least = SPARSE ? seen : all_see<KIND>(q.lk, x, q.len, q.rows);
+            const uint32_t least = SPARSE ? seen : all_see<KIND>(q.lk, x, q.len, OWN ? q.rows : a.M);
             bool odd = false;
             if (least != ~0u) {
                 // a value that is not finite where only later rows look: those
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
             uint32_t now = most;
             int turn = 0;  // a wave
             if (KIND == kNear && odd) {
-                tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), q.base + row_of(0)));
+                tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), (OWN ? q.base : q.len - a.M + 1) + row_of(0)));
                 __syncthreads();
             }
             do {
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
                     fifth();
                     __builtin_amdgcn_s_waitcnt(wait_vm(0));
                     __syncthreads();
-                    tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), q.base + row_of(turn)));
+                    tile_clear<F>(T, ~visible<KIND>(q.lk, tile_at<KIND>(q.lk, x), (OWN ? q.base : q.len - a.M + 1) + row_of(turn)));
                     __syncthreads();
                     continue;
                 }
@@ -645,12 +645,16 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
     p.per = plan.per;
     p.chunks = plan.chunks;
     p.spread = plan.spread;
-    p.alone = plan.slots == 0;
+    // prompts: no parts, and rows whose ends lie more than a tile apart
+    const bool own = plan.slots == 0 && a.M > kPT;
     auto launch = [&]() -> int32_t {
         const unsigned wgs = (unsigned)(((int64_t)p.most * p.chunks + 7) / 8 * 8);
         int tok = timing_begin(ctx, F::kCodes ? "paged_codes" : "paged_mfma");
-        if constexpr (F::kCodes) launch_codes(ctx, p, KIND, wgs);
-        else hipLaunchKernelGGL((k_paged_mfma<F, KIND>), dim3(wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
+        if constexpr (F::kCodes) launch_codes(ctx, p, KIND, own, wgs);
+        else if (KIND != kListed && own)
+            hipLaunchKernelGGL((k_paged_mfma<F, KIND, KIND != kListed>), dim3(wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
+        else
+            hipLaunchKernelGGL((k_paged_mfma<F, KIND, false>), dim3(wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
         timing_end(ctx, tok);
         return launch_check(ctx, F::kCodes ? "k_paged_codes" : "k_paged_mfma");
     };
