@@ -296,8 +296,12 @@ template <int COPIES> __device__ __forceinline__ void meet() {
 }
 
 // A column group's queries (under(): what is to start behind their loads), and
-// nothing summed up yet.
-template <class B> __device__ __forceinline__ void load_queries(const PagedArgs &a, const Seg &q, CodesWave &w, B &&under) {
+// nothing summed up yet; only under() for a wave without one.
+template <class B> __device__ __forceinline__ void load_queries(const PagedArgs &a, const Seg &q, bool active, CodesWave &w, B &&under) {
+    if (!active) {
+        under();
+        return;
+    }
     const int l = lane_anew(), h = q.h0 + (l & 15), g = l >> 4;
     const int64_t row = q.row + (h < a.H ? h : a.H - 1);
     const __bf16 *qa = (const __bf16 *)a.qabs + row * kPL, *qr = (const __bf16 *)a.qrope + row * (kPD - kPL);
@@ -406,7 +410,7 @@ __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4) void k_paged_codes
     if (!walk.next(p, rg, gr, q)) return;
     bool begun = false;
     while (true) {
-        load_queries(a, q, wv, [&]() {
+        load_queries(a, q, active, wv, [&]() {
             if (!begun) start(q);
             begun = true;
         });
