@@ -330,7 +330,10 @@ template <class F> __device__ __forceinline__ bool tile_odd(uint8_t *T, uint32_t
 // the same tiles.  Four (f16x2: two) tiles fit the LDS: the products of one
 // run while the next three (one) are on their way.  A table entry is read a
 // tile before its copy, and the copies issue between the products.
-template <class F, int KIND, bool OWN>
+// FEW: some waves have no heads, and load no queries (one row over 509 positions
+// 16.5 us where all load some, 14.5 so; with the branch where all have heads, 64
+// sequences of up to 8192 positions 130 us instead of 126).
+template <class F, int KIND, bool OWN, bool FEW>
 __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(PagedMfmaArgs p) {
     constexpr bool SPARSE = KIND == kListed;
     constexpr int NW = F::kWaves, PL = F::kPlanes, STAGES = 4 / PL, ROW = kPD * 2 * PL, TILE = 36 * PL * 1024;
@@ -396,14 +399,17 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
     bool begun = false;
     while (true) {
         const int64_t row = q.row + (q.h0 + col < a.H ? q.h0 + col : a.H - 1);
-        const float c = a.scale * kLog2e * F::load(wv.q, a.qabs, a.qrope, row, g);
+        float c = 0.0f;
+        if (!FEW || active) c = a.scale * kLog2e * F::load(wv.q, a.qabs, a.qrope, row, g);
         if (!begun) start(q);
         begun = true;
-        F::arrive(wv.q);
-        wv.m = kLow;
-        wv.l = 0.0f;
+        if (!FEW || active) {
+            F::arrive(wv.q);
+            wv.m = kLow;
+            wv.l = 0.0f;
 #pragma unroll
-        for (int mt = 0; mt < 32; mt++) wv.o[mt] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int mt = 0; mt < 32; mt++) wv.o[mt] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
         uint32_t seen = visible<KIND>(q.lk, tile_at<KIND>(q.lk, q.b0), q.n);
         for (int32_t x = q.b0; x < q.b1; x++) {
             const uint32_t ps = (uint32_t)(x - q.b0) % STAGES * TILE;
@@ -652,9 +658,11 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
         int tok = timing_begin(ctx, F::kCodes ? "paged_codes" : "paged_mfma");
         if constexpr (F::kCodes) launch_codes(ctx, p, KIND, own, wgs);
         else if (KIND != kListed && own)
-            hipLaunchKernelGGL((k_paged_mfma<F, KIND, KIND != kListed>), dim3(wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
+            hipLaunchKernelGGL((k_paged_mfma<F, KIND, KIND != kListed, false>), dim3(wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
+        else if (p.per < F::kCosts.waves)
+            hipLaunchKernelGGL((k_paged_mfma<F, KIND, false, true>), dim3(wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
         else
-            hipLaunchKernelGGL((k_paged_mfma<F, KIND, false>), dim3(wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
+            hipLaunchKernelGGL((k_paged_mfma<F, KIND, false, false>), dim3(wgs), dim3(F::kWaves * 64), 0, ctx->stream, p);
         timing_end(ctx, tok);
         return launch_check(ctx, F::kCodes ? "k_paged_codes" : "k_paged_mfma");
     };
