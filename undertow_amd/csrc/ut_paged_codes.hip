@@ -33,12 +33,13 @@
 // - 128 heads: instructions.  A tile takes 2.35 us a CU where its data come from L2
 //   (512 prompt rows over 8192 positions 1177 us, 0.96 PFLOP/s; without the priority
 //   8 % more; bf16 pages, which need no conversion, 984), 2.6 to 2.8 with the traffic
-//   of decoding: 64 sequences of up to 8192 117 us (bf16 117).
+//   of decoding: 64 sequences of up to 8192 113 to 117 us, as bf16.
 // - 16 heads: memory, 1.03 us a tile and CU (4.7 TB/s), once it runs: 37 sequences
-//   of up to 12001 48 us in all (132 MB), of which its start, the ranges' ends and
-//   the join are half.
-// - few rows: latency.  A call over one tile takes 9.7 us, 1.7 of them that tile's,
-//   over four 15.5.
+//   of up to 12001 46 us in all (132 MB), of which its start, the ranges' ends and
+//   the join take 18.
+// - few rows: latency.  Of a call over one tile, 9.7 us, the lengths and the range
+//   take 0.8, the walk's values 0.5, the queries' issue 0.8 and their digits 1.1,
+//   the tile 1.9, the end 1.5.
 #include "ut_paged_attend.h"
 
 namespace ut {
