@@ -1,0 +1,105 @@
+"""Attention over 8-bit pages whose positions differ in size by more than f32's
+range holds, or have the smallest and largest sizes, against 64 bits.
+
+Tolerances stand at paged8_ref.close; everything is taken times 2^-size, size
+the largest of the sequence's positions, so that they are relative to it."""
+import pytest
+import torch
+
+import paged8_ref as R8
+import paged_ref as R
+from test_gpu_paged import SCALE
+
+pytestmark = pytest.mark.gpu
+WIDTHS = [(128, 512, 64), (16, 512, 64), (4, 64, 16)]
+ZERO = None  # a position whose latent values are zeros
+
+
+def sized(seed, runs, scale, H, L, P):
+    """A pool of sequences whose latent values have sizes runs[b] = [(positions,
+    log2 of their size), ..], and queries.  Head 0's are zeros, so that all its
+    weights are equal; latent queries meet the largest values at size 1, those
+    beyond 2^100 are zeros (a query's own range)."""
+    runs = [[(n * scale, s) for n, s in run] for run in runs]
+    pool = R8.Pool8(seed, [sum(n for n, _ in run) for run in runs], 64, L, P)
+    qabs, qrope = pool.queries(1, H)
+    qrope[:, :, 0] = 0.0
+    sizes = []
+    for b, run in enumerate(runs):
+        at, top = 0, max([s for _, s in run if s is not ZERO], default=0)
+        for n, s in run:
+            x = pool.randn(n, L + P)
+            x[:, :L] *= 0.0 if s is ZERO else 2.0 ** s
+            pool.put(b, at, x)
+            at += n
+        qabs[b] *= 2.0 ** -top if 0 < top <= 100 else 0.0 if top > 0 else 1.0
+        sizes.append(top)
+    qabs[:, :, 0] = 0.0
+    return pool, qabs, qrope, sizes
+
+
+def compare(pool, qabs, qrope, sizes, got, **near):
+    L = pool.L
+    for b, n in enumerate(pool.lens):
+        kv = pool.rows(b, R8.positions(n, **near)).cuda()
+        q = torch.cat([qabs[b, 0], qrope[b, 0]], -1).double().cuda()
+        out, spread, mass = R.attend(kv, q, L, SCALE)
+        down = 2.0 ** -sizes[b]
+        R8.close("i8", got[b, 0].double() * down, out * down, spread * down, mass * down,
+                 R8.score_step(kv, q, L, SCALE)[:, None].cpu(), R8.largest(kv, q, L, SCALE).cpu() * down)
+
+
+def attend(ctx, pool, qabs, qrope, **near):
+    cache, where = pool.cuda(ctx=ctx), (pool.table.cuda(), pool.lens32().cuda(), qabs.cuda(), qrope.cuda(), SCALE)
+    got = cache.attend_window(*where, near["window"], near["sinks"]) if near else cache.attend(*where)
+    ctx.synchronize()
+    return got
+
+
+@pytest.mark.parametrize("scale", [1, 60])  # whole, and cut into ranges
+@pytest.mark.parametrize("H,L,P", WIDTHS)
+@pytest.mark.parametrize("run", [
+    [(40, -60), (60, 70)], [(60, 70), (40, -60)], [(40, -100), (60, 20)], [(40, -100), (60, 100)], [(60, 100), (40, -100)],
+    [(30, -100), (30, 0), (30, 100)], [(30, 0), (64, -100), (31, 90)]])
+def test_sizes_further_apart_than_f32_holds(ctx, run, H, L, P, scale):
+    """All positions keep their weight in the sum, whatever their size."""
+    case = sized(61, [run, [(9, run[0][1])]], scale, H, L, P)
+    compare(*case, attend(ctx, *case[:3]))
+
+
+@pytest.mark.parametrize("scale", [1, 60])
+@pytest.mark.parametrize("H,L,P", WIDTHS)
+@pytest.mark.parametrize("size", [-110, -90, -80, -40, 0, 90])
+def test_zeros_before_values_of_any_size(ctx, size, H, L, P, scale):
+    """Positions of zero latent values weigh, and settle nothing about the
+    others' size; a sequence of them alone has a context of zeros."""
+    case = sized(62, [[(40, ZERO), (60, size)], [(70, ZERO)], [(3, size), (40, ZERO), (64, size)]], scale, H, L, P)
+    got = attend(ctx, *case[:3])
+    assert (got[1] == 0).all()
+    compare(*case, got)
+
+
+@pytest.mark.parametrize("H,L,P", WIDTHS)
+def test_sizes_in_a_window(ctx, H, L, P):
+    case = sized(63, [[(40, -100), (300, ZERO), (70, 100)], [(40, 80), (300, 0), (70, -90)]], 1, H, L, P)
+    compare(*case, attend(ctx, *case[:3], window=90, sinks=35), window=90, sinks=35)
+
+
+@pytest.mark.parametrize("scale", [1, 120])
+@pytest.mark.parametrize("H,L,P", WIDTHS)
+@pytest.mark.parametrize("size", [-115, 115])
+def test_smallest_and_largest_sizes(ctx, size, H, L, P, scale):
+    """Contexts of bf16's smallest normal numbers and of its largest."""
+    case = sized(64, [[(70, size)], [(30, size)]], scale, H, L, P)
+    compare(*case, attend(ctx, *case[:3]))
+
+
+@pytest.mark.parametrize("scale", [1, 120])
+@pytest.mark.parametrize("H", [128, 16])
+def test_sums_of_the_largest_values(ctx, H, scale):
+    """Many values near f32's largest, all of one sign: neither a part's context
+    nor the parts' sum leaves the range that their mean lies in."""
+    case = sized(65, [[(70, 122)], [(30, 0), (40, 122)]], scale, H, 512, 64)
+    pool = case[0]
+    pool.pages[..., :512] = pool.pages[..., :512].clamp(min=-127).abs()
+    compare(*case, attend(ctx, *case[:3]))

@@ -36,7 +36,7 @@ struct PagedMfmaArgs {
     float spread;     // plan_ranges'
     int32_t whole;    // a range is a unit (most: units), and there is no join
     void *part_o;     // [slot][group][128 quads][16 columns][4], f32 or (8-bit pages) f16
-    float *part_ml;   // [slot][group][16 columns][2]; with f16 [4], the third what part_o is to be taken times
+    float *part_ml;   // [slot][group][16 columns][2], offset and sum; with f16 [4], the third part_o's own offset
     int64_t *plan;    // [units] first tile of each, then W (where there is more than one range)
     int32_t lead;     // empty tiles before every unit with tiles but the first
 };

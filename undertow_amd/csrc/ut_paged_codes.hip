@@ -11,16 +11,15 @@
 // rate for one of it, sums exact in 32 bits, a query off by 2^-16 of its part's
 // largest at most.  Values: codes as f16, which holds them exactly, converted once
 // for a workgroup's waves; a weight meets its position's scale before it is
-// rounded to f16, w = e^(s - m) a.  Scales may be of any size: m is a column's
-// offset that puts the largest such product so far at 2^10 to 2^15, so that one
-// loses bits from 2^-24 of the largest down; the sum of the weights themselves,
-// in f32, takes the size that they have then.  m leaves the largest weight at
-// 2^60 or below, and where the first scales that a column meets are so small that
-// this is not enough, they and all behind them are taken times a power of two.
-// (A column loses bits where its largest products are below 2^-74 of that first
-// scale's size, and come with scores that let all before them vanish; and its sum
-// those weights that are below 2^-36 of the largest at scales of 2^100, 2^-15 at the
-// largest number's.)
+// rounded to f16, w = 2^up e^(s - m) a, the largest so far at 2^10 to 2^16, so that
+// one loses bits from 2^-24 of the largest down.  Scales may be of any size, and
+// the sum of the weights themselves, in f32, must not depend on that: a column has
+// an offset m for its scores and a power of two, up, for its products.  m does
+// what it can of both: up is 0 as long as m, so chosen, puts the largest weight, or
+// the sum where that is larger, at 2^-10 to 2^60 when it moves (2^90 before it has
+// to move; the sum of 2^31 of those stays in f32).  So weights below 2^-116 of the
+// largest may be lost, and nothing above them.  All are powers of two, so that a
+// move changes no bit.
 //
 // A position is 584 bytes, half a bf16 one, for the same products at the same
 // rate, so that memory bounds up to some 64 heads and the matrix cores 128.  A
@@ -50,21 +49,15 @@ typedef uint32_t pu32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kCW = kCostsI8.waves, kCodesPerCu = kCostsI8.slots;
 // LDS: two tiles of codes (32 x 512 latent ones in 16 blocks of 8 rows and 128
-// bytes, 32 x 64 rotary ones), the scales of four tiles, one tile's values.
+// bytes, 32 x 64 rotary ones), the scales of four tiles, one tile's values, the columns' up.
 constexpr int kCBlocks = 4, kCRope = 16 * 1024, kCTile = 18 * 1024, kCStages = 2;
-constexpr int kCScales = kCStages * kCTile, kCValues = kCScales + 4 * 256, kCLds = kCValues + 32 * 1024;
+constexpr int kCScales = kCStages * kCTile, kCValues = kCScales + 4 * 256, kCUps = kCValues + 32 * 1024, kCLds = kCUps + kCW * 64;
 static_assert(kCodesPerCu * (kCLds + 1024) <= 160 * 1024, "the workgroups of a CU share its LDS");
 constexpr int kCCopies = 6;  // of a wave and tile: four latent blocks, rotary codes, scales
-constexpr float kCMost = 60.0f, kCRise = 30.0f;  // log2 of the largest weight: after m moves, and before it has to
-
-// A column's 16 heads: queries as digits, 16 dims of a step of 64 in w[2 ks]
-// (high) and w[2 ks + 1] (low).
-struct CodesWave {
-    pu32x4 w[18];
-    float lat, rope;  // what a digit is worth in each part, times the scores' scale
-    pf32x4 o[32];     // context^T: dim 16 mt + 4 (l >> 4) + i, column l & 15
-    float m, l, up;   // offset (log2 units) and sum; the power of two that values are taken times
-};
+// log2 of the largest weight: after m moves, and by how much it may rise before it has to
+constexpr float kCMost = 60.0f, kCLeast = 10.0f, kCRise = 30.0f;
+// the largest product that f16 is to hold, and a little less than its log2
+constexpr float kCTop = 61440.0f, kCTopLog = 15.9f;
 
 // The lane, as if not known yet: what is worked out of it is worked out anew for
 // each tile, since the products need the registers that it would be kept in.
@@ -73,6 +66,21 @@ __device__ __forceinline__ int lane_anew() {
     asm volatile("" : "+v"(l));
     return l;
 }
+// A column's 16 heads: queries as digits, 16 dims of a step of 64 in w[2 ks]
+// (high) and w[2 ks + 1] (low).
+struct CodesWave {
+    pu32x4 w[18];
+    float lat, rope;  // what a digit is worth in each part, times the scores' scale
+    pf32x4 o[32];     // context^T: dim 16 mt + 4 (l >> 4) + i, column l & 15
+    float m, l;       // offset (a whole number of log2 units) and sum
+    bool ups;         // some column's up is not 0: all are in LDS, where they take no registers from the products
+};
+// The power of two that a column's products of weights and scales are taken times,
+// of a wave's at U.
+__device__ __forceinline__ __attribute__((address_space(3))) int *column_up(uint32_t U) {
+    return (__attribute__((address_space(3))) int *)(U + (lane_anew() & 15) * 4);
+}
+
 // The rotary codes of row r, 64 bytes: chunks of 16 XORed with 0, 2, 3 and 1 for the
 // rows 0 to 3, .. 12 to 15, so that the 16 lanes that a read takes at a time (0 to 3
 // with 12 to 15 and 20 to 27, the others likewise) meet the LDS's 16 slots once.
@@ -210,22 +218,28 @@ __device__ __forceinline__ void tile_scores(const CodesWave &x, uint32_t T, uint
 }
 
 // The weights of a tile's scores, each times its position's scale.  seen: the
-// tile's visible positions; fresh: none was before it.  Codes are finite, so that
-// what a row does not see of them needs no care.
-__device__ __forceinline__ pf16x8 tile_weights(CodesWave &w, uint32_t seen, bool &fresh, float (&t)[8], float (&s)[8]) {
+// tile's visible positions; fresh: some column has met no score but -inf yet.  Codes
+// are finite, so that what a row does not see of them needs no care.
+__device__ __forceinline__ pf16x8 tile_weights(CodesWave &w, uint32_t U, uint32_t S, uint32_t seen, bool &fresh, float (&t)[8], float (&s)[8]) {
     const int g = lane_anew() >> 4;
-    if (seen != ~0u) {
-        const uint32_t mine = seen >> (4 * g);
+    const uint32_t mine = seen >> (4 * g);
+    auto hidden = [&](int i) { return !((mine >> ((i >> 2) * 16 + (i & 3))) & 1); };
+    if (seen != ~0u)
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (!((mine >> ((i >> 2) * 16 + (i & 3))) & 1)) {  // a hidden position's scale is any
+            if (hidden(i)) {  // a hidden position's scale is any
                 t[i] = -INFINITY;
                 s[i] = 0.0f;
             }
-    }
-    if (__any(w.up != 1.0f))
+    // (one that is out of range so has a weight below 2^-116 of the largest, or a product below 2^-24)
+    auto times_up = [&]() {
+        if (w.ups) {
+            const int up = *column_up(U);
 #pragma unroll
-        for (int i = 0; i < 8; i++) s[i] = __fmul_rn(s[i], w.up);
+            for (int i = 0; i < 8; i++) s[i] = fminf(fmaxf(ldexpf(s[i], up), kLow), -kLow);
+        }
+    };
+    times_up();
     float e[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(t[i]);
@@ -235,27 +249,41 @@ __device__ __forceinline__ pf16x8 tile_weights(CodesWave &w, uint32_t seen, bool
     float size = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) size = fmaxf(size, fabsf(__fmul_rn(e[i], s[i])));
-    if (fresh || __any(size > 32768.0f || most(t) > kCMost + kCRise)) {
+    if (fresh || __any(size > kCTop || most(t) > kCMost + kCRise)) {
+        int up0 = 0;
+        if (w.ups) {  // the scales anew
+            up0 = *column_up(U);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const pf32x4 v = lds_read<pf32x4>(S + 32 * g + (i >> 2) * 128 + (i & 2) * 8);
+                s[i] = hidden(i) ? 0.0f : v[0];
+                s[i + 1] = hidden(i + 1) ? 0.0f : v[2];
+            }
+        }
+        // the largest product and weight, and the sum, less m; scales below f32's normal
+        // numbers, and 0, count as the least of those: what is so put too low has 13 bits to spare
         float u = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; i++) u = fmaxf(u, t[i] + __builtin_amdgcn_logf(fabsf(s[i])));
+        for (int i = 0; i < 8; i++) u = fmaxf(u, t[i] + fmaxf(__builtin_amdgcn_logf(fabsf(s[i])), -126.0f));
         u = col_max(u);
-        const float top = col_max(most(t)), to = fmaxf(u - 10.0f, top - kCMost);
-        const bool move = (fresh || u > 15.0f || top > kCMost + kCRise) && fabsf(to) < INFINITY;
-        const float by = move ? to : 0.0f, f = fresh ? 0.0f : __builtin_amdgcn_exp2f(-by);
-        if (fresh) {
-            const float low = top - kCMost - (u - 10.0f);  // (log2) too small for m alone
-            w.up = move && low > 0.0f && low < INFINITY ? ldexpf(1.0f, low < 120.0f ? (int)low : 120) : 1.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) s[i] = __fmul_rn(s[i], w.up);
-        }
-        w.m += by;
-        w.l *= f;
+        const float sum = col_sum(w.l), top = fmaxf(col_max(most(t)), __builtin_amdgcn_logf(sum));
+        const bool none = sum == 0.0f, rise = none || u + (float)up0 > kCTopLog;
+        const bool move = (rise || top > kCMost + kCRise) && fabsf(top) < INFINITY;
+        // where products of size 1 are to lie, less m; the weights of size 1 beside them if that may be
+        const float to = rise ? floorf(u - 10.0f) : -(float)up0;
+        const float by = move ? fminf(fmaxf(to, floorf(top - kCMost)), floorf(top + kCLeast)) : 0.0f;
+        const int up = move ? (int)(by - to) : up0;
+        const float f = none ? 0.0f : __builtin_amdgcn_exp2f((float)(up - up0) - by);
 #pragma unroll
         for (int mt = 0; mt < 32; mt++) w.o[mt] *= f;
+        w.l = ldexpf(w.l, (int)-by);
+        w.m += by;
+        w.ups = __any(up != 0);
+        if (w.ups) *column_up(U) = up;
+        times_up();
 #pragma unroll
         for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(t[i] - by);
-        fresh = false;
+        fresh = __any(top == -INFINITY);
     }
     w.l = __fadd_rn(w.l, __fadd_rn(__fadd_rn(__fadd_rn(e[0], e[1]), __fadd_rn(e[2], e[3])), __fadd_rn(__fadd_rn(e[4], e[5]), __fadd_rn(e[6], e[7]))));
     pf16x8 p;
@@ -315,20 +343,21 @@ template <class B> __device__ __forceinline__ void load_queries(const PagedArgs 
     // whole, and here: not in the loop at their first use
 #pragma unroll
     for (int i = 0; i < 18; i++) asm volatile("" : "+v"(w.w[i]));
-    w.m = kLow;
+    w.m = 0.0f;
     w.l = 0.0f;
-    w.up = 1.0f;
+    w.ups = false;
 #pragma unroll
     for (int mt = 0; mt < 32; mt++) w.o[mt] = pf32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 // A unit's context, or a range's part of it.
 template <int KIND>
-__device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, int r, int grp, bool active, const Seg &q, CodesWave &w) {
+__device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, int r, int grp, bool active, const Seg &q, CodesWave &w, uint32_t U) {
     const PagedArgs &a = p.a;
     const float sum = col_sum(w.l);
+    const int up = active && w.ups ? *column_up(U) : 0;
     const int l = lane_anew(), g = l >> 4, col = l & 15, h = q.h0 + col;
     if (active && ((KIND == kListed && p.whole) || (q.b0 == 0 && q.b1 == q.tiles))) {
-        const float inv = sum == 0.0f ? 0.0f : __fmul_rn(1.0f / sum, 1.0f / w.up);
+        const float inv = sum == 0.0f ? 0.0f : __fmul_rn(1.0f / sum, ldexpf(1.0f, -up));
         __bf16 *out = (__bf16 *)a.out + (q.row + h) * kPL + 4 * g;
         if (h < a.H)
 #pragma unroll
@@ -341,15 +370,16 @@ __device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, 
     } else if (active) {
         // a part's context in f16, which is 1/8 of what the output's own rounding to
         // bf16 may take, times a power of two of the column that puts the largest at
-        // 2^13 to 2^14
+        // 2^13 to 2^14; what that leaves of its size, and the sum's, apart: the join
+        // must not lose one to the other
         float top = 0.0f;
 #pragma unroll
         for (int mt = 0; mt < 32; mt++)
 #pragma unroll
             for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(w.o[mt][i]));
         top = col_max(top);
-        const int e = (int)(__float_as_uint(top) >> 23) - 127, up = top > 0.0f && top < INFINITY ? (13 - e < 120 ? 13 - e : 120) : 0;
-        const float f = ldexpf(1.0f, up);
+        const int e = (int)(__float_as_uint(top) >> 23) - 127, by = top > 0.0f && top < INFINITY ? (13 - e < 120 ? 13 - e : 120) : 0;
+        const float f = ldexpf(1.0f, by);
         const int64_t slot = plan_slot(r, rg.s <= q.first) * p.groups + grp;
         pf16x4 *po = (pf16x4 *)p.part_o + slot * 128 * kCols + g * kCols + col;
 #pragma unroll
@@ -359,7 +389,9 @@ __device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, 
             for (int i = 0; i < 4; i++) v[i] = (_Float16)__fmul_rn(w.o[mt][i], f);
             po[mt * 4 * kCols] = v;
         }
-        if (g == 0) *(float4 *)(p.part_ml + (slot * kCols + col) * 4) = make_float4(w.m, sum, __fmul_rn(ldexpf(1.0f, -up), 1.0f / w.up), 0.0f);
+        const int z = __builtin_amdgcn_frexp_expf(sum);
+        const float k = top == 0.0f ? kLow : w.m - (float)(by + up);
+        if (g == 0) *(float4 *)(p.part_ml + (slot * kCols + col) * 4) = make_float4(sum == 0.0f ? kLow : w.m + (float)z, ldexpf(sum, -z), k, 0.0f);
     }
 }
 
@@ -385,6 +417,7 @@ __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4) void k_paged_codes
     const bool active = w < p.per && grp < p.groups;
     const int gr = active ? grp : 0;
     const uint32_t stage0 = (uint32_t)(uintptr_t)(lds_u8 *)stage;
+    const uint32_t ups0 = __builtin_amdgcn_readfirstlane(stage0 + kCUps + w * 64);
     CodesWave wv;
     bool bad = false;
     int32_t entry = 0;  // the next copy's, of this wave's eight rows
@@ -425,10 +458,7 @@ __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4) void k_paged_codes
             convert_tile(T, V, w);
             float t[8], s[8];
             const bool some = active && seen;
-            if (some) {
-                if (fresh) wv.m = 0.0f;
-                tile_scores(wv, T, stage0 + kCScales + (n & 3) * 256, wv.m, t, s);
-            }
+            if (some) tile_scores(wv, T, stage0 + kCScales + (n & 3) * 256, wv.m, t, s);
             meet<-1>();
             // the wave that is through with its scores goes first, so that the other of its SIMD
             // is at its own scores under these products (512 prompt rows over 8192 positions 1327
@@ -438,14 +468,14 @@ __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4) void k_paged_codes
                 copy(q, x + kCStages);
                 entry = entry_of(q, x + kCStages + 1);
             }
-            if (some) tile_context(wv, tile_weights(wv, seen, fresh, t, s), V);
+            if (some) tile_context(wv, tile_weights(wv, ups0, stage0 + kCScales + (n & 3) * 256, seen, fresh, t, s), V);
             __builtin_amdgcn_s_setprio(0);
         }
         __syncthreads();  // the stages may be filled again: with the next part's first tiles
         Seg nx;
         const bool more = walk.next(p, rg, gr, nx);
         if (more) start(nx);
-        finish<KIND>(p, rg, r, grp, active, q, wv);
+        finish<KIND>(p, rg, r, grp, active, q, wv, ups0);
         if (!more) break;
         q = nx;
     }

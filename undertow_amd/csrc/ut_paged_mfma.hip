@@ -523,18 +523,20 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
 }
 
 // Joins the parts of a unit that lies in more than one range:
-// out = sum_r o_r 2^(m_r - M) / sum_r l_r 2^(m_r - M).  A workgroup takes one
-// column group and 16 NQ dims, each of its NW waves every NW-th part, as many at
-// a time as there are, with all their loads under way; the waves' results meet
-// in LDS.  Bound by the parts' bytes: 82 MB in 16.9 us (4.9 TB/s); 8 parts of
-// one row take 4.2.  NQ = 1 where that gives no more workgroups than CUs: one row
-// over 32768 positions in 8 bits 41.7 us with 4, 38.9 with 1 (bf16 37.4 and 36.0,
-// f16x2 59.1 and 56.8); two such rows, on 512 workgroups, 47.0 and 49.4.
+// out = sum_r o_r 2^(m_r - M) / sum_r l_r 2^(m_r - M); of 8-bit pages the contexts
+// have offsets of their own, k_r and K.  A workgroup takes one column group and 16
+// NQ dims, each of its NW waves every NW-th part, as many at a time as there are,
+// with all their loads under way; the waves' results meet in LDS.  Bound by the
+// parts' bytes: 82 MB in 16.9 us (4.9 TB/s); 8 parts of one row take 4.2.  NQ = 1
+// where that gives no more workgroups than CUs: one row over 32768 positions in 8
+// bits 41.7 us with 4, 38.9 with 1 (bf16 37.4 and 36.0, f16x2 59.1 and 56.8); two
+// such rows, on 512 workgroups, 47.0 and 49.4.
 template <class F, int KIND, int NW, int NQ> __global__ __launch_bounds__(NW * 64) void k_paged_join(PagedMfmaArgs p) {
     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
     typedef typename F::part_t p4 __attribute__((ext_vector_type(4)));
     __shared__ __attribute__((aligned(16))) pf32x4 so[NW][4 * NQ][kCols + 1];  // one more: other banks
     __shared__ float2 sml[NW][kCols];
+    __shared__ float sk[NW][kCols];  // 8-bit pages
     const PagedArgs &a = p.a;
     const int u = blockIdx.x / p.groups, grp = blockIdx.x - u * p.groups, tid = threadIdx.x;
     const int w = tid >> 6, col = tid & 15, qd = (tid >> 4) & 3;
@@ -544,13 +546,13 @@ template <class F, int KIND, int NW, int NQ> __global__ __launch_bounds__(NW * 6
     const int64_t N = plan_ranges(W, p.most, p.spread);
     const int r0 = (int)plan_range_of(W, N, first), r1 = (int)plan_range_of(W, N, first + tiles - 1);
     if (r0 == r1) return;
-    float m = kLow, L = 0.0f;
+    float m = kLow, L = 0.0f, at = kLow;
     pf32x4 t[NQ] = {};
     // some parts: r and every NW-th behind it
     auto add = [&](int r, auto many) {
         constexpr int COUNT = decltype(many)::value;
         float2 ml[COUNT];
-        float unit[COUNT];  // of the part's context
+        float k[COUNT];  // the contexts' offsets
         p4 v[COUNT][NQ];
 #pragma unroll
         for (int i = 0; i < COUNT; i++) {
@@ -559,32 +561,35 @@ template <class F, int KIND, int NW, int NQ> __global__ __launch_bounds__(NW * 6
             if constexpr (F::kCodes) {
                 const float4 x = *(const float4 *)(p.part_ml + (slot * kCols + col) * 4);
                 ml[i] = make_float2(x.x, x.y);
-                unit[i] = x.z;
+                k[i] = x.z;
             } else {
                 ml[i] = *(const float2 *)(p.part_ml + (slot * kCols + col) * 2);
-                unit[i] = 1.0f;
+                k[i] = kLow;  // (none: as the sum's)
             }
 #pragma unroll
-            for (int k = 0; k < NQ; k++)
-                v[i][k] = ((const p4 *)p.part_o)[(slot * 128 + blockIdx.y * 4 * NQ + qd + 4 * k) * kCols + col];
+            for (int j = 0; j < NQ; j++)
+                v[i][j] = ((const p4 *)p.part_o)[(slot * 128 + blockIdx.y * 4 * NQ + qd + 4 * j) * kCols + col];
         }
-        float mn = m;
-#pragma unroll
-        for (int i = 0; i < COUNT; i++) mn = fmaxf(mn, ml[i].x);
-        const float f0 = __builtin_amdgcn_exp2f(m - mn);
-        L *= f0;
-#pragma unroll
-        for (int k = 0; k < NQ; k++) t[k] *= f0;
+        float mn = m, kn = at;
 #pragma unroll
         for (int i = 0; i < COUNT; i++) {
-            const float f = __builtin_amdgcn_exp2f(ml[i].x - mn);
-            L = __builtin_fmaf(ml[i].y, f, L);
-            const float fo = F::kCodes ? __fmul_rn(f, unit[i]) : f;
-#pragma unroll
-            for (int k = 0; k < NQ; k++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) t[k][e] = __builtin_fmaf((float)v[i][k][e], fo, t[k][e]);
+            mn = fmaxf(mn, ml[i].x);
+            if constexpr (F::kCodes) kn = fmaxf(kn, k[i]);
         }
+        const float f0 = __builtin_amdgcn_exp2f(m - mn), g0 = F::kCodes ? __builtin_amdgcn_exp2f(at - kn) : f0;
+        L *= f0;
+#pragma unroll
+        for (int j = 0; j < NQ; j++) t[j] *= g0;
+#pragma unroll
+        for (int i = 0; i < COUNT; i++) {
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - mn), g = F::kCodes ? __builtin_amdgcn_exp2f(k[i] - kn) : f;
+            L = __builtin_fmaf(ml[i].y, f, L);
+#pragma unroll
+            for (int j = 0; j < NQ; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) t[j][e] = __builtin_fmaf((float)v[i][j][e], g, t[j][e]);
+        }
+        at = kn;
         m = mn;
     };
     int r = r0 + w;
@@ -599,6 +604,7 @@ template <class F, int KIND, int NW, int NQ> __global__ __launch_bounds__(NW * 6
     }
     if (r <= r1) add(r, std::integral_constant<int, 1>());
     if (qd == 0) sml[w][col] = make_float2(m, L);
+    if (F::kCodes && qd == 0) sk[w][col] = at;
 #pragma unroll
     for (int k = 0; k < NQ; k++) so[w][qd + 4 * k][col] = t[k];
     __syncthreads();
@@ -608,22 +614,28 @@ template <class F, int KIND, int NW, int NQ> __global__ __launch_bounds__(NW * 6
     const int64_t row = SPARSE ? u : (int64_t)u * a.M + grp / per_row;
 #pragma unroll
     for (int c = tid / (4 * NQ); c < kCols; c += 16 * NW / NQ) {
-        float M = kLow, sum = 0.0f;
+        float M = kLow, K = kLow, sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NW; i++) M = fmaxf(M, sml[i][c].x);
+        for (int i = 0; i < NW; i++) {
+            M = fmaxf(M, sml[i][c].x);
+            if (F::kCodes) K = fmaxf(K, sk[i][c]);
+        }
         pf32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NW; i++) {
-            const float f = __builtin_amdgcn_exp2f(sml[i][c].x - M);
+            const float f = __builtin_amdgcn_exp2f(sml[i][c].x - M), g = F::kCodes ? __builtin_amdgcn_exp2f(sk[i][c] - K) : f;
             const pf32x4 v = so[i][d][c];
             sum = __builtin_fmaf(sml[i][c].y, f, sum);
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(v[e], f, o[e]);
+            for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(v[e], g, o[e]);
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         o4 v;
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = (typename F::out_t)__fmul_rn(o[e], inv);
+        for (int e = 0; e < 4; e++) {
+            const float x = __fmul_rn(o[e], inv);
+            v[e] = (typename F::out_t)(F::kCodes ? ldexpf(x, (int)(K - M)) : x);
+        }
         const int h = (SPARSE ? grp : grp % per_row) * kCols + c;
         if (h < a.H) *(o4 *)((typename F::out_t *)a.out + (row * a.H + h) * kPL + blockIdx.y * 16 * NQ + 4 * d) = v;
     }
