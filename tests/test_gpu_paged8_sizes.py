@@ -103,3 +103,27 @@ def test_sums_of_the_largest_values(ctx, H, scale):
     pool = case[0]
     pool.pages[..., :512] = pool.pages[..., :512].clamp(min=-127).abs()
     compare(*case, attend(ctx, *case[:3]))
+
+
+@pytest.mark.parametrize("size", [-118, 0, 118])
+def test_long_prompts_of_the_smallest_and_largest_sizes(ctx, size):
+    """Rows whose sequence no other workgroup shares, and so no join, over
+    thousands of positions of like weight."""
+    M, H, n = 300, 128, 8400
+    pool = R8.Pool8(66, [n], 64, 512, 64, fill=False)
+    x = pool.randn(n, 576)
+    x[:, :512] *= 2.0 ** size
+    x[:, :512] += 2.0 ** (size + 1)  # means as large as the values
+    pool.put(0, 0, x)
+    qabs, qrope = pool.queries(M, H)
+    qabs.zero_()
+    qrope[:, :, 0] = 0.0
+    got = pool.cuda(ctx=ctx).attend(pool.table.cuda(), pool.lens32().cuda(), qabs.cuda(), qrope.cuda(), SCALE)
+    ctx.synchronize()
+    down = 2.0 ** -size
+    for j in (0, 151, 299):
+        kv = pool.rows(0, torch.arange(n - M + j + 1)).cuda()
+        q = torch.cat([qabs[0, j], qrope[0, j]], -1).double().cuda()
+        out, spread, mass = R.attend(kv, q, 512, SCALE)
+        R8.close("i8", got[0, j].double() * down, out * down, spread * down, mass * down,
+                 R8.score_step(kv, q, 512, SCALE)[:, None].cpu(), R8.largest(kv, q, 512, SCALE).cpu() * down)

@@ -357,14 +357,14 @@ __device__ __forceinline__ void finish(const PagedMfmaArgs &p, const Range &rg, 
     const int up = active && w.ups ? *column_up(U) : 0;
     const int l = lane_anew(), g = l >> 4, col = l & 15, h = q.h0 + col;
     if (active && ((KIND == kListed && p.whole) || (q.b0 == 0 && q.b1 == q.tiles))) {
-        const float inv = sum == 0.0f ? 0.0f : __fmul_rn(1.0f / sum, ldexpf(1.0f, -up));
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         __bf16 *out = (__bf16 *)a.out + (q.row + h) * kPL + 4 * g;
         if (h < a.H)
 #pragma unroll
             for (int mt = 0; mt < 32; mt++) {
                 pbf16x4 v;
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = (__bf16)__fmul_rn(w.o[mt][i], inv);
+                for (int i = 0; i < 4; i++) v[i] = (__bf16)ldexpf(__fmul_rn(w.o[mt][i], inv), -up);  // (apart: both may be tiny)
                 *(pbf16x4 *)(out + 16 * mt) = v;
             }
     } else if (active) {
