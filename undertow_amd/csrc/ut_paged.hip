@@ -1057,7 +1057,6 @@ struct DeviceScope {
 };
 
 constexpr int64_t kMostRows = 65535;         // query rows of a call
-constexpr int64_t kMostGroups = 1ll << 22;   // workgroups along a grid's first axis, where pages set them
 static int32_t paged_args(ut_ctx *ctx, const DeviceScope &dev, const char *what, const ut_mla_pages *kv,
                           const int32_t *table, int64_t stride, int64_t max_pages,
                           const int32_t *lens, int64_t B, int64_t M, int64_t H, int64_t most_rows,
@@ -1193,22 +1192,24 @@ extern "C" int32_t ut_mla_paged_append(ut_ctx *ctx, const ut_mla_pages *kv,
     }
     // pages that `rows` positions can fall into
     const int64_t page = kv->page, touched = (rows + page - 2) / page + 1;
-    if (touched > kMostGroups && max_pages > kMostGroups) {
-        set_error(ctx, "ut_mla_paged_append: rows of more than %lld pages in a call", (long long)kMostGroups);
+    const int threads = kv->fmt == UT_KV_I8 ? kAppendWaves * 64 : 576;
+    const int64_t most = most_groups(threads);
+    if (touched > most && max_pages > most) {
+        set_error(ctx, "ut_mla_paged_append: rows of more than %lld pages in a call", (long long)most);
         return UT_ERR_SHAPE;
     }
     const size_t lds = kv->mean ? (size_t)(a.L + a.P) * 4 * sizeof(double) : 0;
     const dim3 grid((unsigned)(touched < max_pages ? touched : max_pages), (unsigned)batch);
     int tok = timing_begin(ctx, "paged_append");
     if (kv->fmt == UT_KV_BF16)
-        hipLaunchKernelGGL(k_paged_append<Bf16>, grid, dim3(576), lds, ctx->stream, a,
+        hipLaunchKernelGGL(k_paged_append<Bf16>, grid, dim3(threads), lds, ctx->stream, a,
                            (uint16_t *)kv->pages, latent_dev, krot_dev, kv->mean, kv->mean_scale);
     else if (kv->fmt == UT_KV_I8)
         hipLaunchKernelGGL((a.L == 512 && a.P == 64 ? k_paged_append_i8<RowWide> : k_paged_append_i8<RowAny>), grid,
-                           dim3(kAppendWaves * 64), 0, ctx->stream, a, (int8_t *)kv->pages, (float2 *)kv->scales,
+                           dim3(threads), 0, ctx->stream, a, (int8_t *)kv->pages, (float2 *)kv->scales,
                            latent_dev, krot_dev, kv->mean, kv->mean_scale);
     else
-        hipLaunchKernelGGL(k_paged_append<F16x2>, grid, dim3(576), lds, ctx->stream, a,
+        hipLaunchKernelGGL(k_paged_append<F16x2>, grid, dim3(threads), lds, ctx->stream, a,
                            (uint16_t *)kv->pages, latent_dev, krot_dev, kv->mean, kv->mean_scale);
     timing_end(ctx, tok);
     return launch_check(ctx, "k_paged_append");
@@ -1231,9 +1232,10 @@ extern "C" int32_t ut_mla_paged_read(ut_ctx *ctx, const ut_mla_pages *kv, const 
     }
     const int per = kReadThreads / ((a.L + a.P) / 4);  // rows of a workgroup at a time
     const int64_t groups = (rows + per * kReadTurns - 1) / (per * kReadTurns);
-    if (groups > kMostGroups) {
+    constexpr int64_t most = most_groups(kReadThreads);
+    if (groups > most) {
         set_error(ctx, "ut_mla_paged_read: more than %lld rows of a sequence in a call",
-                  (long long)(kMostGroups * per * kReadTurns));
+                  (long long)(most * per * kReadTurns));
         return UT_ERR_SHAPE;
     }
     const dim3 grid((unsigned)groups, (unsigned)batch);
@@ -1322,9 +1324,10 @@ extern "C" int32_t ut_mla_page_select(ut_ctx *ctx, const ut_mla_pages *kv, const
                   (long long)top_k, (long long)keep_first, (long long)keep_last);
         return UT_ERR_ARG;
     }
-    if (max_pages > kMostGroups * kScorePages) {
+    constexpr int64_t most = most_groups(256) * kScorePages;
+    if (max_pages > most) {
         set_error(ctx, "ut_mla_page_select: a row chooses among at most %lld pages, the table holds %lld",
-                  (long long)(kMostGroups * kScorePages), (long long)max_pages);
+                  (long long)most, (long long)max_pages);
         return UT_ERR_SHAPE;
     }
     a.qabs = qabs_dev;

@@ -229,6 +229,12 @@ UT_PLAN_FN uint32_t near_every(int32_t v0, int32_t n, int32_t M, int32_t window,
 // Positions of a sequence or a selection: tile and page counts may step past
 // the end by some tiles and stay in 32 bits.
 constexpr int64_t kMostPositions = INT32_MAX - 1023;
+// Workgroups along a grid's first axis, where pages set them: 2^22, and of larger
+// ones as many as have fewer than 2^32 threads, the most that a launch takes.
+constexpr int64_t most_groups(int64_t threads) {
+    const int64_t n = ((int64_t(1) << 32) - 1) / threads;
+    return n < (1 << 22) ? n : 1 << 22;
+}
 // A length cut to what the table can hold; a page id cut to the pool.
 UT_PLAN_FN int32_t plan_len(int32_t n, int64_t cap, bool &bad) {
     if (n >= 0 && n <= cap) return n;
