@@ -127,3 +127,47 @@ def test_long_prompts_of_the_smallest_and_largest_sizes(ctx, size):
         out, spread, mass = R.attend(kv, q, 512, SCALE)
         R8.close("i8", got[0, j].double() * down, out * down, spread * down, mass * down,
                  R8.score_step(kv, q, 512, SCALE)[:, None].cpu(), R8.largest(kv, q, 512, SCALE).cpu() * down)
+
+
+@pytest.mark.parametrize("scale", [1, 60])
+@pytest.mark.parametrize("H", [128, 16])
+def test_scores_below_f32_before_others(ctx, H, scale):
+    """Positions whose scores are -inf in f32 weigh nothing, and those behind
+    them, far below 0 themselves, share the whole weight."""
+    n, far = 100 * scale, 40 * scale
+    pool = R8.Pool8(67, [n, 70], 64, 512, 64, fill=False)
+    for b, m in enumerate((n, 70)):
+        x = pool.randn(m, 576)
+        size = torch.full((m, 1), 2.0 ** -100)
+        size[:far if b == 0 else 33] = 2.0 ** 40
+        x[:, :512] = x[:, :512].abs() * size
+        x[:, 512:] = 1.0 + x[:, 512:] * 0.05
+        pool.put(b, 0, x)
+    qabs, qrope = pool.queries(1, H)
+    qabs, qrope = -(qabs.abs() * 2.0 ** 100), -(qrope.abs() + 40.0)
+    got = attend(ctx, pool, qabs, qrope)
+    for b, m in enumerate((n, 70)):
+        kv = pool.rows(b, torch.arange(far if b == 0 else 33, m)).cuda()
+        q = torch.cat([qabs[b, 0], qrope[b, 0]], -1).double().cuda()
+        assert float((q @ kv.T * SCALE).max()) < -150.0
+        out, spread, mass = R.attend(kv, q, 512, SCALE)
+        # f32 scores of size s carry s 2^-22 or so, beside the queries' steps
+        step = R8.score_step(kv, q, 512, SCALE)[:, None].cpu() + float((q @ kv.T * SCALE).abs().max()) * 2.0 ** -21
+        up = 2.0 ** 100
+        R8.close("i8", got[b, 0].double() * up, out * up, spread * up, mass * up, step, R8.largest(kv, q, 512, SCALE).cpu() * up)
+
+
+@pytest.mark.parametrize("order", [[0, 1, 2, 3, 4, 5], [5, 4, 3, 2, 1, 0], [2, 5, 0, -1, 4]])
+@pytest.mark.parametrize("H", [128, 16])
+def test_sizes_on_listed_pages(ctx, H, order):
+    pool, qabs, qrope, sizes = sized(68, [[(64, -100), (64, ZERO), (64, 100), (64, 0), (64, -115), (30, 100)]], 1, H, 512, 64)
+    sel = torch.tensor([[order]], dtype=torch.int32)
+    got = pool.cuda(ctx=ctx).attend_pages(pool.table.cuda(), pool.lens32().cuda(), qabs.cuda(), qrope.cuda(), SCALE, sel.cuda())
+    ctx.synchronize()
+    at = torch.cat([torch.arange(64 * k, min(64 * k + 64, 350)) for k in order if k >= 0])
+    kv = pool.rows(0, at).cuda()
+    q = torch.cat([qabs[0, 0], qrope[0, 0]], -1).double().cuda()
+    out, spread, mass = R.attend(kv, q, 512, SCALE)
+    down = 2.0 ** -100
+    R8.close("i8", got[0, 0].double() * down, out * down, spread * down, mass * down,
+             R8.score_step(kv, q, 512, SCALE)[:, None].cpu(), R8.largest(kv, q, 512, SCALE).cpu() * down)
