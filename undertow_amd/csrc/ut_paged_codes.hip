@@ -29,10 +29,10 @@
 // Hence two workgroups a CU, four waves each, that know nothing of one another, and
 // a higher priority for the one that is past its scores.  What bounds it now, with
 // tiles of 32 positions:
-// - 128 heads: instructions.  A tile takes 2.35 us a CU where its data come from L2
-//   (512 prompt rows over 8192 positions 1177 us, 0.96 PFLOP/s; without the priority
-//   8 % more; bf16 pages, which need no conversion, 984), 2.6 to 2.8 with the traffic
-//   of decoding: 64 sequences of up to 8192 113 to 117 us, as bf16.
+// - 128 heads: instructions.  A tile takes 2.4 us a CU where its data come from L2
+//   (512 prompt rows over 8192 positions 1220 us, 0.91 PFLOP/s; without the priority
+//   6 % more; bf16 pages, which need no conversion, 1020), 2.6 to 2.8 with the traffic
+//   of decoding: 64 sequences of up to 8192 118 us, as bf16.
 // - 16 heads: memory, 1.03 us a tile and CU (4.7 TB/s), once it runs: 37 sequences
 //   of up to 12001 46 us in all (132 MB), of which its start, the ranges' ends and
 //   the join take 18.
@@ -54,7 +54,8 @@ constexpr int kCBlocks = 4, kCRope = 16 * 1024, kCTile = 18 * 1024, kCStages = 2
 constexpr int kCScales = kCStages * kCTile, kCValues = kCScales + 4 * 256, kCUps = kCValues + 32 * 1024, kCLds = kCUps + kCW * 64;
 static_assert(kCodesPerCu * (kCLds + 1024) <= 160 * 1024, "the workgroups of a CU share its LDS");
 constexpr int kCCopies = 6;  // of a wave and tile: four latent blocks, rotary codes, scales
-// log2 of the largest weight: after m moves, and by how much it may rise before it has to
+// log2 of the largest weight, or of the sum where that is larger: 60 at most and -10 at
+// least after m moves, and by how much a weight may rise above that before it has to
 constexpr float kCMost = 60.0f, kCLeast = 10.0f, kCRise = 30.0f;
 // the largest product that f16 is to hold, and a little less than its log2
 constexpr float kCTop = 61440.0f, kCTopLog = 15.9f;
@@ -148,8 +149,8 @@ template <int I0, int I1> __device__ __forceinline__ float query_digits(pu32x4 (
 // and 64 values that the transposing reads take; wave w: row block w.  A lane
 // takes 16 codes of a row, which become two of a block's eight chunks of a row:
 // those of odd blocks are XORed with one more, so that the eight lanes of a row
-// write to different slots (1192 us for 512 prompt rows over 8192 positions; with
-// reads of 8 codes, in halves by turns, that met in slots, 1230).
+// write to different slots (with reads of 8 codes, in halves by turns, that met in
+// slots, 512 prompt rows over 8192 positions take 3 % more).
 //   f16(code) = (1024 + (code + 128)) - 1152, each step exact.
 __device__ __forceinline__ void convert_tile(uint32_t T, uint32_t V, int w) {
     const pf16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
@@ -461,8 +462,8 @@ __global__ __launch_bounds__(kCW * 64, kCodesPerCu * kCW / 4) void k_paged_codes
             if (some) tile_scores(wv, T, stage0 + kCScales + (n & 3) * 256, wv.m, t, s);
             meet<-1>();
             // the wave that is through with its scores goes first, so that the other of its SIMD
-            // is at its own scores under these products (512 prompt rows over 8192 positions 1327
-            // us without, 1227 with; at the scores 1290, at the context's products 1255)
+            // is at its own scores under these products (512 prompt rows over 8192 positions 1296
+            // us without, 1222 with; at the scores 1276, at the context's products 1246)
             __builtin_amdgcn_s_setprio(1);
             if (x + kCStages < q.b1) {
                 copy(q, x + kCStages);

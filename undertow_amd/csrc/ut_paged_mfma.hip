@@ -331,8 +331,8 @@ template <class F> __device__ __forceinline__ bool tile_odd(uint8_t *T, uint32_t
 // run while the next three (one) are on their way.  A table entry is read a
 // tile before its copy, and the copies issue between the products.
 // FEW: some waves have no heads, and load no queries (one row over 509 positions
-// 16.5 us where all load some, 14.5 so; with the branch where all have heads, 64
-// sequences of up to 8192 positions 130 us instead of 126).
+// 15.5 us where all load some, 12.3 so; with the branch where all have heads, 64
+// sequences of up to 8192 positions 121 us instead of 117).
 template <class F, int KIND, bool OWN, bool FEW>
 __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(PagedMfmaArgs p) {
     constexpr bool SPARSE = KIND == kListed;
@@ -529,8 +529,8 @@ __global__ __launch_bounds__(F::kWaves * 64, F::kWaves / 4) void k_paged_mfma(Pa
 // with all their loads under way; the waves' results meet in LDS.  Bound by the
 // parts' bytes: 82 MB in 16.9 us (4.9 TB/s); 8 parts of one row take 4.2.  NQ = 1
 // where that gives no more workgroups than CUs: one row over 32768 positions in 8
-// bits 41.7 us with 4, 38.9 with 1 (bf16 37.4 and 36.0, f16x2 59.1 and 56.8); two
-// such rows, on 512 workgroups, 47.0 and 49.4.
+// bits 39.1 us with 4, 36.8 with 1 (bf16 34.0 and 32.8, f16x2 54.2 and 52.2); two
+// such rows, on 512 workgroups, 44.8 and 46.0 (bf16 45.7 and 44.9).
 template <class F, int KIND, int NW, int NQ> __global__ __launch_bounds__(NW * 64) void k_paged_join(PagedMfmaArgs p) {
     typedef typename F::out_t o4 __attribute__((ext_vector_type(4)));
     typedef typename F::part_t p4 __attribute__((ext_vector_type(4)));
@@ -692,7 +692,7 @@ template <class F, int KIND> static int32_t launch_fmt(ut_ctx *ctx, const PagedA
     const dim3 grid((unsigned)((int64_t)p.units * p.groups), kPlanJoinSlices);
     int tok = timing_begin(ctx, "paged_join");
     // (8-bit pages: one wave where a unit has few parts, so that more workgroups run at a time: 256
-    // sequences of up to 2048 positions 158 us with four, 147 with two, 143 with one)
+    // sequences of up to 2048 positions 148 us with four, 137 with two, 133 with one)
     if (F::kCodes && p.most <= 8 * p.units)
         hipLaunchKernelGGL((k_paged_join<F, KIND, 1, 4>), grid, dim3(64), 0, ctx->stream, p);
     else if (plan.wide && (int64_t)grid.x * 4 * kPlanJoinSlices <= ctx->multiprocessors)

@@ -80,26 +80,28 @@ inline int32_t plan_lead(const PlanCostsMany &c, int32_t groups) { return groups
 inline int32_t plan_wide(const PlanCostsMany &c, int32_t units, int32_t groups) {
     return groups <= c.waves && units < 4 ? 8 : 2 * units;
 }
-// lead: 64 sequences of up to 8192 positions take 135 us with 0, 132 with 2, 126
-// with 4, 115 with 8, 117 with 16.  ratio: one row over 32768 positions 48 us
-// with 2, 44 with 3, 42 with 4, 41 with 8, and 59 in as many ranges as CUs; 4
-// rows over 500 positions 19.8, 20.8, 20.4, 24.3.  bytes_ratio (2 x 32 KB at a 5
-// TB/s that all share): 5 x 4 rows over up to 2083 positions 39.3 us without,
-// 36.4 with 150, 35.3 with 75; 49 rows of up to 24 20.3, 18.5, 24.7.
+// lead: 64 sequences of up to 8192 positions take 134 us with 0, 127 with 4, 117
+// with 8, 118 with 16.  ratio: one row over 32768 positions 33.9 us with 2, 32.8
+// with 4, 32.3 with 8; 4 rows over up to 500 14.7, 14.9, 15.4.  bytes_ratio (2 x
+// 32 KB at a 5 TB/s that all share): 5 x 4 rows over up to 2083 positions 39.1 us
+// without, 35.9 with 150, 32.8 with 75, which was the worst for short sequences
+// (49 rows of up to 24) before these went whole.
 constexpr PlanCosts kCostsBf16 = {8, 8, 4, 150, 2.5f, 20};
-// (a tile takes twice as long) lead: 11 x 3 rows 103 us with 0, 96.1 with 2, 96.4
-// with 4, 99.7 with 8.  ratio: one row over 500 positions 22.0 us with 4, 19.5
-// with 16; over 10000 43.2 in as many ranges as CUs, 40.0 with 16, 40.6 with 32.
-// bytes_ratio: 63 x 4 rows of up to 25 positions 66.5 us without and with 280,
-// 80.4 with 140.
+// (a tile takes twice as long) lead: 11 x 3 rows 104 to 111 us with 0, 96.2 with 2,
+// 96.3 with 4, 99.4 with 8.  ratio: one row over 500 positions 18.6 us with 4, 15.8
+// with 16 and 32; over 10000 40.1, 35.1 and 32.8.  bytes_ratio: 63 x 4 rows of up to
+// 25 positions took 66.5 us without and with 280, 80.4 with 140, before these went
+// whole (51.1).
 constexpr PlanCosts kCostsF16x2 = {4, 4, 16, 280, 1.3f, 10};
 // (two workgroups of four waves a CU; a part in f16 is half as many bytes)  ratio:
-// one row over 32768 positions 47.8 us with 4, 43.4 with 8, 46.4 with 12.
-// bytes_ratio: 64 sequences of up to 600 47 us with 150, 41.5 with 300; 256 of up to
-// 1024 97 with 300, 110 with 600.  lead: those 256 109 us with 4, 97 with 8, 98 with
-// 14; with 64 heads 77 with 0, 64 with 2, 60 with 4, 64 with 8, with 16 heads 53, 44,
-// 43.5 and 46.  One row over 32768 with its heads spread over the CUs' places 54 us, over the
-// CUs alone, which then take two ranges each, 47.8.
+// one row over 32768 positions 42.3 us with 4, 36.7 with 8, 40.1 with 12, over 8192
+// 26.1, 23.1 and 24.9.  bytes_ratio: 64 sequences of up to 600 44.4 us with 150, 37.5
+// with 300, 35.4 with 600; 20 x 3 rows over up to 1500 50.5, 44.6 and 44.6; 12 of up
+// to 3000 37.5, 35.0 and 32.8; 256 of up to 2048 133 with each.  lead: 256 of up to
+// 1024 86.6 us with 4, 91.6 with 8, 93.6 with 14.  few: the same with 64 heads 60.5
+// with 2, 56.9 with 4, 59.7 with 8, with 16 heads 37.3, 38.2 and 41.4.  (Heads are
+// spread over the CUs, which then take two ranges each, and not over their places:
+// one row over 32768 took 13 % more so.)
 constexpr PlanCostsMany kCostsI8 = {{4, 8, 8, 300, 2.5f, 20}, 2, 4};
 struct PlanCall {
     int32_t whole;        // a range is a unit: no parts, no join
@@ -111,8 +113,8 @@ struct PlanCall {
 };
 // Where n ranges (or whole units) leave CUs free, a call's heads are spread
 // over them: a workgroup of few columns issues its queries, tiles' products and
-// results sooner (one row over 509 positions 18.9 us with 8 column groups a
-// workgroup, 15.8 with one; one row over 32 listed pages of 64 23.7 and 21.1).
+// results sooner (one row over 509 positions 18.4 us with 8 column groups a
+// workgroup, 12.3 with one; one row over 32 listed pages of 64 23.1 and 16.0).
 inline void plan_heads(PlanCall &p, const PlanCosts &c, int32_t cus, int32_t groups, int32_t n) {
     const int32_t free = n < cus ? cus / n : 1;
     p.per = free < groups ? (groups + free - 1) / free : 1;
@@ -128,24 +130,24 @@ inline void plan_heads(PlanCall &p, const PlanCosts &c, int32_t cus, int32_t gro
 // tiles do not count for the heads' spread) and their join, whichever takes
 // fewer tiles' time: whole units that of the longest one, ranges that of the
 // tiles there are.  Cut and whole, lengths spread evenly up to the longest: 64
-// sequences of up to 1024 positions 45 and 48 us, of up to 8192 113 and 313; 256
-// of up to 1024 105 and 85, of up to 4096 218 and 264; 64 x 4 of up to 1024 94 and
-// 78, of up to 4096 189 and 245.  All of them that long: 256 of 2048 204 and 177,
+// sequences of up to 1024 positions 44 and 46 us, of up to 8192 117 and 347; 256
+// of up to 1024 105 and 85, of up to 4096 220 and 257; 64 x 4 of up to 1024 94 and
+// 76, of up to 4096 194 and 236.  All of them that long: 256 of 2048 204 and 177,
 // 64 x 4 of 4096 309 and 291; one of them, the others a sixteenth: 65 and 127, 75
 // and 229; none of them, all a sixteenth of the table: 66 and 32, 55 and 38 (a
 // table cut to the pages in use is cheaper).
 // Up to `brief` tiles a sequence the ranges' tiles count in full: they save
 // little where one is long, and cost more where all are.  64 of up to 600
-// positions 40 and 34 us, all of them that long 47 and 36, one of them 32 and 34.
+// positions 40 and 31 us, all of them that long 47 and 36, one of them 32 and 34.
 //
 // Where a unit's column groups alone fill the CUs (prompt rows), there is one
 // range: its workgroups each go through all units, in rounds over the CUs,
 // leave no parts and need no join.  Their tiles differ only by their rows' place
 // in a unit, where whole units of differing lengths may leave CUs idle, so these
 // have to be fewer by a tenth.  Of 128 heads, whole and as one range: 4 x 256 rows
-// over up to 4096 positions 705 and 711 us, 3 x 777 over up to 1900 710 and 735 (in
-// f16 pairs 2131 and 2220, in 8 bits 805 and 832), 5 x 300 over up to 300 177 and
-// 201, 2 x 512 over up to 1024 212 and 207.
+// over up to 4096 positions 707 and 720 us, 3 x 777 over up to 1900 689 and 724 (in
+// f16 pairs 2134 and 2243, in 8 bits 800 and 839), 5 x 300 over up to 300 176 and
+// 201, 2 x 512 over up to 1024 211 and 207.
 template <class Costs>
 PlanCall plan_call(const Costs &c, int32_t cus, int32_t units, int32_t groups, int64_t each, int64_t listed,
                    bool lists) {
@@ -176,13 +178,13 @@ PlanCall plan_call(const Costs &c, int32_t cus, int32_t units, int32_t groups, i
     }
     if (p.most == 1) return p;
     // The join takes 16 waves a workgroup, and twice the ranges pay, where there
-    // are few units of many parts: one row over 32768 positions 42.8 us with 4
-    // waves, 39.5 with 16, 37.2 with the ranges (over 509, 8 parts, 15.5 and 15.9).
+    // are few units of many parts: one row over 32768 positions 38.4 us with 4
+    // waves, 33.9 with 16, 32.8 with the ranges (over 509, 8 parts, they gain nothing).
     // A few units of 8-bit pages whose heads a workgroup has all take few places, so
-    // that they get eight units' in all: 64 heads over 32768 positions 35.0 us with
-    // twice, 34.6 with four times, 31.3 with eight times the ranges, 16 heads 30.5,
-    // 28.7 and 26.0, two rows of 16 heads over up to 4096 19.8, 18.2 and 19.0, four
-    // 20.6, 21.3 and 22.8; 128 heads over 32768 38.6, 40.4 and 39.6.
+    // that they get eight units' in all: 64 heads over 32768 positions 32.4 us with
+    // twice, 32.6 with four times, 30.2 with eight times the ranges, 16 heads 28.2,
+    // 26.3 and 24.1, two rows of 16 heads over up to 4096 17.2, 17.2 and 15.4, four
+    // 17.6, 19.2 and 17.7; 128 heads over 32768 36.7, 38.4 and 37.6.
     p.wide = (int64_t)units * groups * kPlanJoinSlices <= cus && p.most > 16 * units;
     if (p.wide) cut(plan_wide(c, units, groups));
     p.slots = plan_slot(p.most, false) * groups;
