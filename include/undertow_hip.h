@@ -369,8 +369,10 @@ int32_t ut_mla_paged_read(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *ta
  * pages keep the weights to 22 bits.  With 8-bit pages of 8 positions and more at
  * those widths each part of a query is rounded to 2^-16 of its largest value, a
  * weight times its position's scale to 2^-11, and so is the context of each part
- * of a sequence that is cut; others compute in f32.  Equal calls give equal bits; a row's
- * rounding may depend on the sizes of the call and the lengths of its batch
+ * of a sequence that is cut; scales may be of any size, scores of parts whose
+ * largest query value lies below 2^-100 lose bits, above 2^100 they may overflow;
+ * others compute in f32.  Equal calls give equal bits; a row's rounding may
+ * depend on the sizes of the call and the lengths of its batch
  * (the work is cut evenly over the device).  Working memory: some 135 MB of the
  * arena at most; none where the rows alone fill the device (prompts). */
 int32_t ut_mla_paged_attend(ut_ctx *ctx, const ut_mla_pages *kv, const int32_t *table_dev,

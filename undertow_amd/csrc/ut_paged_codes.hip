@@ -18,8 +18,10 @@
 // what it can of both: up is 0 as long as m, so chosen, puts the largest weight, or
 // the sum where that is larger, at 2^-10 to 2^60 when it moves (2^90 before it has
 // to move; the sum of 2^31 of those stays in f32).  So weights below 2^-116 of the
-// largest may be lost, and nothing above them.  All are powers of two, so that a
-// move changes no bit.
+// sum may be lost, and nothing above them.  All are powers of two, so that a move
+// changes no bit.  (What a query's digit is worth is an f32 number, and its product
+// with the codes' sum another: scores of parts whose largest value lies below 2^-100
+// lose bits, above 2^100 they may overflow.)
 //
 // A position is 584 bytes, half a bf16 one, for the same products at the same
 // rate, so that memory bounds up to some 64 heads and the matrix cores 128.  A
@@ -232,7 +234,7 @@ __device__ __forceinline__ pf16x8 tile_weights(CodesWave &w, uint32_t U, uint32_
                 t[i] = -INFINITY;
                 s[i] = 0.0f;
             }
-    // (one that is out of range so has a weight below 2^-116 of the largest, or a product below 2^-24)
+    // (one that is out of range so has a weight below 2^-116 of the sum, or a product below 2^-24)
     auto times_up = [&]() {
         if (w.ups) {
             const int up = *column_up(U);
